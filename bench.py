@@ -460,8 +460,8 @@ KERNEL_SOURCES = (
     ("int8_gemm", ("int8_gemm.hip",)),
     ("sage_kmean", ("sage_quant.hip", "sage_prep.h")),
     ("sage_quant", ("sage_quant.hip", "sage_prep.h")),
-    ("sage_v_prep", ("sage_attn.hip", "attn_common.h", "attn_plan.h", "sage_prep.h")),
-    ("sage_attn", ("sage_attn.hip", "attn_common.h", "attn_plan.h", "sage_prep.h")),
+    ("sage_v_prep", ("sage_attn.hip", "attn_common.h", "attn_plan.h", "sage_prep.h", "sage_tile.h")),
+    ("sage_attn", ("sage_attn.hip", "attn_common.h", "attn_plan.h", "sage_prep.h", "sage_tile.h")),
 )
 
 
