@@ -457,7 +457,7 @@ CSRC_DIR = os.path.join(ROOT, "comfyui-turing-utils_amd", "csrc")
 # includes are added by kernel_sources_digest).
 KERNEL_SOURCES = (
     ("convrot_quant", ("convrot_quant.hip", "ln_common.h")),
-    ("int8_gemm", ("int8_gemm.hip",)),
+    ("int8_gemm", ("int8_gemm.hip", "adapters.h")),
     ("sage_kmean", ("sage_quant.hip", "sage_prep.h")),
     ("sage_quant", ("sage_quant.hip", "sage_prep.h")),
     ("sage_v_prep", ("sage_attn.hip", "attn_common.h", "attn_plan.h", "sage_prep.h", "sage_tile.h")),

@@ -24,6 +24,7 @@ from .ops import (
     turing_layer_norm_affine_int8_convrot_quantize,
     turing_swiglu_int8_convrot_quantize,
 )
+from .adapters import LinearAdapters, turing_int8_linear_adapters
 from . import turing_sage
 
 # Version gates of the plugin compare against the reference's 0.29.1 ABI
@@ -32,12 +33,14 @@ from . import turing_sage
 __version__ = "0.29.1"
 
 __all__ = [
+    "LinearAdapters",
     "turing_bf16_gelu_int8_convrot_quantize",
     "turing_bf16_int8_convrot_quantize",
     "turing_dequantize_int8_bf16",
     "turing_gelu_int8_convrot_quantize",
     "turing_int8_gemm_i32",
     "turing_int8_linear",
+    "turing_int8_linear_adapters",
     "turing_int8_linear_out",
     "turing_layer_norm_adaln",
     "turing_layer_norm_adaln_int8_convrot_quantize",

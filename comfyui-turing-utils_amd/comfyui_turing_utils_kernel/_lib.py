@@ -163,9 +163,30 @@ SIGNATURES: dict[str, tuple[object, list[object]]] = {
         _i32,
         [_c_void_p, _c_void_p, _c_void_p, _c_void_p, _c_void_p, _i64, _i64, _f32, _c_void_p],
     ),
+    "tu_int8_gemm_adapters_workspace": (_i64, [_i64, _i64, _i64, _i64, _i32]),
+    "tu_int8_gemm_adapters": (
+        _i32,
+        [_c_void_p, _c_void_p, _c_void_p, _c_void_p, _c_void_p, _c_void_p, _c_void_p, _c_void_p, _c_void_p, _i64,
+         _i64, _i64, _c_void_p, _c_void_p, _i64, _c_void_p, _i64, _i64, _i64, _i32, _c_void_p, _i64, _c_void_p],
+    ),
+    "tu_sage_block_select_workspace": (_i64, [_i64, _i64, _i64, _i64, _i64, _i64]),
+    "tu_sage_block_select": (
+        _i32,
+        [_c_void_p, _c_void_p, _i64, _c_void_p, _c_void_p, _i64, _i64, _i64, _i64, _i64, _i64, _i64,
+         _i64, _i64, _i64, _i64, _i64, _i64, _c_void_p, _c_void_p, _i64, _i64, _i64, _i32, _c_void_p, _i64,
+         _c_void_p, _c_void_p],
+    ),
+    "tu_sage_block_attn_workspace": (_i64, [_i64, _i64, _i64, _i64, _i64, _i32]),
+    "tu_sage_block_attn": (
+        _i32,
+        [_c_void_p, _c_void_p, _i64, _c_void_p, _c_void_p, _i64, _c_void_p, _i64, _c_void_p, _i64, _c_void_p,
+         _i64, _i64, _i64, _i64, _i64, _i64,
+         _i64, _i64, _i64, _i64, _i64, _i64, _i64, _i64, _i64,
+         _c_void_p, _c_void_p, _f32, _i32, _i32, _c_void_p, _i64, _c_void_p],
+    ),
 }
 
-ABI_VERSION = 18
+ABI_VERSION = 19
 
 _lock = threading.Lock()
 _lib: ctypes.CDLL | None = None

@@ -7,6 +7,11 @@ Facade functions with the reference's names (``turing_sage/__init__.py``):
 dense W8A8 path: ``w8a8attn``, ``w8a8attn_compiled``, ``prequantize_sol_sageattn``,
 ``prequantize_sol_sageattn_from_qk``, ``sol_sparse_sageattn_from_prequantized``,
 ``preflight_w8a8``.
+
+Beside them, without a counterpart in the reference's facade (and so not in
+``__all__``, which is the reference's list): the block-sparse attention of
+``sparse.py``, ``sparse_sageattn``, ``sparse_sageattn_from_prequantized``,
+``select_key_blocks`` and ``key_block_attention``.
 """
 from __future__ import annotations
 
@@ -199,6 +204,12 @@ def preflight_w8a8(device: torch.device) -> None:
 
 # Registers the torch.ops.turing_utils attention ops on import.
 from . import custom_ops  # noqa: E402,F401
+from .sparse import (  # noqa: E402,F401
+    key_block_attention,
+    select_key_blocks,
+    sparse_sageattn,
+    sparse_sageattn_from_prequantized,
+)
 
 __all__ = [
     "available",

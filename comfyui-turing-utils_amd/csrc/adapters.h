@@ -1,0 +1,40 @@
+// What the two halves of a projection with low-rank adapters share: the
+// down-projection (adapters.hip) writes its rows, the INT8 GEMM's epilogue
+// (int8_gemm.hip) reads them.
+#pragma once
+
+#include "tu_common.h"
+
+namespace tu {
+
+// h holds `parts` planes [m][rank] of fp32 partial sums (ranges of K), scaled
+// by the row's activation scale and its adapter's scaling; rows without an
+// adapter are not written.
+struct Adapters {
+    const float *h;
+    const uint16_t *up;    // bf16 [count][n][rank]
+    const int32_t *ids;    // adapter of rows i * id_rows .. (i + 1) * id_rows - 1
+    int64_t id_rows;
+    int rank, count, parts;
+};
+
+// The adapter of a row, -1 for none (also where the id names no adapter).
+__device__ __forceinline__ int adapter_of(const int32_t *ids, int64_t id_rows, int count, int64_t row, int64_t m) {
+    if (row >= m) return -1;
+    const int64_t i = (row | id_rows) >> 32 ? row / id_rows : static_cast<uint32_t>(row) / static_cast<uint32_t>(id_rows);
+    const int a = ids[i];
+    return static_cast<uint32_t>(a) < static_cast<uint32_t>(count) ? a : -1;
+}
+
+// Ranges of K, and workgroups that share a row tile's adapters, of the
+// down-projection.
+struct DownPlan {
+    int parts, slots;
+    int64_t per;  // bytes of K per range, a multiple of 64
+};
+DownPlan down_plan(int64_t m, int64_t k, int64_t rank, int64_t count, int cus);
+
+int32_t launch_down(const int8_t *a, const float *a_scale, const uint16_t *down, const float *scaling,
+                    const Adapters &ad, const DownPlan &plan, float *h, int64_t m, int64_t k, hipStream_t st);
+
+}  // namespace tu

@@ -1,0 +1,478 @@
+// Sage INT8 attention over listed key blocks (block-sparse attention) for
+// gfx950.  No counterpart among the reference's kernels that this build
+// restates; arithmetic and operand layouts are those of sage_attn.hip.
+//
+//   out_r = sum_j p_rj v_j / sum_j p_rj over the keys j of the listed blocks
+//           that the row sees, p = 2^(s - m), m a running row maximum
+//   s     = float(q8 . k8) * (sm_scale * log2 e) * q_scale * k_scale
+// A list belongs to 128 query rows of one head and names blocks of 64 keys; an
+// entry counts if it lies in [0, blocks) and is larger than every entry before
+// it, so a block counts once whatever the list holds.  Rows at or past their
+// sample's length, and rows that see no key, are zeros.
+//
+// MI355X mapping
+//   * A workgroup is 4 waves = 128 query rows, one list, 32 rows a wave, one
+//     wave per SIMD; two workgroups share a CU (72 KiB of rings each at
+//     head_dim 128), and as nothing ties them together one's softmax runs
+//     beside the other's MFMAs.
+//   * K and V^T tiles stream through rings of three stages each.  A tile's K
+//     is used one interval before its V^T, so in interval t (QK of tile t + 1,
+//     PV of tile t) the loads of K(t + 3) and V^T(t + 2) start at once, into
+//     the stages that interval t - 1 read last, and have two intervals to land.
+//   * The list is compacted into LDS 256 entries at a time, with each block's
+//     scale beside it; the loop reads two entries ahead, so no tile waits for
+//     its address.
+//   * Few rows (a short grid) split their lists into ranges, one workgroup
+//     each, merged by a second kernel.
+#include <algorithm>
+
+#include "attn_common.h"
+#include "attn_plan.h"
+#include "sage_tile.h"
+
+namespace tu {
+namespace {
+
+constexpr int kBlockThreads = 256;
+constexpr int kBlockRows = 128;
+constexpr int kRing = 3;
+constexpr int kSegment = 256;  // list entries compacted at a time
+// exponent base of a row that has seen no key yet: finite, so that a tile
+// without a visible key gives 2^-inf = 0 and not a NaN
+constexpr float kNoBase = -1e30f;
+
+struct BlockPlan {
+    uint32_t nqb, bh;  // query blocks of a head, batch * hq
+    uint32_t width;    // entries of a list
+    uint32_t parts;    // ranges of a list
+    uint32_t per;      // entries of a range
+};
+
+template <int D>
+struct Ring {
+    static constexpr int kV0 = kRing * Geo<D>::kKTileBytes;  // V^T stages follow the K stages
+    static constexpr int kBytes = kRing * Geo<D>::kStageBytes;
+};
+
+// Loads of one tile's K rows, or its V^T columns, into a ring stage (the two
+// halves of issue_tile; same lanes, same swizzle).
+#define TU_ISSUE_K_BODY(D)                                                                                          \
+    constexpr int kK = Geo<D>::kKLoads;                                                                             \
+    _Pragma("unroll") for (int i = 0; i < kK; ++i)                                                                  \
+        __builtin_amdgcn_raw_ptr_buffer_load_lds(krs, (lds_void *)(stage + (kK * wave + i) * 1024), 16,             \
+                                                 gm.k_src[i] + key0 * k_sl, 0, 0, 0);
+#define TU_ISSUE_V_BODY(D)                                                                                          \
+    constexpr int kV = Geo<D>::kVLoads;                                                                             \
+    _Pragma("unroll") for (int i = 0; i < kV; ++i)                                                                  \
+        __builtin_amdgcn_raw_ptr_buffer_load_lds(vrs, (lds_void *)(stage + (kV * wave + i) * 1024), 16, gm.v_src[i], \
+                                                 key0 * 2, 0, 0);
+#define TU_ISSUE(D)                                                                                                  \
+    __device__ __forceinline__ void issue_k(int8_t *stage, __amdgpu_buffer_rsrc_t krs, const LaneGeom<D> &gm,         \
+                                            uint32_t k_sl, uint32_t key0, int wave) {                                 \
+        TU_ISSUE_K_BODY(D)                                                                                            \
+    }                                                                                                                 \
+    __device__ __forceinline__ void issue_v(int8_t *stage, __amdgpu_buffer_rsrc_t vrs, const LaneGeom<D> &gm,         \
+                                            uint32_t key0, int wave) {                                                \
+        TU_ISSUE_V_BODY(D)                                                                                            \
+    }
+TU_ISSUE(128)
+TU_ISSUE(64)
+#undef TU_ISSUE
+#undef TU_ISSUE_K_BODY
+#undef TU_ISSUE_V_BODY
+
+__device__ __forceinline__ int sample_end(const int32_t *lengths, uint32_t b, int64_t len) {
+    return lengths ? min(max(lengths[b], 0), static_cast<int>(len)) : static_cast<int>(len);
+}
+
+// A tile of the compacted list.
+struct ListEntry {
+    int32_t block;
+    float scale;
+};
+
+// kSplit: ranges of a list write the unnormalized O with each row's exponent
+// base and row sum to `part` for block_merge_kernel.
+template <int D, bool kCausal, bool kSplit>
+__global__ __launch_bounds__(kBlockThreads, 2) void block_attn_kernel(
+    const int8_t *__restrict__ q8, const float *__restrict__ q_scale, uint32_t blkq, uint32_t nbq,
+    const int8_t *__restrict__ k8, const float *__restrict__ k_scale, int kscale_shift, uint32_t nbk,
+    const uint16_t *__restrict__ vt, const int32_t *__restrict__ index, uint16_t *__restrict__ o, uint32_t hq,
+    uint32_t groups, int64_t lq, int64_t lk, int64_t lpad, const int32_t *__restrict__ q_len,
+    const int32_t *__restrict__ k_len, int64_t q_sb, int64_t q_sh, int64_t q_sl, int64_t k_sb, int64_t k_sh,
+    int64_t k_sl, int64_t o_sb, int64_t o_sh, int64_t o_sl, float sm_log2, BlockPlan plan, float *__restrict__ part) {
+    constexpr int kSl = Geo<D>::kKSlices;
+    constexpr int kLoadsPerTile = Geo<D>::kLoadsPerTile;
+    __shared__ __align__(1024) int8_t lds[Ring<D>::kBytes];
+    __shared__ ListEntry list[kSegment];
+    __shared__ int scan[2][kBlockThreads / 64];
+
+    const int tid = threadIdx.x;
+    const int lane = tid & 63;
+    const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int g = lane >> 4;
+    const int lc = lane & 15;
+    auto kst = [&](int t) { return lds + (t % kRing) * Geo<D>::kKTileBytes; };
+    // pv_tile and mfma_cluster add kKTileBytes to reach a stage's V^T
+    auto vst = [&](int t) { return lds + Ring<D>::kV0 + (t % kRing) * Geo<D>::kVTileBytes - Geo<D>::kKTileBytes; };
+
+    // Head-major numbering, a contiguous eighth per XCD: neighbouring query
+    // blocks of a head, whose lists are alike, share an L2.
+    uint32_t id = xcd_chunk(blockIdx.x, gridDim.x);
+    uint32_t z = 0;
+    if constexpr (kSplit) {
+        z = id % plan.parts;
+        id /= plan.parts;
+    }
+    const uint32_t bh = id / plan.nqb, qb = id % plan.nqb;
+    const uint32_t b = bh / hq, h = bh % hq, hk = h / groups, hkv = hq / groups;
+    const int q_end = sample_end(q_len, b, lq), k_end = sample_end(k_len, b, lk);
+    const int64_t qblock0 = static_cast<int64_t>(qb) * kBlockRows;
+    const int64_t q0 = qblock0 + wave * kWaveQ;
+
+    const int8_t *qp = q8 + b * q_sb + h * q_sh;
+    const int8_t *kp = k8 + b * k_sb + hk * k_sh;
+    const uint16_t *vtp = vt + static_cast<int64_t>(b * hkv + hk) * D * lpad;
+    const float *ks_row = k_scale + static_cast<int64_t>(b * hkv + hk) * nbk;
+    const int32_t *entries = index + (static_cast<int64_t>(bh) * plan.nqb + qb) * plan.width;
+
+    // blocks this query block can see at all
+    int seen_end = k_end;
+    if constexpr (kCausal) seen_end = static_cast<int>(min<int64_t>(k_end, min<int64_t>(qblock0 + kBlockRows, q_end)));
+    const int blocks = qblock0 < q_end ? (seen_end + kBKey - 1) / kBKey : 0;
+
+    const LaneGeom<D> gm = lane_geom<D>(wave, lane, k_sl, lpad);
+    const __amdgpu_buffer_rsrc_t krs = make_rsrc(kp, static_cast<uint32_t>(lk * k_sl));
+    const __amdgpu_buffer_rsrc_t vrs = make_rsrc(vtp, static_cast<uint32_t>(D * lpad * 2));
+    const uint32_t k_sl32 = static_cast<uint32_t>(k_sl);
+
+    i32x4 qf[kQT][kSl];
+    float qsc[kQT];
+#pragma unroll
+    for (int qt = 0; qt < kQT; ++qt) {
+        const int64_t qi = min(q0 + 16 * qt + lc, lq - 1);
+#pragma unroll
+        for (int ds = 0; ds < kSl; ++ds)
+            qf[qt][ds] = *reinterpret_cast<const i32x4 *>(qp + qi * q_sl + 64 * ds + 16 * g);
+        qsc[qt] = q_scale[static_cast<int64_t>(bh) * nbq + static_cast<uint32_t>(qi) / blkq] * sm_log2;
+    }
+    SoftmaxState<D> st;
+#pragma unroll
+    for (int qt = 0; qt < kQT; ++qt) {
+        st.m_used[qt] = kNoBase;
+        st.acc_l[qt] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+        for (int ds = 0; ds < Geo<D>::kDS; ++ds) st.acc_o[ds][qt] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+    }
+    bf16x8 ones;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) ones[e] = static_cast<__bf16>(1.0f);
+
+    i32x4 s[4][kQT];
+    bf16x8 pb[2][kQT];
+
+    // first entry of this workgroup's range, and the end of it
+    int first = 0, end = blocks > 0 ? static_cast<int>(plan.width) : 0;
+    int before = -1;  // largest entry in front of the next segment
+    if constexpr (kSplit) {
+        first = static_cast<int>(z * plan.per);
+        end = min(end, first + static_cast<int>(plan.per));
+        if (end > first) {
+            int m = -1;
+            for (int i = tid; i < first; i += kBlockThreads) m = max(m, entries[i]);
+#pragma unroll
+            for (int d = 1; d < 64; d <<= 1) m = max(m, __shfl_xor(m, d));
+            if (lane == 0) scan[0][wave] = m;
+            __syncthreads();
+#pragma unroll
+            for (int w = 0; w < kBlockThreads / 64; ++w) before = max(before, scan[0][w]);
+            __syncthreads();
+        }
+    }
+
+    for (int seg = first; seg < end; seg += kSegment) {
+        // Compaction of entries seg .. seg + 255: an inclusive running maximum
+        // over the threads, then the rank among the entries that count.
+        const int at = seg + tid;
+        const int e = at < end ? entries[at] : -1;
+        int top = e;
+#pragma unroll
+        for (int d = 1; d < 64; d <<= 1) {
+            const int other = __shfl_up(top, d);
+            if (lane >= d) top = max(top, other);
+        }
+        if (lane == 63) scan[0][wave] = top;
+        int prev = __shfl_up(top, 1);
+        if (lane == 0) prev = -1;
+        __syncthreads();
+        prev = max(prev, before);
+#pragma unroll
+        for (int w = 0; w < kBlockThreads / 64; ++w) {
+            if (w < wave) prev = max(prev, scan[0][w]);
+            before = max(before, scan[0][w]);
+        }
+        const bool counts = e > prev && e < blocks;
+        const uint64_t mask = __ballot(counts);
+        if (lane == 0) scan[1][wave] = __builtin_popcountll(mask);
+        __syncthreads();
+        int rank = __builtin_popcountll(mask & ((1ull << lane) - 1)), n = 0;
+#pragma unroll
+        for (int w = 0; w < kBlockThreads / 64; ++w) {
+            if (w < wave) rank += scan[1][w];
+            n += scan[1][w];
+        }
+        if (counts) list[rank] = ListEntry{e, ks_row[e >> kscale_shift]};
+        __syncthreads();
+        n = __builtin_amdgcn_readfirstlane(n);
+        if (n == 0) continue;
+
+        auto block_at = [&](int t) { return __builtin_amdgcn_readfirstlane(list[min(t, n - 1)].block); };
+        auto softmax = [&](int t) {
+            const ListEntry le = list[t];
+            const int key0 = __builtin_amdgcn_readfirstlane(le.block) * kBKey;
+            float f[kQT];
+            // a scale of zero would make a masked score 0 * -inf
+#pragma unroll
+            for (int qt = 0; qt < kQT; ++qt) f[qt] = fmaxf(qsc[qt] * le.scale, 1e-37f);
+            bool masked = key0 + kBKey > k_end;
+            if constexpr (kCausal) masked = masked || key0 + kBKey > q0 + 1;
+            if (masked) {
+                const int key_lim = min(k_end - key0, kBKey);
+                const int q_rel = static_cast<int>(max(min(q0 - key0, static_cast<int64_t>(kBKey)), static_cast<int64_t>(-kBlockRows)));
+                mask_tile<kCausal>(s, key_lim, q_rel, g, lc);
+            }
+            softmax_tile(s, f, st, pb);
+        };
+
+        // K(0), V(0), K(1), V(1), K(2) are in flight; tile 0 and K(1) land first
+        issue_k(kst(0), krs, gm, k_sl32, block_at(0) * kBKey, wave);
+        issue_v(lds + Ring<D>::kV0, vrs, gm, block_at(0) * kBKey, wave);
+        issue_k(kst(1), krs, gm, k_sl32, block_at(1) * kBKey, wave);
+        issue_v(lds + Ring<D>::kV0 + Geo<D>::kVTileBytes, vrs, gm, block_at(1) * kBKey, wave);
+        issue_k(kst(2), krs, gm, k_sl32, block_at(2) * kBKey, wave);
+        __builtin_amdgcn_s_waitcnt(vmcnt_imm(kLoadsPerTile));
+        wg_barrier();
+        qk_tile(lds, gm, qf, s);
+        softmax(0);
+        wg_barrier();  // K(0)'s stage is free for K(3)
+#pragma clang loop unroll(disable)
+        for (int t = 0; t < n; ++t) {
+            // K(t + 3) and V(t + 2) into stages last read in interval t - 1
+            const uint32_t k3 = block_at(t + 3) * kBKey, v2 = block_at(t + 2) * kBKey;
+            issue_k(kst(t), krs, gm, k_sl32, k3, wave);
+            issue_v(lds + Ring<D>::kV0 + ((t + 2) % kRing) * Geo<D>::kVTileBytes, vrs, gm, v2, wave);
+            // V^T columns at or past the sample's last key may hold anything:
+            // as zeros they add nothing (their p is zero, but zero times a NaN
+            // is not)
+            const int key0 = block_at(t) * kBKey;
+            if (key0 + kBKey > k_end) {
+                int8_t *v = lds + Ring<D>::kV0 + (t % kRing) * Geo<D>::kVTileBytes;
+                const int from = k_end - key0;  // 1 .. 63
+                for (int i = tid; i < D * 8; i += kBlockThreads) {
+                    const int row = i >> 3, chunk = i & 7;  // 8 keys
+                    if (chunk * 8 + 8 <= from) continue;
+                    auto *p = reinterpret_cast<uint16_t *>(v + row * 128 + ((chunk ^ ((row >> 1) & 7)) << 4));
+                    for (int k = max(from - chunk * 8, 0); k < 8; ++k) p[k] = 0;
+                }
+                __syncthreads();
+            }
+            if (t + 1 < n) {
+                mfma_cluster(kst(t + 1), vst(t), gm, qf, s, pb, st, ones);
+                softmax(t + 1);
+            } else {
+                pv_tile(vst(t), gm, pb, st, ones);
+            }
+            // K(t + 2) and V(t + 1) resident
+            __builtin_amdgcn_s_waitcnt(vmcnt_imm(kLoadsPerTile));
+            wg_barrier();
+        }
+        __builtin_amdgcn_s_waitcnt(vmcnt_imm(0));
+        __syncthreads();
+    }
+
+    // acc_o[ds][qt][r] = O[q0 + 16 qt + lc][16 ds + 4 g + r]; acc_l[qt][*] = l.
+    if constexpr (kSplit) {
+        const int64_t rows = static_cast<int64_t>(plan.bh) * lq;
+        const int64_t row0 = z * rows + static_cast<int64_t>(bh) * lq;
+        float *po = part + row0 * D;
+        float *pml = part + plan.parts * rows * D + row0 * 2;
+#pragma unroll
+        for (int qt = 0; qt < kQT; ++qt) {
+            const int64_t qi = q0 + 16 * qt + lc;
+            if (qi >= lq) continue;
+#pragma unroll
+            for (int ds = 0; ds < Geo<D>::kDS; ++ds)
+                *reinterpret_cast<f32x4 *>(po + qi * D + 16 * ds + 4 * g) = st.acc_o[ds][qt];
+            // a row past its sample's end has seen nothing
+            if (g == 0)
+                *reinterpret_cast<f32x2 *>(pml + qi * 2) =
+                    f32x2{qi < q_end ? st.m_used[qt] : kNoBase, qi < q_end ? st.acc_l[qt][0] : 0.0f};
+        }
+        return;
+    }
+    uint16_t *op = o + b * o_sb + h * o_sh;
+    const bool wide = ((reinterpret_cast<uintptr_t>(o) >> 1 | o_sb | o_sh | o_sl) & 7) == 0;
+#pragma unroll
+    for (int qt = 0; qt < kQT; ++qt) {
+        const int64_t qi = q0 + 16 * qt + lc;
+        const float l = st.acc_l[qt][0];
+        const bool some = l > 0.0f && qi < q_end;
+        const float inv = 1.0f / l;
+#pragma unroll
+        for (int ds = 0; ds < Geo<D>::kDS; ds += 2) {
+            uint32_t w[2][2];
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+                const f32x4 a = st.acc_o[ds + i][qt];
+                w[i][0] = some ? hw_bf16x2_bits(a[0] * inv, a[1] * inv) : 0;
+                w[i][1] = some ? hw_bf16x2_bits(a[2] * inv, a[3] * inv) : 0;
+            }
+            // each lane ends with 8 contiguous channels of one row
+            auto lo = __builtin_amdgcn_permlane16_swap(w[0][0], w[1][0], false, false);
+            auto hi = __builtin_amdgcn_permlane16_swap(w[0][1], w[1][1], false, false);
+            if (qi >= lq) continue;
+            uint16_t *dst = op + qi * o_sl + 16 * (ds + (g & 1)) + 8 * (g >> 1);
+            if (wide) {
+                *reinterpret_cast<u32x4 *>(dst) = u32x4{lo[0], hi[0], lo[1], hi[1]};
+            } else {
+                reinterpret_cast<u32x2 *>(dst)[0] = u32x2{lo[0], hi[0]};
+                reinterpret_cast<u32x2 *>(dst)[1] = u32x2{lo[1], hi[1]};
+            }
+        }
+    }
+}
+
+// Merges the ranges of each row: M = max m_s, w_s = 2^(m_s - M),
+// out = sum w_s O_s / sum w_s l_s, zeros where no range saw a key.
+template <int D>
+__global__ __launch_bounds__(256) void block_merge_kernel(const float *__restrict__ part, BlockPlan plan, uint32_t hq,
+                                                          int64_t lq, uint16_t *__restrict__ o, int64_t o_sb,
+                                                          int64_t o_sh, int64_t o_sl) {
+    constexpr int kTpr = D / 8;  // threads per row, 8 channels each
+    const int64_t row = static_cast<int64_t>(blockIdx.x) * (256 / kTpr) + threadIdx.x / kTpr;
+    const int d0 = (threadIdx.x % kTpr) * 8;
+    const int64_t rows = static_cast<int64_t>(plan.bh) * lq;
+    if (row >= rows) return;
+    const int64_t bh = row / lq, q = row - bh * lq;
+    const float *ml = part + plan.parts * rows * D;
+    float m = kNoBase;
+    for (uint32_t sp = 0; sp < plan.parts; ++sp) m = fmaxf(m, ml[(sp * rows + row) * 2]);
+    float l = 0.0f, acc[8] = {};
+    for (uint32_t sp = 0; sp < plan.parts; ++sp) {
+        const float ls = ml[(sp * rows + row) * 2 + 1];
+        if (!(ls > 0.0f)) continue;  // nothing seen in this range
+        const float w = __builtin_amdgcn_exp2f(ml[(sp * rows + row) * 2] - m);
+        l = __builtin_fmaf(w, ls, l);
+        const f32x4 *src = reinterpret_cast<const f32x4 *>(part + (sp * rows + row) * D + d0);
+        const f32x4 a = src[0], c = src[1];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            acc[e] = __builtin_fmaf(w, a[e], acc[e]);
+            acc[4 + e] = __builtin_fmaf(w, c[e], acc[4 + e]);
+        }
+    }
+    const float inv = l > 0.0f ? 1.0f / l : 0.0f;
+    uint16_t *dst = o + (bh / hq) * o_sb + (bh % hq) * o_sh + q * o_sl + d0;
+    u32x2 lo, hi;
+    lo.x = pack_bf16x2(acc[0] * inv, acc[1] * inv);
+    lo.y = pack_bf16x2(acc[2] * inv, acc[3] * inv);
+    hi.x = pack_bf16x2(acc[4] * inv, acc[5] * inv);
+    hi.y = pack_bf16x2(acc[6] * inv, acc[7] * inv);
+    reinterpret_cast<u32x2 *>(dst)[0] = lo;
+    reinterpret_cast<u32x2 *>(dst)[1] = hi;
+}
+
+// Ranges of a list: as many as fill two workgroups a CU, of at least four
+// entries each.
+BlockPlan block_plan(int64_t batch, int64_t hq, int64_t lq, int64_t width, int64_t cus, int64_t max_parts) {
+    BlockPlan p{};
+    p.nqb = static_cast<uint32_t>((lq + kBlockRows - 1) / kBlockRows);
+    p.bh = static_cast<uint32_t>(batch * hq);
+    p.width = static_cast<uint32_t>(width);
+    const int64_t blocks = static_cast<int64_t>(p.nqb) * p.bh;
+    int64_t parts = std::max<int64_t>(1, std::min({2 * cus / blocks, width / 4, max_parts}));
+    p.per = static_cast<uint32_t>((width + parts - 1) / parts);
+    p.parts = static_cast<uint32_t>((width + p.per - 1) / p.per);
+    return p;
+}
+
+int64_t block_workspace(const BlockPlan &p, int64_t lq, int64_t dim) {
+    return p.parts > 1 ? static_cast<int64_t>(p.parts) * p.bh * lq * (dim + 2) * static_cast<int64_t>(sizeof(float)) : 0;
+}
+
+}  // namespace
+}  // namespace tu
+
+extern "C" int64_t tu_sage_block_attn_workspace(int64_t batch, int64_t hq, int64_t lq, int64_t dim, int64_t width,
+                                                int32_t cus) {
+    using namespace tu;
+    if (batch <= 0 || hq <= 0 || lq <= 0 || dim <= 0 || width <= 0 || cus <= 0) return 0;
+    return block_workspace(block_plan(batch, hq, lq, width, cus, 64), lq, dim);
+}
+
+extern "C" int32_t tu_sage_block_attn(const int8_t *q8, const float *q_scale, int64_t blkq, const int8_t *k8,
+                                      const float *k_scale, int64_t blkk, const void *vt_bf16, int64_t lpad,
+                                      const int32_t *index, int64_t width, void *o_bf16, int64_t batch, int64_t hq,
+                                      int64_t hkv, int64_t lq, int64_t lk, int64_t dim, int64_t q_sb, int64_t q_sh,
+                                      int64_t q_sl, int64_t k_sb, int64_t k_sh, int64_t k_sl, int64_t o_sb,
+                                      int64_t o_sh, int64_t o_sl, const int32_t *q_lengths, const int32_t *k_lengths,
+                                      float sm_scale, int32_t causal, int32_t cus, void *workspace,
+                                      int64_t workspace_bytes, void *stream) {
+    using namespace tu;
+    TU_REQUIRE(dim == 64 || dim == 128, "block attention requires head_dim 64 or 128, got %lld",
+               static_cast<long long>(dim));
+    TU_REQUIRE(batch > 0 && hq > 0 && hkv > 0 && hq % hkv == 0, "block attention: hq must be a positive multiple of hkv");
+    TU_REQUIRE(lq > 0 && lk > 0 && width > 0 && cus > 0 && lq <= 0x7fffff00 && lk <= 0x7fffff00 && width <= 0x3fffffff,
+               "block attention sizes out of range");
+    TU_REQUIRE(lpad >= lk && lpad % kBKey == 0, "block attention: V^T padded length must cover lk, multiple of 64");
+    TU_REQUIRE(blkq > 0 && blkk > 0 && blkk % kBKey == 0 && ((blkk / kBKey) & (blkk / kBKey - 1)) == 0 &&
+                   blkq <= 0x7fffffff && blkk <= 0x7fffffff,
+               "block attention needs blkq > 0 and blkk = 64 * 2^n");
+    TU_REQUIRE(lk * k_sl < (int64_t{1} << 32) && dim * lpad * 2 < (int64_t{1} << 32),
+               "block attention: one head's K or V^T exceeds 4 GiB of addressable bytes");
+    TU_REQUIRE(q8 && q_scale && k8 && k_scale && vt_bf16 && index && o_bf16, "block attention pointers must be non-null");
+    TU_REQUIRE(sm_scale > 0.0f, "block attention sm_scale must be positive");
+    TU_REQUIRE(q_sl % 16 == 0 && q_sh % 16 == 0 && q_sb % 16 == 0 && (reinterpret_cast<uintptr_t>(q8) & 15) == 0 &&
+                   k_sl % 16 == 0 && k_sh % 16 == 0 && k_sb % 16 == 0 && (reinterpret_cast<uintptr_t>(k8) & 15) == 0,
+               "block attention Q/K rows must be 16-byte aligned");
+    TU_REQUIRE((reinterpret_cast<uintptr_t>(vt_bf16) & 15) == 0 && o_sl % 4 == 0 && o_sh % 4 == 0 && o_sb % 4 == 0 &&
+                   (reinterpret_cast<uintptr_t>(o_bf16) & 7) == 0,
+               "block attention V^T/O must be aligned");
+    TU_REQUIRE((reinterpret_cast<uintptr_t>(workspace) & 15) == 0, "block attention workspace must be 16-byte aligned");
+    const int64_t per_part = batch * hq * lq * (dim + 2) * static_cast<int64_t>(sizeof(float));
+    const BlockPlan plan = block_plan(batch, hq, lq, width, cus,
+                                      workspace ? std::min<int64_t>(64, workspace_bytes / per_part) : 1);
+    const int64_t grid = static_cast<int64_t>(plan.nqb) * plan.bh * plan.parts;
+    TU_REQUIRE(batch * hq <= 65535 && grid <= 0x7fffffff / kBlockThreads, "block attention grid too large");
+    if (require_gfx950()) return -1;
+    int kscale_shift = 0;
+    while ((kBKey << kscale_shift) < blkk) ++kscale_shift;
+    auto *part = static_cast<float *>(workspace);
+    hipStream_t st = static_cast<hipStream_t>(stream);
+#define TU_BLOCK_ATTN(D, CAUSAL, SPLIT)                                                                                \
+    block_attn_kernel<D, CAUSAL, SPLIT><<<dim3(static_cast<unsigned>(grid)), kBlockThreads, 0, st>>>(                  \
+        q8, q_scale, static_cast<uint32_t>(blkq), static_cast<uint32_t>((lq + blkq - 1) / blkq), k8, k_scale,          \
+        kscale_shift, static_cast<uint32_t>((lk + blkk - 1) / blkk), static_cast<const uint16_t *>(vt_bf16), index,    \
+        static_cast<uint16_t *>(o_bf16), static_cast<uint32_t>(hq), static_cast<uint32_t>(hq / hkv), lq, lk, lpad,     \
+        q_lengths, k_lengths, q_sb, q_sh, q_sl, k_sb, k_sh, k_sl, o_sb, o_sh, o_sl, sm_scale * kLog2e, plan, part)
+#define TU_BLOCK_FORMS(D)                                                                                              \
+    do {                                                                                                               \
+        if (plan.parts > 1) {                                                                                          \
+            if (causal) TU_BLOCK_ATTN(D, true, true);                                                                  \
+            else TU_BLOCK_ATTN(D, false, true);                                                                        \
+            constexpr int kRowsPerWg = 256 / (D / 8);                                                                  \
+            block_merge_kernel<D><<<dim3(static_cast<unsigned>((batch * hq * lq + kRowsPerWg - 1) / kRowsPerWg)), 256, \
+                                    0, st>>>(part, plan, static_cast<uint32_t>(hq), lq,                                \
+                                             static_cast<uint16_t *>(o_bf16), o_sb, o_sh, o_sl);                       \
+        } else if (causal) {                                                                                           \
+            TU_BLOCK_ATTN(D, true, false);                                                                             \
+        } else {                                                                                                       \
+            TU_BLOCK_ATTN(D, false, false);                                                                            \
+        }                                                                                                              \
+    } while (0)
+    if (dim == 128) TU_BLOCK_FORMS(128);
+    else TU_BLOCK_FORMS(64);
+#undef TU_BLOCK_FORMS
+#undef TU_BLOCK_ATTN
+    return check_launch("tu_sage_block_attn");
+}

@@ -39,6 +39,7 @@
 //     pollutes L2).
 #include <type_traits>
 
+#include "adapters.h"
 #include "tu_common.h"
 
 namespace tu {
@@ -263,6 +264,89 @@ __device__ __forceinline__ uint32_t residual_pair(uint32_t y, uint32_t r, uint32
     return pack_bf16x2(lo, hi);
 }
 
+// Adds the adapters' up-projection to a wave's fp32 tile (v[i][j]: weight rows
+// 16 i of col_base, activation rows 16 j of row_base, in the MFMA's layout).
+// The adapters of the wave's rows are walked one after the other; a fragment
+// whose rows all have the adapter accumulates in place, one with other rows
+// beside it adds only to its own (a product with masked zeros would carry an
+// infinite weight of one request's adapter into another's rows).  h, a sum in
+// fp32, goes to the MFMA as the sum of two bf16 values (16 bits of it), so
+// that the adapter's part is no coarser than the projection's.
+template <int kFragsM, int kFragsN>
+__device__ __forceinline__ void add_adapters(i32x4 (&v)[kFragsN][kFragsM], const Adapters &ad, int64_t row_base,
+                                             int64_t col_base, int64_t m, int64_t n, int frow, int g) {
+    int id[kFragsM];
+    uint64_t pending[kFragsM], any = 0;
+#pragma unroll
+    for (int j = 0; j < kFragsM; ++j) {
+        id[j] = adapter_of(ad.ids, ad.id_rows, ad.count, row_base + 16 * j + frow, m);
+        pending[j] = __ballot(id[j] >= 0);
+        any |= pending[j];
+    }
+    const int64_t plane = m * ad.rank;
+    while (any) {
+        int which = 0;
+#pragma unroll
+        for (int j = kFragsM - 1; j >= 0; --j)
+            if (pending[j]) which = __builtin_amdgcn_readlane(id[j], __builtin_ctzll(pending[j]));
+        uint64_t mine[kFragsM];
+        any = 0;
+#pragma unroll
+        for (int j = 0; j < kFragsM; ++j) {
+            mine[j] = __ballot(id[j] == which);
+            pending[j] &= ~mine[j];
+            any |= pending[j];
+        }
+        const uint16_t *up = ad.up + static_cast<int64_t>(which) * n * ad.rank;
+        for (int r0 = 0; r0 < ad.rank; r0 += 32) {
+            const int r = r0 + 8 * g;  // this lane's 8 ranks; the rank is a multiple of 8
+            const bool in = r < ad.rank;
+            bf16x8 w[kFragsN];
+#pragma unroll
+            for (int i = 0; i < kFragsN; ++i) {
+                const u32x4 bits = *reinterpret_cast<const u32x4 *>(up + min(col_base + 16 * i + frow, n - 1) * ad.rank +
+                                                                    (in ? r : 0));
+                w[i] = __builtin_bit_cast(bf16x8, in ? bits : u32x4{0, 0, 0, 0});
+            }
+#pragma unroll
+            for (int j = 0; j < kFragsM; ++j) {
+                if (!mine[j]) continue;
+                const bool own_row = id[j] == which;
+                f32x4 x[2] = {{0.0f, 0.0f, 0.0f, 0.0f}, {0.0f, 0.0f, 0.0f, 0.0f}};
+                if (own_row && in) {
+                    const float *src = ad.h + (row_base + 16 * j + frow) * ad.rank + r;
+                    for (int p = 0; p < ad.parts; ++p, src += plane) {
+                        x[0] += *reinterpret_cast<const f32x4 *>(src);
+                        x[1] += *reinterpret_cast<const f32x4 *>(src + 4);
+                    }
+                }
+                u32x4 hi, lo;
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    const float a = x[e >> 1][2 * (e & 1)], b = x[e >> 1][2 * (e & 1) + 1];
+                    hi[e] = hw_bf16x2_bits(a, b);
+                    lo[e] = hw_bf16x2_bits(a - __uint_as_float(hi[e] << 16), b - __uint_as_float(hi[e] & 0xffff0000u));
+                }
+                const bf16x8 hb = __builtin_bit_cast(bf16x8, hi), lb = __builtin_bit_cast(bf16x8, lo);
+                const bool whole = mine[j] == ~0ull;
+#pragma unroll
+                for (int i = 0; i < kFragsN; ++i) {
+                    const f32x4 c = __builtin_bit_cast(f32x4, v[i][j]);
+                    if (whole) {
+                        f32x4 d = __builtin_amdgcn_mfma_f32_16x16x32_bf16(w[i], hb, c, 0, 0, 0);
+                        d = __builtin_amdgcn_mfma_f32_16x16x32_bf16(w[i], lb, d, 0, 0, 0);
+                        v[i][j] = __builtin_bit_cast(i32x4, d);
+                    } else {
+                        f32x4 d = __builtin_amdgcn_mfma_f32_16x16x32_bf16(w[i], hb, f32x4{0.0f, 0.0f, 0.0f, 0.0f}, 0, 0, 0);
+                        d = __builtin_amdgcn_mfma_f32_16x16x32_bf16(w[i], lb, d, 0, 0, 0);
+                        v[i][j] = __builtin_bit_cast(i32x4, own_row ? c + d : c);
+                    }
+                }
+            }
+        }
+    }
+}
+
 // kResidual: out = bf16_rn(fma(y, gate[row / gate_rows][col], residual[row][col]))
 // with y the bf16 epilogue value (gate 1 when absent).  residual may be out
 // (in place), so neither carries __restrict__: each output chunk is read as
@@ -271,12 +355,14 @@ __device__ __forceinline__ uint32_t residual_pair(uint32_t y, uint32_t r, uint32
 // that are never stored).
 // NST: stages of the LDS ring.  WPE: waves per SIMD, 2 (one workgroup on a
 // CU) or 4 (two).
-template <int BM, int BN, int NST, int WPE, int kOut, bool kResidual>
+// kAdapters: each row's low-rank adapter joins the fp32 epilogue value,
+// y += sum_r up[a][n][r] h[m][r], before the rounding (adapters.hip makes h).
+template <int BM, int BN, int NST, int WPE, int kOut, bool kResidual, bool kAdapters = false>
 __global__ __launch_bounds__(kThreads, WPE) void int8_gemm_kernel(
     const int8_t *__restrict__ a, const int8_t *__restrict__ w, const float *__restrict__ as,
     const float *__restrict__ ws, const float *__restrict__ bias, void *out,
     int64_t m, int64_t n, int64_t k, int tiles_m, int tiles_n, const uint16_t *residual, const uint16_t *gate,
-    int64_t gate_rows) {
+    int64_t gate_rows, Adapters ad) {
     constexpr int kBM = BM;
     constexpr int kFragsM = Tile<BM, BN>::kFragsM;
     constexpr int kFragsN = Tile<BM, BN>::kFragsN;
@@ -533,6 +619,25 @@ __global__ __launch_bounds__(kThreads, WPE) void int8_gemm_kernel(
             }
         const bool hw_round = !kResidual &&
             __builtin_amdgcn_ballot_w64(finite_max >= 0x7f800000u || ws_max >= 0x7f7fffffu) == 0;
+        if constexpr (kAdapters) {
+            // The fp32 epilogue values, in the accumulators' registers.
+#pragma unroll
+            for (int j = 0; j < kFragsM; ++j)
+#pragma unroll
+                for (int i = 0; i < kFragsN; ++i) {
+                    f32x4 v;
+#pragma unroll
+                    for (int r = 0; r < 4; ++r) {
+                        float x = static_cast<float>(acc[i][j][r]);
+                        x = x * arow[j];
+                        x = x * wsv[i][r];
+                        if (bias) x = x + bv[i][r];
+                        v[r] = x;
+                    }
+                    acc[i][j] = __builtin_bit_cast(i32x4, v);
+                }
+            add_adapters<kFragsM, kFragsN>(acc, ad, row_base, col_base, m, n, frow, g);
+        }
         __syncthreads();
         int8_t *tile = lds_mem + wave * kRows * 256;
         auto stage_tile = [&](auto hw) {
@@ -544,6 +649,10 @@ __global__ __launch_bounds__(kThreads, WPE) void int8_gemm_kernel(
                     float v[4];
 #pragma unroll
                     for (int r = 0; r < 4; ++r) {
+                        if constexpr (kAdapters) {
+                            v[r] = __int_as_float(acc[i][j][r]);
+                            continue;
+                        }
                         float x = static_cast<float>(acc[i][j][r]);
                         x = x * arow[j];
                         x = x * wsv[i][r];
@@ -744,10 +853,11 @@ const TileCost &pick_tile(int64_t m, int64_t n, int64_t k, int cus) {
     return *best;
 }
 
-template <int kOut, bool kResidual = false>
+template <int kOut, bool kResidual = false, bool kAdapters = false>
 int32_t launch_gemm(const int8_t *a, const int8_t *w, const float *as, const float *ws, const float *bias,
                     void *out, int64_t m, int64_t n, int64_t k, void *stream, const uint16_t *residual = nullptr,
-                    const uint16_t *gate = nullptr, int64_t gate_rows = 1, int policy = TU_GEMM_TILE_AUTO) {
+                    const uint16_t *gate = nullptr, int64_t gate_rows = 1, int policy = TU_GEMM_TILE_AUTO,
+                    const Adapters &ad = Adapters{}) {
     if (m == 0) return 0;
     if (policy == TU_GEMM_TILE_AUTO) {
         int cus = 0;
@@ -758,8 +868,8 @@ int32_t launch_gemm(const int8_t *a, const int8_t *w, const float *as, const flo
 #define TU_TILE(BM, BN, NST, WPE)                                                                                 \
     do {                                                                                                        \
         const int tiles_m = static_cast<int>((m + BM - 1) / BM), tiles_n = static_cast<int>((n + BN - 1) / BN);     \
-        int8_gemm_kernel<BM, BN, NST, WPE, kOut, kResidual><<<dim3(tiles_m * tiles_n), kThreads, 0, st>>>(           \
-            a, w, as, ws, bias, out, m, n, k, tiles_m, tiles_n, residual, gate, gate_rows);                      \
+        int8_gemm_kernel<BM, BN, NST, WPE, kOut, kResidual, kAdapters><<<dim3(tiles_m * tiles_n), kThreads, 0, st>>>( \
+            a, w, as, ws, bias, out, m, n, k, tiles_m, tiles_n, residual, gate, gate_rows, ad);                  \
     } while (0)
     switch (policy) {
     case TU_GEMM_TILE_128: TU_TILE(128, 256, 3, 2); break;
@@ -771,7 +881,8 @@ int32_t launch_gemm(const int8_t *a, const int8_t *w, const float *as, const flo
     default: TU_TILE(256, 256, 2, 2); break;
     }
 #undef TU_TILE
-    return check_launch(kOut == kOutI32   ? "tu_int8_gemm_i32"
+    return check_launch(kAdapters         ? "tu_int8_gemm_adapters"
+                        : kOut == kOutI32 ? "tu_int8_gemm_i32"
                         : kResidual       ? "tu_int8_gemm_bf16_residual"
                         : kOut == kOutF16 ? "tu_int8_gemm_f16"
                         : kOut == kOutF32 ? "tu_int8_gemm_f32"
@@ -827,6 +938,52 @@ extern "C" int32_t tu_int8_gemm_bf16_residual(const int8_t *a, const int8_t *w, 
     return launch_gemm<kOutBf16, true>(a, w, a_scale, w_scale, bias, out_bf16, m, n, k, stream,
                                     static_cast<const uint16_t *>(residual_bf16),
                                     static_cast<const uint16_t *>(gate_bf16), gate_bf16 ? gate_rows : 1);
+}
+
+extern "C" int64_t tu_int8_gemm_adapters_workspace(int64_t m, int64_t k, int64_t rank, int64_t count, int32_t cus) {
+    using namespace tu;
+    if (m <= 0 || k <= 0 || rank <= 0 || count <= 0 || cus <= 0) return 0;
+    return down_plan(m, k, rank, count, cus).parts * m * rank * static_cast<int64_t>(sizeof(float));
+}
+
+extern "C" int32_t tu_int8_gemm_adapters(const int8_t *a, const int8_t *w, const float *a_scale, const float *w_scale,
+                                         const float *bias, const void *down_bf16, const void *up_bf16,
+                                         const float *scaling, const int32_t *ids, int64_t id_rows, int64_t rank,
+                                         int64_t count, const void *residual_bf16, const void *gate_bf16,
+                                         int64_t gate_rows, void *out_bf16, int64_t m, int64_t n, int64_t k,
+                                         int32_t cus, void *workspace, int64_t workspace_bytes, void *stream) {
+    using namespace tu;
+    TU_REQUIRE(rank > 0 && rank % 8 == 0 && rank <= 4096, "adapter rank must be a positive multiple of 8 up to 4096, got %lld",
+               static_cast<long long>(rank));
+    TU_REQUIRE(count > 0 && count <= 0x7fffffff && id_rows > 0 && cus > 0,
+               "adapter count, rows per id and compute units must be positive");
+    TU_REQUIRE(down_bf16 && up_bf16 && scaling && ids, "adapter pointers must be non-null");
+    TU_REQUIRE((reinterpret_cast<uintptr_t>(down_bf16) & 15) == 0 && (reinterpret_cast<uintptr_t>(up_bf16) & 15) == 0 &&
+                   (reinterpret_cast<uintptr_t>(residual_bf16) & 15) == 0 &&
+                   (reinterpret_cast<uintptr_t>(gate_bf16) & 15) == 0,
+               "adapter weights, residual and gate must be 16-byte aligned");
+    TU_REQUIRE(!gate_bf16 || (residual_bf16 && gate_rows > 0), "a gate needs a residual and positive gate_rows");
+    TU_REQUIRE((m + 31) / 32 <= 0x7fffffff / 512, "adapter grid too large");
+    const bool sized = m > 0 && k > 0;
+    const DownPlan plan = sized ? down_plan(m, k, rank, count, cus) : DownPlan{1, 1, 64};
+    const int64_t need = sized ? plan.parts * m * rank * static_cast<int64_t>(sizeof(float)) : 0;
+    TU_REQUIRE(!sized || (workspace && (reinterpret_cast<uintptr_t>(workspace) & 15) == 0 && workspace_bytes >= need),
+               "adapter workspace must be 16-byte aligned and hold %lld bytes", static_cast<long long>(need));
+    if (check_epilogue_args(a_scale, w_scale, bias) || check_gemm_args(a, w, out_bf16, m, n, k)) return -1;
+    if (m == 0) return 0;
+    auto *h = static_cast<float *>(workspace);
+    const Adapters ad{h, static_cast<const uint16_t *>(up_bf16), ids, id_rows, static_cast<int>(rank),
+                      static_cast<int>(count), plan.parts};
+    if (launch_down(a, a_scale, static_cast<const uint16_t *>(down_bf16), scaling, ad, plan, h, m, k,
+                    static_cast<hipStream_t>(stream)))
+        return -1;
+    const auto *res = static_cast<const uint16_t *>(residual_bf16);
+    const auto *gate = static_cast<const uint16_t *>(gate_bf16);
+    if (res)
+        return launch_gemm<kOutBf16, true, true>(a, w, a_scale, w_scale, bias, out_bf16, m, n, k, stream, res, gate,
+                                                 gate ? gate_rows : 1, TU_GEMM_TILE_AUTO, ad);
+    return launch_gemm<kOutBf16, false, true>(a, w, a_scale, w_scale, bias, out_bf16, m, n, k, stream, nullptr, nullptr,
+                                              1, TU_GEMM_TILE_AUTO, ad);
 }
 
 extern "C" int32_t tu_int8_gemm_i32(const int8_t *a, const int8_t *w, int32_t *acc, int64_t m, int64_t n,

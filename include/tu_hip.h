@@ -164,6 +164,29 @@ int32_t tu_int8_gemm_bf16_residual(const int8_t *a, const int8_t *w, const float
                                    const void *gate_bf16, int64_t gate_rows, void *out_bf16, int64_t m,
                                    int64_t n, int64_t k, void *stream);
 
+/* The GEMM with each row's low-rank adapter beside the projection:
+ *   y[m][n] = ((float(acc) * a_scale[m]) * w_scale[n]) + bias[n]
+ *             + sum_r up[a][n][r] * h[m][r]
+ *   h[m][r] = scaling[a] * a_scale[m] * sum_k code[m][k] * down[a][r][k]
+ * with a = ids[m / id_rows]; a row whose id is outside [0, count) has no
+ * adapter and gets tu_int8_gemm_bf16's bits.  out = bf16_rn(y), or with a
+ * residual bf16_rn(fma(bf16_rn(y), gate, residual)) as
+ * tu_int8_gemm_bf16_residual.  Codes are those of a rotated activation, so
+ * down holds the adapter's rows rotated alike.  h is in fp32 and reaches the
+ * matrix pipe as two bf16 terms.  down: bf16 [count, rank, k]; up: bf16
+ * [count, n, rank]; scaling: fp32 [count]; ids: int32 [ceil(m / id_rows)];
+ * rank a multiple of 8 up to 4096; down, up, residual and gate 16-byte
+ * aligned; the rest as above.  workspace: 16-byte aligned, at least
+ * tu_int8_gemm_adapters_workspace(...) bytes for the same sizes and compute
+ * units (`cus`).  Two launches.  No counterpart in the reference. */
+int64_t tu_int8_gemm_adapters_workspace(int64_t m, int64_t k, int64_t rank, int64_t count, int32_t cus);
+int32_t tu_int8_gemm_adapters(const int8_t *a, const int8_t *w, const float *a_scale, const float *w_scale,
+                              const float *bias, const void *down_bf16, const void *up_bf16,
+                              const float *scaling, const int32_t *ids, int64_t id_rows, int64_t rank,
+                              int64_t count, const void *residual_bf16, const void *gate_bf16,
+                              int64_t gate_rows, void *out_bf16, int64_t m, int64_t n, int64_t k,
+                              int32_t cus, void *workspace, int64_t workspace_bytes, void *stream);
+
 /* acc[m][n] = sum_k a[m][k] * w[n][k] as int32, row-major [m, n].  Same
  * kernel as tu_int8_gemm_bf16 with the epilogue replaced by an int32 store;
  * the accumulator half of the reference's cuBLAS INT8 + epilogue split
@@ -316,6 +339,56 @@ int32_t tu_sage_attn_fwd_auto(const int8_t *q8, const float *q_scale, int64_t bl
                               int64_t k_sh, int64_t k_sl, int64_t o_sb, int64_t o_sh, int64_t o_sl,
                               float sm_scale, int32_t causal, int32_t cus, void *workspace,
                               int64_t workspace_bytes, void *stream);
+
+/* Sage attention over selected key blocks ---------------------------------- */
+
+/* For each block of 128 queries the key blocks of 64 it is to attend to:
+ *   mq_i, mk_j = mean rows of scale * code over the block's rows in front of
+ *                the sample's end (q_lengths / k_lengths int32 [batch], or
+ *                NULL: all of them), in fp64
+ *   S_ij = mq_i . mk_j in fp64
+ * Block j is visible to block i if i has rows below the sample's length,
+ * 64 j < the sample's key length and, causal, 64 j <= i's last row.  Of the
+ * visible ones the first `keep` are taken by: forced blocks (j < sink_blocks;
+ * with local_blocks = w > 0, 2 i - (w - 1) <= j <= 2 i + w), then the larger
+ * S, NaN last, then the lower j.  index: int32 [batch, hq, ceil(lq / 128),
+ * min(keep, ceil(lk / 64))], ascending, -1 behind the last.  Codes, scales and
+ * strides as tu_sage_attn_fwd's.  workspace: 16-byte aligned, at least
+ * tu_sage_block_select_workspace(...) bytes.  No counterpart in the reference
+ * (its Sol router, comfyui_turing_utils/attention/sparse.py, selects by
+ * another rule). */
+int64_t tu_sage_block_select_workspace(int64_t batch, int64_t hq, int64_t hkv, int64_t lq, int64_t lk,
+                                       int64_t dim);
+int32_t tu_sage_block_select(const int8_t *q8, const float *q_scale, int64_t blkq, const int8_t *k8,
+                             const float *k_scale, int64_t blkk, int64_t batch, int64_t hq, int64_t hkv,
+                             int64_t lq, int64_t lk, int64_t dim, int64_t q_sb, int64_t q_sh, int64_t q_sl,
+                             int64_t k_sb, int64_t k_sh, int64_t k_sl, const int32_t *q_lengths,
+                             const int32_t *k_lengths, int64_t keep, int64_t sink_blocks,
+                             int64_t local_blocks, int32_t causal, void *workspace,
+                             int64_t workspace_bytes, int32_t *index, void *stream);
+
+/* tu_sage_attn_fwd over listed key blocks: query rows 128 i .. 128 i + 127 of
+ * a head attend to the keys of the blocks of 64 that index [batch, hq,
+ * ceil(lq / 128), width] names for them.  An entry counts if it lies in
+ * [0, ceil(lk / 64)) and is larger than every entry before it.  Keys at or
+ * past k_lengths[b] are not seen (codes and values there may be anything);
+ * rows at or past q_lengths[b], and rows that see no key, are zeros.  Causal:
+ * top-left aligned.  Grids of few workgroups on a device of `cus` compute
+ * units split their lists into ranges that a second kernel merges, as many as
+ * `workspace` (16-byte aligned, workspace_bytes long) holds;
+ * tu_sage_block_attn_workspace gives the bytes for all of them (0: no split),
+ * and without one (NULL, 0) nothing is split.  The rest as tu_sage_attn_fwd.
+ * No counterpart in the reference's kernels that this build restates. */
+int64_t tu_sage_block_attn_workspace(int64_t batch, int64_t hq, int64_t lq, int64_t dim, int64_t width,
+                                     int32_t cus);
+int32_t tu_sage_block_attn(const int8_t *q8, const float *q_scale, int64_t blkq, const int8_t *k8,
+                           const float *k_scale, int64_t blkk, const void *vt_bf16, int64_t lpad,
+                           const int32_t *index, int64_t width, void *o_bf16, int64_t batch, int64_t hq,
+                           int64_t hkv, int64_t lq, int64_t lk, int64_t dim, int64_t q_sb, int64_t q_sh,
+                           int64_t q_sl, int64_t k_sb, int64_t k_sh, int64_t k_sl, int64_t o_sb, int64_t o_sh,
+                           int64_t o_sl, const int32_t *q_lengths, const int32_t *k_lengths, float sm_scale,
+                           int32_t causal, int32_t cus, void *workspace, int64_t workspace_bytes,
+                           void *stream);
 
 /* Sage attention: fused Q/K preprocessing -------------------------------- */
 
