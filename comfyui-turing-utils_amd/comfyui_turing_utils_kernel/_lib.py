@@ -163,7 +163,7 @@ SIGNATURES: dict[str, tuple[object, list[object]]] = {
         _i32,
         [_c_void_p, _c_void_p, _c_void_p, _c_void_p, _c_void_p, _i64, _i64, _f32, _c_void_p],
     ),
-    "tu_int8_gemm_adapters_workspace": (_i64, [_i64, _i64, _i64, _i64, _i32]),
+    "tu_int8_gemm_adapters_workspace": (_i64, [_i64, _i64]),
     "tu_int8_gemm_adapters": (
         _i32,
         [_c_void_p, _c_void_p, _c_void_p, _c_void_p, _c_void_p, _c_void_p, _c_void_p, _c_void_p, _c_void_p, _i64,

@@ -82,8 +82,8 @@ def _linear_adapters(activation, weight, activation_scale, weight_scale, bias, d
     out = torch.empty((m, n), dtype=torch.bfloat16, device=device)
     if m == 0:
         return out
-    lib, cus, (count, rank, _) = _lib.load(), _compute_units(device), down.shape
-    nbytes = int(lib.tu_int8_gemm_adapters_workspace(m, k, rank, count, cus))
+    cus, (count, rank, _) = _compute_units(device), down.shape
+    nbytes = int(_lib.load().tu_int8_gemm_adapters_workspace(m, rank))
     with torch.cuda.device(device):
         workspace = torch.empty(nbytes, dtype=torch.uint8, device=device)
         _lib.call(

@@ -7,15 +7,15 @@
 
 namespace tu {
 
-// h holds `parts` planes [m][rank] of fp32 partial sums (ranges of K), scaled
-// by the row's activation scale and its adapter's scaling; rows without an
-// adapter are not written.
+// A row of h holds its ranks as two bf16 terms, [hi | lo] (hi + lo is the fp32
+// sum to 2^-16 of it), scaled by the row's activation scale and its adapter's
+// scaling; rows without an adapter are not written.
 struct Adapters {
-    const float *h;
+    const uint16_t *h;     // [m][2 rank]
     const uint16_t *up;    // bf16 [count][n][rank]
     const int32_t *ids;    // adapter of rows i * id_rows .. (i + 1) * id_rows - 1
     int64_t id_rows;
-    int rank, count, parts;
+    int rank, count;
 };
 
 // The adapter of a row, -1 for none (also where the id names no adapter).
@@ -26,15 +26,7 @@ __device__ __forceinline__ int adapter_of(const int32_t *ids, int64_t id_rows, i
     return static_cast<uint32_t>(a) < static_cast<uint32_t>(count) ? a : -1;
 }
 
-// Ranges of K, and workgroups that share a row tile's adapters, of the
-// down-projection.
-struct DownPlan {
-    int parts, slots;
-    int64_t per;  // bytes of K per range, a multiple of 64
-};
-DownPlan down_plan(int64_t m, int64_t k, int64_t rank, int64_t count, int cus);
-
 int32_t launch_down(const int8_t *a, const float *a_scale, const uint16_t *down, const float *scaling,
-                    const Adapters &ad, const DownPlan &plan, float *h, int64_t m, int64_t k, hipStream_t st);
+                    const Adapters &ad, uint16_t *h, int64_t m, int64_t k, int cus, hipStream_t st);
 
 }  // namespace tu

@@ -51,7 +51,9 @@ struct BlockPlan {
 template <int D>
 struct Ring {
     static constexpr int kV0 = kRing * Geo<D>::kKTileBytes;  // V^T stages follow the K stages
-    static constexpr int kBytes = kRing * Geo<D>::kStageBytes;
+    static constexpr int kList = kRing * Geo<D>::kStageBytes;  // the compacted entries follow the rings
+    static constexpr int kScan = kList + kSegment * 8;         // and the waves' counts
+    static constexpr int kBytes = kScan + 2 * (kBlockThreads / 64) * 4;
 };
 
 // Loads of one tile's K rows, or its V^T columns, into a ring stage (the two
@@ -103,9 +105,11 @@ __global__ __launch_bounds__(kBlockThreads, 2) void block_attn_kernel(
     int64_t k_sl, int64_t o_sb, int64_t o_sh, int64_t o_sl, float sm_log2, BlockPlan plan, float *__restrict__ part) {
     constexpr int kSl = Geo<D>::kKSlices;
     constexpr int kLoadsPerTile = Geo<D>::kLoadsPerTile;
+    // One array: with several the compiler waits for all direct-to-LDS loads
+    // before a tile's fragment reads.
     __shared__ __align__(1024) int8_t lds[Ring<D>::kBytes];
-    __shared__ ListEntry list[kSegment];
-    __shared__ int scan[2][kBlockThreads / 64];
+    auto *list = reinterpret_cast<ListEntry *>(lds + Ring<D>::kList);
+    auto *scan = reinterpret_cast<int(*)[kBlockThreads / 64]>(lds + Ring<D>::kScan);
 
     const int tid = threadIdx.x;
     const int lane = tid & 63;

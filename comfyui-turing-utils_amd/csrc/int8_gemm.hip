@@ -264,88 +264,167 @@ __device__ __forceinline__ uint32_t residual_pair(uint32_t y, uint32_t r, uint32
     return pack_bf16x2(lo, hi);
 }
 
-// Adds the adapters' up-projection to a wave's fp32 tile (v[i][j]: weight rows
-// 16 i of col_base, activation rows 16 j of row_base, in the MFMA's layout).
-// The adapters of the wave's rows are walked one after the other; a fragment
-// whose rows all have the adapter accumulates in place, one with other rows
-// beside it adds only to its own (a product with masked zeros would carry an
-// infinite weight of one request's adapter into another's rows).  h, a sum in
-// fp32, goes to the MFMA as the sum of two bf16 values (16 bits of it), so
-// that the adapter's part is no coarser than the projection's.
-template <int kFragsM, int kFragsN>
-__device__ __forceinline__ void add_adapters(i32x4 (&v)[kFragsN][kFragsM], const Adapters &ad, int64_t row_base,
-                                             int64_t col_base, int64_t m, int64_t n, int frow, int g) {
+// The adapters of a wave's rows (16 kFragsM of them, row j of a lane being
+// 16 j + lane % 16), and the products that the epilogue adds for them.
+//
+// Each row's h, its own adapter's, is held in registers as its two bf16 terms,
+// up to 64 ranks at a time (chunks of 32, one MFMA a term).  Where one adapter
+// has all rows the products accumulate in place; else the adapters are walked
+// one after the other, each product added to that adapter's own rows (one with
+// masked zeros would carry an infinite weight of one request's adapter into
+// another's).
+template <int kFragsM>
+struct RowAdapters {
     int id[kFragsM];
-    uint64_t pending[kFragsM], any = 0;
-#pragma unroll
-    for (int j = 0; j < kFragsM; ++j) {
-        id[j] = adapter_of(ad.ids, ad.id_rows, ad.count, row_base + 16 * j + frow, m);
-        pending[j] = __ballot(id[j] >= 0);
-        any |= pending[j];
-    }
-    const int64_t plane = m * ad.rank;
-    while (any) {
-        int which = 0;
+    uint64_t left[kFragsM];  // rows with an adapter
+    bool whole;              // all rows have the same one
+    int first, second;       // the first two, -1 where there are fewer
+    bool more;               // there are others
+    int64_t row_base, col_base, m, n;
+    int frow, g;
+
+    // The next adapter among the rows of `rest`, which lose its rows; -1 for none.
+    __device__ __forceinline__ int take(uint64_t (&rest)[kFragsM]) const {
+        int which = -1;
 #pragma unroll
         for (int j = kFragsM - 1; j >= 0; --j)
-            if (pending[j]) which = __builtin_amdgcn_readlane(id[j], __builtin_ctzll(pending[j]));
-        uint64_t mine[kFragsM];
-        any = 0;
+            if (rest[j]) which = __builtin_amdgcn_readlane(id[j], __builtin_ctzll(rest[j]));
+        if (which >= 0) {
 #pragma unroll
-        for (int j = 0; j < kFragsM; ++j) {
-            mine[j] = __ballot(id[j] == which);
-            pending[j] &= ~mine[j];
-            any |= pending[j];
+            for (int j = 0; j < kFragsM; ++j) rest[j] &= ~__ballot(id[j] == which);
         }
-        const uint16_t *up = ad.up + static_cast<int64_t>(which) * n * ad.rank;
-        for (int r0 = 0; r0 < ad.rank; r0 += 32) {
-            const int r = r0 + 8 * g;  // this lane's 8 ranks; the rank is a multiple of 8
-            const bool in = r < ad.rank;
-            bf16x8 w[kFragsN];
+        return which;
+    }
+
+    __device__ __forceinline__ void ids(const Adapters &ad, int64_t row_base_, int64_t m_, int frow_) {
+        row_base = row_base_, m = m_, frow = frow_;
 #pragma unroll
-            for (int i = 0; i < kFragsN; ++i) {
-                const u32x4 bits = *reinterpret_cast<const u32x4 *>(up + min(col_base + 16 * i + frow, n - 1) * ad.rank +
-                                                                    (in ? r : 0));
-                w[i] = __builtin_bit_cast(bf16x8, in ? bits : u32x4{0, 0, 0, 0});
-            }
+        for (int j = 0; j < kFragsM; ++j) id[j] = adapter_of(ad.ids, ad.id_rows, ad.count, row_base + 16 * j + frow, m);
+    }
+
+    __device__ __forceinline__ void find(int64_t col_base_, int64_t n_, int g_) {
+        col_base = col_base_, n = n_, g = g_;
+        uint64_t rest[kFragsM];
+#pragma unroll
+        for (int j = 0; j < kFragsM; ++j) rest[j] = left[j] = __ballot(id[j] >= 0);
+        first = take(rest);
+        second = take(rest);
+        uint64_t others = 0;
+#pragma unroll
+        for (int j = 0; j < kFragsM; ++j) others |= rest[j];
+        more = others != 0;
+        bool all = true;
+        // rows past the last one are never stored
+#pragma unroll
+        for (int j = 0; j < kFragsM; ++j) all = all && (id[j] == first || row_base + 16 * j + frow >= m);
+        whole = __all(all);
+    }
+
+    // The terms of h of kC chunks from rank r0 on, zeros where there is none.
+    template <int kC>
+    struct Held {
+        bf16x8 h[kC][2][kFragsM];
+    };
+    template <int kC>
+    __device__ __forceinline__ void load(Held<kC> &x, const Adapters &ad, int r0) const {
+#pragma unroll
+        for (int c = 0; c < kC; ++c)
 #pragma unroll
             for (int j = 0; j < kFragsM; ++j) {
-                if (!mine[j]) continue;
-                const bool own_row = id[j] == which;
-                f32x4 x[2] = {{0.0f, 0.0f, 0.0f, 0.0f}, {0.0f, 0.0f, 0.0f, 0.0f}};
-                if (own_row && in) {
-                    const float *src = ad.h + (row_base + 16 * j + frow) * ad.rank + r;
-                    for (int p = 0; p < ad.parts; ++p, src += plane) {
-                        x[0] += *reinterpret_cast<const f32x4 *>(src);
-                        x[1] += *reinterpret_cast<const f32x4 *>(src + 4);
-                    }
-                }
-                u32x4 hi, lo;
+                const int r = r0 + 32 * c + 8 * g;
+                const bool in = id[j] >= 0 && r < ad.rank;
+                const uint16_t *src = ad.h + (in ? (row_base + 16 * j + frow) * 2 * ad.rank + r : 0);
 #pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                    const float a = x[e >> 1][2 * (e & 1)], b = x[e >> 1][2 * (e & 1) + 1];
-                    hi[e] = hw_bf16x2_bits(a, b);
-                    lo[e] = hw_bf16x2_bits(a - __uint_as_float(hi[e] << 16), b - __uint_as_float(hi[e] & 0xffff0000u));
+                for (int t = 0; t < 2; ++t) {
+                    u32x4 v = *reinterpret_cast<const u32x4 *>(src + t * ad.rank);
+                    x.h[c][t][j] = __builtin_bit_cast(bf16x8, in ? v : u32x4{0, 0, 0, 0});
                 }
-                const bf16x8 hb = __builtin_bit_cast(bf16x8, hi), lb = __builtin_bit_cast(bf16x8, lo);
-                const bool whole = mine[j] == ~0ull;
+            }
+    }
+
+    // up of the same ranks for column fragment i.
+    template <int kC>
+    struct Up {
+        bf16x8 w[kC];
+    };
+    template <int kC>
+    __device__ __forceinline__ void load(Up<kC> &x, const Adapters &ad, int which, int r0, int i) const {
 #pragma unroll
-                for (int i = 0; i < kFragsN; ++i) {
-                    const f32x4 c = __builtin_bit_cast(f32x4, v[i][j]);
-                    if (whole) {
-                        f32x4 d = __builtin_amdgcn_mfma_f32_16x16x32_bf16(w[i], hb, c, 0, 0, 0);
-                        d = __builtin_amdgcn_mfma_f32_16x16x32_bf16(w[i], lb, d, 0, 0, 0);
-                        v[i][j] = __builtin_bit_cast(i32x4, d);
-                    } else {
-                        f32x4 d = __builtin_amdgcn_mfma_f32_16x16x32_bf16(w[i], hb, f32x4{0.0f, 0.0f, 0.0f, 0.0f}, 0, 0, 0);
-                        d = __builtin_amdgcn_mfma_f32_16x16x32_bf16(w[i], lb, d, 0, 0, 0);
-                        v[i][j] = __builtin_bit_cast(i32x4, own_row ? c + d : c);
-                    }
+        for (int c = 0; c < kC; ++c) {
+            const int r = r0 + 32 * c + 8 * g;
+            const bool in = which >= 0 && r < ad.rank;
+            const u32x4 v = *reinterpret_cast<const u32x4 *>(
+                ad.up + (static_cast<int64_t>(max(which, 0)) * n + min(col_base + 16 * i + frow, n - 1)) * ad.rank + (in ? r : 0));
+            x.w[c] = __builtin_bit_cast(bf16x8, in ? v : u32x4{0, 0, 0, 0});
+        }
+    }
+
+    // Adds a product to every row ...
+    template <int kC>
+    __device__ __forceinline__ void add(f32x4 (&v)[kFragsM], const Up<kC> &w, const Held<kC> &x) const {
+#pragma unroll
+        for (int c = 0; c < kC; ++c)
+#pragma unroll
+            for (int t = 0; t < 2; ++t)
+#pragma unroll
+                for (int j = 0; j < kFragsM; ++j)
+                    v[j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(w.w[c], x.h[c][t][j], v[j], 0, 0, 0);
+    }
+    // ... or to the adapter's own.
+    template <int kC>
+    __device__ __forceinline__ void add_own(f32x4 (&v)[kFragsM], const Up<kC> &w, const Held<kC> &x, int which) const {
+        f32x4 d[kFragsM];
+#pragma unroll
+        for (int j = 0; j < kFragsM; ++j) d[j] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+        add(d, w, x);
+#pragma unroll
+        for (int j = 0; j < kFragsM; ++j)
+#pragma unroll
+            for (int r = 0; r < 4; ++r) v[j][r] = which >= 0 && id[j] == which ? v[j][r] + d[j][r] : v[j][r];
+    }
+
+    // The products of kI column fragments from i on, whatever adapters the rows
+    // have: kBatch adapters' loads are in flight while the batch before is used.
+    template <int kI>
+    __device__ __forceinline__ void add_any(f32x4 (&v)[kI][kFragsM], const Adapters &ad, int i) const {
+        constexpr int kBatch = kFragsM >= 4 ? 1 : 4;
+#pragma clang loop unroll(disable)
+        for (int r0 = 0; r0 < ad.rank; r0 += 32) {
+            Held<1> x;
+            load(x, ad, r0);
+            uint64_t rest[kFragsM];
+#pragma unroll
+            for (int j = 0; j < kFragsM; ++j) rest[j] = left[j];
+            int which[kBatch];
+            Up<1> w[kBatch][kI];
+            auto fetch = [&] {
+#pragma unroll
+                for (int u = 0; u < kBatch; ++u) {
+                    which[u] = take(rest);
+#pragma unroll
+                    for (int c = 0; c < kI; ++c) load(w[u][c], ad, which[u], r0, i + c);
                 }
+            };
+            fetch();
+#pragma clang loop unroll(disable)
+            while (which[0] >= 0) {
+                int now[kBatch];
+                Up<1> wn[kBatch][kI];
+#pragma unroll
+                for (int u = 0; u < kBatch; ++u) {
+                    now[u] = which[u];
+#pragma unroll
+                    for (int c = 0; c < kI; ++c) wn[u][c] = w[u][c];
+                }
+                fetch();
+#pragma unroll
+                for (int u = 0; u < kBatch; ++u)
+#pragma unroll
+                    for (int c = 0; c < kI; ++c) add_own(v[c], wn[u][c], x, now[u]);
             }
         }
     }
-}
+};
 
 // kResidual: out = bf16_rn(fma(y, gate[row / gate_rows][col], residual[row][col]))
 // with y the bf16 epilogue value (gate 1 when absent).  residual may be out
@@ -367,7 +446,12 @@ __global__ __launch_bounds__(kThreads, WPE) void int8_gemm_kernel(
     constexpr int kFragsM = Tile<BM, BN>::kFragsM;
     constexpr int kFragsN = Tile<BM, BN>::kFragsN;
     constexpr int kStageBytes = Tile<BM, BN>::kStageBytes;
-    __shared__ __align__(1024) int8_t lds_mem[Tile<BM, BN>::lds_bytes(NST)];
+    // kAdapters: behind the ring, each wave's column scales and bias, as the
+    // adapters' operands need the registers that hold them otherwise (256 x 256
+    // spilled 122 of them).  One array: with two the compiler waits for all
+    // direct-to-LDS loads before a step's fragment reads.
+    constexpr int kColsBytes = kAdapters ? kWaves * BN * 4 : 0;
+    __shared__ __align__(1024) int8_t lds_mem[Tile<BM, BN>::lds_bytes(NST) + kColsBytes];
     auto lds = [&](int st) { return lds_mem + st * kStageBytes; };
 
     const int tid = threadIdx.x;
@@ -588,15 +672,20 @@ __global__ __launch_bounds__(kThreads, WPE) void int8_gemm_kernel(
         // retire in order, so loads interleaved with their uses would each
         // wait a full round trip.
         const float *bp = bias ? bias : ws;
+        [[maybe_unused]] constexpr int kMma = Tile<BM, BN>::kMma;
+        [[maybe_unused]] RowAdapters<kFragsM> rows;
+        if constexpr (kAdapters) rows.ids(ad, row_base, m, frow);
         float arow[kFragsM];
-        f32x4 wsv[kFragsN], bv[kFragsN];
+        f32x4 wsv[kAdapters ? 1 : kFragsN], bv[kAdapters ? 1 : kFragsN];
 #pragma unroll
         for (int j = 0; j < kFragsM; ++j) arow[j] = as[min(row_base + j * 16 + frow, m - 1)];
+        if constexpr (!kAdapters) {
 #pragma unroll
-        for (int i = 0; i < kFragsN; ++i) {
-            const int64_t col = min(col_base + i * 16 + 4 * g, n - 4);
-            wsv[i] = *reinterpret_cast<const f32x4 *>(ws + col);
-            bv[i] = *reinterpret_cast<const f32x4 *>(bp + col);
+            for (int i = 0; i < kFragsN; ++i) {
+                const int64_t col = min(col_base + i * 16 + 4 * g, n - 4);
+                wsv[i] = *reinterpret_cast<const f32x4 *>(ws + col);
+                bv[i] = *reinterpret_cast<const f32x4 *>(bp + col);
+            }
         }
         // With finite row scales and bias and finite nonzero column scales no
         // value of the wave's tile can be NaN: float(acc) is finite, a product
@@ -609,38 +698,36 @@ __global__ __launch_bounds__(kThreads, WPE) void int8_gemm_kernel(
         uint32_t finite_max = 0, ws_max = 0;
 #pragma unroll
         for (int j = 0; j < kFragsM; ++j) finite_max = max(finite_max, __float_as_uint(arow[j]) & 0x7fffffffu);
-#pragma unroll
-        for (int i = 0; i < kFragsN; ++i)
-#pragma unroll
-            for (int r = 0; r < 4; ++r) {
-                finite_max = max(finite_max, __float_as_uint(bv[i][r]) & 0x7fffffffu);
-                // |ws| bits - 1 (unsigned): 0 wraps to 0xffffffff
-                ws_max = max(ws_max, (__float_as_uint(wsv[i][r]) & 0x7fffffffu) - 1u);
-            }
-        const bool hw_round = !kResidual &&
-            __builtin_amdgcn_ballot_w64(finite_max >= 0x7f800000u || ws_max >= 0x7f7fffffu) == 0;
+        // scales, then bias, of this wave's BN / 2 columns
+        [[maybe_unused]] float *cols =
+            reinterpret_cast<float *>(lds_mem + Tile<BM, BN>::lds_bytes(NST)) + (kAdapters ? wave * BN : 0);
         if constexpr (kAdapters) {
-            // The fp32 epilogue values, in the accumulators' registers.
+            rows.find(col_base, n, g);
 #pragma unroll
-            for (int j = 0; j < kFragsM; ++j)
+            for (int c = 0; c < BN / 2; c += 64) {
+                if (c + lane >= BN / 2) break;
+                const int64_t col = min(col_base + c + lane, n - 1);
+                const float w = ws[col], b = bp[col];
+                cols[c + lane] = w;
+                cols[BN / 2 + c + lane] = b;
+                finite_max = max(finite_max, __float_as_uint(b) & 0x7fffffffu);
+                ws_max = max(ws_max, (__float_as_uint(w) & 0x7fffffffu) - 1u);
+            }
+        } else {
 #pragma unroll
-                for (int i = 0; i < kFragsN; ++i) {
-                    f32x4 v;
+            for (int i = 0; i < kFragsN; ++i)
 #pragma unroll
-                    for (int r = 0; r < 4; ++r) {
-                        float x = static_cast<float>(acc[i][j][r]);
-                        x = x * arow[j];
-                        x = x * wsv[i][r];
-                        if (bias) x = x + bv[i][r];
-                        v[r] = x;
-                    }
-                    acc[i][j] = __builtin_bit_cast(i32x4, v);
+                for (int r = 0; r < 4; ++r) {
+                    finite_max = max(finite_max, __float_as_uint(bv[i][r]) & 0x7fffffffu);
+                    // |ws| bits - 1 (unsigned): 0 wraps to 0xffffffff
+                    ws_max = max(ws_max, (__float_as_uint(wsv[i][r]) & 0x7fffffffu) - 1u);
                 }
-            add_adapters<kFragsM, kFragsN>(acc, ad, row_base, col_base, m, n, frow, g);
         }
+        const bool finite = __builtin_amdgcn_ballot_w64(finite_max >= 0x7f800000u || ws_max >= 0x7f7fffffu) == 0;
+        const bool hw_round = !kResidual && finite;
         __syncthreads();
         int8_t *tile = lds_mem + wave * kRows * 256;
-        auto stage_tile = [&](auto hw) {
+        [[maybe_unused]] auto stage_tile = [&](auto hw) {
 #pragma unroll
             for (int j = 0; j < kFragsM; ++j) {
                 const int lrow = j * 16 + frow;
@@ -649,10 +736,6 @@ __global__ __launch_bounds__(kThreads, WPE) void int8_gemm_kernel(
                     float v[4];
 #pragma unroll
                     for (int r = 0; r < 4; ++r) {
-                        if constexpr (kAdapters) {
-                            v[r] = __int_as_float(acc[i][j][r]);
-                            continue;
-                        }
                         float x = static_cast<float>(acc[i][j][r]);
                         x = x * arow[j];
                         x = x * wsv[i][r];
@@ -682,8 +765,101 @@ __global__ __launch_bounds__(kThreads, WPE) void int8_gemm_kernel(
                 }
             }
         };
-        if (hw_round) stage_tile(std::true_type{});
-        else stage_tile(std::false_type{});
+        if constexpr (kAdapters) {
+            // Column fragment i: the fp32 epilogue values, and (with the
+            // adapters' part) their rounding, as in stage_tile.
+            auto values = [&](int i, f32x4 (&v)[kFragsM]) {
+                const f32x4 wv = *reinterpret_cast<const f32x4 *>(&cols[16 * i + 4 * g]);
+                const f32x4 bv4 = *reinterpret_cast<const f32x4 *>(&cols[BN / 2 + 16 * i + 4 * g]);
+#pragma unroll
+                for (int j = 0; j < kFragsM; ++j)
+#pragma unroll
+                    for (int r = 0; r < 4; ++r) {
+                        float x = static_cast<float>(acc[i][j][r]);
+                        x = x * arow[j];
+                        x = x * wv[r];
+                        if (bias) x = x + bv4[r];
+                        v[j][r] = x;
+                    }
+            };
+            auto store = [&](int i, const f32x4 (&v)[kFragsM]) {
+#pragma unroll
+                for (int j = 0; j < kFragsM; ++j) {
+                    const int lrow = j * 16 + frow;
+                    u32x2 packed;
+                    if (finite) {
+                        packed.x = hw_bf16x2_bits(v[j][0], v[j][1]);
+                        packed.y = hw_bf16x2_bits(v[j][2], v[j][3]);
+                    } else {
+                        packed.x = pack_bf16x2(v[j][0], v[j][1]);
+                        packed.y = pack_bf16x2(v[j][2], v[j][3]);
+                    }
+                    const int chunk = (2 * i + (g >> 1)) ^ (lrow & 15);
+                    *reinterpret_cast<u32x2 *>(tile + lrow * 256 + chunk * 16 + (g & 1) * 8) = packed;
+                }
+            };
+            // kWhole: all rows have the first adapter; else the first two are
+            // those of a border between requests.  A fragment's weights are
+            // loaded while the one before is computed.
+            auto held = [&](auto chunks, auto whole) {
+                constexpr int kC = decltype(chunks)::value;
+                constexpr bool kWhole = decltype(whole)::value;
+                typename RowAdapters<kFragsM>::template Held<kC> x;
+                typename RowAdapters<kFragsM>::template Up<kC> w[2], w2[2];
+                rows.load(x, ad, 0);
+                rows.load(w[0], ad, rows.first, 0, 0);
+                if constexpr (!kWhole) rows.load(w2[0], ad, rows.second, 0, 0);
+#pragma unroll
+                for (int i = 0; i < kFragsN; ++i) {
+                    f32x4 v[kFragsM];
+                    values(i, v);
+                    if (i + 1 < kFragsN) {
+                        rows.load(w[(i + 1) & 1], ad, rows.first, 0, i + 1);
+                        if constexpr (!kWhole) rows.load(w2[(i + 1) & 1], ad, rows.second, 0, i + 1);
+                    }
+                    if constexpr (kWhole) {
+                        rows.add(v, w[i & 1], x);
+                    } else {
+                        rows.add_own(v, w[i & 1], x, rows.first);
+                        rows.add_own(v, w2[i & 1], x, rows.second);
+                    }
+                    store(i, v);
+                }
+            };
+            constexpr std::integral_constant<int, 1> one{};
+            constexpr std::integral_constant<int, 2> two{};
+            if (rows.first < 0) {
+#pragma unroll
+                for (int i = 0; i < kFragsN; ++i) {
+                    f32x4 v[kFragsM];
+                    values(i, v);
+                    store(i, v);
+                }
+            } else if (rows.whole && ad.rank <= 32) {
+                held(one, std::true_type{});
+            } else if (rows.whole && ad.rank <= 64) {
+                held(two, std::true_type{});
+            } else if (kFragsM > 1 && !rows.more && ad.rank <= 32) {
+                held(one, std::false_type{});
+            } else if (kFragsM > 1 && kMma < 32 && !rows.more && ad.rank <= 64) {
+                held(two, std::false_type{});
+            } else {
+                constexpr int kI = kFragsM == 1 ? kFragsN : 1;
+#pragma unroll
+                for (int i = 0; i < kFragsN; i += kI) {
+                    f32x4 v[kI][kFragsM];
+#pragma unroll
+                    for (int c = 0; c < kI; ++c) values(i + c, v[c]);
+                    rows.template add_any<kI>(v, ad, i);
+#pragma unroll
+                    for (int c = 0; c < kI; ++c) store(i + c, v[c]);
+                }
+            }
+        } else if (hw_round) {
+            stage_tile(std::true_type{});
+        } else {
+            stage_tile(std::false_type{});
+        }
         __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
         __builtin_amdgcn_wave_barrier();
         __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
@@ -940,10 +1116,8 @@ extern "C" int32_t tu_int8_gemm_bf16_residual(const int8_t *a, const int8_t *w, 
                                     static_cast<const uint16_t *>(gate_bf16), gate_bf16 ? gate_rows : 1);
 }
 
-extern "C" int64_t tu_int8_gemm_adapters_workspace(int64_t m, int64_t k, int64_t rank, int64_t count, int32_t cus) {
-    using namespace tu;
-    if (m <= 0 || k <= 0 || rank <= 0 || count <= 0 || cus <= 0) return 0;
-    return down_plan(m, k, rank, count, cus).parts * m * rank * static_cast<int64_t>(sizeof(float));
+extern "C" int64_t tu_int8_gemm_adapters_workspace(int64_t m, int64_t rank) {
+    return m > 0 && rank > 0 ? m * rank * 4 : 0;
 }
 
 extern "C" int32_t tu_int8_gemm_adapters(const int8_t *a, const int8_t *w, const float *a_scale, const float *w_scale,
@@ -963,18 +1137,16 @@ extern "C" int32_t tu_int8_gemm_adapters(const int8_t *a, const int8_t *w, const
                    (reinterpret_cast<uintptr_t>(gate_bf16) & 15) == 0,
                "adapter weights, residual and gate must be 16-byte aligned");
     TU_REQUIRE(!gate_bf16 || (residual_bf16 && gate_rows > 0), "a gate needs a residual and positive gate_rows");
-    TU_REQUIRE((m + 31) / 32 <= 0x7fffffff / 512, "adapter grid too large");
-    const bool sized = m > 0 && k > 0;
-    const DownPlan plan = sized ? down_plan(m, k, rank, count, cus) : DownPlan{1, 1, 64};
-    const int64_t need = sized ? plan.parts * m * rank * static_cast<int64_t>(sizeof(float)) : 0;
-    TU_REQUIRE(!sized || (workspace && (reinterpret_cast<uintptr_t>(workspace) & 15) == 0 && workspace_bytes >= need),
+    TU_REQUIRE((m + 15) / 16 <= 0x7fffffff / 512, "adapter grid too large");
+    const int64_t need = tu_int8_gemm_adapters_workspace(m, rank);
+    TU_REQUIRE(m <= 0 || (workspace && (reinterpret_cast<uintptr_t>(workspace) & 15) == 0 && workspace_bytes >= need),
                "adapter workspace must be 16-byte aligned and hold %lld bytes", static_cast<long long>(need));
     if (check_epilogue_args(a_scale, w_scale, bias) || check_gemm_args(a, w, out_bf16, m, n, k)) return -1;
     if (m == 0) return 0;
-    auto *h = static_cast<float *>(workspace);
+    auto *h = static_cast<uint16_t *>(workspace);
     const Adapters ad{h, static_cast<const uint16_t *>(up_bf16), ids, id_rows, static_cast<int>(rank),
-                      static_cast<int>(count), plan.parts};
-    if (launch_down(a, a_scale, static_cast<const uint16_t *>(down_bf16), scaling, ad, plan, h, m, k,
+                      static_cast<int>(count)};
+    if (launch_down(a, a_scale, static_cast<const uint16_t *>(down_bf16), scaling, ad, h, m, k, cus,
                     static_cast<hipStream_t>(stream)))
         return -1;
     const auto *res = static_cast<const uint16_t *>(residual_bf16);

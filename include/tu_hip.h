@@ -172,14 +172,14 @@ int32_t tu_int8_gemm_bf16_residual(const int8_t *a, const int8_t *w, const float
  * adapter and gets tu_int8_gemm_bf16's bits.  out = bf16_rn(y), or with a
  * residual bf16_rn(fma(bf16_rn(y), gate, residual)) as
  * tu_int8_gemm_bf16_residual.  Codes are those of a rotated activation, so
- * down holds the adapter's rows rotated alike.  h is in fp32 and reaches the
- * matrix pipe as two bf16 terms.  down: bf16 [count, rank, k]; up: bf16
+ * down holds the adapter's rows rotated alike.  h is summed in fp32 and kept
+ * as two bf16 terms (to 2^-16 of it).  down: bf16 [count, rank, k]; up: bf16
  * [count, n, rank]; scaling: fp32 [count]; ids: int32 [ceil(m / id_rows)];
  * rank a multiple of 8 up to 4096; down, up, residual and gate 16-byte
  * aligned; the rest as above.  workspace: 16-byte aligned, at least
- * tu_int8_gemm_adapters_workspace(...) bytes for the same sizes and compute
- * units (`cus`).  Two launches.  No counterpart in the reference. */
-int64_t tu_int8_gemm_adapters_workspace(int64_t m, int64_t k, int64_t rank, int64_t count, int32_t cus);
+ * tu_int8_gemm_adapters_workspace(m, rank) bytes (h).  cus: the device's
+ * compute units.  Two launches.  No counterpart in the reference. */
+int64_t tu_int8_gemm_adapters_workspace(int64_t m, int64_t rank);
 int32_t tu_int8_gemm_adapters(const int8_t *a, const int8_t *w, const float *a_scale, const float *w_scale,
                               const float *bias, const void *down_bf16, const void *up_bf16,
                               const float *scaling, const int32_t *ids, int64_t id_rows, int64_t rank,

@@ -144,9 +144,8 @@ def test_workspaces():
     assert lib.tu_sage_block_attn_workspace(1, 40, 32760, 128, 128, 256) == 0
     assert lib.tu_sage_block_attn_workspace(1, 1, 1, 128, 3, 256) == 0
     assert lib.tu_sage_block_attn_workspace(4, 16, 1, 128, 32, 256) > 0
-    for m, k, rank, count in ((1, 16, 8, 1), (61, 5120, 24, 16), (32760, 13824, 64, 2)):
-        n = lib.tu_int8_gemm_adapters_workspace(m, k, rank, count, 256)
-        assert n >= 4 * m * rank and n % (4 * m * rank) == 0
+    # two bf16 terms a row and rank
+    assert lib.tu_int8_gemm_adapters_workspace(61, 24) == 61 * 24 * 4
 
 
 @pytest.mark.parametrize("group", [128, 256])
