@@ -224,7 +224,7 @@ class _GeneralRoute:
     def int8_linear(*args):
         return None
 
-    sageattn = w8a8attn = int8_linear
+    sageattn = w8a8attn = select_key_blocks = key_block_attention = int8_linear_adapters = int8_linear
 
 
 _host = None

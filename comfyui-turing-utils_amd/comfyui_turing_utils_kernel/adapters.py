@@ -23,19 +23,10 @@ import torch
 
 from . import _lib, ops
 from .ops import _check_residual, _linear_args
+from .turing_sage.core import _compute_units
 
 RANK_MULTIPLE = 8  # the kernels read 16-byte pieces of a rank
 MAX_RANK = 4096
-
-_CU_COUNT: dict = {}
-
-
-def _compute_units(device: torch.device) -> int:
-    index = device.index if device.index is not None else torch.cuda.current_device()
-    if index not in _CU_COUNT:
-        _CU_COUNT[index] = int(torch.cuda.get_device_properties(index).multi_processor_count)
-    return _CU_COUNT[index]
-
 
 def _check_adapters(m, n, k, down, up, scaling, adapter_ids, adapter_rows) -> None:
     if down.dtype != torch.bfloat16 or up.dtype != torch.bfloat16:
@@ -151,10 +142,13 @@ def turing_int8_linear_adapters(
     bf16 [count, N, rank], ``scaling`` fp32 [count], ``adapter_ids`` int32
     [ceil(M / adapter_rows)]; the rank is a multiple of 8.  The op is
     ``torch.ops.turing_utils.int8_linear_adapters``; it has no backward."""
-    call = _int8_linear_adapters_op if torch.compiler.is_compiling() or activation.device.type != "cuda" \
-        else _linear_adapters
-    return call(activation, weight, activation_scale, weight_scale, bias, down, up, scaling, adapter_ids,
-                adapter_rows, residual, gate, gate_rows)
+    args = (activation, weight, activation_scale, weight_scale, bias, down, up, scaling, adapter_ids, adapter_rows,
+            residual, gate, gate_rows)
+    if torch.compiler.is_compiling() or not activation.is_cuda:
+        return _int8_linear_adapters_op(*args)
+    out = _lib.host_calls().int8_linear_adapters(*args, _compute_units(activation.device),
+                                                 _lib.raw_stream(activation.get_device()))
+    return _linear_adapters(*args) if out is None else out
 
 
 _R4 = ((1, 1, 1, -1), (1, 1, -1, 1), (1, -1, 1, 1), (-1, 1, 1, 1))

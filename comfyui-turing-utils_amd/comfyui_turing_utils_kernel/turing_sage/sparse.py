@@ -147,9 +147,17 @@ def select_key_blocks(
     and w - 1 more on each side), then the larger product of the blocks' mean
     rows (64-bit, over the rows in front of the sample's end), NaN last, then
     the lower j."""
-    call = sage_block_select if torch.compiler.is_compiling() or query_int8.device.type != "cuda" else _select
-    return call(query_int8, query_scale, key_int8, key_scale, tensor_layout, int(keep), bool(is_causal),
-                int(sink_blocks), int(local_blocks), int(blkq), int(blkk), query_lengths, key_lengths)
+    args = (tensor_layout, int(keep), bool(is_causal), int(sink_blocks), int(local_blocks), int(blkq), int(blkk),
+            query_lengths, key_lengths)
+    if torch.compiler.is_compiling() or not query_int8.is_cuda:
+        return sage_block_select(query_int8, query_scale, key_int8, key_scale, *args)
+    if tensor_layout in ("HND", "NHD"):
+        index = _lib.host_calls().select_key_blocks(query_int8, query_scale, key_int8, key_scale,
+                                                    tensor_layout == "NHD", *args[1:],
+                                                    _lib.raw_stream(query_int8.get_device()))
+        if index is not None:
+            return index
+    return _select(query_int8, query_scale, key_int8, key_scale, *args)
 
 
 def _check_attend(query_int8, query_scale, key_int8, key_scale, value_t, block_index, tensor_layout, blkq, blkk):
@@ -261,9 +269,18 @@ def key_block_attention(
     Output: bf16 in the layout and shape of ``query_int8``."""
     if sm_scale is not None and not 0.0 < float(sm_scale) < float("inf"):
         raise ValueError("sm_scale must be a positive finite number")
-    call = sage_block_attention if torch.compiler.is_compiling() or query_int8.device.type != "cuda" else _attend
-    return call(query_int8, query_scale, key_int8, key_scale, value_t, block_index, tensor_layout, bool(is_causal),
-                -1.0 if sm_scale is None else float(sm_scale), int(blkq), int(blkk), query_lengths, key_lengths)
+    tensors = (query_int8, query_scale, key_int8, key_scale, value_t, block_index)
+    args = (tensor_layout, bool(is_causal), -1.0 if sm_scale is None else float(sm_scale), int(blkq), int(blkk),
+            query_lengths, key_lengths)
+    if torch.compiler.is_compiling() or not query_int8.is_cuda:
+        return sage_block_attention(*tensors, *args)
+    if tensor_layout in ("HND", "NHD"):
+        out = _lib.host_calls().key_block_attention(*tensors, tensor_layout == "NHD", *args[1:],
+                                                    _compute_units(query_int8.device),
+                                                    _lib.raw_stream(query_int8.get_device()))
+        if out is not None:
+            return out
+    return _attend(*tensors, *args)
 
 
 def sparse_sageattn_from_prequantized(

@@ -1,5 +1,5 @@
-// The whole host side of the three hot calls as one native function each:
-// checks, output and scratch tensors, launches.
+// The whole host side of the hot calls as one native function each: checks,
+// output and scratch tensors, launches.
 //
 // A short call is bound by its host work, not by its kernels: from Python the
 // W8A8 linear of one row spent 42 us on the host (two dispatched custom ops,
@@ -282,9 +282,194 @@ PyObject *w8a8attn(PyObject *, PyObject *const *args, Py_ssize_t nargs) {
     END_HANDLE_TH_ERRORS
 }
 
+// An optional tensor argument that is contiguous, of one type and 16-byte aligned.
+bool optional(PyObject *obj, const Tensor **out, c10::Device device, at::ScalarType type) {
+    *out = nullptr;
+    if (obj == Py_None) return true;
+    return plain(obj, out, device) && (*out)->scalar_type() == type && (*out)->is_contiguous() && aligned(**out, 16);
+}
+
+// Optional int32 lengths of a padded batch; their data or null.
+bool lengths(PyObject *obj, const int32_t **out, c10::Device device, int64_t batch) {
+    *out = nullptr;
+    if (obj == Py_None) return true;
+    const Tensor *t;
+    if (!plain(obj, &t, device) || t->scalar_type() != at::kInt || t->dim() != 1 || t->size(0) != batch || !t->is_contiguous())
+        return false;
+    *out = t->data_ptr<int32_t>();
+    return true;
+}
+
+// Quantized Q / K (codes, scales) of the block-sparse calls.
+struct CodesQk {
+    const Tensor *q, *qs, *k, *ks;
+    int64_t batch, hq, hkv, lq, lk, dim, blkq, blkk;
+    int head, seq;
+    c10::Device device = c10::kCPU;
+    int64_t sb(const Tensor &t) const { return t.stride(0); }
+    int64_t sh(const Tensor &t) const { return t.stride(head); }
+    int64_t sl(const Tensor &t) const { return t.stride(seq); }
+};
+
+bool codes_aligned(const Tensor &t) {
+    return t.stride(3) == 1 && t.stride(0) % 16 == 0 && t.stride(1) % 16 == 0 && t.stride(2) % 16 == 0 && aligned(t, 16);
+}
+
+bool unpack_codes(PyObject *const *args, int64_t nhd, CodesQk &a) {
+    if (!THPVariable_CheckTypeExact(Py_TYPE(args[0]))) return false;
+    a.device = THPVariable_Unpack(args[0]).device();
+    if (!a.device.is_cuda() || !plain_context(a.device.index()) || !plain(args[0], &a.q, a.device) ||
+        !plain(args[1], &a.qs, a.device) || !plain(args[2], &a.k, a.device) || !plain(args[3], &a.ks, a.device))
+        return false;
+    const Tensor &q = *a.q, &k = *a.k, &qs = *a.qs, &ks = *a.ks;
+    if (q.scalar_type() != at::kChar || k.scalar_type() != at::kChar || q.dim() != 4 || k.dim() != 4 ||
+        qs.scalar_type() != at::kFloat || ks.scalar_type() != at::kFloat || qs.dim() != 3 || ks.dim() != 3 ||
+        !qs.is_contiguous() || !ks.is_contiguous())
+        return false;
+    a.head = nhd ? 2 : 1;
+    a.seq = nhd ? 1 : 2;
+    a.batch = q.size(0);
+    a.hq = q.size(a.head);
+    a.lq = q.size(a.seq);
+    a.hkv = k.size(a.head);
+    a.lk = k.size(a.seq);
+    a.dim = q.size(3);
+    return (a.dim == 64 || a.dim == 128) && k.size(0) == a.batch && k.size(3) == a.dim && a.batch > 0 && a.hq > 0 &&
+           a.lq > 0 && a.lk > 0 && a.hkv > 0 && a.hq % a.hkv == 0 && a.blkq > 0 && a.blkk > 0 && a.blkk % 64 == 0 &&
+           qs.size(0) == a.batch && qs.size(1) == a.hq && qs.size(2) == ceil_div(a.lq, a.blkq) &&
+           ks.size(0) == a.batch && ks.size(1) == a.hkv && ks.size(2) == ceil_div(a.lk, a.blkk) && codes_aligned(q) &&
+           codes_aligned(k);
+}
+
+// select_key_blocks(q8, qs, k8, ks, nhd, keep, causal, sink, local, blkq, blkk, q_lengths, k_lengths, stream)
+PyObject *select_key_blocks(PyObject *, PyObject *const *args, Py_ssize_t nargs) {
+    HANDLE_TH_ERRORS
+    CodesQk a;
+    int64_t nhd, keep, causal, sink, local, stream;
+    const int32_t *ql, *kl;
+    if (nargs != 14 || !integer(args[4], &nhd) || !integer(args[5], &keep) || !integer(args[6], &causal) ||
+        !integer(args[7], &sink) || !integer(args[8], &local) || !integer(args[9], &a.blkq) ||
+        !integer(args[10], &a.blkk) || !integer(args[13], &stream) || keep < 1 || sink < 0 || local < 0 ||
+        sink > 0x3fffffff || local > 0x3fffffff || !unpack_codes(args, nhd, a) ||
+        !lengths(args[11], &ql, a.device, a.batch) || !lengths(args[12], &kl, a.device, a.batch))
+        Py_RETURN_NONE;
+    Tensor index;
+    {
+        ReleaseGil nogil;
+        const int64_t nkb = ceil_div(a.lk, 64);
+        keep = keep < nkb ? keep : nkb;
+        index = empty({a.batch, a.hq, ceil_div(a.lq, 128), keep}, at::kInt, a.device);
+        const int64_t bytes = tu_sage_block_select_workspace(a.batch, a.hq, a.hkv, a.lq, a.lk, a.dim);
+        const Tensor work = empty({bytes}, at::kByte, a.device);
+        if (tu_sage_block_select(a.q->data_ptr<int8_t>(), a.qs->data_ptr<float>(), a.blkq, a.k->data_ptr<int8_t>(),
+                                 a.ks->data_ptr<float>(), a.blkk, a.batch, a.hq, a.hkv, a.lq, a.lk, a.dim, a.sb(*a.q),
+                                 a.sh(*a.q), a.sl(*a.q), a.sb(*a.k), a.sh(*a.k), a.sl(*a.k), ql, kl, keep, sink, local,
+                                 causal != 0, work.data_ptr(), bytes, index.data_ptr<int32_t>(),
+                                 reinterpret_cast<void *>(stream)))
+            failed("tu_sage_block_select");
+    }
+    return THPVariable_Wrap(std::move(index));
+    END_HANDLE_TH_ERRORS
+}
+
+// key_block_attention(q8, qs, k8, ks, vt, index, nhd, causal, scale, blkq, blkk, q_lengths, k_lengths, cus, stream)
+PyObject *key_block_attention(PyObject *, PyObject *const *args, Py_ssize_t nargs) {
+    HANDLE_TH_ERRORS
+    CodesQk a;
+    int64_t nhd, causal, cus, stream;
+    const int32_t *ql, *kl;
+    const Tensor *vt, *index;
+    if (nargs != 15 || !integer(args[6], &nhd) || !integer(args[7], &causal) || !PyFloat_Check(args[8]) ||
+        !integer(args[9], &a.blkq) || !integer(args[10], &a.blkk) || !integer(args[13], &cus) ||
+        !integer(args[14], &stream) || !unpack_codes(args, nhd, a) || !plain(args[4], &vt, a.device) ||
+        !plain(args[5], &index, a.device) || !lengths(args[11], &ql, a.device, a.batch) ||
+        !lengths(args[12], &kl, a.device, a.batch))
+        Py_RETURN_NONE;
+    const double given = PyFloat_AS_DOUBLE(args[8]);
+    const float scale = given > 0.0 ? static_cast<float>(given) : static_cast<float>(1.0 / std::sqrt(static_cast<double>(a.dim)));
+    const int64_t lpad = ceil_div(a.lk, 64) * 64, tiles = a.blkk / 64;
+    if (!(scale > 0.0f && std::isfinite(scale)) || (tiles & (tiles - 1)) || vt->scalar_type() != at::kBFloat16 ||
+        vt->dim() != 4 || vt->size(0) != a.batch || vt->size(1) != a.hkv || vt->size(2) != a.dim || vt->size(3) != lpad ||
+        !vt->is_contiguous() || !aligned(*vt, 16) || index->scalar_type() != at::kInt || index->dim() != 4 ||
+        index->size(0) != a.batch || index->size(1) != a.hq || index->size(2) != ceil_div(a.lq, 128) ||
+        index->size(3) < 1 || !index->is_contiguous())
+        Py_RETURN_NONE;
+    Tensor out;
+    {
+        ReleaseGil nogil;
+        const int64_t width = index->size(3);
+        out = nhd ? empty({a.batch, a.lq, a.hq, a.dim}, at::kBFloat16, a.device)
+                  : empty({a.batch, a.hq, a.lq, a.dim}, at::kBFloat16, a.device);
+        const int64_t bytes =
+            tu_sage_block_attn_workspace(a.batch, a.hq, a.lq, a.dim, width, static_cast<int32_t>(cus));
+        Tensor part;
+        if (bytes > 0) part = empty({bytes}, at::kByte, a.device);
+        if (tu_sage_block_attn(a.q->data_ptr<int8_t>(), a.qs->data_ptr<float>(), a.blkq, a.k->data_ptr<int8_t>(),
+                               a.ks->data_ptr<float>(), a.blkk, vt->data_ptr(), lpad, index->data_ptr<int32_t>(), width,
+                               out.data_ptr(), a.batch, a.hq, a.hkv, a.lq, a.lk, a.dim, a.sb(*a.q), a.sh(*a.q),
+                               a.sl(*a.q), a.sb(*a.k), a.sh(*a.k), a.sl(*a.k), a.sb(out), a.sh(out), a.sl(out), ql, kl,
+                               scale, causal != 0, static_cast<int32_t>(cus), ptr(part), bytes,
+                               reinterpret_cast<void *>(stream)))
+            failed("tu_sage_block_attn");
+    }
+    return THPVariable_Wrap(std::move(out));
+    END_HANDLE_TH_ERRORS
+}
+
+// int8_linear_adapters(activation, weight, activation_scale, weight_scale, bias, down, up, scaling, adapter_ids,
+//                      adapter_rows, residual, gate, gate_rows, cus, stream)
+PyObject *int8_linear_adapters(PyObject *, PyObject *const *args, Py_ssize_t nargs) {
+    HANDLE_TH_ERRORS
+    int64_t id_rows, gate_rows, cus, stream;
+    if (nargs != 15 || !integer(args[9], &id_rows) || !integer(args[12], &gate_rows) || !integer(args[13], &cus) ||
+        !integer(args[14], &stream) || !THPVariable_CheckTypeExact(Py_TYPE(args[0])))
+        Py_RETURN_NONE;
+    const c10::Device device = THPVariable_Unpack(args[0]).device();
+    const Tensor *x, *w, *xs, *ws, *bias, *down, *up, *scaling, *ids, *residual, *gate;
+    if (!device.is_cuda() || !plain_context(device.index()) || !plain(args[0], &x, device) ||
+        !plain(args[1], &w, device) || !plain(args[2], &xs, device) || !plain(args[3], &ws, device) ||
+        !optional(args[4], &bias, device, at::kFloat) || !plain(args[5], &down, device) || !plain(args[6], &up, device) ||
+        !plain(args[7], &scaling, device) || !plain(args[8], &ids, device) ||
+        !optional(args[10], &residual, device, at::kBFloat16) || !optional(args[11], &gate, device, at::kBFloat16))
+        Py_RETURN_NONE;
+    if (x->scalar_type() != at::kChar || x->dim() != 2 || w->scalar_type() != at::kChar || w->dim() != 2 ||
+        down->scalar_type() != at::kBFloat16 || down->dim() != 3 || up->scalar_type() != at::kBFloat16 || up->dim() != 3)
+        Py_RETURN_NONE;
+    const int64_t m = x->size(0), k = x->size(1), n = w->size(0), count = down->size(0), rank = down->size(1);
+    for (const Tensor *t : {x, w, down, up})
+        if (!t->is_contiguous() || !aligned(*t, 16)) Py_RETURN_NONE;
+    for (const Tensor *t : {xs, ws, scaling})
+        if (t->scalar_type() != at::kFloat || !t->is_contiguous()) Py_RETURN_NONE;
+    if (m < 1 || k < 1 || k % 16 || k >= 131072 || n < 1 || n % 8 || w->size(1) != k || xs->numel() != m ||
+        ws->numel() != n || !aligned(*ws, 16) || (bias && bias->numel() != n) || count < 1 || rank < 1 || rank % 8 ||
+        rank > 4096 || down->size(2) != k || up->size(0) != count || up->size(1) != n || up->size(2) != rank ||
+        scaling->dim() != 1 || scaling->size(0) != count || ids->scalar_type() != at::kInt || ids->dim() != 1 ||
+        !ids->is_contiguous() || id_rows < 1 || ids->size(0) != ceil_div(m, id_rows) || (gate && !residual) ||
+        (residual && (residual->dim() != 2 || residual->size(0) != m || residual->size(1) != n)) ||
+        (gate && (gate_rows < 1 || gate->numel() != ceil_div(m, gate_rows) * n)))
+        Py_RETURN_NONE;
+    Tensor out;
+    {
+        ReleaseGil nogil;
+        out = empty({m, n}, at::kBFloat16, device);
+        const int64_t bytes = tu_int8_gemm_adapters_workspace(m, rank);
+        const Tensor work = empty({bytes}, at::kByte, device);
+        if (tu_int8_gemm_adapters(x->data_ptr<int8_t>(), w->data_ptr<int8_t>(), xs->data_ptr<float>(),
+                                  ws->data_ptr<float>(), bias ? bias->data_ptr<float>() : nullptr, down->data_ptr(),
+                                  up->data_ptr(), scaling->data_ptr<float>(), ids->data_ptr<int32_t>(), id_rows, rank,
+                                  count, residual ? residual->data_ptr() : nullptr, gate ? gate->data_ptr() : nullptr,
+                                  gate ? gate_rows : 1, out.data_ptr(), m, n, k, static_cast<int32_t>(cus),
+                                  work.data_ptr(), bytes, reinterpret_cast<void *>(stream)))
+            failed("tu_int8_gemm_adapters");
+    }
+    return THPVariable_Wrap(std::move(out));
+    END_HANDLE_TH_ERRORS
+}
+
 #define TU_METHOD(NAME) \
     {#NAME, reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(NAME)), METH_FASTCALL, nullptr}
-PyMethodDef methods[] = {TU_METHOD(int8_linear), TU_METHOD(sageattn), TU_METHOD(w8a8attn), {nullptr, nullptr, 0, nullptr}};
+PyMethodDef methods[] = {TU_METHOD(int8_linear), TU_METHOD(sageattn), TU_METHOD(w8a8attn), TU_METHOD(select_key_blocks),
+                         TU_METHOD(key_block_attention), TU_METHOD(int8_linear_adapters), {nullptr, nullptr, 0, nullptr}};
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "_host_calls", nullptr, -1, methods, nullptr, nullptr, nullptr, nullptr};
 
 }  // namespace
