@@ -11,19 +11,23 @@
 // sample's length, and rows that see no key, are zeros.
 //
 // MI355X mapping
-//   * A workgroup is 4 waves = 128 query rows, one list, 32 rows a wave, one
-//     wave per SIMD; two workgroups share a CU (72 KiB of rings each at
-//     head_dim 128), and as nothing ties them together one's softmax runs
-//     beside the other's MFMAs.
-//   * K and V^T tiles stream through rings of three stages each.  A tile's K
-//     is used one interval before its V^T, so in interval t (QK of tile t + 1,
-//     PV of tile t) the loads of K(t + 3) and V^T(t + 2) start at once, into
-//     the stages that interval t - 1 read last, and have two intervals to land.
+//   * A unit of work is 128 query rows with their list, or a range of it; a
+//     workgroup is two groups of 4 waves, a unit each, 32 rows a wave, so that
+//     every SIMD holds one wave of each group.  The groups share nothing but a
+//     barrier per tile, which keeps them in opposite phases: group 0 runs its
+//     MFMA cluster then its softmax, group 1 the softmax first.  (Two
+//     workgroups of one unit each fell into step, both in their MFMAs, then
+//     both in their softmax: 53 % MFMA busy, 3.29 ms at B1 H40 L32760 D128 with
+//     102 of 512 blocks.)
+//   * K and V^T tiles of a group stream through rings of three stages each.  A
+//     tile's K is used one interval before its V^T, so in interval t (QK of
+//     tile t + 1, PV of tile t) the loads of K(t + 3) and V^T(t + 2) start at
+//     once, into the stages that interval t - 1 read last, and have two
+//     intervals to land.
 //   * The list is compacted into LDS 256 entries at a time, with each block's
-//     scale beside it; the loop reads two entries ahead, so no tile waits for
-//     its address.
-//   * Few rows (a short grid) split their lists into ranges, one workgroup
-//     each, merged by a second kernel.
+//     scale beside it.
+//   * Few rows (a short grid) split their lists into ranges, a unit each,
+//     merged by a second kernel.
 #include <algorithm>
 
 #include "attn_common.h"
@@ -33,13 +37,16 @@
 namespace tu {
 namespace {
 
-constexpr int kBlockThreads = 256;
+constexpr int kGroupThreads = 256;
+constexpr int kBlockThreads = 2 * kGroupThreads;
 constexpr int kBlockRows = 128;
 constexpr int kRing = 3;
 constexpr int kSegment = 256;  // list entries compacted at a time
 // exponent base of a row that has seen no key yet: finite, so that a tile
 // without a visible key gives 2^-inf = 0 and not a NaN
 constexpr float kNoBase = -1e30f;
+// a scale of zero would make a masked score 0 * -inf
+constexpr float kLeastScale = 1e-18f;
 
 struct BlockPlan {
     uint32_t nqb, bh;  // query blocks of a head, batch * hq
@@ -52,8 +59,9 @@ template <int D>
 struct Ring {
     static constexpr int kV0 = kRing * Geo<D>::kKTileBytes;  // V^T stages follow the K stages
     static constexpr int kList = kRing * Geo<D>::kStageBytes;  // the compacted entries follow the rings
-    static constexpr int kScan = kList + kSegment * 8;         // and the waves' counts
-    static constexpr int kBytes = kScan + 2 * (kBlockThreads / 64) * 4;
+    static constexpr int kScan = kList + kSegment * 8;         // and the group's waves' counts
+    static constexpr int kGroup = (kScan + 3 * 4 * 4 + 1023) / 1024 * 1024;
+    static constexpr int kBytes = 2 * kGroup;
 };
 
 // Loads of one tile's K rows, or its V^T columns, into a ring stage (the two
@@ -93,10 +101,38 @@ struct ListEntry {
     float scale;
 };
 
+// O^T += V^T P for a tile whose keys from `from` on (1 .. 63) are behind the
+// sample's end: their p is zero, but what stands there may be no number, so
+// their values are zeroed as well.
+template <int D>
+__device__ __forceinline__ void pv_tail(const int8_t *stage, const LaneGeom<D> &gm, const bf16x8 (&p)[2][kQT],
+                                        SoftmaxState<D> &st, const bf16x8 &ones, int from, int g) {
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+        u32x4 keep;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            const int key = 32 * h + 8 * g + 2 * e;
+            keep[e] = (key < from ? 0x0000ffffu : 0u) | (key + 1 < from ? 0xffff0000u : 0u);
+        }
+#pragma unroll
+        for (int ds = 0; ds < Geo<D>::kDS; ++ds) {
+            const u32x4 v = *reinterpret_cast<const u32x4 *>(stage + gm.v_rd[h] + ds * 16 * 128) & keep;
+#pragma unroll
+            for (int qt = 0; qt < kQT; ++qt)
+                st.acc_o[ds][qt] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, v), p[h][qt],
+                                                                           st.acc_o[ds][qt], 0, 0, 0);
+        }
+#pragma unroll
+        for (int qt = 0; qt < kQT; ++qt)
+            st.acc_l[qt] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(ones, p[h][qt], st.acc_l[qt], 0, 0, 0);
+    }
+}
+
 // kSplit: ranges of a list write the unnormalized O with each row's exponent
 // base and row sum to `part` for block_merge_kernel.
 template <int D, bool kCausal, bool kSplit>
-__global__ __launch_bounds__(kBlockThreads, 2) void block_attn_kernel(
+__global__ __launch_bounds__(kBlockThreads, 1) void block_attn_kernel(
     const int8_t *__restrict__ q8, const float *__restrict__ q_scale, uint32_t blkq, uint32_t nbq,
     const int8_t *__restrict__ k8, const float *__restrict__ k_scale, int kscale_shift, uint32_t nbk,
     const uint16_t *__restrict__ vt, const int32_t *__restrict__ index, uint16_t *__restrict__ o, uint32_t hq,
@@ -107,22 +143,24 @@ __global__ __launch_bounds__(kBlockThreads, 2) void block_attn_kernel(
     constexpr int kLoadsPerTile = Geo<D>::kLoadsPerTile;
     // One array: with several the compiler waits for all direct-to-LDS loads
     // before a tile's fragment reads.
-    __shared__ __align__(1024) int8_t lds[Ring<D>::kBytes];
-    auto *list = reinterpret_cast<ListEntry *>(lds + Ring<D>::kList);
-    auto *scan = reinterpret_cast<int(*)[kBlockThreads / 64]>(lds + Ring<D>::kScan);
+    __shared__ __align__(1024) int8_t lds_mem[Ring<D>::kBytes];
 
-    const int tid = threadIdx.x;
-    const int lane = tid & 63;
-    const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int lane = threadIdx.x & 63;
+    const int wave8 = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int grp = wave8 >> 2;
+    const int wave = wave8 & 3;
+    const int tid = wave * 64 + lane;  // within the group
     const int g = lane >> 4;
     const int lc = lane & 15;
-    auto kst = [&](int t) { return lds + (t % kRing) * Geo<D>::kKTileBytes; };
-    // pv_tile and mfma_cluster add kKTileBytes to reach a stage's V^T
-    auto vst = [&](int t) { return lds + Ring<D>::kV0 + (t % kRing) * Geo<D>::kVTileBytes - Geo<D>::kKTileBytes; };
-
+    int8_t *lds = lds_mem + grp * Ring<D>::kGroup;
+    auto *list = reinterpret_cast<ListEntry *>(lds + Ring<D>::kList);
+    auto *scan = reinterpret_cast<int(*)[4]>(lds + Ring<D>::kScan);
     // Head-major numbering, a contiguous eighth per XCD: neighbouring query
     // blocks of a head, whose lists are alike, share an L2.
-    uint32_t id = xcd_chunk(blockIdx.x, gridDim.x);
+    const uint32_t units = plan.bh * plan.nqb * plan.parts;
+    uint32_t id = 2 * xcd_chunk(blockIdx.x, gridDim.x) + grp;
+    const bool idle = id >= units;  // the second group of an odd last pair
+    if (idle) id = units - 1;
     uint32_t z = 0;
     if constexpr (kSplit) {
         z = id % plan.parts;
@@ -143,7 +181,10 @@ __global__ __launch_bounds__(kBlockThreads, 2) void block_attn_kernel(
     // blocks this query block can see at all
     int seen_end = k_end;
     if constexpr (kCausal) seen_end = static_cast<int>(min<int64_t>(k_end, min<int64_t>(qblock0 + kBlockRows, q_end)));
-    const int blocks = qblock0 < q_end ? (seen_end + kBKey - 1) / kBKey : 0;
+    const int blocks = qblock0 < q_end && !idle ? (seen_end + kBKey - 1) / kBKey : 0;
+    // the first block that the sample's end or a diagonal cuts
+    int masked_from = k_end / kBKey;
+    if constexpr (kCausal) masked_from = static_cast<int>(min<int64_t>(masked_from, qblock0 / kBKey));
 
     const LaneGeom<D> gm = lane_geom<D>(wave, lane, k_sl, lpad);
     const __amdgpu_buffer_rsrc_t krs = make_rsrc(kp, static_cast<uint32_t>(lk * k_sl));
@@ -158,7 +199,7 @@ __global__ __launch_bounds__(kBlockThreads, 2) void block_attn_kernel(
 #pragma unroll
         for (int ds = 0; ds < kSl; ++ds)
             qf[qt][ds] = *reinterpret_cast<const i32x4 *>(qp + qi * q_sl + 64 * ds + 16 * g);
-        qsc[qt] = q_scale[static_cast<int64_t>(bh) * nbq + static_cast<uint32_t>(qi) / blkq] * sm_log2;
+        qsc[qt] = fmaxf(q_scale[static_cast<int64_t>(bh) * nbq + static_cast<uint32_t>(qi) / blkq], kLeastScale) * sm_log2;
     }
     SoftmaxState<D> st;
 #pragma unroll
@@ -175,29 +216,29 @@ __global__ __launch_bounds__(kBlockThreads, 2) void block_attn_kernel(
     i32x4 s[4][kQT];
     bf16x8 pb[2][kQT];
 
-    // first entry of this workgroup's range, and the end of it
-    int first = 0, end = blocks > 0 ? static_cast<int>(plan.width) : 0;
+    // first entry of this group's range, and the end of it.  Both groups walk
+    // as many segments and tiles as the longer one, for the barriers.
+    int first = 0;
+    const int per = static_cast<int>(plan.per);
     int before = -1;  // largest entry in front of the next segment
     if constexpr (kSplit) {
-        first = static_cast<int>(z * plan.per);
-        end = min(end, first + static_cast<int>(plan.per));
-        if (end > first) {
-            int m = -1;
-            for (int i = tid; i < first; i += kBlockThreads) m = max(m, entries[i]);
+        first = static_cast<int>(z) * per;
+        int m = -1;
+        for (int i = tid; i < first; i += kGroupThreads) m = max(m, entries[i]);
 #pragma unroll
-            for (int d = 1; d < 64; d <<= 1) m = max(m, __shfl_xor(m, d));
-            if (lane == 0) scan[0][wave] = m;
-            __syncthreads();
+        for (int d = 1; d < 64; d <<= 1) m = max(m, __shfl_xor(m, d));
+        if (lane == 0) scan[0][wave] = m;
+        __syncthreads();
 #pragma unroll
-            for (int w = 0; w < kBlockThreads / 64; ++w) before = max(before, scan[0][w]);
-            __syncthreads();
-        }
+        for (int w = 0; w < 4; ++w) before = max(before, scan[0][w]);
+        __syncthreads();
     }
+    const int end = min(static_cast<int>(plan.width), first + per);
 
-    for (int seg = first; seg < end; seg += kSegment) {
-        // Compaction of entries seg .. seg + 255: an inclusive running maximum
-        // over the threads, then the rank among the entries that count.
-        const int at = seg + tid;
+    for (int seg = 0; seg < per; seg += kSegment) {
+        // Compaction of the next 256 entries: an inclusive running maximum over
+        // the group's threads, then the rank among the entries that count.
+        const int at = first + seg + tid;
         const int e = at < end ? entries[at] : -1;
         int top = e;
 #pragma unroll
@@ -211,89 +252,139 @@ __global__ __launch_bounds__(kBlockThreads, 2) void block_attn_kernel(
         __syncthreads();
         prev = max(prev, before);
 #pragma unroll
-        for (int w = 0; w < kBlockThreads / 64; ++w) {
+        for (int w = 0; w < 4; ++w) {
             if (w < wave) prev = max(prev, scan[0][w]);
             before = max(before, scan[0][w]);
         }
         const bool counts = e > prev && e < blocks;
         const uint64_t mask = __ballot(counts);
-        if (lane == 0) scan[1][wave] = __builtin_popcountll(mask);
+        // tiles with masked keys stand last, as the list ascends
+        const uint64_t plain = __ballot(counts && e < masked_from);
+        if (lane == 0) {
+            scan[1][wave] = __builtin_popcountll(mask);
+            scan[2][wave] = __builtin_popcountll(plain);
+        }
         __syncthreads();
-        int rank = __builtin_popcountll(mask & ((1ull << lane) - 1)), n = 0;
+        int rank = __builtin_popcountll(mask & ((1ull << lane) - 1)), n = 0, whole = 0;
 #pragma unroll
-        for (int w = 0; w < kBlockThreads / 64; ++w) {
+        for (int w = 0; w < 4; ++w) {
             if (w < wave) rank += scan[1][w];
             n += scan[1][w];
+            whole += scan[2][w];
         }
-        if (counts) list[rank] = ListEntry{e, ks_row[e >> kscale_shift]};
-        __syncthreads();
+        if (counts) list[rank] = ListEntry{e, fmaxf(ks_row[e >> kscale_shift], kLeastScale)};
+        // the other group's tiles, for the barriers
+        const auto *theirs = reinterpret_cast<const int *>(lds_mem + (1 - grp) * Ring<D>::kGroup + Ring<D>::kScan) + 4;
+        int most = theirs[0] + theirs[1] + theirs[2] + theirs[3];
         n = __builtin_amdgcn_readfirstlane(n);
-        if (n == 0) continue;
+        whole = __builtin_amdgcn_readfirstlane(whole);
+        most = __builtin_amdgcn_readfirstlane(max(n, most));
+        __syncthreads();
+        if (most == 0) continue;
 
-        auto block_at = [&](int t) { return __builtin_amdgcn_readfirstlane(list[min(t, n - 1)].block); };
-        auto softmax = [&](int t) {
-            const ListEntry le = list[t];
-            const int key0 = __builtin_amdgcn_readfirstlane(le.block) * kBKey;
+        auto entry_at = [&](int t) { return list[min(t, n - 1)]; };
+        auto block_of = [&](const ListEntry &le) { return __builtin_amdgcn_readfirstlane(le.block); };
+        auto softmax = [&](int t, float scale, auto mask_tag) {
             float f[kQT];
-            // a scale of zero would make a masked score 0 * -inf
 #pragma unroll
-            for (int qt = 0; qt < kQT; ++qt) f[qt] = fmaxf(qsc[qt] * le.scale, 1e-37f);
-            bool masked = key0 + kBKey > k_end;
-            if constexpr (kCausal) masked = masked || key0 + kBKey > q0 + 1;
-            if (masked) {
+            for (int qt = 0; qt < kQT; ++qt) f[qt] = qsc[qt] * scale;
+            if (decltype(mask_tag)::value && t >= whole) {
+                const int key0 = block_of(list[t]) * kBKey;
                 const int key_lim = min(k_end - key0, kBKey);
                 const int q_rel = static_cast<int>(max(min(q0 - key0, static_cast<int64_t>(kBKey)), static_cast<int64_t>(-kBlockRows)));
                 mask_tile<kCausal>(s, key_lim, q_rel, g, lc);
             }
             softmax_tile(s, f, st, pb);
         };
+        // K of a tile, or its V^T, into a ring stage
+        auto load_k = [&](int stage, int block) {
+            issue_k(lds + stage * Geo<D>::kKTileBytes, krs, gm, k_sl32, block * kBKey, wave);
+        };
+        auto load_v = [&](int stage, int block) {
+            issue_v(lds + Ring<D>::kV0 + stage * Geo<D>::kVTileBytes, vrs, gm, block * kBKey, wave);
+        };
 
-        // K(0), V(0), K(1), V(1), K(2) are in flight; tile 0 and K(1) land first
-        issue_k(kst(0), krs, gm, k_sl32, block_at(0) * kBKey, wave);
-        issue_v(lds + Ring<D>::kV0, vrs, gm, block_at(0) * kBKey, wave);
-        issue_k(kst(1), krs, gm, k_sl32, block_at(1) * kBKey, wave);
-        issue_v(lds + Ring<D>::kV0 + Geo<D>::kVTileBytes, vrs, gm, block_at(1) * kBKey, wave);
-        issue_k(kst(2), krs, gm, k_sl32, block_at(2) * kBKey, wave);
-        __builtin_amdgcn_s_waitcnt(vmcnt_imm(kLoadsPerTile));
-        wg_barrier();
-        qk_tile(lds, gm, qf, s);
-        softmax(0);
-        wg_barrier();  // K(0)'s stage is free for K(3)
-#pragma clang loop unroll(disable)
-        for (int t = 0; t < n; ++t) {
-            // K(t + 3) and V(t + 2) into stages last read in interval t - 1
-            const uint32_t k3 = block_at(t + 3) * kBKey, v2 = block_at(t + 2) * kBKey;
-            issue_k(kst(t), krs, gm, k_sl32, k3, wave);
-            issue_v(lds + Ring<D>::kV0 + ((t + 2) % kRing) * Geo<D>::kVTileBytes, vrs, gm, v2, wave);
-            // V^T columns at or past the sample's last key may hold anything:
-            // as zeros they add nothing (their p is zero, but zero times a NaN
-            // is not)
-            const int key0 = block_at(t) * kBKey;
-            if (key0 + kBKey > k_end) {
-                int8_t *v = lds + Ring<D>::kV0 + (t % kRing) * Geo<D>::kVTileBytes;
-                const int from = k_end - key0;  // 1 .. 63
-                for (int i = tid; i < D * 8; i += kBlockThreads) {
-                    const int row = i >> 3, chunk = i & 7;  // 8 keys
-                    if (chunk * 8 + 8 <= from) continue;
-                    auto *p = reinterpret_cast<uint16_t *>(v + row * 128 + ((chunk ^ ((row >> 1) & 7)) << 4));
-                    for (int k = max(from - chunk * 8, 0); k < 8; ++k) p[k] = 0;
-                }
-                __syncthreads();
-            }
-            if (t + 1 < n) {
-                mfma_cluster(kst(t + 1), vst(t), gm, qf, s, pb, st, ones);
-                softmax(t + 1);
-            } else {
-                pv_tile(vst(t), gm, pb, st, ones);
-            }
-            // K(t + 2) and V(t + 1) resident
+        // block2, block3: blocks of tiles t + 2 and t + 3; scale1 .. 3: scales
+        // of tiles t + 1 .. t + 3
+        int block2 = 0, block3 = 0;
+        float scale1 = 0.0f, scale2 = 0.0f, scale3 = 0.0f;
+        auto uniform = [](float x) { return __int_as_float(__builtin_amdgcn_readfirstlane(__float_as_int(x))); };
+        if (n > 0) {
+            // K(0), V(0), K(1), V(1), K(2) in flight; tile 0 and K(1) land first
+            const ListEntry e0 = entry_at(0), e1 = entry_at(1), e2 = entry_at(2), e3 = entry_at(3);
+            load_k(0, block_of(e0));
+            load_v(0, block_of(e0));
+            load_k(1, block_of(e1));
+            load_v(1, block_of(e1));
+            block2 = block_of(e2), block3 = block_of(e3);
+            scale1 = uniform(e1.scale), scale2 = uniform(e2.scale), scale3 = uniform(e3.scale);
+            load_k(2, block2);
             __builtin_amdgcn_s_waitcnt(vmcnt_imm(kLoadsPerTile));
-            wg_barrier();
+        }
+        wg_barrier();
+        if (n > 0) {
+            qk_tile(lds, gm, qf, s);
+            if (grp == 0) softmax(0, list[0].scale, std::true_type{});
+        }
+        wg_barrier();  // K(0)'s stage is free for K(3)
+        if (grp == 1 && n > 0) softmax(0, list[0].scale, std::true_type{});
+        __builtin_amdgcn_s_waitcnt(lgkmcnt_imm(0));
+        // Interval t + 1: group 0 [M_t, softmax(t + 1)], group 1 [softmax(t),
+        // M_t] with M_t = {QK(t + 1), PV(t)}; the same sequence, group 1's
+        // barrier between its two halves.  Before it a wave waits for its loads
+        // of K(t + 2) and V(t + 1), issued an interval ago.
+        const int main_steps = max(0, min(n, whole) - 1);
+        int s0 = 0, s1 = 1, s2 = 2;  // stages of tiles t, t + 1, t + 2
+#pragma clang loop unroll(disable)
+        for (int t = 0; t < main_steps; ++t) {
+            mfma_cluster(lds + s1 * Geo<D>::kKTileBytes,
+                         lds + Ring<D>::kV0 + s0 * Geo<D>::kVTileBytes - Geo<D>::kKTileBytes, gm, qf, s, pb, st, ones);
+            const ListEntry e4 = entry_at(t + 4);
+            // K(t + 3) and V(t + 2) into stages last read in interval t - 1
+            load_k(s0, block3);
+            load_v(s2, block2);
+            if (grp == 1) {
+                __builtin_amdgcn_s_waitcnt(vmcnt_imm(kLoadsPerTile));
+                wg_barrier();
+            }
+            softmax(t + 1, scale1, std::false_type{});
+            block2 = block3, block3 = block_of(e4);
+            scale1 = scale2, scale2 = scale3, scale3 = uniform(e4.scale);
+            const int free = s0;
+            s0 = s1, s1 = s2, s2 = free;
+            if (grp == 0) {
+                __builtin_amdgcn_s_waitcnt(vmcnt_imm(kLoadsPerTile));
+                wg_barrier();
+            }
+        }
+        // Masked tiles, the last tile, and intervals that only the other group
+        // still has work for.
+#pragma clang loop unroll(disable)
+        for (int t = main_steps; t < most; ++t) {
+            if (t < n) {
+                const int8_t *vst = lds + Ring<D>::kV0 + (t % kRing) * Geo<D>::kVTileBytes - Geo<D>::kKTileBytes;
+                if (t + 1 < n) qk_tile(lds + (t + 1) % kRing * Geo<D>::kKTileBytes, gm, qf, s);
+                const int from = k_end - block_of(list[t]) * kBKey;  // valid keys of tile t
+                if (from >= kBKey) pv_tile(vst, gm, pb, st, ones);
+                else pv_tail(vst, gm, pb, st, ones, from, g);
+                load_k(t % kRing, block_of(entry_at(t + 3)));
+                load_v((t + 2) % kRing, block_of(entry_at(t + 2)));
+            }
+            if (grp == 1) {
+                __builtin_amdgcn_s_waitcnt(vmcnt_imm(kLoadsPerTile));
+                wg_barrier();
+            }
+            if (t + 1 < n) softmax(t + 1, list[t + 1].scale, std::true_type{});
+            if (grp == 0) {
+                __builtin_amdgcn_s_waitcnt(vmcnt_imm(kLoadsPerTile));
+                wg_barrier();
+            }
         }
         __builtin_amdgcn_s_waitcnt(vmcnt_imm(0));
         __syncthreads();
     }
 
+    if (idle) return;
     // acc_o[ds][qt][r] = O[q0 + 16 qt + lc][16 ds + 4 g + r]; acc_l[qt][*] = l.
     if constexpr (kSplit) {
         const int64_t rows = static_cast<int64_t>(plan.bh) * lq;
@@ -386,7 +477,7 @@ __global__ __launch_bounds__(256) void block_merge_kernel(const float *__restric
     reinterpret_cast<u32x2 *>(dst)[1] = hi;
 }
 
-// Ranges of a list: as many as fill two workgroups a CU, of at least four
+// Ranges of a list: as many as give every CU its two units, of at least four
 // entries each.
 BlockPlan block_plan(int64_t batch, int64_t hq, int64_t lq, int64_t width, int64_t cus, int64_t max_parts) {
     BlockPlan p{};
@@ -446,7 +537,7 @@ extern "C" int32_t tu_sage_block_attn(const int8_t *q8, const float *q_scale, in
     const int64_t per_part = batch * hq * lq * (dim + 2) * static_cast<int64_t>(sizeof(float));
     const BlockPlan plan = block_plan(batch, hq, lq, width, cus,
                                       workspace ? std::min<int64_t>(64, workspace_bytes / per_part) : 1);
-    const int64_t grid = static_cast<int64_t>(plan.nqb) * plan.bh * plan.parts;
+    const int64_t grid = (static_cast<int64_t>(plan.nqb) * plan.bh * plan.parts + 1) / 2;
     TU_REQUIRE(batch * hq <= 65535 && grid <= 0x7fffffff / kBlockThreads, "block attention grid too large");
     if (require_gfx950()) return -1;
     int kscale_shift = 0;
