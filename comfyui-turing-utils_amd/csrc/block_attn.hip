@@ -11,23 +11,24 @@
 // sample's length, and rows that see no key, are zeros.
 //
 // MI355X mapping
-//   * A unit of work is 128 query rows with their list, or a range of it; a
-//     workgroup is two groups of 4 waves, a unit each, 32 rows a wave, so that
-//     every SIMD holds one wave of each group.  The groups share nothing but a
-//     barrier per tile, which keeps them in opposite phases: group 0 runs its
-//     MFMA cluster then its softmax, group 1 the softmax first.  (Two
-//     workgroups of one unit each fell into step, both in their MFMAs, then
-//     both in their softmax: 53 % MFMA busy, 3.29 ms at B1 H40 L32760 D128 with
-//     102 of 512 blocks.)
-//   * K and V^T tiles of a group stream through rings of three stages each.  A
-//     tile's K is used one interval before its V^T, so in interval t (QK of
-//     tile t + 1, PV of tile t) the loads of K(t + 3) and V^T(t + 2) start at
-//     once, into the stages that interval t - 1 read last, and have two
-//     intervals to land.
-//   * The list is compacted into LDS 256 entries at a time, with each block's
-//     scale beside it.
-//   * Few rows (a short grid) split their lists into ranges, a unit each,
-//     merged by a second kernel.
+//   * A unit of work is 128 query rows with their list, or a range of it: a
+//     workgroup of 4 waves, 32 rows a wave, one wave per SIMD.  Two workgroups
+//     share a CU (72 KiB of rings each at head_dim 128), and one's start-up and
+//     end, 10 us beside 1.4 us a tile and so most of a short list, runs beside
+//     the other's tiles.  (A persistent workgroup of two such groups with a
+//     common barrier, in opposite phases by construction, took 1.40 us a tile
+//     but stood still in both groups' start-ups: B1 H40 L32760 D128, 102 of 512
+//     blocks, 3.13 ms, and 85 us against 65 for lists of 16.)
+//   * Left alone the two fall into step, both in their MFMAs and then both in
+//     their softmax, so the wave in a SIMD's odd slot has the higher priority.
+//   * K and V^T tiles stream through rings of three stages each.  A tile's K is
+//     used one interval before its V^T, so in interval t (QK of tile t + 1, PV
+//     of tile t) the loads of K(t + 3) and V^T(t + 2) go into the stages that
+//     interval t - 1 read last, and have an interval to land.
+//   * The list is compacted into LDS 256 entries at a time, by every wave for
+//     itself (the same values), without a barrier.
+//   * Lists past the last full round of units, and those of a short grid, are
+//     split into ranges, a unit each, merged by a second kernel.
 #include <algorithm>
 
 #include "attn_common.h"
@@ -37,8 +38,7 @@
 namespace tu {
 namespace {
 
-constexpr int kGroupThreads = 256;
-constexpr int kBlockThreads = 2 * kGroupThreads;
+constexpr int kBlockThreads = 256;
 constexpr int kBlockRows = 128;
 constexpr int kRing = 3;
 constexpr int kSegment = 256;  // list entries compacted at a time
@@ -49,19 +49,20 @@ constexpr float kNoBase = -1e30f;
 constexpr float kLeastScale = 1e-18f;
 
 struct BlockPlan {
-    uint32_t nqb, bh;  // query blocks of a head, batch * hq
-    uint32_t width;    // entries of a list
-    uint32_t parts;    // ranges of a list
-    uint32_t per;      // entries of a range
+    uint32_t nqb;    // query blocks of a head
+    uint32_t blocks; // query blocks of all heads
+    uint32_t whole;  // of these, numbered head-major, run as one unit each; the later ones as `parts`
+    uint32_t width;  // entries of a list
+    uint32_t parts;  // ranges of a split list
+    uint32_t per;    // entries of a range
+    uint32_t rows;   // partial rows of a split query block
 };
 
 template <int D>
 struct Ring {
     static constexpr int kV0 = kRing * Geo<D>::kKTileBytes;  // V^T stages follow the K stages
     static constexpr int kList = kRing * Geo<D>::kStageBytes;  // the compacted entries follow the rings
-    static constexpr int kScan = kList + kSegment * 8;         // and the group's waves' counts
-    static constexpr int kGroup = (kScan + 3 * 4 * 4 + 1023) / 1024 * 1024;
-    static constexpr int kBytes = 2 * kGroup;
+    static constexpr int kBytes = kList + kSegment * 4;
 };
 
 // Loads of one tile's K rows, or its V^T columns, into a ring stage (the two
@@ -87,6 +88,11 @@ struct Ring {
     }
 TU_ISSUE(128)
 TU_ISSUE(64)
+// A tile's scale by a vector load whatever its address is: the waits of the
+// main loop count it beside the tile's loads.
+__device__ __forceinline__ float load_scale(__amdgpu_buffer_rsrc_t rs, int at) {
+    return __int_as_float(__builtin_amdgcn_raw_buffer_load_b32(rs, at * 4, 0, 0));
+}
 #undef TU_ISSUE
 #undef TU_ISSUE_K_BODY
 #undef TU_ISSUE_V_BODY
@@ -95,15 +101,9 @@ __device__ __forceinline__ int sample_end(const int32_t *lengths, uint32_t b, in
     return lengths ? min(max(lengths[b], 0), static_cast<int>(len)) : static_cast<int>(len);
 }
 
-// A tile of the compacted list.
-struct ListEntry {
-    int32_t block;
-    float scale;
-};
-
-// O^T += V^T P for a tile whose keys from `from` on (1 .. 63) are behind the
-// sample's end: their p is zero, but what stands there may be no number, so
-// their values are zeroed as well.
+// O^T += V^T P for a tile whose keys from `from` on may be behind the sample's
+// end: their p is zero, but what stands there may be no number, so their values
+// are zeroed as well.
 template <int D>
 __device__ __forceinline__ void pv_tail(const int8_t *stage, const LaneGeom<D> &gm, const bf16x8 (&p)[2][kQT],
                                         SoftmaxState<D> &st, const bf16x8 &ones, int from, int g) {
@@ -129,10 +129,42 @@ __device__ __forceinline__ void pv_tail(const int8_t *stage, const LaneGeom<D> &
     }
 }
 
-// kSplit: ranges of a list write the unnormalized O with each row's exponent
-// base and row sum to `part` for block_merge_kernel.
+// One list, or a range of it.
+struct Unit {
+    uint32_t bh, qb;  // batch * head, query block
+    int z;            // range of a split list, -1 for a whole one
+    int first, end;   // its entries
+};
+
+// Unit i of an XCD's sequence (its eighth of the whole lists, then of the
+// ranges of the others); end 0 past the last one.
+__device__ __forceinline__ Unit unit_at(const BlockPlan &p, uint32_t xcd, uint32_t i) {
+    auto chunk = [&](uint32_t n) { return n / 8 * xcd + min(n % 8, xcd); };
+    const uint32_t mine = p.whole / 8 + (xcd < p.whole % 8);
+    Unit u;
+    uint32_t block;
+    if (i < mine) {
+        block = chunk(p.whole) + i;
+        u.z = -1;
+        u.first = 0;
+        u.end = static_cast<int>(p.width);
+    } else {
+        const uint32_t ranges = (p.blocks - p.whole) * p.parts;
+        if (i - mine >= ranges / 8 + (xcd < ranges % 8)) return Unit{0, 0, 0, 0, 0};
+        const uint32_t v = chunk(ranges) + i - mine;
+        block = p.whole + v / p.parts;
+        u.z = static_cast<int>(v % p.parts);
+        u.first = u.z * static_cast<int>(p.per);
+        u.end = min(static_cast<int>(p.width), u.first + static_cast<int>(p.per));
+    }
+    u.bh = block / p.nqb;
+    u.qb = block % p.nqb;
+    return u;
+}
+// kSplit: some lists are split; a range writes the unnormalized O with each
+// row's exponent base and row sum to `part` for block_merge_kernel.
 template <int D, bool kCausal, bool kSplit>
-__global__ __launch_bounds__(kBlockThreads, 1) void block_attn_kernel(
+__global__ __launch_bounds__(kBlockThreads, 2) void block_attn_kernel(
     const int8_t *__restrict__ q8, const float *__restrict__ q_scale, uint32_t blkq, uint32_t nbq,
     const int8_t *__restrict__ k8, const float *__restrict__ k_scale, int kscale_shift, uint32_t nbk,
     const uint16_t *__restrict__ vt, const int32_t *__restrict__ index, uint16_t *__restrict__ o, uint32_t hq,
@@ -140,70 +172,89 @@ __global__ __launch_bounds__(kBlockThreads, 1) void block_attn_kernel(
     const int32_t *__restrict__ k_len, int64_t q_sb, int64_t q_sh, int64_t q_sl, int64_t k_sb, int64_t k_sh,
     int64_t k_sl, int64_t o_sb, int64_t o_sh, int64_t o_sl, float sm_log2, BlockPlan plan, float *__restrict__ part) {
     constexpr int kSl = Geo<D>::kKSlices;
-    constexpr int kLoadsPerTile = Geo<D>::kLoadsPerTile;
+    // a tile's loads, and the one of a later tile's scale beside them
+    constexpr int kLoads = Geo<D>::kLoadsPerTile + 1;
     // One array: with several the compiler waits for all direct-to-LDS loads
     // before a tile's fragment reads.
     __shared__ __align__(1024) int8_t lds_mem[Ring<D>::kBytes];
 
     const int lane = threadIdx.x & 63;
-    const int wave8 = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const int grp = wave8 >> 2;
-    const int wave = wave8 & 3;
-    const int tid = wave * 64 + lane;  // within the group
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int g = lane >> 4;
     const int lc = lane & 15;
-    int8_t *lds = lds_mem + grp * Ring<D>::kGroup;
-    auto *list = reinterpret_cast<ListEntry *>(lds + Ring<D>::kList);
-    auto *scan = reinterpret_cast<int(*)[4]>(lds + Ring<D>::kScan);
-    // Head-major numbering, a contiguous eighth per XCD: neighbouring query
-    // blocks of a head, whose lists are alike, share an L2.
-    const uint32_t units = plan.bh * plan.nqb * plan.parts;
-    uint32_t id = 2 * xcd_chunk(blockIdx.x, gridDim.x) + grp;
-    const bool idle = id >= units;  // the second group of an odd last pair
-    if (idle) id = units - 1;
-    uint32_t z = 0;
-    if constexpr (kSplit) {
-        z = id % plan.parts;
-        id /= plan.parts;
-    }
-    const uint32_t bh = id / plan.nqb, qb = id % plan.nqb;
-    const uint32_t b = bh / hq, h = bh % hq, hk = h / groups, hkv = hq / groups;
-    const int q_end = sample_end(q_len, b, lq), k_end = sample_end(k_len, b, lk);
-    const int64_t qblock0 = static_cast<int64_t>(qb) * kBlockRows;
-    const int64_t q0 = qblock0 + wave * kWaveQ;
+    int8_t *lds = lds_mem;
+    auto *list = reinterpret_cast<int *>(lds + Ring<D>::kList);
+    // the wave's slot in its SIMD (hardware id register, 4 bits from bit 0)
+    if (__builtin_amdgcn_s_getreg(4 | 3 << 11) & 1) __builtin_amdgcn_s_setprio(2);
 
-    const int8_t *qp = q8 + b * q_sb + h * q_sh;
+    // Each XCD owns a contiguous eighth of the head-major units: neighbouring
+    // query blocks of a head, whose lists are alike, share an L2.
+    const Unit cur = unit_at(plan, blockIdx.x & 7, blockIdx.x >> 3);
+    if (cur.end == 0) return;  // the grid is rounded up to the XCDs
+    const int32_t *entries = index + (static_cast<int64_t>(cur.bh) * plan.nqb + cur.qb) * plan.width;
+    // Entries `at` .. of the list, 4 a lane (-1 past the unit's end).
+    auto fetch = [&](int at, int (&e)[4]) {
+#pragma unroll
+        for (int c = 0; c < 4; ++c) {
+            const int i = at + 64 * c + lane;
+            e[c] = entries[min(i, static_cast<int>(plan.width) - 1)];
+            if (i >= cur.end) e[c] = -1;
+        }
+    };
+    int e[4];
+    fetch(cur.first, e);
+
+    const uint32_t b = cur.bh / hq, h = cur.bh % hq, hk = h / groups, hkv = hq / groups;
+    const int q_end = sample_end(q_len, b, lq), k_end = sample_end(k_len, b, lk);
+    const int64_t qblock0 = static_cast<int64_t>(cur.qb) * kBlockRows;
+    const int64_t q0 = qblock0 + wave * kWaveQ;
+    // blocks this query block can see at all, and the first that the sample's
+    // end or a diagonal cuts
+    int seen_end = k_end, masked_from = k_end / kBKey;
+    if constexpr (kCausal) {
+        seen_end = static_cast<int>(min<int64_t>(k_end, min<int64_t>(qblock0 + kBlockRows, q_end)));
+        masked_from = static_cast<int>(min<int64_t>(masked_from, qblock0 / kBKey));
+    }
+    const int blocks = qblock0 < q_end ? (seen_end + kBKey - 1) / kBKey : 0;
     const int8_t *kp = k8 + b * k_sb + hk * k_sh;
     const uint16_t *vtp = vt + static_cast<int64_t>(b * hkv + hk) * D * lpad;
     const float *ks_row = k_scale + static_cast<int64_t>(b * hkv + hk) * nbk;
-    const int32_t *entries = index + (static_cast<int64_t>(bh) * plan.nqb + qb) * plan.width;
-
-    // blocks this query block can see at all
-    int seen_end = k_end;
-    if constexpr (kCausal) seen_end = static_cast<int>(min<int64_t>(k_end, min<int64_t>(qblock0 + kBlockRows, q_end)));
-    const int blocks = qblock0 < q_end && !idle ? (seen_end + kBKey - 1) / kBKey : 0;
-    // the first block that the sample's end or a diagonal cuts
-    int masked_from = k_end / kBKey;
-    if constexpr (kCausal) masked_from = static_cast<int>(min<int64_t>(masked_from, qblock0 / kBKey));
-
-    const LaneGeom<D> gm = lane_geom<D>(wave, lane, k_sl, lpad);
+    const __amdgpu_buffer_rsrc_t srs = make_rsrc(ks_row, nbk * 4);
     const __amdgpu_buffer_rsrc_t krs = make_rsrc(kp, static_cast<uint32_t>(lk * k_sl));
     const __amdgpu_buffer_rsrc_t vrs = make_rsrc(vtp, static_cast<uint32_t>(D * lpad * 2));
+    const LaneGeom<D> gm = lane_geom<D>(wave, lane, k_sl, lpad);
     const uint32_t k_sl32 = static_cast<uint32_t>(k_sl);
+    // K of a tile, or its V^T, into a ring stage
+    auto load_k = [&](int stage, int block) {
+        issue_k(lds + stage * Geo<D>::kKTileBytes, krs, gm, k_sl32, block * kBKey, wave);
+    };
+    auto load_v = [&](int stage, int block) {
+        issue_v(lds + Ring<D>::kV0 + stage * Geo<D>::kVTileBytes, vrs, gm, block * kBKey, wave);
+    };
 
     i32x4 qf[kQT][kSl];
     float qsc[kQT];
+    {
+        const int8_t *qp = q8 + b * q_sb + h * q_sh;
 #pragma unroll
-    for (int qt = 0; qt < kQT; ++qt) {
-        const int64_t qi = min(q0 + 16 * qt + lc, lq - 1);
+        for (int qt = 0; qt < kQT; ++qt) {
+            const int64_t qi = min(q0 + 16 * qt + lc, lq - 1);
 #pragma unroll
-        for (int ds = 0; ds < kSl; ++ds)
-            qf[qt][ds] = *reinterpret_cast<const i32x4 *>(qp + qi * q_sl + 64 * ds + 16 * g);
-        qsc[qt] = fmaxf(q_scale[static_cast<int64_t>(bh) * nbq + static_cast<uint32_t>(qi) / blkq], kLeastScale) * sm_log2;
+            for (int ds = 0; ds < kSl; ++ds)
+                qf[qt][ds] = *reinterpret_cast<const i32x4 *>(qp + qi * q_sl + 64 * ds + 16 * g);
+            qsc[qt] = q_scale[static_cast<int64_t>(cur.bh) * nbq + static_cast<uint32_t>(qi) / blkq];
+        }
+    }
+    int before = -1;  // largest entry in front of the segment
+    if constexpr (kSplit) {
+        for (int i = lane; i < cur.first; i += 64) before = max(before, entries[i]);
+#pragma unroll
+        for (int d = 1; d < 64; d <<= 1) before = max(before, __shfl_xor(before, d));
     }
     SoftmaxState<D> st;
 #pragma unroll
     for (int qt = 0; qt < kQT; ++qt) {
+        qsc[qt] = fmaxf(qsc[qt], kLeastScale) * sm_log2;
         st.m_used[qt] = kNoBase;
         st.acc_l[qt] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
@@ -211,197 +262,147 @@ __global__ __launch_bounds__(kBlockThreads, 1) void block_attn_kernel(
     }
     bf16x8 ones;
 #pragma unroll
-    for (int e = 0; e < 8; ++e) ones[e] = static_cast<__bf16>(1.0f);
-
+    for (int i = 0; i < 8; ++i) ones[i] = static_cast<__bf16>(1.0f);
     i32x4 s[4][kQT];
     bf16x8 pb[2][kQT];
 
-    // first entry of this group's range, and the end of it.  Both groups walk
-    // as many segments and tiles as the longer one, for the barriers.
-    int first = 0;
-    const int per = static_cast<int>(plan.per);
-    int before = -1;  // largest entry in front of the next segment
-    if constexpr (kSplit) {
-        first = static_cast<int>(z) * per;
-        int m = -1;
-        for (int i = tid; i < first; i += kGroupThreads) m = max(m, entries[i]);
+    for (int seg = cur.first; seg < cur.end; seg += kSegment) {
+        if (seg > cur.first) fetch(seg, e);
+        // Compaction of the segment.  Ascending lists with nothing but -1 behind
+        // them need no running maximum.
+        bool ordered = true;
+        int prev[4];
 #pragma unroll
-        for (int d = 1; d < 64; d <<= 1) m = max(m, __shfl_xor(m, d));
-        if (lane == 0) scan[0][wave] = m;
-        __syncthreads();
-#pragma unroll
-        for (int w = 0; w < 4; ++w) before = max(before, scan[0][w]);
-        __syncthreads();
-    }
-    const int end = min(static_cast<int>(plan.width), first + per);
-
-    for (int seg = 0; seg < per; seg += kSegment) {
-        // Compaction of the next 256 entries: an inclusive running maximum over
-        // the group's threads, then the rank among the entries that count.
-        const int at = first + seg + tid;
-        const int e = at < end ? entries[at] : -1;
-        int top = e;
-#pragma unroll
-        for (int d = 1; d < 64; d <<= 1) {
-            const int other = __shfl_up(top, d);
-            if (lane >= d) top = max(top, other);
+        for (int c = 0; c < 4; ++c) {
+            prev[c] = __shfl_up(e[c], 1);
+            const int last = c ? __builtin_amdgcn_readlane(e[c - (c > 0)], 63) : before;
+            if (lane == 0) prev[c] = last;
+            ordered = ordered && (e[c] < 0 || (e[c] > prev[c] && (prev[c] >= 0 || (c == 0 && lane == 0))));
         }
-        if (lane == 63) scan[0][wave] = top;
-        int prev = __shfl_up(top, 1);
-        if (lane == 0) prev = -1;
-        __syncthreads();
-        prev = max(prev, before);
+        if (!__all(ordered)) {
+            int top = before;
 #pragma unroll
-        for (int w = 0; w < 4; ++w) {
-            if (w < wave) prev = max(prev, scan[0][w]);
-            before = max(before, scan[0][w]);
-        }
-        const bool counts = e > prev && e < blocks;
-        const uint64_t mask = __ballot(counts);
-        // tiles with masked keys stand last, as the list ascends
-        const uint64_t plain = __ballot(counts && e < masked_from);
-        if (lane == 0) {
-            scan[1][wave] = __builtin_popcountll(mask);
-            scan[2][wave] = __builtin_popcountll(plain);
-        }
-        __syncthreads();
-        int rank = __builtin_popcountll(mask & ((1ull << lane) - 1)), n = 0, whole = 0;
+            for (int c = 0; c < 4; ++c) {
+                int m = e[c];
 #pragma unroll
-        for (int w = 0; w < 4; ++w) {
-            if (w < wave) rank += scan[1][w];
-            n += scan[1][w];
-            whole += scan[2][w];
+                for (int d = 1; d < 64; d <<= 1) {
+                    const int other = __shfl_up(m, d);
+                    if (lane >= d) m = max(m, other);
+                }
+                prev[c] = __shfl_up(m, 1);
+                prev[c] = lane == 0 ? top : max(prev[c], top);
+                top = max(top, __builtin_amdgcn_readlane(m, 63));
+            }
         }
-        if (counts) list[rank] = ListEntry{e, fmaxf(ks_row[e >> kscale_shift], kLeastScale)};
-        // the other group's tiles, for the barriers
-        const auto *theirs = reinterpret_cast<const int *>(lds_mem + (1 - grp) * Ring<D>::kGroup + Ring<D>::kScan) + 4;
-        int most = theirs[0] + theirs[1] + theirs[2] + theirs[3];
+        int n = 0, whole = 0, top = before;
+#pragma unroll
+        for (int c = 0; c < 4; ++c) {
+            const bool counts = e[c] > prev[c] && e[c] >= 0 && e[c] < blocks;
+            const uint64_t mask = __ballot(counts);
+            if (counts) list[n + __builtin_popcountll(mask & ((1ull << lane) - 1))] = e[c];
+            n += __builtin_popcountll(mask);
+            // tiles with masked keys stand last, as the list ascends
+            whole += __builtin_popcountll(__ballot(counts && e[c] < masked_from));
+            top = max(top, e[c]);
+        }
         n = __builtin_amdgcn_readfirstlane(n);
         whole = __builtin_amdgcn_readfirstlane(whole);
-        most = __builtin_amdgcn_readfirstlane(max(n, most));
-        __syncthreads();
-        if (most == 0) continue;
 
-        auto entry_at = [&](int t) { return list[min(t, n - 1)]; };
-        auto block_of = [&](const ListEntry &le) { return __builtin_amdgcn_readfirstlane(le.block); };
+        auto block_at = [&](int t) { return __builtin_amdgcn_readfirstlane(list[min(t, n - 1)]); };
+#pragma unroll
+        for (int d = 1; d < 64; d <<= 1) top = max(top, __shfl_xor(top, d));
+        before = top;
+        if (n == 0) continue;
+
         auto softmax = [&](int t, float scale, auto mask_tag) {
             float f[kQT];
 #pragma unroll
             for (int qt = 0; qt < kQT; ++qt) f[qt] = qsc[qt] * scale;
             if (decltype(mask_tag)::value && t >= whole) {
-                const int key0 = block_of(list[t]) * kBKey;
+                const int key0 = block_at(t) * kBKey;
                 const int key_lim = min(k_end - key0, kBKey);
                 const int q_rel = static_cast<int>(max(min(q0 - key0, static_cast<int64_t>(kBKey)), static_cast<int64_t>(-kBlockRows)));
                 mask_tile<kCausal>(s, key_lim, q_rel, g, lc);
             }
             softmax_tile(s, f, st, pb);
         };
-        // K of a tile, or its V^T, into a ring stage
-        auto load_k = [&](int stage, int block) {
-            issue_k(lds + stage * Geo<D>::kKTileBytes, krs, gm, k_sl32, block * kBKey, wave);
+        auto uniform = [](float x) {
+            return fmaxf(__int_as_float(__builtin_amdgcn_readfirstlane(__float_as_int(x))), kLeastScale);
         };
-        auto load_v = [&](int stage, int block) {
-            issue_v(lds + Ring<D>::kV0 + stage * Geo<D>::kVTileBytes, vrs, gm, block * kBKey, wave);
-        };
-
-        // block2, block3: blocks of tiles t + 2 and t + 3; scale1 .. 3: scales
-        // of tiles t + 1 .. t + 3
-        int block2 = 0, block3 = 0;
-        float scale1 = 0.0f, scale2 = 0.0f, scale3 = 0.0f;
-        auto uniform = [](float x) { return __int_as_float(__builtin_amdgcn_readfirstlane(__float_as_int(x))); };
-        if (n > 0) {
-            // K(0), V(0), K(1), V(1), K(2) in flight; tile 0 and K(1) land first
-            const ListEntry e0 = entry_at(0), e1 = entry_at(1), e2 = entry_at(2), e3 = entry_at(3);
-            load_k(0, block_of(e0));
-            load_v(0, block_of(e0));
-            load_k(1, block_of(e1));
-            load_v(1, block_of(e1));
-            block2 = block_of(e2), block3 = block_of(e3);
-            scale1 = uniform(e1.scale), scale2 = uniform(e2.scale), scale3 = uniform(e3.scale);
-            load_k(2, block2);
-            __builtin_amdgcn_s_waitcnt(vmcnt_imm(kLoadsPerTile));
-        }
+        // scale1 .. 3: scales of tiles t + 1 .. t + 3; block2, block3: blocks of
+        // tiles t + 2 and t + 3
+        const int block0 = block_at(0), block1 = block_at(1);
+        int block2 = block_at(2), block3 = block_at(3);
+        float scale0 = load_scale(srs, block0 >> kscale_shift), scale1 = load_scale(srs, block1 >> kscale_shift);
+        float scale2 = load_scale(srs, block2 >> kscale_shift), scale3 = load_scale(srs, block3 >> kscale_shift);
+        load_k(0, block0);
+        load_v(0, block0);
+        load_k(1, block1);
+        load_v(1, block1);
+        load_k(2, block2);
+        // K(0), V(0), K(1) land, and with them every older load
+        __builtin_amdgcn_s_waitcnt(vmcnt_imm(Geo<D>::kLoadsPerTile));
+        scale0 = uniform(scale0), scale1 = uniform(scale1), scale2 = uniform(scale2);
         wg_barrier();
-        if (n > 0) {
-            qk_tile(lds, gm, qf, s);
-            if (grp == 0) softmax(0, list[0].scale, std::true_type{});
-        }
-        wg_barrier();  // K(0)'s stage is free for K(3)
-        if (grp == 1 && n > 0) softmax(0, list[0].scale, std::true_type{});
+        qk_tile(lds, gm, qf, s);
+        softmax(0, scale0, std::true_type{});
         __builtin_amdgcn_s_waitcnt(lgkmcnt_imm(0));
-        // Interval t + 1: group 0 [M_t, softmax(t + 1)], group 1 [softmax(t),
-        // M_t] with M_t = {QK(t + 1), PV(t)}; the same sequence, group 1's
-        // barrier between its two halves.  Before it a wave waits for its loads
-        // of K(t + 2) and V(t + 1), issued an interval ago.
+        wg_barrier();  // K(0)'s stage is free for K(3)
+        // Interval t: QK of tile t + 1 and PV of tile t, then the softmax of
+        // tile t + 1.  At its end a wave waits for its loads of K(t + 2) and
+        // V(t + 1), issued an interval ago.
         const int main_steps = max(0, min(n, whole) - 1);
         int s0 = 0, s1 = 1, s2 = 2;  // stages of tiles t, t + 1, t + 2
 #pragma clang loop unroll(disable)
         for (int t = 0; t < main_steps; ++t) {
-            mfma_cluster(lds + s1 * Geo<D>::kKTileBytes,
-                         lds + Ring<D>::kV0 + s0 * Geo<D>::kVTileBytes - Geo<D>::kKTileBytes, gm, qf, s, pb, st, ones);
-            const ListEntry e4 = entry_at(t + 4);
+            mfma_cluster<D, false>(lds + s1 * Geo<D>::kKTileBytes,
+                                   lds + Ring<D>::kV0 + s0 * Geo<D>::kVTileBytes - Geo<D>::kKTileBytes, gm, qf, s, pb, st, ones);
+            const int e4 = list[min(t + 4, n - 1)];
             // K(t + 3) and V(t + 2) into stages last read in interval t - 1
             load_k(s0, block3);
             load_v(s2, block2);
-            if (grp == 1) {
-                __builtin_amdgcn_s_waitcnt(vmcnt_imm(kLoadsPerTile));
-                wg_barrier();
-            }
+            const float scale4 = load_scale(srs, e4 >> kscale_shift);
             softmax(t + 1, scale1, std::false_type{});
-            block2 = block3, block3 = block_of(e4);
-            scale1 = scale2, scale2 = scale3, scale3 = uniform(e4.scale);
+            block2 = block3, block3 = __builtin_amdgcn_readfirstlane(e4);
             const int free = s0;
             s0 = s1, s1 = s2, s2 = free;
-            if (grp == 0) {
-                __builtin_amdgcn_s_waitcnt(vmcnt_imm(kLoadsPerTile));
-                wg_barrier();
-            }
+            __builtin_amdgcn_s_waitcnt(vmcnt_imm(kLoads));
+            wg_barrier();
+            scale1 = scale2, scale2 = uniform(scale3), scale3 = scale4;
         }
-        // Masked tiles, the last tile, and intervals that only the other group
-        // still has work for.
+        // Masked tiles and the last one.
 #pragma clang loop unroll(disable)
-        for (int t = main_steps; t < most; ++t) {
-            if (t < n) {
-                const int8_t *vst = lds + Ring<D>::kV0 + (t % kRing) * Geo<D>::kVTileBytes - Geo<D>::kKTileBytes;
-                if (t + 1 < n) qk_tile(lds + (t + 1) % kRing * Geo<D>::kKTileBytes, gm, qf, s);
-                const int from = k_end - block_of(list[t]) * kBKey;  // valid keys of tile t
-                if (from >= kBKey) pv_tile(vst, gm, pb, st, ones);
-                else pv_tail(vst, gm, pb, st, ones, from, g);
-                load_k(t % kRing, block_of(entry_at(t + 3)));
-                load_v((t + 2) % kRing, block_of(entry_at(t + 2)));
-            }
-            if (grp == 1) {
-                __builtin_amdgcn_s_waitcnt(vmcnt_imm(kLoadsPerTile));
-                wg_barrier();
-            }
-            if (t + 1 < n) softmax(t + 1, list[t + 1].scale, std::true_type{});
-            if (grp == 0) {
-                __builtin_amdgcn_s_waitcnt(vmcnt_imm(kLoadsPerTile));
-                wg_barrier();
-            }
+        for (int t = main_steps; t < n; ++t) {
+            if (t + 3 < n) load_k(t % kRing, block_at(t + 3));
+            if (t + 2 < n) load_v((t + 2) % kRing, block_at(t + 2));
+            const int8_t *v = lds + Ring<D>::kV0 + (t % kRing) * Geo<D>::kVTileBytes - Geo<D>::kKTileBytes;
+            if (t + 1 < n) qk_tile(lds + (t + 1) % kRing * Geo<D>::kKTileBytes, gm, qf, s);
+            pv_tail(v, gm, pb, st, ones, k_end - block_at(t) * kBKey, g);
+            if (t + 1 < n)
+                softmax(t + 1, uniform(load_scale(srs, block_at(t + 1) >> kscale_shift)), std::true_type{});
+            __builtin_amdgcn_s_waitcnt(vmcnt_imm(0));
+            wg_barrier();
         }
-        __builtin_amdgcn_s_waitcnt(vmcnt_imm(0));
-        __syncthreads();
     }
 
-    if (idle) return;
     // acc_o[ds][qt][r] = O[q0 + 16 qt + lc][16 ds + 4 g + r]; acc_l[qt][*] = l.
-    if constexpr (kSplit) {
-        const int64_t rows = static_cast<int64_t>(plan.bh) * lq;
-        const int64_t row0 = z * rows + static_cast<int64_t>(bh) * lq;
+    if (kSplit && cur.z >= 0) {
+        // [parts][rows of the split blocks][D] fp32, then [..][2]
+        const int64_t rows = static_cast<int64_t>(plan.blocks - plan.whole) * plan.rows;
+        const int64_t row0 = cur.z * rows + static_cast<int64_t>(cur.bh * plan.nqb + cur.qb - plan.whole) * plan.rows +
+                             wave * kWaveQ;
         float *po = part + row0 * D;
         float *pml = part + plan.parts * rows * D + row0 * 2;
 #pragma unroll
         for (int qt = 0; qt < kQT; ++qt) {
-            const int64_t qi = q0 + 16 * qt + lc;
-            if (qi >= lq) continue;
+            const int r = 16 * qt + lc;
+            if (q0 + r >= lq) continue;
 #pragma unroll
             for (int ds = 0; ds < Geo<D>::kDS; ++ds)
-                *reinterpret_cast<f32x4 *>(po + qi * D + 16 * ds + 4 * g) = st.acc_o[ds][qt];
+                *reinterpret_cast<f32x4 *>(po + r * D + 16 * ds + 4 * g) = st.acc_o[ds][qt];
             // a row past its sample's end has seen nothing
-            if (g == 0)
-                *reinterpret_cast<f32x2 *>(pml + qi * 2) =
-                    f32x2{qi < q_end ? st.m_used[qt] : kNoBase, qi < q_end ? st.acc_l[qt][0] : 0.0f};
+            const bool in = q0 + r < q_end;
+            if (g == 0) *reinterpret_cast<f32x2 *>(pml + r * 2) = f32x2{in ? st.m_used[qt] : kNoBase, in ? st.acc_l[qt][0] : 0.0f};
         }
         return;
     }
@@ -437,33 +438,53 @@ __global__ __launch_bounds__(kBlockThreads, 1) void block_attn_kernel(
     }
 }
 
-// Merges the ranges of each row: M = max m_s, w_s = 2^(m_s - M),
+// Merges the ranges of the split lists' rows: M = max m_s, w_s = 2^(m_s - M),
 // out = sum w_s O_s / sum w_s l_s, zeros where no range saw a key.
 template <int D>
 __global__ __launch_bounds__(256) void block_merge_kernel(const float *__restrict__ part, BlockPlan plan, uint32_t hq,
                                                           int64_t lq, uint16_t *__restrict__ o, int64_t o_sb,
                                                           int64_t o_sh, int64_t o_sl) {
     constexpr int kTpr = D / 8;  // threads per row, 8 channels each
+    constexpr int kAhead = 8;    // ranges whose loads are in flight together
     const int64_t row = static_cast<int64_t>(blockIdx.x) * (256 / kTpr) + threadIdx.x / kTpr;
     const int d0 = (threadIdx.x % kTpr) * 8;
-    const int64_t rows = static_cast<int64_t>(plan.bh) * lq;
+    const int64_t rows = static_cast<int64_t>(plan.blocks - plan.whole) * plan.rows;
     if (row >= rows) return;
-    const int64_t bh = row / lq, q = row - bh * lq;
+    const uint32_t block = plan.whole + static_cast<uint32_t>(row / plan.rows);
+    const uint32_t bh = block / plan.nqb;
+    const int64_t q = static_cast<int64_t>(block % plan.nqb) * kBlockRows + row % plan.rows;
+    if (q >= lq) return;
     const float *ml = part + plan.parts * rows * D;
-    float m = kNoBase;
-    for (uint32_t sp = 0; sp < plan.parts; ++sp) m = fmaxf(m, ml[(sp * rows + row) * 2]);
-    float l = 0.0f, acc[8] = {};
-    for (uint32_t sp = 0; sp < plan.parts; ++sp) {
-        const float ls = ml[(sp * rows + row) * 2 + 1];
-        if (!(ls > 0.0f)) continue;  // nothing seen in this range
-        const float w = __builtin_amdgcn_exp2f(ml[(sp * rows + row) * 2] - m);
-        l = __builtin_fmaf(w, ls, l);
-        const f32x4 *src = reinterpret_cast<const f32x4 *>(part + (sp * rows + row) * D + d0);
-        const f32x4 a = src[0], c = src[1];
+    const int parts = static_cast<int>(plan.parts);
+    float m = kNoBase, l = 0.0f, acc[8] = {};
+    for (int p0 = 0; p0 < parts; p0 += kAhead) {
+        f32x2 x[kAhead];
+        f32x4 a[kAhead], c[kAhead];
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-            acc[e] = __builtin_fmaf(w, a[e], acc[e]);
-            acc[4 + e] = __builtin_fmaf(w, c[e], acc[4 + e]);
+        for (int u = 0; u < kAhead; ++u) {
+            const int64_t at = min(p0 + u, parts - 1) * rows + row;
+            x[u] = *reinterpret_cast<const f32x2 *>(ml + at * 2);
+            a[u] = *reinterpret_cast<const f32x4 *>(part + at * D + d0);
+            c[u] = *reinterpret_cast<const f32x4 *>(part + at * D + d0 + 4);
+        }
+        float top = m;
+#pragma unroll
+        for (int u = 0; u < kAhead; ++u) top = fmaxf(top, x[u][0]);
+        const float old = __builtin_amdgcn_exp2f(m - top);
+        m = top;
+        l *= old;
+#pragma unroll
+        for (int k = 0; k < 8; ++k) acc[k] *= old;
+#pragma unroll
+        for (int u = 0; u < kAhead; ++u) {
+            if (p0 + u >= parts || !(x[u][1] > 0.0f)) continue;  // nothing seen in this range
+            const float w = __builtin_amdgcn_exp2f(x[u][0] - m);
+            l = __builtin_fmaf(w, x[u][1], l);
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+                acc[k] = __builtin_fmaf(w, a[u][k], acc[k]);
+                acc[4 + k] = __builtin_fmaf(w, c[u][k], acc[4 + k]);
+            }
         }
     }
     const float inv = l > 0.0f ? 1.0f / l : 0.0f;
@@ -477,22 +498,48 @@ __global__ __launch_bounds__(256) void block_merge_kernel(const float *__restric
     reinterpret_cast<u32x2 *>(dst)[1] = hi;
 }
 
-// Ranges of a list: as many as give every CU its two units, of at least four
-// entries each.
-BlockPlan block_plan(int64_t batch, int64_t hq, int64_t lq, int64_t width, int64_t cus, int64_t max_parts) {
-    BlockPlan p{};
-    p.nqb = static_cast<uint32_t>((lq + kBlockRows - 1) / kBlockRows);
-    p.bh = static_cast<uint32_t>(batch * hq);
-    p.width = static_cast<uint32_t>(width);
-    const int64_t blocks = static_cast<int64_t>(p.nqb) * p.bh;
-    int64_t parts = std::max<int64_t>(1, std::min({2 * cus / blocks, width / 4, max_parts}));
-    p.per = static_cast<uint32_t>((width + parts - 1) / parts);
-    p.parts = static_cast<uint32_t>((width + p.per - 1) / p.per);
-    return p;
+// Two units a CU run at a time.  Lists past the last full round of them are
+// split where that shortens the round, into ranges of at least four entries;
+// a round costs its tiles, a fixed part and, split, the partial rows and the
+// merge (in tiles of 1.4 us).
+constexpr double kUnitTiles = 2.5;
+constexpr double kMergeTiles = 4.0;
+
+int64_t block_workspace(const BlockPlan &p, int64_t dim) {
+    return p.parts > 1 ? static_cast<int64_t>(p.parts) * (p.blocks - p.whole) * p.rows * (dim + 2) *
+                             static_cast<int64_t>(sizeof(float))
+                       : 0;
 }
 
-int64_t block_workspace(const BlockPlan &p, int64_t lq, int64_t dim) {
-    return p.parts > 1 ? static_cast<int64_t>(p.parts) * p.bh * lq * (dim + 2) * static_cast<int64_t>(sizeof(float)) : 0;
+BlockPlan block_plan(int64_t batch, int64_t hq, int64_t lq, int64_t dim, int64_t width, int64_t cus, int64_t max_bytes) {
+    BlockPlan p{};
+    p.nqb = static_cast<uint32_t>((lq + kBlockRows - 1) / kBlockRows);
+    p.blocks = static_cast<uint32_t>(batch * hq * p.nqb);
+    p.rows = static_cast<uint32_t>(std::min<int64_t>(lq, kBlockRows));
+    p.width = static_cast<uint32_t>(width);
+    p.whole = p.blocks;
+    p.parts = 1;
+    p.per = p.width;
+    const int64_t slots = 2 * cus, rest = p.blocks % slots;
+    double best = static_cast<double>(width) + kUnitTiles;
+    for (int64_t parts = 2; rest > 0 && parts <= 64; ++parts) {
+        const int64_t per = (width + parts - 1) / parts;
+        if (per < 4) break;
+        if ((width + per - 1) / per != parts) continue;
+        BlockPlan c = p;
+        c.whole = static_cast<uint32_t>(p.blocks - rest);
+        c.parts = static_cast<uint32_t>(parts);
+        c.per = static_cast<uint32_t>(per);
+        if (block_workspace(c, dim) > max_bytes) break;
+        const double cost = static_cast<double>((rest * parts + slots - 1) / slots) * (per + kUnitTiles) + kMergeTiles;
+        if (cost < best) {
+            best = cost;
+            p.whole = c.whole;
+            p.parts = c.parts;
+            p.per = c.per;
+        }
+    }
+    return p;
 }
 
 }  // namespace
@@ -502,7 +549,7 @@ extern "C" int64_t tu_sage_block_attn_workspace(int64_t batch, int64_t hq, int64
                                                 int32_t cus) {
     using namespace tu;
     if (batch <= 0 || hq <= 0 || lq <= 0 || dim <= 0 || width <= 0 || cus <= 0) return 0;
-    return block_workspace(block_plan(batch, hq, lq, width, cus, 64), lq, dim);
+    return block_workspace(block_plan(batch, hq, lq, dim, width, cus, INT64_MAX), dim);
 }
 
 extern "C" int32_t tu_sage_block_attn(const int8_t *q8, const float *q_scale, int64_t blkq, const int8_t *k8,
@@ -534,18 +581,18 @@ extern "C" int32_t tu_sage_block_attn(const int8_t *q8, const float *q_scale, in
                    (reinterpret_cast<uintptr_t>(o_bf16) & 7) == 0,
                "block attention V^T/O must be aligned");
     TU_REQUIRE((reinterpret_cast<uintptr_t>(workspace) & 15) == 0, "block attention workspace must be 16-byte aligned");
-    const int64_t per_part = batch * hq * lq * (dim + 2) * static_cast<int64_t>(sizeof(float));
-    const BlockPlan plan = block_plan(batch, hq, lq, width, cus,
-                                      workspace ? std::min<int64_t>(64, workspace_bytes / per_part) : 1);
-    const int64_t grid = (static_cast<int64_t>(plan.nqb) * plan.bh * plan.parts + 1) / 2;
-    TU_REQUIRE(batch * hq <= 65535 && grid <= 0x7fffffff / kBlockThreads, "block attention grid too large");
+    TU_REQUIRE(batch * hq <= 65535 && batch * hq * ((lq + kBlockRows - 1) / kBlockRows) <= 0x1fffffff,
+               "block attention grid too large");
+    const BlockPlan plan = block_plan(batch, hq, lq, dim, width, cus, workspace ? workspace_bytes : 0);
+    // an eighth of the whole lists and of the ranges each, rounded up, for every XCD
+    const unsigned grid = 8 * ((plan.whole + 7) / 8 + ((plan.blocks - plan.whole) * plan.parts + 7) / 8);
     if (require_gfx950()) return -1;
     int kscale_shift = 0;
     while ((kBKey << kscale_shift) < blkk) ++kscale_shift;
     auto *part = static_cast<float *>(workspace);
     hipStream_t st = static_cast<hipStream_t>(stream);
 #define TU_BLOCK_ATTN(D, CAUSAL, SPLIT)                                                                                \
-    block_attn_kernel<D, CAUSAL, SPLIT><<<dim3(static_cast<unsigned>(grid)), kBlockThreads, 0, st>>>(                  \
+    block_attn_kernel<D, CAUSAL, SPLIT><<<dim3(grid), kBlockThreads, 0, st>>>(                                              \
         q8, q_scale, static_cast<uint32_t>(blkq), static_cast<uint32_t>((lq + blkq - 1) / blkq), k8, k_scale,          \
         kscale_shift, static_cast<uint32_t>((lk + blkk - 1) / blkk), static_cast<const uint16_t *>(vt_bf16), index,    \
         static_cast<uint16_t *>(o_bf16), static_cast<uint32_t>(hq), static_cast<uint32_t>(hq / hkv), lq, lk, lpad,     \
@@ -556,9 +603,9 @@ extern "C" int32_t tu_sage_block_attn(const int8_t *q8, const float *q_scale, in
             if (causal) TU_BLOCK_ATTN(D, true, true);                                                                  \
             else TU_BLOCK_ATTN(D, false, true);                                                                        \
             constexpr int kRowsPerWg = 256 / (D / 8);                                                                  \
-            block_merge_kernel<D><<<dim3(static_cast<unsigned>((batch * hq * lq + kRowsPerWg - 1) / kRowsPerWg)), 256, \
-                                    0, st>>>(part, plan, static_cast<uint32_t>(hq), lq,                                \
-                                             static_cast<uint16_t *>(o_bf16), o_sb, o_sh, o_sl);                       \
+            const int64_t rows = static_cast<int64_t>(plan.blocks - plan.whole) * plan.rows;                           \
+            block_merge_kernel<D><<<dim3(static_cast<unsigned>((rows + kRowsPerWg - 1) / kRowsPerWg)), 256, 0, st>>>(  \
+                part, plan, static_cast<uint32_t>(hq), lq, static_cast<uint16_t *>(o_bf16), o_sb, o_sh, o_sl);         \
         } else if (causal) {                                                                                           \
             TU_BLOCK_ATTN(D, true, false);                                                                             \
         } else {                                                                                                       \
