@@ -19,16 +19,16 @@
 //     common barrier, in opposite phases by construction, took 1.40 us a tile
 //     but stood still in both groups' start-ups: B1 H40 L32760 D128, 102 of 512
 //     blocks, 3.13 ms, and 85 us against 65 for lists of 16.)
-//   * Left alone the two fall into step, both in their MFMAs and then both in
-//     their softmax, so the wave in a SIMD's odd slot has the higher priority.
+//   * The MFMA cluster has priority over the other workgroup's softmax, as in
+//     the dense kernel: 3.00 ms at that shape, 3.07 without.
 //   * K and V^T tiles stream through rings of three stages each.  A tile's K is
 //     used one interval before its V^T, so in interval t (QK of tile t + 1, PV
 //     of tile t) the loads of K(t + 3) and V^T(t + 2) go into the stages that
 //     interval t - 1 read last, and have an interval to land.
 //   * The list is compacted into LDS 256 entries at a time, by every wave for
 //     itself (the same values), without a barrier.
-//   * Lists past the last full round of units, and those of a short grid, are
-//     split into ranges, a unit each, merged by a second kernel.
+//   * A grid that leaves workgroups' places empty splits its lists into
+//     ranges, a unit each, merged by a second kernel.
 #include <algorithm>
 
 #include "attn_common.h"
@@ -51,11 +51,10 @@ constexpr float kLeastScale = 1e-18f;
 struct BlockPlan {
     uint32_t nqb;    // query blocks of a head
     uint32_t blocks; // query blocks of all heads
-    uint32_t whole;  // of these, numbered head-major, run as one unit each; the later ones as `parts`
     uint32_t width;  // entries of a list
-    uint32_t parts;  // ranges of a split list
+    uint32_t parts;  // ranges of a list, a unit each
     uint32_t per;    // entries of a range
-    uint32_t rows;   // partial rows of a split query block
+    uint32_t rows;   // partial rows of a query block
 };
 
 template <int D>
@@ -129,42 +128,15 @@ __device__ __forceinline__ void pv_tail(const int8_t *stage, const LaneGeom<D> &
     }
 }
 
-// One list, or a range of it.
-struct Unit {
-    uint32_t bh, qb;  // batch * head, query block
-    int z;            // range of a split list, -1 for a whole one
-    int first, end;   // its entries
-};
+// kSplit: a range of a list writes the unnormalized O with each row's exponent
+// base and row sum to `part` for block_merge_kernel.
+// Workgroups of a CU: 2 fill the LDS at head_dim 128; at 64, 3 fill the
+// registers (4 spill: 82 us for 53 at B2 H9 L6000 with 24 of 94 blocks).
+template <int D>
+constexpr int kWgsPerCu = D == 64 ? 3 : 2;
 
-// Unit i of an XCD's sequence (its eighth of the whole lists, then of the
-// ranges of the others); end 0 past the last one.
-__device__ __forceinline__ Unit unit_at(const BlockPlan &p, uint32_t xcd, uint32_t i) {
-    auto chunk = [&](uint32_t n) { return n / 8 * xcd + min(n % 8, xcd); };
-    const uint32_t mine = p.whole / 8 + (xcd < p.whole % 8);
-    Unit u;
-    uint32_t block;
-    if (i < mine) {
-        block = chunk(p.whole) + i;
-        u.z = -1;
-        u.first = 0;
-        u.end = static_cast<int>(p.width);
-    } else {
-        const uint32_t ranges = (p.blocks - p.whole) * p.parts;
-        if (i - mine >= ranges / 8 + (xcd < ranges % 8)) return Unit{0, 0, 0, 0, 0};
-        const uint32_t v = chunk(ranges) + i - mine;
-        block = p.whole + v / p.parts;
-        u.z = static_cast<int>(v % p.parts);
-        u.first = u.z * static_cast<int>(p.per);
-        u.end = min(static_cast<int>(p.width), u.first + static_cast<int>(p.per));
-    }
-    u.bh = block / p.nqb;
-    u.qb = block % p.nqb;
-    return u;
-}
-// kSplit: some lists are split; a range writes the unnormalized O with each
-// row's exponent base and row sum to `part` for block_merge_kernel.
 template <int D, bool kCausal, bool kSplit>
-__global__ __launch_bounds__(kBlockThreads, 2) void block_attn_kernel(
+__global__ __launch_bounds__(kBlockThreads, kWgsPerCu<D>) void block_attn_kernel(
     const int8_t *__restrict__ q8, const float *__restrict__ q_scale, uint32_t blkq, uint32_t nbq,
     const int8_t *__restrict__ k8, const float *__restrict__ k_scale, int kscale_shift, uint32_t nbk,
     const uint16_t *__restrict__ vt, const int32_t *__restrict__ index, uint16_t *__restrict__ o, uint32_t hq,
@@ -184,29 +156,32 @@ __global__ __launch_bounds__(kBlockThreads, 2) void block_attn_kernel(
     const int lc = lane & 15;
     int8_t *lds = lds_mem;
     auto *list = reinterpret_cast<int *>(lds + Ring<D>::kList);
-    // the wave's slot in its SIMD (hardware id register, 4 bits from bit 0)
-    if (__builtin_amdgcn_s_getreg(4 | 3 << 11) & 1) __builtin_amdgcn_s_setprio(2);
-
     // Each XCD owns a contiguous eighth of the head-major units: neighbouring
     // query blocks of a head, whose lists are alike, share an L2.
-    const Unit cur = unit_at(plan, blockIdx.x & 7, blockIdx.x >> 3);
-    if (cur.end == 0) return;  // the grid is rounded up to the XCDs
-    const int32_t *entries = index + (static_cast<int64_t>(cur.bh) * plan.nqb + cur.qb) * plan.width;
+    uint32_t id = xcd_chunk(blockIdx.x, gridDim.x), z = 0;
+    if constexpr (kSplit) {
+        z = id % plan.parts;
+        id /= plan.parts;
+    }
+    const uint32_t bh = id / plan.nqb, qb = id % plan.nqb;
+    const int first = static_cast<int>(z * plan.per);
+    const int end = min(static_cast<int>(plan.width), first + static_cast<int>(plan.per));
+    const int32_t *entries = index + (static_cast<int64_t>(bh) * plan.nqb + qb) * plan.width;
     // Entries `at` .. of the list, 4 a lane (-1 past the unit's end).
     auto fetch = [&](int at, int (&e)[4]) {
 #pragma unroll
         for (int c = 0; c < 4; ++c) {
             const int i = at + 64 * c + lane;
             e[c] = entries[min(i, static_cast<int>(plan.width) - 1)];
-            if (i >= cur.end) e[c] = -1;
+            if (i >= end) e[c] = -1;
         }
     };
     int e[4];
-    fetch(cur.first, e);
+    fetch(first, e);
 
-    const uint32_t b = cur.bh / hq, h = cur.bh % hq, hk = h / groups, hkv = hq / groups;
+    const uint32_t b = bh / hq, h = bh % hq, hk = h / groups, hkv = hq / groups;
     const int q_end = sample_end(q_len, b, lq), k_end = sample_end(k_len, b, lk);
-    const int64_t qblock0 = static_cast<int64_t>(cur.qb) * kBlockRows;
+    const int64_t qblock0 = static_cast<int64_t>(qb) * kBlockRows;
     const int64_t q0 = qblock0 + wave * kWaveQ;
     // blocks this query block can see at all, and the first that the sample's
     // end or a diagonal cuts
@@ -242,12 +217,12 @@ __global__ __launch_bounds__(kBlockThreads, 2) void block_attn_kernel(
 #pragma unroll
             for (int ds = 0; ds < kSl; ++ds)
                 qf[qt][ds] = *reinterpret_cast<const i32x4 *>(qp + qi * q_sl + 64 * ds + 16 * g);
-            qsc[qt] = q_scale[static_cast<int64_t>(cur.bh) * nbq + static_cast<uint32_t>(qi) / blkq];
+            qsc[qt] = q_scale[static_cast<int64_t>(bh) * nbq + static_cast<uint32_t>(qi) / blkq];
         }
     }
     int before = -1;  // largest entry in front of the segment
     if constexpr (kSplit) {
-        for (int i = lane; i < cur.first; i += 64) before = max(before, entries[i]);
+        for (int i = lane; i < first; i += 64) before = max(before, entries[i]);
 #pragma unroll
         for (int d = 1; d < 64; d <<= 1) before = max(before, __shfl_xor(before, d));
     }
@@ -266,8 +241,8 @@ __global__ __launch_bounds__(kBlockThreads, 2) void block_attn_kernel(
     i32x4 s[4][kQT];
     bf16x8 pb[2][kQT];
 
-    for (int seg = cur.first; seg < cur.end; seg += kSegment) {
-        if (seg > cur.first) fetch(seg, e);
+    for (int seg = first; seg < end; seg += kSegment) {
+        if (seg > first) fetch(seg, e);
         // Compaction of the segment.  Ascending lists with nothing but -1 behind
         // them need no running maximum.
         bool ordered = true;
@@ -355,8 +330,8 @@ __global__ __launch_bounds__(kBlockThreads, 2) void block_attn_kernel(
         int s0 = 0, s1 = 1, s2 = 2;  // stages of tiles t, t + 1, t + 2
 #pragma clang loop unroll(disable)
         for (int t = 0; t < main_steps; ++t) {
-            mfma_cluster<D, false>(lds + s1 * Geo<D>::kKTileBytes,
-                                   lds + Ring<D>::kV0 + s0 * Geo<D>::kVTileBytes - Geo<D>::kKTileBytes, gm, qf, s, pb, st, ones);
+            mfma_cluster(lds + s1 * Geo<D>::kKTileBytes,
+                         lds + Ring<D>::kV0 + s0 * Geo<D>::kVTileBytes - Geo<D>::kKTileBytes, gm, qf, s, pb, st, ones);
             const int e4 = list[min(t + 4, n - 1)];
             // K(t + 3) and V(t + 2) into stages last read in interval t - 1
             load_k(s0, block3);
@@ -386,11 +361,10 @@ __global__ __launch_bounds__(kBlockThreads, 2) void block_attn_kernel(
     }
 
     // acc_o[ds][qt][r] = O[q0 + 16 qt + lc][16 ds + 4 g + r]; acc_l[qt][*] = l.
-    if (kSplit && cur.z >= 0) {
-        // [parts][rows of the split blocks][D] fp32, then [..][2]
-        const int64_t rows = static_cast<int64_t>(plan.blocks - plan.whole) * plan.rows;
-        const int64_t row0 = cur.z * rows + static_cast<int64_t>(cur.bh * plan.nqb + cur.qb - plan.whole) * plan.rows +
-                             wave * kWaveQ;
+    if constexpr (kSplit) {
+        // [parts][rows][D] fp32, then [parts][rows][2]
+        const int64_t rows = static_cast<int64_t>(plan.blocks) * plan.rows;
+        const int64_t row0 = z * rows + static_cast<int64_t>(id) * plan.rows + wave * kWaveQ;
         float *po = part + row0 * D;
         float *pml = part + plan.parts * rows * D + row0 * 2;
 #pragma unroll
@@ -438,7 +412,7 @@ __global__ __launch_bounds__(kBlockThreads, 2) void block_attn_kernel(
     }
 }
 
-// Merges the ranges of the split lists' rows: M = max m_s, w_s = 2^(m_s - M),
+// Merges the ranges of each row: M = max m_s, w_s = 2^(m_s - M),
 // out = sum w_s O_s / sum w_s l_s, zeros where no range saw a key.
 template <int D>
 __global__ __launch_bounds__(256) void block_merge_kernel(const float *__restrict__ part, BlockPlan plan, uint32_t hq,
@@ -448,9 +422,9 @@ __global__ __launch_bounds__(256) void block_merge_kernel(const float *__restric
     constexpr int kAhead = 8;    // ranges whose loads are in flight together
     const int64_t row = static_cast<int64_t>(blockIdx.x) * (256 / kTpr) + threadIdx.x / kTpr;
     const int d0 = (threadIdx.x % kTpr) * 8;
-    const int64_t rows = static_cast<int64_t>(plan.blocks - plan.whole) * plan.rows;
+    const int64_t rows = static_cast<int64_t>(plan.blocks) * plan.rows;
     if (row >= rows) return;
-    const uint32_t block = plan.whole + static_cast<uint32_t>(row / plan.rows);
+    const uint32_t block = static_cast<uint32_t>(row / plan.rows);
     const uint32_t bh = block / plan.nqb;
     const int64_t q = static_cast<int64_t>(block % plan.nqb) * kBlockRows + row % plan.rows;
     if (q >= lq) return;
@@ -498,15 +472,16 @@ __global__ __launch_bounds__(256) void block_merge_kernel(const float *__restric
     reinterpret_cast<u32x2 *>(dst)[1] = hi;
 }
 
-// Two units a CU run at a time.  Lists past the last full round of them are
-// split where that shortens the round, into ranges of at least four entries;
-// a round costs its tiles, a fixed part and, split, the partial rows and the
-// merge (in tiles of 1.4 us).
-constexpr double kUnitTiles = 2.5;
+// Lists are split where the grid leaves places empty, into ranges of at least
+// four entries: a round of units costs their tiles and a fixed part, and split
+// the merge (in tiles of 1.4 us).  Splitting only the lists past a full round
+// did not pay: a unit that has its CU to itself is faster (B1 H12 L8190 D128,
+// 768 units: 97 us with the last 256 split, 87 without).
+constexpr double kUnitTiles = 5.0;
 constexpr double kMergeTiles = 4.0;
 
 int64_t block_workspace(const BlockPlan &p, int64_t dim) {
-    return p.parts > 1 ? static_cast<int64_t>(p.parts) * (p.blocks - p.whole) * p.rows * (dim + 2) *
+    return p.parts > 1 ? static_cast<int64_t>(p.parts) * p.blocks * p.rows * (dim + 2) *
                              static_cast<int64_t>(sizeof(float))
                        : 0;
 }
@@ -517,24 +492,21 @@ BlockPlan block_plan(int64_t batch, int64_t hq, int64_t lq, int64_t dim, int64_t
     p.blocks = static_cast<uint32_t>(batch * hq * p.nqb);
     p.rows = static_cast<uint32_t>(std::min<int64_t>(lq, kBlockRows));
     p.width = static_cast<uint32_t>(width);
-    p.whole = p.blocks;
     p.parts = 1;
     p.per = p.width;
-    const int64_t slots = 2 * cus, rest = p.blocks % slots;
+    const int64_t slots = (dim == 64 ? kWgsPerCu<64> : kWgsPerCu<128>) * cus;
     double best = static_cast<double>(width) + kUnitTiles;
-    for (int64_t parts = 2; rest > 0 && parts <= 64; ++parts) {
+    for (int64_t parts = 2; p.blocks < slots && parts <= 64; ++parts) {
         const int64_t per = (width + parts - 1) / parts;
         if (per < 4) break;
         if ((width + per - 1) / per != parts) continue;
         BlockPlan c = p;
-        c.whole = static_cast<uint32_t>(p.blocks - rest);
         c.parts = static_cast<uint32_t>(parts);
         c.per = static_cast<uint32_t>(per);
         if (block_workspace(c, dim) > max_bytes) break;
-        const double cost = static_cast<double>((rest * parts + slots - 1) / slots) * (per + kUnitTiles) + kMergeTiles;
+        const double cost = static_cast<double>((p.blocks * parts + slots - 1) / slots) * (per + kUnitTiles) + kMergeTiles;
         if (cost < best) {
             best = cost;
-            p.whole = c.whole;
             p.parts = c.parts;
             p.per = c.per;
         }
@@ -584,8 +556,7 @@ extern "C" int32_t tu_sage_block_attn(const int8_t *q8, const float *q_scale, in
     TU_REQUIRE(batch * hq <= 65535 && batch * hq * ((lq + kBlockRows - 1) / kBlockRows) <= 0x1fffffff,
                "block attention grid too large");
     const BlockPlan plan = block_plan(batch, hq, lq, dim, width, cus, workspace ? workspace_bytes : 0);
-    // an eighth of the whole lists and of the ranges each, rounded up, for every XCD
-    const unsigned grid = 8 * ((plan.whole + 7) / 8 + ((plan.blocks - plan.whole) * plan.parts + 7) / 8);
+    const unsigned grid = plan.blocks * plan.parts;
     if (require_gfx950()) return -1;
     int kscale_shift = 0;
     while ((kBKey << kscale_shift) < blkk) ++kscale_shift;
@@ -603,7 +574,7 @@ extern "C" int32_t tu_sage_block_attn(const int8_t *q8, const float *q_scale, in
             if (causal) TU_BLOCK_ATTN(D, true, true);                                                                  \
             else TU_BLOCK_ATTN(D, false, true);                                                                        \
             constexpr int kRowsPerWg = 256 / (D / 8);                                                                  \
-            const int64_t rows = static_cast<int64_t>(plan.blocks - plan.whole) * plan.rows;                           \
+            const int64_t rows = static_cast<int64_t>(plan.blocks) * plan.rows;                                        \
             block_merge_kernel<D><<<dim3(static_cast<unsigned>((rows + kRowsPerWg - 1) / kRowsPerWg)), 256, 0, st>>>(  \
                 part, plan, static_cast<uint32_t>(hq), lq, static_cast<uint16_t *>(o_bf16), o_sb, o_sh, o_sl);         \
         } else if (causal) {                                                                                           \

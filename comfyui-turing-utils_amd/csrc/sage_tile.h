@@ -288,7 +288,7 @@ __device__ __forceinline__ void pv_tile(const int8_t *stage, const LaneGeom<D> &
 // MFMA cluster of a steady-state step: QK^T of the tile in kst and PV of the
 // tile in vst, with the LDS fragment reads issued a group of MFMAs ahead of
 // their first use.
-template <int D, bool kRaise = true>
+template <int D>
 __device__ __forceinline__ void mfma_cluster(const int8_t *kst, const int8_t *vst, const LaneGeom<D> &gm,
                                              const i32x4 (&qf)[kQT][Geo<D>::kKSlices], i32x4 (&s)[4][kQT],
                                              const bf16x8 (&p)[2][kQT], SoftmaxState<D> &st, const bf16x8 &ones) {
@@ -296,7 +296,7 @@ __device__ __forceinline__ void mfma_cluster(const int8_t *kst, const int8_t *vs
     // This wave's MFMA cluster is the critical path of its interval: raise its
     // issue priority over the other group's softmax VALU on the same SIMD
     // (measured about 1 % faster; raising the softmax instead was slower).
-    if constexpr (kRaise) __builtin_amdgcn_s_setprio(3);
+    __builtin_amdgcn_s_setprio(3);
     i32x4 kf[4][kSl];
     bf16x8 va[kDS], vb[kDS];
     // first-slice K fragments first: the first QK^T MFMAs only need those
@@ -366,7 +366,7 @@ __device__ __forceinline__ void mfma_cluster(const int8_t *kst, const int8_t *vs
         __builtin_amdgcn_sched_group_barrier(0x100, 4, 0);
         __builtin_amdgcn_sched_group_barrier(0x008, 15, 0);
     }
-    if constexpr (kRaise) __builtin_amdgcn_s_setprio(0);
+    __builtin_amdgcn_s_setprio(0);
 }
 
 }  // namespace
