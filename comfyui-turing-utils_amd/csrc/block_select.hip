@@ -19,11 +19,13 @@
 namespace tu {
 namespace {
 
+typedef double f64x2 __attribute__((ext_vector_type(2)));
 typedef double f64x4 __attribute__((ext_vector_type(4)));
 
 constexpr int kQBlock = 128;  // rows of a query block
 constexpr int kKBlock = 64;   // keys of a key block
 constexpr int kThreads = 256;
+constexpr int kSelectThreads = 512;
 constexpr int kTileQ = 16;         // query blocks of a scoring workgroup (one MFMA's rows)
 constexpr int kMaxLdsBlocks = 1024;  // key blocks whose keys fit LDS (16 rows of 8 KiB)
 
@@ -160,30 +162,39 @@ __device__ __forceinline__ uint64_t forced_or(uint64_t key, int qb, int j, const
     return near || j < static_cast<int>(c.sink) ? ~0ull : key;
 }
 
-// The `take` largest of n keys (key(p) is the lane's key of block 64 p + lane,
-// 0 past n), ties to the lower block, written in ascending order with -1
-// behind: the threshold is found bit by bit, counting keys at or above it.
-template <typename Key>
-__device__ __forceinline__ void select_row(int n, int take, int width, int lane, Key key, int32_t *__restrict__ out) {
-    const int parts = (n + 63) / 64;
-    uint64_t t = 0;
+// The `take` largest of the keys (key(p) is the lane's key of block 64 p +
+// lane, 0 past the visible blocks and at least 1 in front), ties to the lower
+// block, written in ascending order with -1 behind: the threshold is found bit
+// by bit, counting keys at or above it, until a count fits.  kParts: keys of a
+// lane, held in registers; 0: `parts` of them, read each time.
+template <int kParts, typename Key>
+__device__ __forceinline__ void select_row(int n, int take, int width, int lane, int parts, Key key,
+                                           int32_t *__restrict__ out) {
+    auto each = [&](auto visit) {
+        if constexpr (kParts > 0) {
+#pragma unroll
+            for (int p = 0; p < kParts; ++p) visit(p);
+        } else {
+            for (int p = 0; p < parts; ++p) visit(p);
+        }
+    };
+    uint64_t t = 1;
     if (take < n) {
+        t = 0;
         for (int bit = 63; bit >= 0; --bit) {
             const uint64_t cand = t | 1ull << bit;
             int count = 0;
-            for (int p = 0; p < parts; ++p) count += __builtin_popcountll(__ballot(key(p) >= cand));
+            each([&](int p) { count += __builtin_popcountll(__ballot(key(p) >= cand)); });
             if (count >= take) t = cand;
             if (count == take) break;
         }
-    } else {
-        t = 1;  // every key of a visible block is at least 1
     }
     int above = 0;
-    for (int p = 0; p < parts; ++p) above += __builtin_popcountll(__ballot(key(p) > t));
+    each([&](int p) { above += __builtin_popcountll(__ballot(key(p) > t)); });
     const int allowed = take - above;
     const uint64_t below = (1ull << lane) - 1;
     int ties = 0, pos = 0;
-    for (int p = 0; p < parts; ++p) {
+    each([&](int p) {
         const uint64_t v = key(p);
         const uint64_t equal = __ballot(v == t);
         const bool chosen = v > t || (v == t && ties + __builtin_popcountll(equal & below) < allowed);
@@ -191,16 +202,18 @@ __device__ __forceinline__ void select_row(int n, int take, int width, int lane,
         if (chosen) out[pos + __builtin_popcountll(mask & below)] = 64 * p + lane;
         ties += __builtin_popcountll(equal);
         pos += __builtin_popcountll(mask);
-    }
+    });
     for (int i = pos + lane; i < width; i += 64) out[i] = -1;
 }
 
 // Scores of 16 query blocks and all key blocks of one head, as ordered keys in
 // LDS (kLds) or in `scores`, then (kLds) the choice, a wave per query block.
-// The four lane groups of the MFMA take a quarter of the channels each, so a
-// lane reads contiguous channels of its row.
+// The MFMA takes any order of the channels, so lane group g reads channels 8 u +
+// 2 g and the next for the products 2 u and 2 u + 1: 64 bytes of a row per load
+// (a quarter of the channels each, 256 bytes apart, fetched every line eight
+// times: 85 us at 256 x 512 blocks of 40 heads).
 template <int D, bool kLds, int kBlocks>
-__global__ __launch_bounds__(kThreads) void block_select_kernel(const double *__restrict__ mean_q,
+__global__ __launch_bounds__(kSelectThreads) void block_select_kernel(const double *__restrict__ mean_q,
                                                                 const double *__restrict__ mean_k, Choice c,
                                                                 uint32_t hq, uint32_t groups, uint32_t nqb,
                                                                 uint32_t nkb, int lq, int lk,
@@ -208,7 +221,7 @@ __global__ __launch_bounds__(kThreads) void block_select_kernel(const double *__
                                                                 const int32_t *__restrict__ k_len,
                                                                 uint64_t *__restrict__ scores,
                                                                 int32_t *__restrict__ index) {
-    __shared__ uint64_t keys[kLds ? kTileQ * kBlocks : 1];
+    __shared__ uint64_t keys[kLds ? kTileQ * kBlocks : 1];  // [query block][key block]
     const int lane = threadIdx.x & 63;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int lc = lane & 15, g = lane >> 4;
@@ -217,20 +230,25 @@ __global__ __launch_bounds__(kThreads) void block_select_kernel(const double *__
     const int i0 = static_cast<int>(blockIdx.x % tiles) * kTileQ;
     const uint32_t b = bh / hq, h = bh % hq, hkv = hq / groups;
     const int q_end = sample_end(q_len, b, lq), k_end = sample_end(k_len, b, lk);
-    const double *mq = mean_q + (static_cast<int64_t>(bh) * nqb + min(i0 + lc, static_cast<int>(nqb) - 1)) * D + g * (D / 4);
-    const double *mk = mean_k + static_cast<int64_t>(b * hkv + h / groups) * nkb * D + g * (D / 4);
-    double a[D / 4];
+    const double *mq = mean_q + (static_cast<int64_t>(bh) * nqb + min(i0 + lc, static_cast<int>(nqb) - 1)) * D + 2 * g;
+    const double *mk = mean_k + static_cast<int64_t>(b * hkv + h / groups) * nkb * D + 2 * g;
+    f64x2 a[D / 8];
 #pragma unroll
-    for (int s = 0; s < D / 4; ++s) a[s] = mq[s];
+    for (int u = 0; u < D / 8; ++u) a[u] = *reinterpret_cast<const f64x2 *>(mq + 8 * u);
     // no row of the tile sees more than its last one
     const int last = min(i0 + kTileQ, static_cast<int>(nqb)) - 1;
     const int most = c.causal ? (min(k_end, (last + 1) * kQBlock) + kKBlock - 1) / kKBlock : (k_end + kKBlock - 1) / kKBlock;
-    for (int j0 = 16 * wave; j0 < most; j0 += 16 * (kThreads / 64)) {
+    for (int j0 = 16 * wave; j0 < most; j0 += 16 * (kSelectThreads / 64)) {
         const int j = j0 + lc;
         const double *kr = mk + static_cast<int64_t>(min(j, static_cast<int>(nkb) - 1)) * D;
         f64x4 acc = {0.0, 0.0, 0.0, 0.0};
+        f64x2 x[D / 8];
 #pragma unroll
-        for (int s = 0; s < D / 4; ++s) acc = __builtin_amdgcn_mfma_f64_16x16x4f64(a[s], kr[s], acc, 0, 0, 0);
+        for (int u = 0; u < D / 8; ++u) x[u] = *reinterpret_cast<const f64x2 *>(kr + 8 * u);
+#pragma unroll
+        for (int u = 0; u < D / 8; ++u)
+#pragma unroll
+            for (int e = 0; e < 2; ++e) acc = __builtin_amdgcn_mfma_f64_16x16x4f64(a[u][e], x[u][e], acc, 0, 0, 0);
         // acc[r] = S of query block i0 + 4 r + g and key block j
 #pragma unroll
         for (int r = 0; r < 4; ++r) {
@@ -245,14 +263,17 @@ __global__ __launch_bounds__(kThreads) void block_select_kernel(const double *__
     }
     if constexpr (kLds) {
         __syncthreads();
-        for (int r = wave; r < kTileQ; r += kThreads / 64) {
+        for (int r = wave; r < kTileQ; r += kSelectThreads / 64) {
             const int i = i0 + r;
             if (i >= static_cast<int>(nqb)) break;
             const int n = visible_blocks(i, q_end, k_end, c.causal);
             int32_t *out = index + (static_cast<int64_t>(bh) * nqb + i) * c.width;
-            const uint64_t *row = keys + r * kBlocks;
-            select_row(n, min(static_cast<int>(c.keep), n), static_cast<int>(c.width), lane,
-                       [&](int p) { return 64 * p + lane < n ? row[64 * p + lane] : 0ull; }, out);
+            uint64_t mine[kBlocks / 64];
+#pragma unroll
+            for (int p = 0; p < kBlocks / 64; ++p)
+                mine[p] = 64 * p + lane < n ? keys[r * kBlocks + 64 * p + lane] : 0ull;
+            select_row<kBlocks / 64>(n, min(static_cast<int>(c.keep), n), static_cast<int>(c.width), lane, 0,
+                       [&](int p) { return mine[p]; }, out);
         }
     }
 }
@@ -269,7 +290,7 @@ __global__ __launch_bounds__(kThreads) void choose_kernel(const uint64_t *__rest
     const uint32_t b = id / nqb / hq;
     const int n = visible_blocks(static_cast<int>(id % nqb), sample_end(q_len, b, lq), sample_end(k_len, b, lk), c.causal);
     const uint64_t *row = scores + static_cast<int64_t>(id) * nkb;
-    select_row(n, min(static_cast<int>(c.keep), n), static_cast<int>(c.width), lane,
+    select_row<0>(n, min(static_cast<int>(c.keep), n), static_cast<int>(c.width), lane, (n + 63) / 64,
                [&](int p) { return 64 * p + lane < n ? row[64 * p + lane] : 0ull; },
                index + static_cast<int64_t>(id) * c.width);
 }
@@ -296,7 +317,7 @@ int32_t launch_select(const Side &q, const Side &k, int64_t batch, int64_t hq, i
         q, k, static_cast<uint32_t>(q_tasks), static_cast<uint32_t>(tasks), mean_q, mean_k);
     const dim3 grid(static_cast<unsigned>(batch * hq * blocks_of(nqb, kTileQ)));
 #define TU_SELECT(LDS, BLOCKS)                                                                                          \
-    block_select_kernel<D, LDS, BLOCKS><<<grid, kThreads, 0, st>>>(                                                    \
+    block_select_kernel<D, LDS, BLOCKS><<<grid, kSelectThreads, 0, st>>>(                                                    \
         mean_q, mean_k, c, static_cast<uint32_t>(hq), static_cast<uint32_t>(hq / hkv), nqb, nkb, static_cast<int>(q.len), \
         static_cast<int>(k.len), q.lengths, k.lengths, scores, index)
     if (nkb <= 128) TU_SELECT(true, 128);
