@@ -60,6 +60,45 @@ def test_more_key_blocks_than_lds_holds(gpu_device):
     _check(gpu_device, 1, 1, 1, 140, 70000, 64, 300, seed=7)
     _check(gpu_device, 1, 1, 1, 140, 70000, 128, 3, causal=True, seed=8)
     _check(gpu_device, 1, 1, 1, 140, 65536, 64, 40, seed=9)
+    _check(gpu_device, 1, 1, 1, 140, 131200, 64, 40, seed=10)
+
+
+def test_near_scores(gpu_device):
+    """Key blocks that differ by one code in 64 x 64: scores closer than 16 or 24 bits tell apart."""
+    dev = gpu_device
+    g = torch.Generator().manual_seed(11)
+    for d, blocks, keep in ((64, 40, 13), (128, 300, 150), (64, 600, 5)):
+        q8, qs = ref.codes(1, 1, 300, d, 128, g, dev)
+        row = torch.randint(-120, 120, (1, 1, 64, d), generator=g, dtype=torch.int8)
+        k8 = row.repeat(1, 1, blocks, 1)
+        for j in range(blocks):
+            k8[0, 0, 64 * j + j % 64, j % d] += int(torch.randint(-3, 4, (1,), generator=g))
+        ks = torch.full((1, 1, blocks), 0.02, device=dev)
+        got = turing_sage.select_key_blocks(q8, qs, k8.to(dev), ks, keep=keep, blkk=64)
+        assert torch.equal(got.cpu(), ref.select(q8, qs, k8.to(dev), ks, keep, "HND", False, 0, 0, 128, 64))
+
+
+@pytest.mark.parametrize("q_factor,k_factor", [(1e-25, 1.0), (1.0, 1e-30), (1e30, 1e25), (1e-36, 1e36), (1e25, 1e-25)])
+def test_scales_at_the_ends_of_fp32(gpu_device, q_factor, k_factor):
+    dev = gpu_device
+    g = torch.Generator().manual_seed(12)
+    q8, qs = ref.codes(1, 2, 260, 64, 128, g, dev)
+    k8, ks = ref.codes(1, 2, 1000, 64, 64, g, dev)
+    qs, ks = qs * q_factor, ks * k_factor
+    got = turing_sage.select_key_blocks(q8, qs, k8, ks, keep=6, blkk=64, local_blocks=1)
+    assert torch.equal(got.cpu(), ref.select(q8, qs, k8, ks, 6, "HND", False, 0, 1, 128, 64))
+
+
+def test_a_few_keys_far_larger_than_the_others(gpu_device):
+    """The margin follows the longest mean: most blocks are then undecided."""
+    dev = gpu_device
+    g = torch.Generator().manual_seed(13)
+    q8, qs = ref.codes(2, 2, 500, 128, 128, g, dev)
+    k8, ks = ref.codes(2, 2, 6400, 128, 64, g, dev)
+    ks[:, :, 7] *= 3e4
+    for keep in (1, 40, 99):
+        got = turing_sage.select_key_blocks(q8, qs, k8, ks, keep=keep, blkk=64)
+        assert torch.equal(got.cpu(), ref.select(q8, qs, k8, ks, keep, "HND", False, 0, 0, 128, 64))
 
 
 def test_equal_scores_go_to_the_lower_block(gpu_device):

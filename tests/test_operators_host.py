@@ -136,10 +136,11 @@ def test_entry_points_refuse_before_any_launch():
 
 def test_workspaces():
     lib = _lib.load()
-    # fp64 mean rows of 3 query and 8 key blocks a head
-    assert lib.tu_sage_block_select_workspace(2, 4, 2, 300, 500, 64) == 2 * (4 * 3 + 2 * 8) * 64 * 8
-    # past 1024 key blocks the scores too
-    assert lib.tu_sage_block_select_workspace(1, 1, 1, 128, 65600, 64) == (1 + 1025) * 64 * 8 + 1025 * 8
+    # 3 query and 8 key blocks a head: mean rows in fp64, as two bf16 terms of 16 blocks each, their lengths
+    assert lib.tu_sage_block_select_workspace(2, 4, 2, 300, 500, 64) == 2 * 28 * (64 * 8 + 4) + 2 * 6 * 16 * 64 * 4
+    # past 2048 key blocks the scores too
+    assert (lib.tu_sage_block_select_workspace(1, 1, 1, 128, 131200, 64)
+            == 2051 * 64 * 8 + 2052 * 4 + (16 + 2064) * 64 * 4 + 2050 * 8)
     # many query blocks: no list is split; one row: lists in ranges of at least four
     assert lib.tu_sage_block_attn_workspace(1, 40, 32760, 128, 128, 256) == 0
     assert lib.tu_sage_block_attn_workspace(1, 1, 1, 128, 3, 256) == 0
