@@ -10,7 +10,7 @@
 // INT8 GEMM's epilogue, where it joins the projection's fp32 value before the
 // one rounding to bf16.
 //
-// A workgroup takes 16 or 32 rows and 16 to 64 ranks, its 8 waves a share of K
+// A workgroup takes 16 to 64 rows and 16 to 64 ranks, its 8 waves a share of K
 // each (they meet in LDS), and walks the distinct adapters of its rows; rows of
 // one request lie together, so that is one adapter except at a border.  Each
 // lane reads 16 codes of a row and the same 16 columns of a rank, which the
@@ -59,11 +59,11 @@ __global__ __launch_bounds__(kThreads) void adapter_down_kernel(const int8_t *__
 
     // the low lanes hold the tile's adapters
     const int id = lane < kRows ? adapter_of(ad.ids, ad.id_rows, ad.count, row0 + lane, m) : -1;
-    uint32_t pending = static_cast<uint32_t>(__ballot(id >= 0));
+    uint64_t pending = __ballot(id >= 0);
     int ordinal = 0;
     while (pending) {
-        const int which = __builtin_amdgcn_readlane(id, __builtin_ctz(pending));
-        const uint32_t mine = static_cast<uint32_t>(__ballot(id == which));
+        const int which = __builtin_amdgcn_readlane(id, __builtin_ctzll(pending));
+        const uint64_t mine = __ballot(id == which);
         pending &= ~mine;
         if (ordinal++ % slots != slot) continue;
         const uint16_t *dn = down + static_cast<int64_t>(which) * ad.rank * k;
@@ -78,51 +78,43 @@ __global__ __launch_bounds__(kThreads) void adapter_down_kernel(const int8_t *__
         const uint16_t *rank_row[kFrags];
 #pragma unroll
         for (int f = 0; f < kFrags; ++f) rank_row[f] = dn + min(r0 + 16 * f + lc, ad.rank - 1) * k;
-        // Steps of 64 columns whose loads are in flight together; the
-        // last ones take zeros past K (a multiple of 16).
-        constexpr int kAhead = kFrags * kRowFrags <= 4 ? 4 : 2;
-        auto steps = [&](int64_t k0, auto count, auto tail) {
-            constexpr int kN = decltype(count)::value;
-            u32x4 c[kN][kRowFrags], d[kN][kFrags][2];
-            bool in[kN];
+        // Steps of 64 columns; the last one takes zeros past K (a multiple of
+        // 16).  The CU's other waves hide a step's loads better than two or
+        // four steps of one wave in flight: 12.6, 13.3 and 13.7 us in all at 4
+        // rows, 135.8, 137.6 and 141.5 at 2050, 850, 858 and 895 at 32760.
+        auto step = [&](int64_t k0, auto tail) {
+            int64_t kk = k0 + 16 * g;
+            const bool in = !decltype(tail)::value || kk < k;
+            kk = in ? kk : 0;
+            u32x4 c[kRowFrags], d[kFrags][2];
 #pragma unroll
-            for (int u = 0; u < kN; ++u) {
-                int64_t kk = k0 + 64 * kWaves * u + 16 * g;
-                in[u] = !decltype(tail)::value || kk < k;
-                kk = in[u] ? kk : 0;
+            for (int i = 0; i < kRowFrags; ++i) c[i] = *reinterpret_cast<const u32x4 *>(code[i] + kk);
 #pragma unroll
-                for (int i = 0; i < kRowFrags; ++i) c[u][i] = *reinterpret_cast<const u32x4 *>(code[i] + kk);
+            for (int f = 0; f < kFrags; ++f)
 #pragma unroll
-                for (int f = 0; f < kFrags; ++f)
+                for (int e = 0; e < 2; ++e) d[f][e] = *reinterpret_cast<const u32x4 *>(rank_row[f] + kk + 8 * e);
 #pragma unroll
-                    for (int e = 0; e < 2; ++e) d[u][f][e] = *reinterpret_cast<const u32x4 *>(rank_row[f] + kk + 8 * e);
-            }
+            for (int e = 0; e < 2; ++e) {
+                bf16x8 x[kRowFrags];
 #pragma unroll
-            for (int u = 0; u < kN; ++u)
-#pragma unroll
-                for (int e = 0; e < 2; ++e) {
-                    bf16x8 x[kRowFrags];
-#pragma unroll
-                    for (int i = 0; i < kRowFrags; ++i) {
-                        x[i] = codes_to_bf16(c[u][i][2 * e], c[u][i][2 * e + 1]);
-                        if (!in[u]) x[i] = __builtin_bit_cast(bf16x8, u32x4{0, 0, 0, 0});
-                    }
-#pragma unroll
-                    for (int f = 0; f < kFrags; ++f) {
-                        const u32x4 y = in[u] ? d[u][f][e] : u32x4{0, 0, 0, 0};
-#pragma unroll
-                        for (int i = 0; i < kRowFrags; ++i)
-                            acc[f][i] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, y), x[i],
-                                                                                acc[f][i], 0, 0, 0);
-                    }
+                for (int i = 0; i < kRowFrags; ++i) {
+                    x[i] = codes_to_bf16(c[i][2 * e], c[i][2 * e + 1]);
+                    if (!in) x[i] = __builtin_bit_cast(bf16x8, u32x4{0, 0, 0, 0});
                 }
+#pragma unroll
+                for (int f = 0; f < kFrags; ++f) {
+                    const u32x4 y = in ? d[f][e] : u32x4{0, 0, 0, 0};
+#pragma unroll
+                    for (int i = 0; i < kRowFrags; ++i)
+                        acc[f][i] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, y), x[i], acc[f][i],
+                                                                            0, 0, 0);
+                }
+            }
         };
         int64_t k0 = 64 * wave;
 #pragma clang loop unroll(disable)
-        for (; k0 + 64 * kWaves * (kAhead - 1) + 64 <= k; k0 += 64 * kWaves * kAhead)
-            steps(k0, std::integral_constant<int, kAhead>{}, std::false_type{});
-#pragma clang loop unroll(disable)
-        for (; k0 < k; k0 += 64 * kWaves * kAhead) steps(k0, std::integral_constant<int, kAhead>{}, std::true_type{});
+        for (; k0 + 64 <= k; k0 += 64 * kWaves) step(k0, std::false_type{});
+        if (k0 < k) step(k0, std::true_type{});
 #pragma unroll
         for (int f = 0; f < kFrags; ++f)
 #pragma unroll
@@ -158,18 +150,24 @@ __global__ __launch_bounds__(kThreads) void adapter_down_kernel(const int8_t *__
 
 int32_t launch_down(const int8_t *a, const float *a_scale, const uint16_t *down, const float *scaling,
                     const Adapters &ad, uint16_t *h, int64_t m, int64_t k, int cus, hipStream_t st) {
-    // The largest tile that gives every CU a workgroup, else the smallest.
+    // The largest tile that gives every CU a workgroup (four of the 32 rows for
+    // one of 64: at 32760 rows of 5120, rank 32, 64 rows take 850 us with the
+    // GEMM where 32 take 877), else the smallest.
     int rows = 32, ranks = ad.rank <= 16 ? 16 : ad.rank <= 32 ? 32 : 64;
     auto tiles = [&] { return (m + rows - 1) / rows * ((ad.rank + ranks - 1) / ranks); };
     while (tiles() < cus && ranks > 16) ranks /= 2;
     if (tiles() < cus) rows = 16;
+    else if (ranks <= 32 && tiles() >= 4 * cus) rows = 64;
     // two at least, so that a tile with a border between requests takes no longer
     const int slots = static_cast<int>(std::min<int64_t>(ad.count, std::min<int64_t>(16, std::max<int64_t>(2, cus / tiles()))));
     const dim3 grid(static_cast<unsigned>((m + rows - 1) / rows), static_cast<unsigned>((ad.rank + ranks - 1) / ranks),
                     static_cast<unsigned>(slots));
 #define TU_DOWN(R, F) adapter_down_kernel<R, F><<<grid, kThreads, 0, st>>>(a, a_scale, down, scaling, ad, slots, h, m, k)
     if (rows == 16) TU_DOWN(16, 1);
-    else if (ranks == 16) TU_DOWN(16, 2);
+    else if (rows == 64) {
+        if (ranks == 16) TU_DOWN(16, 4);
+        else TU_DOWN(32, 4);
+    } else if (ranks == 16) TU_DOWN(16, 2);
     else if (ranks == 32) TU_DOWN(32, 2);
     else TU_DOWN(64, 2);
 #undef TU_DOWN

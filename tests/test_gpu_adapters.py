@@ -76,6 +76,12 @@ def test_every_tile(gpu_device, m, n, residual):
     _check(_inputs(gpu_device, m, 256, n, 32, 3, rows, residual=residual, gate=residual, seed=n))
 
 
+@pytest.mark.parametrize("rank", [8, 16, 32])
+def test_many_rows(gpu_device, rank):
+    """The tall tile of the down-projection, borders inside it."""
+    _check(_inputs(gpu_device, 33001, 160, 64, rank, 5, 37, seed=rank))
+
+
 def test_sizes_reach_every_tile(gpu_device):
     from comfyui_turing_utils_kernel import _lib
 
