@@ -40,17 +40,25 @@ per token (the rotation is orthogonal, so rot(x) . rot(w) = x . w).  The
 residual stream x is bf16; each residual add, x + y * gate, runs in the
 epilogue of the projection that produces y (``turing_utils::int8_linear_residual``):
 bf16_rn(fma(y, gate, x)) with y the bf16 projection output.
+
+Two options of a forward, off by default: each sample of a batch with the
+low-rank adapters of its own request on any of the linears (``set_adapters``,
+``adapter_ids``; ``turing_utils::int8_linear_adapters``), and self-attention
+over the key blocks chosen per query block (``BlockSparsity``;
+``turing_sage.sparse_sageattn_from_prequantized``).
 """
 from __future__ import annotations
 
 import math
 from dataclasses import dataclass
-from typing import Optional
+from typing import Mapping, Optional
 
 import torch
 
 from . import ops  # noqa: F401  (registers torch.ops.turing_utils.*)
+from .adapters import LinearAdapters, turing_int8_linear_adapters
 from .turing_sage import core as sage_core
+from .turing_sage.sparse import sparse_sageattn_from_prequantized
 
 GROUP = 128
 
@@ -110,10 +118,18 @@ class W8A8Linear:
         return cls(codes, scale, bias, group)
 
     def __call__(self, x, gelu: bool = False, residual: Optional[torch.Tensor] = None,
-                 gate: Optional[torch.Tensor] = None, gate_rows: int = 1) -> torch.Tensor:
+                 gate: Optional[torch.Tensor] = None, gate_rows: int = 1, adapters: Optional[LinearAdapters] = None,
+                 adapter_ids: Optional[torch.Tensor] = None, adapter_rows: int = 1) -> torch.Tensor:
         """y = x W^T + b, or residual + y * gate[row // gate_rows] (gate 1 when
         None) fused into the GEMM epilogue when ``residual`` [M, N] is given.
-        x: bf16 [M, K], or a QuantizedActivation of this linear's group."""
+        x: bf16 [M, K], or a QuantizedActivation of this linear's group.
+        With ``adapter_ids`` (int32) y also has adapter
+        adapter_ids[row // adapter_rows] of ``adapters`` in it (see
+        ``turing_int8_linear_adapters``)."""
+        if (adapters is None) != (adapter_ids is None):
+            raise ValueError("adapters need adapter_ids, and adapter_ids need adapters")
+        if adapters is not None and adapters.group != self.group:
+            raise ValueError(f"adapters at ConvRot group {adapters.group} on a W8A8 linear of group {self.group}")
         if isinstance(x, QuantizedActivation):
             if gelu or x.group != self.group or x.codes.shape[1] != self.in_features:
                 raise ValueError(f"W8A8 linear expects codes of [M, {self.in_features}] at group {self.group} "
@@ -125,6 +141,10 @@ class W8A8Linear:
             quantize = (torch.ops.turing_utils.bf16_gelu_int8_convrot_quantize if gelu
                         else torch.ops.turing_utils.bf16_int8_convrot_quantize)
             codes, scale = quantize(x.contiguous(), self.group)
+        if adapters is not None:
+            return turing_int8_linear_adapters(codes, self.weight, scale, self.weight_scale, self.bias, adapters.down,
+                                               adapters.up, adapters.scaling, adapter_ids, adapter_rows, residual, gate,
+                                               gate_rows)
         if residual is None:
             return torch.ops.turing_utils.int8_linear(codes, self.weight, scale, self.weight_scale, self.bias)
         return torch.ops.turing_utils.int8_linear_residual(codes, self.weight, scale, self.weight_scale, self.bias,
@@ -184,6 +204,16 @@ class WanBlockConfig:
         return self.dim // self.heads
 
 
+@dataclass(frozen=True)
+class BlockSparsity:
+    """Self-attention over ``keep`` key blocks of 64 for each query block of
+    128, the first ``sink_blocks`` and the ``local_blocks`` on either side of
+    the query block's own always among them (``turing_sage.select_key_blocks``)."""
+    keep: int
+    sink_blocks: int = 0
+    local_blocks: int = 0
+
+
 class WanTextEmbeddingW8A8:
     """Linear(text_dim, C), tanh-GELU, Linear(C, C) on the text context."""
 
@@ -198,6 +228,8 @@ class WanTextEmbeddingW8A8:
 
 class WanBlockW8A8:
     """One Wan 2.1 attention block; see the module docstring for the math."""
+
+    LINEARS = ("self_qkv", "self_o", "cross_q", "cross_kv", "cross_o", "ffn_up", "ffn_down")
 
     def __init__(self, cfg: WanBlockConfig, *, modulation: torch.Tensor,
                  self_qkv: W8A8Linear, self_o: W8A8Linear, self_norm_q: torch.Tensor, self_norm_k: torch.Tensor,
@@ -223,41 +255,75 @@ class WanBlockW8A8:
         self.ffn_up, self.ffn_down = ffn_up, ffn_down
         self.norm3_weight = norm3_weight.to(torch.bfloat16).reshape(c).contiguous()
         self.norm3_bias = norm3_bias.to(torch.bfloat16).reshape(c).contiguous()
+        self.adapters: dict[str, LinearAdapters] = {}
+
+    def set_adapters(self, adapters: Mapping[str, LinearAdapters]) -> None:
+        """The adapters that ``adapter_ids`` of a forward choose from, by the
+        name of their linear (``LINEARS``); all of one count.  self_qkv and
+        cross_kv take ``LinearAdapters.concat`` of q, k and v, or of k and v.
+        An empty mapping takes them off."""
+        for name, a in adapters.items():
+            if name not in self.LINEARS:
+                raise ValueError(f"no linear {name!r} in a Wan block, it has {', '.join(self.LINEARS)}")
+            lin = getattr(self, name)
+            if (a.down.shape[2], a.up.shape[1], a.group) != (lin.in_features, lin.out_features, lin.group):
+                raise ValueError(f"adapters [{a.up.shape[1]}, {a.down.shape[2]}] at group {a.group} do not fit {name}, "
+                                 f"[{lin.out_features}, {lin.in_features}] at group {lin.group}")
+        if len({a.count for a in adapters.values()}) > 1:
+            raise ValueError("the linears' adapters must be of one count")
+        self.adapters = dict(adapters)
+
+    def _adapted(self, name: str, adapter_ids: Optional[torch.Tensor], rows: int) -> dict:
+        """The adapter arguments of a linear whose samples have ``rows`` rows each."""
+        if adapter_ids is None or name not in self.adapters:
+            return {}
+        return dict(adapters=self.adapters[name], adapter_ids=adapter_ids, adapter_rows=rows)
 
     # -- sublayers (each takes and returns bf16 [B, L, C]) ---------------------
 
     # (h: bf16 [B, L, C] or its QuantizedActivation for the first projection)
 
+    # adapter_ids: int32 [B], the adapter of each sample (outside [0, count): none)
+
     def self_attention(self, h, freqs: torch.Tensor, residual: Optional[torch.Tensor] = None,
-                       gate: Optional[torch.Tensor] = None) -> torch.Tensor:
+                       gate: Optional[torch.Tensor] = None, adapter_ids: Optional[torch.Tensor] = None,
+                       sparsity: Optional[BlockSparsity] = None) -> torch.Tensor:
         """The attention output projected by o; with ``residual`` [B, L, C],
         residual + that * gate (gate [B, 1, C] or None) from one epilogue."""
         cfg = self.cfg
         b, l, c = h.shape
-        qkv = self.self_qkv(_token_rows(h)).view(b, l, 3, cfg.heads, cfg.head_dim)
+        qkv = self.self_qkv(_token_rows(h), **self._adapted("self_qkv", adapter_ids, l))
+        qkv = qkv.view(b, l, 3, cfg.heads, cfg.head_dim)
         q, k, v = qkv[:, :, 0], qkv[:, :, 1], qkv[:, :, 2]
         qk = sage_core.prequantize_rms_rope_qk(
             q, k, self.self_norm_q, self.self_norm_k, freqs, epsilon=cfg.eps, rot_dim=cfg.head_dim,
             tensor_layout="NHD", norm_scope="row")
         state = sage_core.prequantize_sageattn_from_qk(qk, v, sm_scale=cfg.head_dim ** -0.5)
         del qkv, q, k, qk
-        out = sage_core.sageattn_from_prequantized(state)
-        return self._project(self.self_o, out.reshape(b * l, c), residual, gate).view(b, l, c)
+        if sparsity is None:
+            out = sage_core.sageattn_from_prequantized(state)
+        else:
+            out = sparse_sageattn_from_prequantized(state, keep=sparsity.keep, sink_blocks=sparsity.sink_blocks,
+                                                    local_blocks=sparsity.local_blocks)
+        return self._project("self_o", out.reshape(b * l, c), b, residual, gate, adapter_ids).view(b, l, c)
 
-    def _project(self, lin: W8A8Linear, x2d: torch.Tensor, residual, gate, gelu: bool = False) -> torch.Tensor:
+    def _project(self, name: str, x2d: torch.Tensor, b: int, residual, gate, adapter_ids,
+                 gelu: bool = False) -> torch.Tensor:
+        lin, adapted = getattr(self, name), self._adapted(name, adapter_ids, x2d.shape[0] // b)
         if residual is None:
-            return lin(x2d, gelu=gelu)
+            return lin(x2d, gelu=gelu, **adapted)
         b, l, c = residual.shape
         g = None if gate is None else gate.reshape(b, c)
-        return lin(x2d, gelu=gelu, residual=residual.reshape(b * l, c), gate=g, gate_rows=l)
+        return lin(x2d, gelu=gelu, residual=residual.reshape(b * l, c), gate=g, gate_rows=l, **adapted)
 
-    def cross_attention(self, h, context: torch.Tensor,
-                        residual: Optional[torch.Tensor] = None) -> torch.Tensor:
+    def cross_attention(self, h, context: torch.Tensor, residual: Optional[torch.Tensor] = None,
+                        adapter_ids: Optional[torch.Tensor] = None) -> torch.Tensor:
         cfg = self.cfg
         b, l, c = h.shape
         lc = context.shape[1]
-        q = self.cross_q(_token_rows(h)).view(b, l, cfg.heads, cfg.head_dim)
-        kv = self.cross_kv(context.reshape(b * lc, c)).view(b, lc, 2, cfg.heads, cfg.head_dim)
+        q = self.cross_q(_token_rows(h), **self._adapted("cross_q", adapter_ids, l)).view(b, l, cfg.heads, cfg.head_dim)
+        kv = self.cross_kv(context.reshape(b * lc, c), **self._adapted("cross_kv", adapter_ids, lc))
+        kv = kv.view(b, lc, 2, cfg.heads, cfg.head_dim)
         k, v = kv[:, :, 0], kv[:, :, 1]
         qk = sage_core.prequantize_rms_rope_qk(
             q, k, self.cross_norm_q, self.cross_norm_k, None, epsilon=cfg.eps, rot_dim=0,
@@ -265,27 +331,35 @@ class WanBlockW8A8:
         state = sage_core.prequantize_sageattn_from_qk(qk, v, sm_scale=cfg.head_dim ** -0.5)
         del q, kv, k, qk
         out = sage_core.sageattn_from_prequantized(state)
-        return self._project(self.cross_o, out.reshape(b * l, c), residual, None).view(b, l, c)
+        return self._project("cross_o", out.reshape(b * l, c), b, residual, None, adapter_ids).view(b, l, c)
 
-    def ffn(self, h, residual: Optional[torch.Tensor] = None,
-            gate: Optional[torch.Tensor] = None) -> torch.Tensor:
+    def ffn(self, h, residual: Optional[torch.Tensor] = None, gate: Optional[torch.Tensor] = None,
+            adapter_ids: Optional[torch.Tensor] = None) -> torch.Tensor:
         b, l, c = h.shape
-        up = self.ffn_up(_token_rows(h))
-        return self._project(self.ffn_down, up, residual, gate, gelu=True).view(b, l, c)
+        up = self.ffn_up(_token_rows(h), **self._adapted("ffn_up", adapter_ids, l))
+        return self._project("ffn_down", up, b, residual, gate, adapter_ids, gelu=True).view(b, l, c)
 
     def modulation_chunks(self, e: torch.Tensor) -> list[torch.Tensor]:
         """(modulation + e) split into the six [B, 1, C] bf16 rows."""
         mod = (self.modulation + e.to(torch.float32)).to(torch.bfloat16)
         return [mod[:, i:i + 1] for i in range(6)]
 
-    def forward(self, x: torch.Tensor, e: torch.Tensor, context: torch.Tensor, freqs: torch.Tensor) -> torch.Tensor:
+    def forward(self, x: torch.Tensor, e: torch.Tensor, context: torch.Tensor, freqs: torch.Tensor,
+                adapter_ids: Optional[torch.Tensor] = None, sparsity: Optional[BlockSparsity] = None) -> torch.Tensor:
         """x bf16 [B, L, C]; e [B, 6, C] time modulation; context bf16 [B, Lc, C]
-        (after the text embedding); freqs [1|B, L, 1, D/2, 2, 2]."""
+        (after the text embedding); freqs [1|B, L, 1, D/2, 2, 2]; adapter_ids
+        int32 [B], the adapter (``set_adapters``) of each sample, none outside
+        [0, count); sparsity: which keys self-attention keeps, all when None."""
         cfg = self.cfg
         if x.dtype != torch.bfloat16 or x.dim() != 3 or x.shape[2] != cfg.dim:
             raise TypeError(f"Wan block input must be bf16 [B, L, {cfg.dim}]")
         if context.dtype != torch.bfloat16 or context.dim() != 3 or context.shape[2] != cfg.dim:
             raise TypeError(f"Wan block context must be bf16 [B, Lc, {cfg.dim}]")
+        if adapter_ids is not None:
+            if not self.adapters:
+                raise ValueError("adapter_ids need adapters: call set_adapters first")
+            if adapter_ids.dtype != torch.int32 or adapter_ids.shape != (x.shape[0],):
+                raise ValueError(f"adapter_ids must be int32 [{x.shape[0]}], one adapter per sample")
         e0, e1, e2, e3, e4, e5 = self.modulation_chunks(e)
         x = x.contiguous()
         b, l, _ = x.shape
@@ -296,11 +370,13 @@ class WanBlockW8A8:
 
         # each norm runs with the next projection's quantizer, each residual
         # add in the epilogue of the projection before it
-        x = self.self_attention(adaln_codes(x, e1, e0, self.self_qkv.group), freqs, residual=x, gate=e2)
+        x = self.self_attention(adaln_codes(x, e1, e0, self.self_qkv.group), freqs, residual=x, gate=e2,
+                                adapter_ids=adapter_ids, sparsity=sparsity)
         codes, rs = torch.ops.turing_utils.layer_norm_affine_int8_convrot_quantize(
             x, self.norm3_weight, self.norm3_bias, cfg.eps, self.cross_q.group)
-        x = self.cross_attention(QuantizedActivation(codes, rs, b, l, self.cross_q.group), context, residual=x)
-        return self.ffn(adaln_codes(x, e4, e3, self.ffn_up.group), residual=x, gate=e5)
+        x = self.cross_attention(QuantizedActivation(codes, rs, b, l, self.cross_q.group), context, residual=x,
+                                 adapter_ids=adapter_ids)
+        return self.ffn(adaln_codes(x, e4, e3, self.ffn_up.group), residual=x, gate=e5, adapter_ids=adapter_ids)
 
     __call__ = forward
 

@@ -203,3 +203,59 @@ def test_reference_attention_is_masked_softmax():
     p = torch.nan_to_num(s.masked_fill(~mask, -float("inf")).softmax(-1))
     want = p @ vt[0, 0, :, :300].double().t()
     assert torch.allclose(out, want, rtol=1e-12, atol=1e-12) and (size >= out.abs() - 1e-12).all()
+
+
+def _block():
+    from comfyui_turing_utils_kernel.wan_block import W8A8Linear, WanBlockConfig, WanBlockW8A8
+
+    def lin(n, k):
+        return W8A8Linear(torch.zeros(n, k, dtype=torch.int8), torch.ones(n), None)
+
+    ones = torch.ones(256)
+    return WanBlockW8A8(WanBlockConfig(dim=256, heads=2, ffn_dim=512, text_dim=256), modulation=torch.zeros(1, 6, 256),
+                        self_qkv=lin(768, 256), self_o=lin(256, 256), self_norm_q=ones, self_norm_k=ones,
+                        norm3_weight=ones, norm3_bias=ones * 0, cross_q=lin(256, 256), cross_kv=lin(512, 256),
+                        cross_o=lin(256, 256), cross_norm_q=ones, cross_norm_k=ones, ffn_up=lin(512, 256),
+                        ffn_down=lin(256, 512))
+
+
+def test_block_adapters_are_checked():
+    from comfyui_turing_utils_kernel import LinearAdapters
+
+    def adapters(n, k, count=2, group=128):
+        return LinearAdapters.from_float([(torch.ones(4, k), torch.ones(n, 4), 1.0)] * count, group)
+
+    block = _block()
+    block.set_adapters({"self_qkv": adapters(768, 256), "ffn_down": adapters(256, 512)})
+    assert set(block.adapters) == {"self_qkv", "ffn_down"}
+    for bad, match in (({"qkv": adapters(768, 256)}, "no linear"), ({"self_o": adapters(512, 256)}, "do not fit"),
+                       ({"self_o": adapters(256, 256, group=256)}, "do not fit"),
+                       ({"self_o": adapters(256, 256), "ffn_up": adapters(512, 256, 3)}, "one count")):
+        with pytest.raises(ValueError, match=match):
+            block.set_adapters(bad)
+    assert set(block.adapters) == {"self_qkv", "ffn_down"}  # a refused mapping changes nothing
+
+    x = torch.zeros(2, 8, 256, dtype=torch.bfloat16)
+    args = (x, torch.zeros(2, 6, 256), x, None)
+    for ids in (torch.zeros(3, dtype=torch.int32), torch.zeros(2, dtype=torch.int64), torch.zeros(1, 2, dtype=torch.int32)):
+        with pytest.raises(ValueError, match="adapter_ids must be"):
+            block(*args, adapter_ids=ids)
+    block.set_adapters({})
+    with pytest.raises(ValueError, match="need adapters"):
+        block(*args, adapter_ids=torch.zeros(2, dtype=torch.int32))
+
+
+def test_linear_adapters_are_checked():
+    from comfyui_turing_utils_kernel import LinearAdapters
+    from comfyui_turing_utils_kernel.wan_block import QuantizedActivation, W8A8Linear
+
+    lin = W8A8Linear(torch.zeros(64, 256, dtype=torch.int8), torch.ones(64), None)
+    x = QuantizedActivation(torch.zeros(8, 256, dtype=torch.int8), torch.ones(8, 1), 1, 8, 128)
+    one = [(torch.ones(4, 256), torch.ones(64, 4), 1.0)]
+    ids = torch.zeros(8, dtype=torch.int32)
+    with pytest.raises(ValueError, match="need adapter_ids"):
+        lin(x, adapters=LinearAdapters.from_float(one))
+    with pytest.raises(ValueError, match="need adapters"):
+        lin(x, adapter_ids=ids)
+    with pytest.raises(ValueError, match="group 256"):
+        lin(x, adapters=LinearAdapters.from_float(one, 256), adapter_ids=ids)
