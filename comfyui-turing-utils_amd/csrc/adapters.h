@@ -7,16 +7,24 @@
 
 namespace tu {
 
-// A row of h holds its ranks as two bf16 terms, [hi | lo] (hi + lo is the fp32
-// sum to 2^-16 of it), scaled by the row's activation scale and its adapter's
-// scaling; rows without an adapter are not written.
+// h holds a row's ranks as two bf16 terms (hi + lo is the fp32 sum to 2^-16 of
+// it), scaled by the row's activation scale and its adapter's scaling, as the
+// epilogue's MFMA reads them: [16 rows][32 ranks][term][row][32], a load of a
+// wave being 1 KiB in one piece.  Rows without an adapter and ranks that pad the
+// last 32 are not written.
 struct Adapters {
-    const uint16_t *h;     // [m][2 rank]
+    const uint16_t *h;
     const uint16_t *up;    // bf16 [count][n][rank]
     const int32_t *ids;    // adapter of rows i * id_rows .. (i + 1) * id_rows - 1
     int64_t id_rows;
     int rank, count;
 };
+
+// Place of a row's rank r in h; its low term lies kLowTerm values on.
+constexpr int kLowTerm = 16 * 32;
+__device__ __forceinline__ int64_t h_at(int64_t row, int rank, int r) {
+    return ((row >> 4) * ((rank + 31) >> 5) + (r >> 5)) * (2 * kLowTerm) + (row & 15) * 32 + (r & 31);
+}
 
 // The adapter of a row, -1 for none (also where the id names no adapter).
 __device__ __forceinline__ int adapter_of(const int32_t *ids, int64_t id_rows, int count, int64_t row, int64_t m) {

@@ -25,8 +25,6 @@
 namespace tu {
 namespace {
 
-constexpr int kWaves = 8;
-constexpr int kThreads = 64 * kWaves;
 
 __device__ __forceinline__ bf16x8 codes_to_bf16(uint32_t lo, uint32_t hi) {
     u32x4 out;
@@ -41,9 +39,10 @@ __device__ __forceinline__ bf16x8 codes_to_bf16(uint32_t lo, uint32_t hi) {
     return __builtin_bit_cast(bf16x8, out);
 }
 
-// kRanks: ranks of a workgroup; kRowFrags: its 16-row fragments.
-template <int kRanks, int kRowFrags>
-__global__ __launch_bounds__(kThreads) void adapter_down_kernel(const int8_t *__restrict__ a, const float *__restrict__ as,
+// kRanks: ranks of a workgroup; kRowFrags: its 16-row fragments; kWaves: waves
+// that share K.
+template <int kRanks, int kRowFrags, int kWaves>
+__global__ __launch_bounds__(64 * kWaves) void adapter_down_kernel(const int8_t *__restrict__ a, const float *__restrict__ as,
                                                                 const uint16_t *__restrict__ down,
                                                                 const float *__restrict__ scaling, Adapters ad, int slots,
                                                                 uint16_t *__restrict__ h, int64_t m, int64_t k) {
@@ -137,9 +136,9 @@ __global__ __launch_bounds__(kThreads) void adapter_down_kernel(const int8_t *__
                     lo[e] = hw_bf16x2_bits(v[2 * e] - __uint_as_float(hi[e] << 16),
                                            v[2 * e + 1] - __uint_as_float(hi[e] & 0xffff0000u));
                 }
-                uint16_t *dst = h + row * 2 * ad.rank + rank;
+                uint16_t *dst = h + h_at(row, ad.rank, rank);
                 *reinterpret_cast<u32x2 *>(dst) = hi;
-                *reinterpret_cast<u32x2 *>(dst + ad.rank) = lo;
+                *reinterpret_cast<u32x2 *>(dst + kLowTerm) = lo;
             }
         }
         __syncthreads();
@@ -162,14 +161,14 @@ int32_t launch_down(const int8_t *a, const float *a_scale, const uint16_t *down,
     const int slots = static_cast<int>(std::min<int64_t>(ad.count, std::min<int64_t>(16, std::max<int64_t>(2, cus / tiles()))));
     const dim3 grid(static_cast<unsigned>((m + rows - 1) / rows), static_cast<unsigned>((ad.rank + ranks - 1) / ranks),
                     static_cast<unsigned>(slots));
-#define TU_DOWN(R, F) adapter_down_kernel<R, F><<<grid, kThreads, 0, st>>>(a, a_scale, down, scaling, ad, slots, h, m, k)
-    if (rows == 16) TU_DOWN(16, 1);
+#define TU_DOWN(R, F, W) adapter_down_kernel<R, F, W><<<grid, 64 * W, 0, st>>>(a, a_scale, down, scaling, ad, slots, h, m, k)
+    if (rows == 16) TU_DOWN(16, 1, 8);
     else if (rows == 64) {
-        if (ranks == 16) TU_DOWN(16, 4);
-        else TU_DOWN(32, 4);
-    } else if (ranks == 16) TU_DOWN(16, 2);
-    else if (ranks == 32) TU_DOWN(32, 2);
-    else TU_DOWN(64, 2);
+        if (ranks == 16) TU_DOWN(16, 4, 8);
+        else TU_DOWN(32, 4, 8);
+    } else if (ranks == 16) TU_DOWN(16, 2, 8);
+    else if (ranks == 32) TU_DOWN(32, 2, 8);
+    else TU_DOWN(64, 2, 8);
 #undef TU_DOWN
     return check_launch("tu_int8_gemm_adapters");
 }

@@ -333,10 +333,10 @@ struct RowAdapters {
             for (int j = 0; j < kFragsM; ++j) {
                 const int r = r0 + 32 * c + 8 * g;
                 const bool in = id[j] >= 0 && r < ad.rank;
-                const uint16_t *src = ad.h + (in ? (row_base + 16 * j + frow) * 2 * ad.rank + r : 0);
+                const uint16_t *src = ad.h + (in ? h_at(row_base + 16 * j + frow, ad.rank, r) : 0);
 #pragma unroll
                 for (int t = 0; t < 2; ++t) {
-                    u32x4 v = *reinterpret_cast<const u32x4 *>(src + t * ad.rank);
+                    u32x4 v = *reinterpret_cast<const u32x4 *>(src + t * kLowTerm);
                     x.h[c][t][j] = __builtin_bit_cast(bf16x8, in ? v : u32x4{0, 0, 0, 0});
                 }
             }
@@ -1117,7 +1117,7 @@ extern "C" int32_t tu_int8_gemm_bf16_residual(const int8_t *a, const int8_t *w, 
 }
 
 extern "C" int64_t tu_int8_gemm_adapters_workspace(int64_t m, int64_t rank) {
-    return m > 0 && rank > 0 ? m * rank * 4 : 0;
+    return m > 0 && rank > 0 ? (m + 15) / 16 * ((rank + 31) / 32) * (2 * tu::kLowTerm * 2) : 0;
 }
 
 extern "C" int32_t tu_int8_gemm_adapters(const int8_t *a, const int8_t *w, const float *a_scale, const float *w_scale,
