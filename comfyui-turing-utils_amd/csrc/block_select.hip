@@ -287,17 +287,20 @@ __device__ __forceinline__ double wave_score(const double *__restrict__ mq, cons
     return s;
 }
 
+template <int kBlocks>
+constexpr int kChooseThreads = kBlocks <= 128 ? 1024 : 512;
+
 // Approximate scores of 16 query blocks and all key blocks of one head into
 // LDS; then a wave per query block makes the choice.
 // Up to 512 key blocks three workgroups fit a CU, so that the 640 of 40 heads
 // and 256 query blocks all run at once (two: 65 us for 60).
 template <int D, int kBlocks>
-__global__ __launch_bounds__(kSelectThreads, kBlocks <= 512 ? 6 : 2) void block_choose_kernel(Means mq, Means mk, Choice c, uint32_t hq,
+__global__ __launch_bounds__(kChooseThreads<kBlocks>, kBlocks <= 512 ? 6 : 2) void block_choose_kernel(Means mq, Means mk, Choice c, uint32_t hq,
                                                                       uint32_t groups, uint32_t nqb, uint32_t nkb,
                                                                       int lq, int lk, const int32_t *__restrict__ q_len,
                                                                       const int32_t *__restrict__ k_len,
                                                                       int32_t *__restrict__ index) {
-    constexpr int kWaves = kSelectThreads / 64, kParts = kBlocks / 64, kChunks = D / 32;
+    constexpr int kWaves = kChooseThreads<kBlocks> / 64, kParts = kBlocks / 64, kChunks = D / 32;
     __shared__ float scores[kTileQ * kBlocks];  // [query block][key block]
     const int lane = threadIdx.x & 63;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -554,8 +557,8 @@ int32_t launch_select(const Side &q, const Side &k, int64_t batch, int64_t hq, i
     const auto hq32 = static_cast<uint32_t>(hq), groups = static_cast<uint32_t>(hq / hkv);
     const int lq = static_cast<int>(q.len), lk = static_cast<int>(k.len);
 #define TU_SELECT(BLOCKS)                                                                                              \
-    block_choose_kernel<D, BLOCKS><<<grid, kSelectThreads, 0, st>>>(mq, mk, c, hq32, groups, nqb, nkb, lq, lk,         \
-                                                                    q.lengths, k.lengths, index)
+    block_choose_kernel<D, BLOCKS><<<grid, kChooseThreads<BLOCKS>, 0, st>>>(mq, mk, c, hq32, groups, nqb, nkb, lq, lk, \
+                                                                            q.lengths, k.lengths, index)
     if (nkb <= 128) TU_SELECT(128);
     else if (nkb <= 512) TU_SELECT(512);
     else if (nkb <= 1024) TU_SELECT(1024);
