@@ -144,11 +144,12 @@ def turing_int8_linear_adapters(
     ``torch.ops.turing_utils.int8_linear_adapters``; it has no backward."""
     args = (activation, weight, activation_scale, weight_scale, bias, down, up, scaling, adapter_ids, adapter_rows,
             residual, gate, gate_rows)
-    if torch.compiler.is_compiling() or not activation.is_cuda:
-        return _int8_linear_adapters_op(*args)
-    out = _lib.host_calls().int8_linear_adapters(*args, _compute_units(activation.device),
-                                                 _lib.raw_stream(activation.get_device()))
-    return _linear_adapters(*args) if out is None else out
+    if not torch.compiler.is_compiling() and activation.is_cuda:
+        out = _lib.host_calls().int8_linear_adapters(*args, _compute_units(activation.device),
+                                                     _lib.raw_stream(activation.get_device()))
+        if out is not None:
+            return out
+    return _int8_linear_adapters_op(*args)
 
 
 _R4 = ((1, 1, 1, -1), (1, 1, -1, 1), (1, -1, 1, 1), (-1, 1, 1, 1))

@@ -149,15 +149,13 @@ def select_key_blocks(
     the lower j."""
     args = (tensor_layout, int(keep), bool(is_causal), int(sink_blocks), int(local_blocks), int(blkq), int(blkk),
             query_lengths, key_lengths)
-    if torch.compiler.is_compiling() or not query_int8.is_cuda:
-        return sage_block_select(query_int8, query_scale, key_int8, key_scale, *args)
-    if tensor_layout in ("HND", "NHD"):
+    if tensor_layout in ("HND", "NHD") and query_int8.is_cuda and not torch.compiler.is_compiling():
         index = _lib.host_calls().select_key_blocks(query_int8, query_scale, key_int8, key_scale,
                                                     tensor_layout == "NHD", *args[1:],
                                                     _lib.raw_stream(query_int8.get_device()))
         if index is not None:
             return index
-    return _select(query_int8, query_scale, key_int8, key_scale, *args)
+    return sage_block_select(query_int8, query_scale, key_int8, key_scale, *args)
 
 
 def _check_attend(query_int8, query_scale, key_int8, key_scale, value_t, block_index, tensor_layout, blkq, blkk):
@@ -272,15 +270,13 @@ def key_block_attention(
     tensors = (query_int8, query_scale, key_int8, key_scale, value_t, block_index)
     args = (tensor_layout, bool(is_causal), -1.0 if sm_scale is None else float(sm_scale), int(blkq), int(blkk),
             query_lengths, key_lengths)
-    if torch.compiler.is_compiling() or not query_int8.is_cuda:
-        return sage_block_attention(*tensors, *args)
-    if tensor_layout in ("HND", "NHD"):
+    if tensor_layout in ("HND", "NHD") and query_int8.is_cuda and not torch.compiler.is_compiling():
         out = _lib.host_calls().key_block_attention(*tensors, tensor_layout == "NHD", *args[1:],
                                                     _compute_units(query_int8.device),
                                                     _lib.raw_stream(query_int8.get_device()))
         if out is not None:
             return out
-    return _attend(*tensors, *args)
+    return sage_block_attention(*tensors, *args)
 
 
 def sparse_sageattn_from_prequantized(

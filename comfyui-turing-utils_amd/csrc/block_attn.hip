@@ -195,7 +195,8 @@ __global__ __launch_bounds__(kBlockThreads, kWgsPerCu<D>) void block_attn_kernel
     const uint16_t *vtp = vt + static_cast<int64_t>(b * hkv + hk) * D * lpad;
     const float *ks_row = k_scale + static_cast<int64_t>(b * hkv + hk) * nbk;
     const __amdgpu_buffer_rsrc_t srs = make_rsrc(ks_row, nbk * 4);
-    const __amdgpu_buffer_rsrc_t krs = make_rsrc(kp, static_cast<uint32_t>(lk * k_sl));
+    // to the last row's end, whatever the stride (one row's may be anything)
+    const __amdgpu_buffer_rsrc_t krs = make_rsrc(kp, static_cast<uint32_t>((lk - 1) * k_sl + D));
     const __amdgpu_buffer_rsrc_t vrs = make_rsrc(vtp, static_cast<uint32_t>(D * lpad * 2));
     const LaneGeom<D> gm = lane_geom<D>(wave, lane, k_sl, lpad);
     const uint32_t k_sl32 = static_cast<uint32_t>(k_sl);
@@ -542,7 +543,7 @@ extern "C" int32_t tu_sage_block_attn(const int8_t *q8, const float *q_scale, in
     TU_REQUIRE(blkq > 0 && blkk > 0 && blkk % kBKey == 0 && ((blkk / kBKey) & (blkk / kBKey - 1)) == 0 &&
                    blkq <= 0x7fffffff && blkk <= 0x7fffffff,
                "block attention needs blkq > 0 and blkk = 64 * 2^n");
-    TU_REQUIRE(lk * k_sl < (int64_t{1} << 32) && dim * lpad * 2 < (int64_t{1} << 32),
+    TU_REQUIRE(k_sl >= 0 && q_sl >= 0 && lk * k_sl < (int64_t{1} << 32) && dim * lpad * 2 < (int64_t{1} << 32),
                "block attention: one head's K or V^T exceeds 4 GiB of addressable bytes");
     TU_REQUIRE(q8 && q_scale && k8 && k_scale && vt_bf16 && index && o_bf16, "block attention pointers must be non-null");
     TU_REQUIRE(sm_scale > 0.0f, "block attention sm_scale must be positive");
