@@ -118,7 +118,9 @@ __device__ __forceinline__ void block_mean(const Side &s, uint32_t bh, uint32_t 
         ++since;
         if (since == per || i == kLoads - 1) {
             const int row = min(t0 + i * kRpl + r0, static_cast<int>(s.len) - 1);
-            const double f = static_cast<double>(scale[static_cast<uint32_t>(row) / g]);
+            // a scale behind the sample's end may be no number
+            const bool some = (i + 1 - since) * kRpl + r0 < valid;
+            const double f = some ? static_cast<double>(scale[static_cast<uint32_t>(row) / g]) : 0.0;
             const int bias = 128 * since;
 #pragma unroll
             for (int w = 0; w < 4; ++w) {

@@ -101,3 +101,26 @@ def test_both_routes_of_the_adapters(gpu_device):
         wide = torch.zeros(m, 384 + 16, dtype=torch.int8, device=gpu_device)
         wide[:, :384] = a["activation"]
         assert torch.equal(want, kernel.turing_int8_linear_adapters(**dict(a, activation=wide[:, :384])))
+
+
+@pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("blkq,blkk", [(16, 64), (32, 128), (128, 64)])
+def test_scales_behind_the_end_are_not_seen(gpu_device, d, blkq, blkk):
+    """Scale groups that begin at or behind a sample's end hold NaN and infinity."""
+    dev = gpu_device
+    g = torch.Generator().manual_seed(d + blkq)
+    q8, qs = ref.codes(3, 2, 300, d, blkq, g, dev)
+    k8, ks = ref.codes(3, 2, 700, d, blkk, g, dev)
+    ql, kl = (torch.tensor(x, dtype=torch.int32, device=dev) for x in ([300, 131, 17], [700, 130, 65]))
+    want = ref.select(q8, qs, k8, ks, 2, "HND", False, 0, 0, blkq, blkk, ql, kl)
+    vt = torch.randn(3, 2, d, 704, generator=g).to(torch.bfloat16).to(dev)
+    kw = dict(blkq=blkq, blkk=blkk, query_lengths=ql, key_lengths=kl)
+    clean = turing_sage.key_block_attention(q8, qs, k8, ks, vt, want.to(dev), **kw)
+    for scales, lengths, blk in ((qs, ql, blkq), (ks, kl, blkk)):
+        first = torch.arange(scales.size(2), device=dev) * blk
+        behind = (first >= lengths[:, None, None]).expand_as(scales)
+        scales[behind] = torch.tensor([float("nan"), float("inf")], device=dev)[torch.arange(int(behind.sum()), device=dev) % 2]
+    got = turing_sage.select_key_blocks(q8, qs, k8, ks, keep=2, **kw)
+    assert torch.equal(got.cpu(), want)
+    out = turing_sage.key_block_attention(q8, qs, k8, ks, vt, got, **kw)
+    assert torch.equal(out, clean) and torch.isfinite(out).all()
