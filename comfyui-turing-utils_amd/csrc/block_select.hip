@@ -43,7 +43,7 @@ constexpr int kMaxLdsBlocks = 2048;  // key blocks whose keys fit LDS (16 rows o
 // |q| |k|, and 384 sums in fp32, rounded or cut, under 2^-14.4 of it: 2^-13.4.
 constexpr float kScoreError = 0x1p-13f;
 
-constexpr int kFewOpen = 8;  // undecided blocks that a wave scores one after the other
+constexpr int kFewOpen = 8;  // undecided blocks that 16 lanes score each
 
 // What block_mean_kernel leaves of one side's blocks: fp64 mean rows, the same
 // as bf16 terms hi and lo, and their lengths (rounded up).  The terms stand as
@@ -279,13 +279,18 @@ __device__ __forceinline__ double exact_score(const double *__restrict__ mq, con
     return s;
 }
 
-// The same by the whole wave, every lane a part of the channels.
+// The same by 16 lanes, every one a part of the channels.
 template <int D>
-__device__ __forceinline__ double wave_score(const double *__restrict__ mq, const double *__restrict__ mk, int lane) {
-    double s = mq[lane] * mk[lane];
-    if constexpr (D == 128) s = __builtin_fma(mq[lane + 64], mk[lane + 64], s);
+__device__ __forceinline__ double group_score(const double *__restrict__ mq, const double *__restrict__ mk, int lc) {
+    double s = 0.0;
 #pragma unroll
-    for (int d = 1; d < 64; d <<= 1) s += __shfl_xor(s, d);
+    for (int d = 2 * lc; d < D; d += 32) {
+        const f64x2 x = *reinterpret_cast<const f64x2 *>(mq + d), y = *reinterpret_cast<const f64x2 *>(mk + d);
+        s = __builtin_fma(x[0], y[0], s);
+        s = __builtin_fma(x[1], y[1], s);
+    }
+#pragma unroll
+    for (int d = 1; d < 16; d <<= 1) s += __shfl_xor(s, d);
     return s;
 }
 
@@ -331,6 +336,10 @@ __global__ __launch_bounds__(kChooseThreads<kBlocks>, kBlocks <= 512 ? 6 : 2) vo
         longest = fmaxf(longest, 64 * p + lane < most ? mk.norm[k_row + 64 * p + lane] : 0.0f);
 #pragma unroll
     for (int d = 1; d < 64; d <<= 1) longest = fmaxf(longest, __shfl_xor(longest, d));
+    constexpr int kRowsOfWave = kTileQ / kWaves;
+    float norms[kRowsOfWave];
+#pragma unroll
+    for (int x = 0; x < kRowsOfWave; ++x) norms[x] = mq.norm[q_row + min(i0 + wave + x * kWaves, static_cast<int>(nqb) - 1)];
     for (int j0 = 16 * wave; j0 < most; j0 += 16 * kWaves) {
         const int j = j0 + lc;
         const uint16_t *ks = k_split + static_cast<int64_t>(j0) * 2 * D;
@@ -352,8 +361,8 @@ __global__ __launch_bounds__(kChooseThreads<kBlocks>, kBlocks <= 512 ? 6 : 2) vo
         for (int r = 0; r < 4; ++r) scores[(4 * g + r) * kBlocks + j] = acc[r];
     }
     __syncthreads();
-    for (int r = wave; r < kTileQ; r += kWaves) {
-        const int i = i0 + r;
+    for (int x = 0; x < kRowsOfWave; ++x) {
+        const int r = wave + x * kWaves, i = i0 + r;
         if (i >= static_cast<int>(nqb)) break;
         const int n = visible_blocks(i, q_end, k_end, c.causal);
         const int take = min(static_cast<int>(c.keep), n), width = static_cast<int>(c.width);
@@ -369,19 +378,19 @@ __global__ __launch_bounds__(kChooseThreads<kBlocks>, kBlocks <= 512 ? 6 : 2) vo
 #pragma unroll
         for (int p = 0; p < kParts; ++p) {
             const int j = 64 * p + lane;
-            const float x = j < n ? scores[r * kBlocks + j] : 0.0f;
+            const float y = j < n ? scores[r * kBlocks + j] : 0.0f;
             const bool first = j < n && forced(i, j, c);
-            finite = finite && __builtin_fabsf(x) < INFINITY;
-            v[p] = j >= n ? -INFINITY : first ? INFINITY : x;
-            lo = j < n && !first ? fminf(lo, x) : lo;
-            hi = j < n && !first ? fmaxf(hi, x) : hi;
+            finite = finite && __builtin_fabsf(y) < INFINITY;
+            v[p] = j >= n ? -INFINITY : first ? INFINITY : y;
+            lo = j < n && !first ? fminf(lo, y) : lo;
+            hi = j < n && !first ? fmaxf(hi, y) : hi;
             force += __builtin_popcountll(__ballot(first));
         }
         if (force >= take) {
             write_row<kParts>(1u, take, width, lane, 0, [&](int p) { return v[p] == INFINITY ? 1u : 0u; }, out);
             continue;
         }
-        const float norm = mq.norm[q_row + i], eps = kScoreError * norm * longest;
+        const float norm = x == 0 ? norms[0] : norms[kRowsOfWave - 1], eps = kScoreError * norm * longest;
         const double *row = mq.mean + (q_row + i) * D;
         uint64_t key[kParts];
         auto exact = [&](int p) {
@@ -394,7 +403,7 @@ __global__ __launch_bounds__(kChooseThreads<kBlocks>, kBlocks <= 512 ? 6 : 2) vo
                 const int j = 64 * p + lane;
                 const uint64_t e = j >= n ? 0ull : forced(i, j, c) ? ~0ull : exact(p);
 #pragma unroll
-                for (int x = 0; x < kParts; ++x) key[x] = x == p ? e : key[x];
+                for (int y = 0; y < kParts; ++y) key[y] = y == p ? e : key[y];
             }
             const uint64_t t = threshold<kParts, uint64_t>(take, 0, [&](int p) { return key[p]; });
             write_row<kParts>(t, take, width, lane, 0, [&](int p) { return key[p]; }, out);
@@ -436,23 +445,38 @@ __global__ __launch_bounds__(kChooseThreads<kBlocks>, kBlocks <= 512 ? 6 : 2) vo
             write_row<kParts>(1u, take, width, lane, 0, [&](int p) { return v[p] >= outside ? 1u : 0u; }, out);
             continue;
         }
-        // A few open blocks in turn, a wave's work each; many, a lane's each.
+        // A few open blocks four at a time, one to 16 lanes; many, one to a lane.
         // (One way for a row: equal scores have to stay equal.)
+        if (open > kFewOpen) {
 #pragma unroll
-        for (int p = 0; p < kParts; ++p) {
-            const bool undecided = v[p] <= in && v[p] >= outside;
-            key[p] = v[p] > in ? ~0ull : 0ull;
-            uint64_t left = __ballot(undecided);
-            if (left == 0) continue;
-            if (open > kFewOpen) {
-                const uint64_t e = undecided ? exact(p) : 0ull;
-                key[p] = undecided ? e : key[p];
-                continue;
+            for (int p = 0; p < kParts; ++p) {
+                const bool undecided = v[p] <= in && v[p] >= outside;
+                key[p] = v[p] > in ? ~0ull : 0ull;
+                if (__any(undecided)) {
+                    const uint64_t e = undecided ? exact(p) : 0ull;
+                    key[p] = undecided ? e : key[p];
+                }
             }
-            for (; left != 0; left &= left - 1) {
-                const int x = __builtin_ctzll(left);
-                const uint64_t e = order_key(wave_score<D>(row, mk.mean + (k_row + 64 * p + x) * D, lane));
-                key[p] = lane == x ? e : key[p];
+        } else {
+            int mine[2] = {0, 0}, place[kParts], n_open = 0;  // of lane / 16's blocks; a block's place among the open
+#pragma unroll
+            for (int p = 0; p < kParts; ++p) {
+                uint64_t left = __ballot(v[p] <= in && v[p] >= outside);
+                place[p] = n_open + __builtin_popcountll(left & ((1ull << lane) - 1));
+                for (; left != 0; left &= left - 1, ++n_open)
+                    if ((lane >> 4) == (n_open & 3)) mine[n_open >> 2] = 64 * p + __builtin_ctzll(left);
+            }
+            double sum[2];
+#pragma unroll
+            for (int q = 0; q < 2; ++q) sum[q] = group_score<D>(row, mk.mean + (k_row + mine[q]) * D, lc);
+#pragma unroll
+            for (int p = 0; p < kParts; ++p) {
+                const bool undecided = v[p] <= in && v[p] >= outside;
+                key[p] = v[p] > in ? ~0ull : 0ull;
+                if (!__any(undecided)) continue;
+                const int from = 16 * (place[p] & 3);
+                const double one = __shfl(sum[0], from), two = __shfl(sum[1], from);
+                key[p] = undecided ? order_key(place[p] < 4 ? one : two) : key[p];
             }
         }
         const uint64_t t = threshold<kParts, uint64_t>(take, 0, [&](int p) { return key[p]; });
