@@ -253,9 +253,10 @@ __global__ __launch_bounds__(kBlockThreads, kWgsPerCu<D>) void block_attn_kernel
         // Compaction of the segment.  Ascending lists with nothing but -1 behind
         // them need no running maximum.
         bool ordered = true;
-        int prev[4];
+        int prev[4] = {};
 #pragma unroll
         for (int c = 0; c < 4; ++c) {
+            if (64 * c >= end - seg) break;  // all -1 from here on
             prev[c] = __shfl_up(e[c], 1);
             const int last = c ? __builtin_amdgcn_readlane(e[c - (c > 0)], 63) : before;
             if (lane == 0) prev[c] = last;
@@ -279,6 +280,7 @@ __global__ __launch_bounds__(kBlockThreads, kWgsPerCu<D>) void block_attn_kernel
         int n = 0, whole = 0, top = before;
 #pragma unroll
         for (int c = 0; c < 4; ++c) {
+            if (64 * c >= end - seg) break;
             const bool counts = e[c] > prev[c] && e[c] >= 0 && e[c] < blocks;
             const uint64_t mask = __ballot(counts);
             if (counts) list[n + __builtin_popcountll(mask & ((1ull << lane) - 1))] = e[c];
@@ -291,9 +293,11 @@ __global__ __launch_bounds__(kBlockThreads, kWgsPerCu<D>) void block_attn_kernel
         whole = __builtin_amdgcn_readfirstlane(whole);
 
         auto block_at = [&](int t) { return __builtin_amdgcn_readfirstlane(list[min(t, n - 1)]); };
+        if (seg + kSegment < end) {
 #pragma unroll
-        for (int d = 1; d < 64; d <<= 1) top = max(top, __shfl_xor(top, d));
-        before = top;
+            for (int d = 1; d < 64; d <<= 1) top = max(top, __shfl_xor(top, d));
+            before = top;
+        }
         if (n == 0) continue;
 
         auto softmax = [&](int t, float scale, auto mask_tag) {
