@@ -18,9 +18,10 @@
 // more than 2 eps above the approximate threshold are in, those more than 2 eps
 // below are out, and only the others (one or two of 512) are computed in fp64.
 //
-// What bounds it at B1 H40 L32760 D128 (336 MB of codes): the means take 82 us,
-// 382 MB read and written at 4.7 TB/s, and the choice 46 us: 22 of products, 12
-// of fp64 scores, whose loads wait one after the other, the rest the search.
+// What bounds it at B1 H40 L32760 D128 (336 MB of codes): the means take 81 us,
+// 384 MB read and written at 4.7 TB/s, and the choice 39 us: 16 of products, 6
+// for the scores' way back from LDS, 9 of search, 8 of fp64 scores and lists;
+// past the products it is bound by instructions, comparisons and bit counts.
 // With every score from fp64 MFMAs and a search bit by bit it was 69 + 73 us.
 #include "tu_common.h"
 #include "attn_plan.h"
@@ -390,24 +391,17 @@ __global__ __launch_bounds__(kChooseThreads<kBlocks>, kBlocks <= 512 ? 6 : 2) vo
             write_row<kParts>(1u, take, width, lane, 0, [&](int p) { return v[p] == INFINITY ? 1u : 0u; }, out);
             continue;
         }
-        const float norm = x == 0 ? norms[0] : norms[kRowsOfWave - 1], eps = kScoreError * norm * longest;
+        const float norm = x == 0 ? norms[0] : norms[kRowsOfWave - 1];
+        float eps = kScoreError * norm * longest;
         const double *row = mq.mean + (q_row + i) * D;
-        uint64_t key[kParts];
-        auto exact = [&](int p) {
-            return order_key(exact_score<D>(row, mk.mean + (k_row + 64 * p + lane) * D));
-        };
         // Sums in fp32 that left its range, or neared its smallest numbers, or
-        // means of NaN say nothing: every score in fp64.
+        // means of NaN say nothing: all blocks that are not forced are open.
         if (!(__all(finite) && norm > 0x1p-40f && norm < 0x1p60f && longest > 0x1p-40f && longest < 0x1p60f)) {
-            for (int p = 0; p < kParts; ++p) {
+            each_part<kParts>(0, [&](int p) {
                 const int j = 64 * p + lane;
-                const uint64_t e = j >= n ? 0ull : forced(i, j, c) ? ~0ull : exact(p);
-#pragma unroll
-                for (int y = 0; y < kParts; ++y) key[y] = y == p ? e : key[y];
-            }
-            const uint64_t t = threshold<kParts, uint64_t>(take, 0, [&](int p) { return key[p]; });
-            write_row<kParts>(t, take, width, lane, 0, [&](int p) { return key[p]; }, out);
-            continue;
+                if (j < n && !forced(i, j, c)) v[p] = 0.0f;
+            });
+            lo = hi = eps = 0.0f;
         }
         // The last score taken lies in lo .. hi: by interpolation and halving
         // in turn, until the two are eps apart or just `take` reach lo.
@@ -435,6 +429,7 @@ __global__ __launch_bounds__(kChooseThreads<kBlocks>, kBlocks <= 512 ? 6 : 2) vo
                 lo = hi;
             }
         }
+        // blocks above `in` are taken, those below `outside` not
         const float in = hi + 2.25f * eps, outside = lo - 2.25f * eps;
         int sure = 0, open = 0;
         each_part<kParts>(0, [&](int p) {
@@ -445,39 +440,50 @@ __global__ __launch_bounds__(kChooseThreads<kBlocks>, kBlocks <= 512 ? 6 : 2) vo
             write_row<kParts>(1u, take, width, lane, 0, [&](int p) { return v[p] >= outside ? 1u : 0u; }, out);
             continue;
         }
-        // A few open blocks four at a time, one to 16 lanes; many, one to a lane.
-        // (One way for a row: equal scores have to stay equal.)
-        if (open > kFewOpen) {
-#pragma unroll
-            for (int p = 0; p < kParts; ++p) {
-                const bool undecided = v[p] <= in && v[p] >= outside;
-                key[p] = v[p] > in ? ~0ull : 0ull;
-                if (__any(undecided)) {
-                    const uint64_t e = undecided ? exact(p) : 0ull;
-                    key[p] = undecided ? e : key[p];
-                }
-            }
-        } else {
-            int mine[2] = {0, 0}, place[kParts], n_open = 0;  // of lane / 16's blocks; a block's place among the open
+        // A few open blocks: scored four at a time, 16 lanes each; lane t then
+        // holds the t-th and counts those before it.
+        if (open <= kFewOpen) {
+            int mine[kFewOpen / 4] = {}, found = 0;  // lane / 16's blocks
 #pragma unroll
             for (int p = 0; p < kParts; ++p) {
                 uint64_t left = __ballot(v[p] <= in && v[p] >= outside);
-                place[p] = n_open + __builtin_popcountll(left & ((1ull << lane) - 1));
-                for (; left != 0; left &= left - 1, ++n_open)
-                    if ((lane >> 4) == (n_open & 3)) mine[n_open >> 2] = 64 * p + __builtin_ctzll(left);
+                for (; left != 0; left &= left - 1, ++found)
+                    if ((lane >> 4) == (found & 3)) mine[found >> 2] = 64 * p + __builtin_ctzll(left);
             }
-            double sum[2];
+            double s[kFewOpen / 4];
 #pragma unroll
-            for (int q = 0; q < 2; ++q) sum[q] = group_score<D>(row, mk.mean + (k_row + mine[q]) * D, lc);
-#pragma unroll
-            for (int p = 0; p < kParts; ++p) {
+            for (int q = 0; q < kFewOpen / 4; ++q)
+                s[q] = __shfl(group_score<D>(row, mk.mean + (k_row + mine[q]) * D, lc), 16 * (lane & 3));
+            const uint64_t own = order_key(lane < 4 ? s[0] : s[1]);
+            int before = 0;
+            for (int t = 0; t < open; ++t) {
+                const uint64_t other = __shfl(own, t);
+                before += other > own || (other == own && t < lane) ? 1 : 0;
+            }
+            const uint64_t win = __ballot(lane < open && before < take - sure);
+            found = 0;
+            each_part<kParts>(0, [&](int p) {
                 const bool undecided = v[p] <= in && v[p] >= outside;
-                key[p] = v[p] > in ? ~0ull : 0ull;
-                if (!__any(undecided)) continue;
-                const int from = 16 * (place[p] & 3);
-                const double one = __shfl(sum[0], from), two = __shfl(sum[1], from);
-                key[p] = undecided ? order_key(place[p] < 4 ? one : two) : key[p];
-            }
+                const uint64_t all = __ballot(undecided);
+                const int place = found + __builtin_popcountll(all & ((1ull << lane) - 1));
+                if (undecided) v[p] = win >> place & 1 ? INFINITY : -INFINITY;
+                found += __builtin_popcountll(all);
+            });
+            write_row<kParts>(1u, take, width, lane, 0, [&](int p) { return v[p] > in ? 2u : 0u; }, out);
+            continue;
+        }
+        // Many: one to a lane.  (One way for a row: equal scores stay equal.)
+        uint64_t key[kParts];
+        each_part<kParts>(0, [&](int p) { key[p] = v[p] > in ? ~0ull : v[p] >= outside ? 1ull : 0ull; });
+#pragma clang loop unroll(disable)
+        for (int p = 0; p < kParts; ++p) {
+            bool undecided = false;
+#pragma unroll
+            for (int y = 0; y < kParts; ++y) undecided = y == p ? key[y] == 1ull : undecided;
+            if (!__any(undecided)) continue;
+            const uint64_t e = undecided ? order_key(exact_score<D>(row, mk.mean + (k_row + 64 * p + lane) * D)) : 0ull;
+#pragma unroll
+            for (int y = 0; y < kParts; ++y) key[y] = y == p && undecided ? e : key[y];
         }
         const uint64_t t = threshold<kParts, uint64_t>(take, 0, [&](int p) { return key[p]; });
         write_row<kParts>(t, take, width, lane, 0, [&](int p) { return key[p]; }, out);
