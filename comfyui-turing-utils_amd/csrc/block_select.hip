@@ -303,21 +303,21 @@ constexpr int kChooseThreads = kBlocks <= 128 ? 1024 : 512;
 // Up to 512 key blocks three workgroups fit a CU, so that the 640 of 40 heads
 // and 256 query blocks all run at once (two: 65 us for 60).
 template <int D, int kBlocks>
-__global__ __launch_bounds__(kChooseThreads<kBlocks>, kBlocks <= 512 ? 6 : 2) void block_choose_kernel(Means mq, Means mk, Choice c, uint32_t hq,
-                                                                      uint32_t groups, uint32_t nqb, uint32_t nkb,
-                                                                      int lq, int lk, const int32_t *__restrict__ q_len,
-                                                                      const int32_t *__restrict__ k_len,
-                                                                      int32_t *__restrict__ index) {
+__global__ __launch_bounds__(kChooseThreads<kBlocks>, kBlocks <= 512 ? 6 : 2) void block_choose_kernel(
+    Means mq, Means mk, Choice c, uint32_t hq, uint32_t groups, uint32_t nqb, uint32_t nkb, int lq, int lk,
+    const int32_t *__restrict__ q_len, const int32_t *__restrict__ k_len, int32_t *__restrict__ index) {
     constexpr int kWaves = kChooseThreads<kBlocks> / 64, kParts = kBlocks / 64, kChunks = D / 32;
     __shared__ float scores[kTileQ * kBlocks];  // [query block][key block]
     const int lane = threadIdx.x & 63;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int lc = lane & 15, g = lane >> 4;
     const uint32_t tiles = (nqb + kTileQ - 1) / kTileQ;
-    // a head's tiles on one die: its key blocks are read once into that die's L2
-    const uint32_t tile = xcd_chunk(blockIdx.x, gridDim.x), bh = tile / tiles;
+    // A head's tiles, and the heads of a K/V head, on one die, whose L2 reads the
+    // key blocks once; a short sample's tiles are spread over all dies.
+    const uint32_t tile = xcd_chunk(blockIdx.x, gridDim.x), order = tile / tiles, hkv = hq / groups;
+    const uint32_t batch = gridDim.x / (tiles * hq), b = order / groups % batch;
+    const uint32_t h = order / groups / batch * groups + order % groups, bh = b * hq + h;
     const int i0 = static_cast<int>(tile % tiles) * kTileQ;
-    const uint32_t b = bh / hq, h = bh % hq, hkv = hq / groups;
     const int q_end = sample_end(q_len, b, lq), k_end = sample_end(k_len, b, lk);
     const int64_t q_row = static_cast<int64_t>(bh) * nqb, k_row = static_cast<int64_t>(b * hkv + h / groups) * nkb;
     // (rows behind the last block hold anything and are not used)
