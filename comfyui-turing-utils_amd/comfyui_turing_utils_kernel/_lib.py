@@ -167,7 +167,7 @@ SIGNATURES: dict[str, tuple[object, list[object]]] = {
     "tu_int8_gemm_adapters": (
         _i32,
         [_c_void_p, _c_void_p, _c_void_p, _c_void_p, _c_void_p, _c_void_p, _c_void_p, _c_void_p, _c_void_p, _i64,
-         _i64, _i64, _c_void_p, _c_void_p, _i64, _c_void_p, _i64, _i64, _i64, _i32, _c_void_p, _i64, _c_void_p],
+         _i64, _i64, _i64, _c_void_p, _c_void_p, _i64, _c_void_p, _i64, _i64, _i64, _i32, _c_void_p, _i64, _c_void_p],
     ),
     "tu_sage_block_select_workspace": (_i64, [_i64, _i64, _i64, _i64, _i64, _i64]),
     "tu_sage_block_select": (

@@ -28,14 +28,17 @@ from .turing_sage.core import _compute_units
 RANK_MULTIPLE = 8  # the kernels read 16-byte pieces of a rank
 MAX_RANK = 4096
 
-def _check_adapters(m, n, k, down, up, scaling, adapter_ids, adapter_rows) -> None:
+def _check_adapters(m, n, k, down, up, scaling, adapter_ids, adapter_rows, parts=1) -> None:
     if down.dtype != torch.bfloat16 or up.dtype != torch.bfloat16:
         raise TypeError("adapter weights must be bfloat16")
-    if down.dim() != 3 or up.dim() != 3 or down.shape[2] != k or up.shape != (down.shape[0], n, down.shape[1]):
-        raise ValueError(f"adapters must be down [count, rank, {k}] and up [count, {n}, rank], got "
-                         f"{tuple(down.shape)} and {tuple(up.shape)}")
+    if parts < 1 or (parts > 1 and n % (16 * parts)):
+        raise ValueError(f"{n} columns do not make {parts} equal parts of a multiple of 16")
+    if down.dim() != 3 or up.dim() != 3 or down.shape[2] != k \
+            or up.shape != (down.shape[0], n, down.shape[1] // parts) or down.shape[1] % parts:
+        raise ValueError(f"adapters must be down [count, rank, {k}] and up [count, {n}, "
+                         f"{'rank' if parts == 1 else f'rank / {parts}'}], got {tuple(down.shape)} and {tuple(up.shape)}")
     rank = down.shape[1]
-    if down.shape[0] < 1 or rank % RANK_MULTIPLE or not 0 < rank <= MAX_RANK:
+    if down.shape[0] < 1 or rank // parts % RANK_MULTIPLE or not 0 < rank <= MAX_RANK:
         raise ValueError(f"adapters need a count of at least 1 and a rank that is a multiple of {RANK_MULTIPLE} up to "
                          f"{MAX_RANK} (zero ranks pad), got {tuple(down.shape)}")
     if scaling.dtype != torch.float32 or scaling.shape != (down.shape[0],):
@@ -55,10 +58,10 @@ def _aligned(t: Optional[torch.Tensor]) -> Optional[torch.Tensor]:
 
 
 def _linear_adapters(activation, weight, activation_scale, weight_scale, bias, down, up, scaling, adapter_ids,
-                     adapter_rows, residual, gate, gate_rows):
+                     adapter_rows, residual, gate, gate_rows, parts):
     activation, weight, activation_scale, weight_scale, bias, m, n, k = _linear_args(
         activation, weight, activation_scale, weight_scale, bias)
-    _check_adapters(m, n, k, down, up, scaling, adapter_ids, adapter_rows)
+    _check_adapters(m, n, k, down, up, scaling, adapter_ids, adapter_rows, parts)
     if residual is not None:
         _check_residual(residual, gate, gate_rows, m, n)
     elif gate is not None:
@@ -80,7 +83,8 @@ def _linear_adapters(activation, weight, activation_scale, weight_scale, bias, d
         _lib.call(
             "tu_int8_gemm_adapters", activation.data_ptr(), weight.data_ptr(), activation_scale.data_ptr(),
             weight_scale.data_ptr(), _lib.ptr(bias), down.data_ptr(), up.data_ptr(), scaling.contiguous().data_ptr(),
-            adapter_ids.contiguous().data_ptr(), int(adapter_rows), rank, count, _lib.ptr(residual), _lib.ptr(gate),
+            adapter_ids.contiguous().data_ptr(), int(adapter_rows), rank, count, int(parts),
+            _lib.ptr(residual), _lib.ptr(gate),
             int(gate_rows) if gate is not None else 1, out.data_ptr(), m, n, k, cus, workspace.data_ptr(), nbytes,
             _lib.stream_of(device))
     return out
@@ -101,16 +105,18 @@ def _int8_linear_adapters_op(
     residual: torch.Tensor | None = None,
     gate: torch.Tensor | None = None,
     gate_rows: int = 1,
+    parts: int = 1,
 ) -> torch.Tensor:
     return _linear_adapters(activation, weight, activation_scale, weight_scale, bias, down, up, scaling, adapter_ids,
-                            adapter_rows, residual, gate, gate_rows)
+                            adapter_rows, residual, gate, gate_rows, parts)
 
 
 @_int8_linear_adapters_op.register_fake
 def _int8_linear_adapters_fake(activation, weight, activation_scale, weight_scale, bias, down, up, scaling,
-                               adapter_ids, adapter_rows=1, residual=None, gate=None, gate_rows=1):
+                               adapter_ids, adapter_rows=1, residual=None, gate=None, gate_rows=1,
+                               parts=1):
     (m, k), n = activation.shape, weight.size(0)
-    _check_adapters(m, n, k, down, up, scaling, adapter_ids, adapter_rows)
+    _check_adapters(m, n, k, down, up, scaling, adapter_ids, adapter_rows, parts)
     if residual is not None:
         _check_residual(residual, gate, gate_rows, m, n)
     return torch.empty((m, n), dtype=torch.bfloat16, device=activation.device)
@@ -130,6 +136,7 @@ def turing_int8_linear_adapters(
     residual: Optional[torch.Tensor] = None,
     gate: Optional[torch.Tensor] = None,
     gate_rows: int = 1,
+    parts: int = 1,
 ) -> torch.Tensor:
     """``int8_linear`` (or, with ``residual``, ``int8_linear_residual``) whose
     fp32 value gains each row's adapter before it is rounded:
@@ -140,10 +147,14 @@ def turing_int8_linear_adapters(
     [0, count) has no adapter and gets int8_linear's bits.  ``down`` bf16
     [count, rank, K] holds rotated rows (``LinearAdapters`` makes them), ``up``
     bf16 [count, N, rank], ``scaling`` fp32 [count], ``adapter_ids`` int32
-    [ceil(M / adapter_rows)]; the rank is a multiple of 8.  The op is
+    [ceil(M / adapter_rows)]; the rank is a multiple of 8.  With ``parts`` the
+    columns and the ranks are so many equal parts (of a multiple of 16 columns
+    and 8 ranks each), the columns of a part see its own ranks alone, and ``up``
+    is [count, N, rank / parts]: the projections of a fused q / k / v have
+    adapters of their own.  The op is
     ``torch.ops.turing_utils.int8_linear_adapters``; it has no backward."""
     args = (activation, weight, activation_scale, weight_scale, bias, down, up, scaling, adapter_ids, adapter_rows,
-            residual, gate, gate_rows)
+            residual, gate, gate_rows, parts)
     if not torch.compiler.is_compiling() and activation.is_cuda:
         out = _lib.host_calls().int8_linear_adapters(*args, _compute_units(activation.device),
                                                      _lib.raw_stream(activation.get_device()))
@@ -169,18 +180,20 @@ def _rotation(group: int, device) -> torch.Tensor:
 
 class LinearAdapters:
     """The adapters of one W8A8 linear, laid out for the kernels: ``down`` bf16
-    [count, rank, K] (rotated), ``up`` bf16 [count, N, rank], ``scaling`` fp32
-    [count].  Adapters of different ranks share the largest, padded with zeros."""
+    [count, rank, K] (rotated), ``up`` bf16 [count, N, rank / parts], ``scaling``
+    fp32 [count]; ``parts`` as in ``turing_int8_linear_adapters``.  Adapters of
+    different ranks share the largest, padded with zeros."""
 
-    def __init__(self, down: torch.Tensor, up: torch.Tensor, scaling: torch.Tensor, group: int = 128):
+    def __init__(self, down: torch.Tensor, up: torch.Tensor, scaling: torch.Tensor, group: int = 128, parts: int = 1):
         if group not in ops.SUPPORTED_GROUP_SIZES:
             raise ValueError(f"ConvRot group must be one of {ops.SUPPORTED_GROUP_SIZES}, got {group}")
         if down.dim() != 3 or up.dim() != 3:
-            raise ValueError("adapters must be down [count, rank, K] and up [count, N, rank]")
+            raise ValueError("adapters must be down [count, rank, K] and up [count, N, rank / parts]")
         # an empty list of rows: the shapes alone
         _check_adapters(0, up.shape[1], down.shape[2], down, up, scaling,
-                        torch.empty(0, dtype=torch.int32, device=down.device), 1)
+                        torch.empty(0, dtype=torch.int32, device=down.device), 1, parts)
         self.down, self.up, self.scaling, self.group = _aligned(down), _aligned(up), scaling.contiguous(), group
+        self.parts = parts
 
     @property
     def count(self) -> int:
@@ -220,17 +233,26 @@ class LinearAdapters:
     @staticmethod
     def concat(parts: "Sequence[LinearAdapters]") -> "LinearAdapters":
         """The adapters of ``W8A8Linear.concat``'s linear from those of its
-        parts (adapter i of each part together): ranks side by side, and each
-        part's output columns see its own ranks only.  Every part needs the
-        same scalings, as one file gives a model's layers."""
+        parts (adapter i of each part together): each part's output columns
+        see its own ranks only.  Equal parts of a multiple of 16 columns stay
+        parts, of the largest's rank; of others, ``up`` is padded with zeros.
+        Every part needs the same scalings, as one file gives a model's layers."""
         if not parts or len({(p.count, p.down.shape[2], p.group) for p in parts}) != 1:
             raise ValueError("concatenated adapters need one count, K and ConvRot group")
         if any(not torch.equal(p.scaling, parts[0].scaling) for p in parts[1:]):
             raise ValueError("concatenated adapters need the same scalings")
-        count, rank, n = parts[0].count, sum(p.rank for p in parts), sum(p.up.shape[1] for p in parts)
-        up = torch.zeros((count, n, rank), dtype=torch.bfloat16, device=parts[0].up.device)
+        if any(p.parts != 1 for p in parts):
+            raise ValueError("concatenated adapters cannot be concatenated again")
+        count, n = parts[0].count, sum(p.up.shape[1] for p in parts)
+        scaling, group = parts[0].scaling, parts[0].group
+        if len({p.up.shape[1] for p in parts}) == 1 and n % (16 * len(parts)) == 0:
+            most = max(p.rank for p in parts)
+            pad = torch.nn.functional.pad
+            return LinearAdapters(torch.cat([pad(p.down, (0, 0, 0, most - p.rank)) for p in parts], 1),
+                                  torch.cat([pad(p.up, (0, most - p.rank)) for p in parts], 1), scaling, group, len(parts))
+        up = torch.zeros((count, n, sum(p.rank for p in parts)), dtype=torch.bfloat16, device=parts[0].up.device)
         row = col = 0
         for p in parts:
             up[:, row:row + p.up.shape[1], col:col + p.rank] = p.up
             row, col = row + p.up.shape[1], col + p.rank
-        return LinearAdapters(torch.cat([p.down for p in parts], 1), up, parts[0].scaling, parts[0].group)
+        return LinearAdapters(torch.cat([p.down for p in parts], 1), up, scaling, group)

@@ -144,7 +144,7 @@ class W8A8Linear:
         if adapters is not None:
             return turing_int8_linear_adapters(codes, self.weight, scale, self.weight_scale, self.bias, adapters.down,
                                                adapters.up, adapters.scaling, adapter_ids, adapter_rows, residual, gate,
-                                               gate_rows)
+                                               gate_rows, adapters.parts)
         if residual is None:
             return torch.ops.turing_utils.int8_linear(codes, self.weight, scale, self.weight_scale, self.bias)
         return torch.ops.turing_utils.int8_linear_residual(codes, self.weight, scale, self.weight_scale, self.bias,

@@ -14,10 +14,13 @@ namespace tu {
 // last 32 are not written.
 struct Adapters {
     const uint16_t *h;
-    const uint16_t *up;    // bf16 [count][n][rank]
+    const uint16_t *up;    // bf16 [count][n][up_rank]
     const int32_t *ids;    // adapter of rows i * id_rows .. (i + 1) * id_rows - 1
     int64_t id_rows;
     int rank, count;
+    // The columns are parts of part_cols (a multiple of 16) side by side, and
+    // those of part p see the up_rank ranks from p * up_rank on.
+    int up_rank, part_cols;
 };
 
 // Place of a row's rank r in h; its low term lies kLowTerm values on.

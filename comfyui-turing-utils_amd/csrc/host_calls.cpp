@@ -417,12 +417,12 @@ PyObject *key_block_attention(PyObject *, PyObject *const *args, Py_ssize_t narg
 }
 
 // int8_linear_adapters(activation, weight, activation_scale, weight_scale, bias, down, up, scaling, adapter_ids,
-//                      adapter_rows, residual, gate, gate_rows, cus, stream)
+//                      adapter_rows, residual, gate, gate_rows, parts, cus, stream)
 PyObject *int8_linear_adapters(PyObject *, PyObject *const *args, Py_ssize_t nargs) {
     HANDLE_TH_ERRORS
-    int64_t id_rows, gate_rows, cus, stream;
-    if (nargs != 15 || !integer(args[9], &id_rows) || !integer(args[12], &gate_rows) || !integer(args[13], &cus) ||
-        !integer(args[14], &stream) || !THPVariable_CheckTypeExact(Py_TYPE(args[0])))
+    int64_t id_rows, gate_rows, parts, cus, stream;
+    if (nargs != 16 || !integer(args[9], &id_rows) || !integer(args[12], &gate_rows) || !integer(args[13], &parts) ||
+        !integer(args[14], &cus) || !integer(args[15], &stream) || !THPVariable_CheckTypeExact(Py_TYPE(args[0])))
         Py_RETURN_NONE;
     const c10::Device device = THPVariable_Unpack(args[0]).device();
     const Tensor *x, *w, *xs, *ws, *bias, *down, *up, *scaling, *ids, *residual, *gate;
@@ -441,8 +441,9 @@ PyObject *int8_linear_adapters(PyObject *, PyObject *const *args, Py_ssize_t nar
     for (const Tensor *t : {xs, ws, scaling})
         if (t->scalar_type() != at::kFloat || !t->is_contiguous()) Py_RETURN_NONE;
     if (m < 1 || k < 1 || k % 16 || k >= 131072 || n < 1 || n % 8 || w->size(1) != k || xs->numel() != m ||
-        ws->numel() != n || !aligned(*ws, 16) || (bias && bias->numel() != n) || count < 1 || rank < 1 || rank % 8 ||
-        rank > 4096 || down->size(2) != k || up->size(0) != count || up->size(1) != n || up->size(2) != rank ||
+        ws->numel() != n || !aligned(*ws, 16) || (bias && bias->numel() != n) || count < 1 || rank < 1 || parts < 1 ||
+        parts > rank || rank % (8 * parts) || (parts > 1 && n % (16 * parts)) || rank > 4096 || down->size(2) != k ||
+        up->size(0) != count || up->size(1) != n || up->size(2) != rank / parts ||
         scaling->dim() != 1 || scaling->size(0) != count || ids->scalar_type() != at::kInt || ids->dim() != 1 ||
         !ids->is_contiguous() || id_rows < 1 || ids->size(0) != ceil_div(m, id_rows) || (gate && !residual) ||
         (residual && (residual->dim() != 2 || residual->size(0) != m || residual->size(1) != n)) ||
@@ -457,7 +458,7 @@ PyObject *int8_linear_adapters(PyObject *, PyObject *const *args, Py_ssize_t nar
         if (tu_int8_gemm_adapters(x->data_ptr<int8_t>(), w->data_ptr<int8_t>(), xs->data_ptr<float>(),
                                   ws->data_ptr<float>(), bias ? bias->data_ptr<float>() : nullptr, down->data_ptr(),
                                   up->data_ptr(), scaling->data_ptr<float>(), ids->data_ptr<int32_t>(), id_rows, rank,
-                                  count, residual ? residual->data_ptr() : nullptr, gate ? gate->data_ptr() : nullptr,
+                                  count, parts, residual ? residual->data_ptr() : nullptr, gate ? gate->data_ptr() : nullptr,
                                   gate ? gate_rows : 1, out.data_ptr(), m, n, k, static_cast<int32_t>(cus),
                                   work.data_ptr(), bytes, reinterpret_cast<void *>(stream)))
             failed("tu_int8_gemm_adapters");

@@ -288,6 +288,12 @@ struct RowAdapters {
     bool more;               // there are others
     int64_t row_base, col_base, m, n;
     int frow, g;
+    int base;    // first rank of the columns at hand
+    bool parted; // the wave's columns are of more than one part
+
+    __device__ __forceinline__ int base_of(const Adapters &ad, int64_t col) const {
+        return static_cast<int>(static_cast<uint32_t>(min(col, n - 1)) / static_cast<uint32_t>(ad.part_cols)) * ad.up_rank;
+    }
 
     // The next adapter among the rows of `rest`, which lose its rows; -1 for none.
     __device__ __forceinline__ int take(uint64_t (&rest)[kFragsM]) const {
@@ -308,8 +314,10 @@ struct RowAdapters {
         for (int j = 0; j < kFragsM; ++j) id[j] = adapter_of(ad.ids, ad.id_rows, ad.count, row_base + 16 * j + frow, m);
     }
 
-    __device__ __forceinline__ void find(int64_t col_base_, int64_t n_, int g_) {
+    __device__ __forceinline__ void find(const Adapters &ad, int64_t col_base_, int cols, int64_t n_, int g_) {
         col_base = col_base_, n = n_, g = g_;
+        base = base_of(ad, col_base);
+        parted = base_of(ad, col_base + cols - 1) != base;
         uint64_t rest[kFragsM];
 #pragma unroll
         for (int j = 0; j < kFragsM; ++j) rest[j] = left[j] = __ballot(id[j] >= 0);
@@ -338,8 +346,8 @@ struct RowAdapters {
 #pragma unroll
             for (int j = 0; j < kFragsM; ++j) {
                 const int r = r0 + 32 * c + 8 * g;
-                const bool in = id[j] >= 0 && r < ad.rank;
-                const uint16_t *src = ad.h + (in ? h_at(row_base + 16 * j + frow, ad.rank, r) : 0);
+                const bool in = id[j] >= 0 && r < ad.up_rank;
+                const uint16_t *src = ad.h + (in ? h_at(row_base + 16 * j + frow, ad.rank, base + r) : 0);
 #pragma unroll
                 for (int t = 0; t < 2; ++t) {
                     u32x4 v = *reinterpret_cast<const u32x4 *>(src + t * kLowTerm);
@@ -358,9 +366,9 @@ struct RowAdapters {
 #pragma unroll
         for (int c = 0; c < kC; ++c) {
             const int r = r0 + 32 * c + 8 * g;
-            const bool in = which >= 0 && r < ad.rank;
+            const bool in = which >= 0 && r < ad.up_rank;
             const u32x4 v = *reinterpret_cast<const u32x4 *>(
-                ad.up + (static_cast<int64_t>(max(which, 0)) * n + min(col_base + 16 * i + frow, n - 1)) * ad.rank + (in ? r : 0));
+                ad.up + (static_cast<int64_t>(max(which, 0)) * n + min(col_base + 16 * i + frow, n - 1)) * ad.up_rank + (in ? r : 0));
             x.w[c] = __builtin_bit_cast(bf16x8, in ? v : u32x4{0, 0, 0, 0});
         }
     }
@@ -395,7 +403,7 @@ struct RowAdapters {
     __device__ __forceinline__ void add_any(f32x4 (&v)[kI][kFragsM], const Adapters &ad, int i) const {
         constexpr int kBatch = kFragsM >= 4 ? 1 : 4;
 #pragma clang loop unroll(disable)
-        for (int r0 = 0; r0 < ad.rank; r0 += 32) {
+        for (int r0 = 0; r0 < ad.up_rank; r0 += 32) {
             Held<1> x;
             load(x, ad, r0);
             uint64_t rest[kFragsM];
@@ -708,7 +716,7 @@ __global__ __launch_bounds__(kThreads, WPE) void int8_gemm_kernel(
         [[maybe_unused]] float *cols =
             reinterpret_cast<float *>(lds_mem + Tile<BM, BN>::lds_bytes(NST)) + (kAdapters ? wave * BN : 0);
         if constexpr (kAdapters) {
-            rows.find(col_base, n, g);
+            rows.find(ad, col_base, BN / 2, n, g);
 #pragma unroll
             for (int c = 0; c < BN / 2; c += 64) {
                 if (c + lane >= BN / 2) break;
@@ -841,18 +849,28 @@ __global__ __launch_bounds__(kThreads, WPE) void int8_gemm_kernel(
                     values(i, v);
                     store(i, v);
                 }
-            } else if (rows.whole && ad.rank <= 32) {
+            } else if (!rows.parted && rows.whole && ad.up_rank <= 32) {
                 held(one, std::true_type{});
-            } else if (rows.whole && ad.rank <= 64) {
+            } else if (!rows.parted && rows.whole && ad.up_rank <= 64) {
                 held(two, std::true_type{});
-            } else if (kFragsM > 1 && !rows.more && ad.rank <= 32) {
+            } else if (kFragsM > 1 && !rows.parted && !rows.more && ad.up_rank <= 32) {
                 held(one, std::false_type{});
-            } else if (kFragsM > 1 && kMma < 32 && !rows.more && ad.rank <= 64) {
+            } else if (kFragsM > 1 && kMma < 32 && !rows.parted && !rows.more && ad.up_rank <= 64) {
                 held(two, std::false_type{});
+            } else if (kFragsM == 1 && rows.parted) {
+#pragma unroll
+                for (int i = 0; i < kFragsN; ++i) {
+                    f32x4 v[1][kFragsM];
+                    values(i, v[0]);
+                    rows.base = rows.base_of(ad, col_base + 16 * i);
+                    rows.template add_any<1>(v, ad, i);
+                    store(i, v[0]);
+                }
             } else {
                 constexpr int kI = kFragsM == 1 ? kFragsN : 1;
 #pragma unroll
                 for (int i = 0; i < kFragsN; i += kI) {
+                    if constexpr (kI == 1) rows.base = rows.base_of(ad, col_base + 16 * i);
                     f32x4 v[kI][kFragsM];
 #pragma unroll
                     for (int c = 0; c < kI; ++c) values(i + c, v[c]);
@@ -1129,12 +1147,14 @@ extern "C" int64_t tu_int8_gemm_adapters_workspace(int64_t m, int64_t rank) {
 extern "C" int32_t tu_int8_gemm_adapters(const int8_t *a, const int8_t *w, const float *a_scale, const float *w_scale,
                                          const float *bias, const void *down_bf16, const void *up_bf16,
                                          const float *scaling, const int32_t *ids, int64_t id_rows, int64_t rank,
-                                         int64_t count, const void *residual_bf16, const void *gate_bf16,
+                                         int64_t count, int64_t parts, const void *residual_bf16, const void *gate_bf16,
                                          int64_t gate_rows, void *out_bf16, int64_t m, int64_t n, int64_t k,
                                          int32_t cus, void *workspace, int64_t workspace_bytes, void *stream) {
     using namespace tu;
     TU_REQUIRE(rank > 0 && rank % 8 == 0 && rank <= 4096, "adapter rank must be a positive multiple of 8 up to 4096, got %lld",
                static_cast<long long>(rank));
+    TU_REQUIRE(parts > 0 && rank % (8 * parts) == 0 && (parts == 1 || n % (16 * parts) == 0),
+               "adapter parts need ranks of a multiple of 8 and columns of a multiple of 16 each");
     TU_REQUIRE(count > 0 && count <= 0x7fffffff && id_rows > 0 && cus > 0,
                "adapter count, rows per id and compute units must be positive");
     TU_REQUIRE(down_bf16 && up_bf16 && scaling && ids, "adapter pointers must be non-null");
@@ -1151,7 +1171,7 @@ extern "C" int32_t tu_int8_gemm_adapters(const int8_t *a, const int8_t *w, const
     if (m == 0) return 0;
     auto *h = static_cast<uint16_t *>(workspace);
     const Adapters ad{h, static_cast<const uint16_t *>(up_bf16), ids, id_rows, static_cast<int>(rank),
-                      static_cast<int>(count)};
+                      static_cast<int>(count), static_cast<int>(rank / parts), static_cast<int>(n / parts)};
     if (launch_down(a, a_scale, static_cast<const uint16_t *>(down_bf16), scaling, ad, h, m, k, cus,
                     static_cast<hipStream_t>(stream)))
         return -1;

@@ -174,8 +174,11 @@ int32_t tu_int8_gemm_bf16_residual(const int8_t *a, const int8_t *w, const float
  * tu_int8_gemm_bf16_residual.  Codes are those of a rotated activation, so
  * down holds the adapter's rows rotated alike.  h is summed in fp32 and kept
  * as two bf16 terms (to 2^-16 of it).  down: bf16 [count, rank, k]; up: bf16
- * [count, n, rank]; scaling: fp32 [count]; ids: int32 [ceil(m / id_rows)];
- * rank a multiple of 8 up to 4096; down, up, residual and gate 16-byte
+ * [count, n, rank / parts]: the columns and the ranks are `parts` equal parts
+ * each (a multiple of 16 columns where there are several), and the columns of
+ * a part see that part's ranks, as projections side by side have adapters of
+ * their own; scaling: fp32 [count]; ids: int32 [ceil(m / id_rows)];
+ * rank a multiple of 8 * parts up to 4096; down, up, residual and gate 16-byte
  * aligned; the rest as above.  workspace: 16-byte aligned, at least
  * tu_int8_gemm_adapters_workspace(m, rank) bytes (h).  cus: the device's
  * compute units.  Two launches.  No counterpart in the reference. */
@@ -183,7 +186,7 @@ int64_t tu_int8_gemm_adapters_workspace(int64_t m, int64_t rank);
 int32_t tu_int8_gemm_adapters(const int8_t *a, const int8_t *w, const float *a_scale, const float *w_scale,
                               const float *bias, const void *down_bf16, const void *up_bf16,
                               const float *scaling, const int32_t *ids, int64_t id_rows, int64_t rank,
-                              int64_t count, const void *residual_bf16, const void *gate_bf16,
+                              int64_t count, int64_t parts, const void *residual_bf16, const void *gate_bf16,
                               int64_t gate_rows, void *out_bf16, int64_t m, int64_t n, int64_t k,
                               int32_t cus, void *workspace, int64_t workspace_bytes, void *stream);
 

@@ -44,13 +44,22 @@ def _plain(a):
     return torch.ops.turing_utils.int8_linear_residual(*args, a["residual"], a.get("gate"), a.get("gate_rows", 1))
 
 
+def _dense(up, parts):
+    """``up`` with zeros where a part's columns do not see a rank."""
+    count, n, rank = up.shape
+    out = torch.zeros(count, parts, n // parts, parts, rank, dtype=up.dtype, device=up.device)
+    for p in range(parts):
+        out[:, p, :, p] = up.view(count, parts, n // parts, rank)[:, p]
+    return out.view(count, n, parts * rank)
+
+
 def _check(a):
     m, k = a["activation"].shape
     print(f"[adapters] M{m} K{k} N{a['weight'].shape[0]} rank {a['down'].shape[1]} count {a['down'].shape[0]} "
           f"rows {a['adapter_rows']}", flush=True)
     got = kernel.turing_int8_linear_adapters(**a)
     want, bound = ref.linear(a["activation"], a["weight"], a["activation_scale"], a["weight_scale"], a["bias"], a["down"],
-                             a["up"], a["scaling"], a["adapter_ids"], a["adapter_rows"], a.get("residual"),
+                             _dense(a["up"], a.get("parts", 1)), a["scaling"], a["adapter_ids"], a["adapter_rows"], a.get("residual"),
                              a.get("gate"), a.get("gate_rows", 1))
     off = (got.double() - want).abs()
     assert got.dtype == torch.bfloat16 and bool((off <= bound).all()), float((off / bound).max())
@@ -80,6 +89,19 @@ def test_every_tile(gpu_device, m, n, residual):
 def test_many_rows(gpu_device, rank):
     """The tall tile of the down-projection, borders inside it."""
     _check(_inputs(gpu_device, 33001, 160, 64, rank, 5, 37, seed=rank))
+
+
+@pytest.mark.parametrize("m,n,rank,parts", [
+    (1, 32, 16, 2), (5, 144, 24, 3), (61, 240, 120, 3), (130, 96, 24, 3), (4096, 256, 64, 2), (512, 4800, 96, 3),
+    (1024, 1584, 192, 3), (1024, 8976, 96, 3), (2050, 2064, 120, 3), (4100, 4800, 192, 3), (4100, 4800, 96, 3),
+    (512, 10176, 240, 3), (4100, 5120, 128, 2)])
+@pytest.mark.parametrize("rows", [1, 1000])
+def test_parts(gpu_device, m, n, rank, parts, rows):
+    """Columns that see their own ranks, with borders of parts inside a wave's columns; every tile."""
+    a = _inputs(gpu_device, m, 256, n, rank, 3, rows, seed=n + rank, residual=rows > 1)
+    a["up"], a["parts"] = a["up"][..., :rank // parts].contiguous(), parts
+    got = _check(a)
+    assert torch.equal(got, torch.ops.turing_utils.int8_linear_adapters(**a))
 
 
 def test_sizes_reach_every_tile(gpu_device):

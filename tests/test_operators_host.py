@@ -103,6 +103,9 @@ def test_attention_refusals():
     (lambda a: a.update(adapter_ids=a["adapter_ids"].long()), "int32"),
     (lambda a: a.update(adapter_ids=a["adapter_ids"][:3]), "adapter_ids"),
     (lambda a: a.update(adapter_rows=0), "adapter_ids"),
+    (lambda a: a.update(parts=0), "parts"),
+    (lambda a: a.update(parts=3), "parts"),
+    (lambda a: a.update(parts=2), "adapters must be"),
     (lambda a: a.update(residual=torch.zeros(3, 64, dtype=torch.bfloat16, device=META)), "residual"),
 ])
 def test_adapter_refusals(change, match):
@@ -128,9 +131,10 @@ def test_entry_points_refuse_before_any_launch():
     for at, value, word in ((16, 32, "head_dim"), (13, 3, "multiple"), (7, 300, "padded"), (5, 192, "blkk"), (28, 0.0, "sm_scale"),
                             (9, 0, "sizes"), (8, None, "non-null"), (30, 0, "sizes"), (31, p + 4, "workspace"), (12, 70000, "grid")):
         assert word in error("tu_sage_block_attn", *(value if i == at else x for i, x in enumerate(attn))), at
-    lora = [p, p, p, p, None, p, p, p, p, 1, 16, 2, None, None, 1, p, 64, 128, 256, 256, p, 1 << 30, None]
+    lora = [p, p, p, p, None, p, p, p, p, 1, 16, 2, 1, None, None, 1, p, 64, 128, 256, 256, p, 1 << 30, None]
     for at, value, word in ((10, 12, "rank"), (10, 0, "rank"), (11, 0, "count"), (9, 0, "rows"), (5, p + 8, "aligned"),
-                            (18, 24, "K%16"), (6, None, "non-null"), (13, p, "gate"), (21, 8, "workspace"), (20, None, "workspace")):
+                            (19, 24, "K%16"), (6, None, "non-null"), (14, p, "gate"), (22, 8, "workspace"), (21, None, "workspace"),
+                            (12, 0, "parts"), (12, 4, "parts"), (12, 3, "parts")):
         assert word in error("tu_int8_gemm_adapters", *(value if i == at else x for i, x in enumerate(lora))), at
 
 
@@ -173,6 +177,16 @@ def test_adapter_layout():
     assert both.down.shape == (2, 24, 256) and both.up.shape == (2, 48, 24)
     assert torch.equal(both.up[:, :40, :16], bank.up) and torch.equal(both.up[:, 40:, 16:], other.up)
     assert (both.up[:, :40, 16:] == 0).all() and (both.up[:, 40:, :16] == 0).all()
+    same = kernel.LinearAdapters.from_float([(a[:2], torch.randn(48, 2, generator=g), s) for a, _, s in pairs], 128)
+    wide = kernel.LinearAdapters.from_float([(a, torch.randn(48, a.shape[0], generator=g), s) for a, _, s in pairs], 128)
+    three = kernel.LinearAdapters.concat([same, wide, same])
+    assert three.parts == 3 and three.rank == 48 and three.up.shape == (2, 144, 16)
+    assert torch.equal(three.down[:, 16:32], wide.down) and torch.equal(three.up[:, 48:96], wide.up)
+    for at in (0, 1):
+        assert torch.equal(three.down[:, 32 * at:32 * at + 8], same.down) and (three.down[:, 32 * at + 8:32 * at + 16] == 0).all()
+        assert torch.equal(three.up[:, 96 * at:96 * at + 48, :8], same.up) and (three.up[:, 96 * at:96 * at + 48, 8:] == 0).all()
+    with pytest.raises(ValueError, match="again"):
+        kernel.LinearAdapters.concat([three, three])
     for bad, match in (([], "at least one"), ([(torch.zeros(2, 200), torch.zeros(8, 2), 1.0)], "divide"),
                        ([(torch.zeros(2, 128), torch.zeros(8, 3), 1.0)], "each adapter")):
         with pytest.raises(ValueError, match=match):
