@@ -38,6 +38,9 @@ __device__ __forceinline__ int adapter_of(const int32_t *ids, int64_t id_rows, i
 }
 
 int32_t launch_down(const int8_t *a, const float *a_scale, const uint16_t *down, const float *scaling,
-                    const Adapters &ad, uint16_t *h, int64_t m, int64_t k, int cus, hipStream_t st);
+                    const Adapters &ad, uint16_t *h, int32_t *sort, int64_t m, int64_t k, int cus, hipStream_t st);
+
+// Bytes of h and, behind it, of what launch_down sorts.
+int64_t adapters_workspace(int64_t m, int64_t rank);
 
 }  // namespace tu

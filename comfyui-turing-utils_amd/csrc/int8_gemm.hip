@@ -1141,7 +1141,7 @@ extern "C" int32_t tu_int8_gemm_bf16_residual(const int8_t *a, const int8_t *w, 
 }
 
 extern "C" int64_t tu_int8_gemm_adapters_workspace(int64_t m, int64_t rank) {
-    return m > 0 && rank > 0 ? (m + 15) / 16 * ((rank + 31) / 32) * (2 * tu::kLowTerm * 2) : 0;
+    return m > 0 && rank > 0 ? tu::adapters_workspace(m, rank) : 0;
 }
 
 extern "C" int32_t tu_int8_gemm_adapters(const int8_t *a, const int8_t *w, const float *a_scale, const float *w_scale,
@@ -1172,7 +1172,8 @@ extern "C" int32_t tu_int8_gemm_adapters(const int8_t *a, const int8_t *w, const
     auto *h = static_cast<uint16_t *>(workspace);
     const Adapters ad{h, static_cast<const uint16_t *>(up_bf16), ids, id_rows, static_cast<int>(rank),
                       static_cast<int>(count), static_cast<int>(rank / parts), static_cast<int>(n / parts)};
-    if (launch_down(a, a_scale, static_cast<const uint16_t *>(down_bf16), scaling, ad, h, m, k, cus,
+    if (launch_down(a, a_scale, static_cast<const uint16_t *>(down_bf16), scaling, ad, h,
+                    reinterpret_cast<int32_t *>(h + (m + 15) / 16 * ((rank + 31) / 32) * (2 * kLowTerm)), m, k, cus,
                     static_cast<hipStream_t>(stream)))
         return -1;
     const auto *res = static_cast<const uint16_t *>(residual_bf16);

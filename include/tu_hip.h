@@ -180,8 +180,9 @@ int32_t tu_int8_gemm_bf16_residual(const int8_t *a, const int8_t *w, const float
  * their own; scaling: fp32 [count]; ids: int32 [ceil(m / id_rows)];
  * rank a multiple of 8 * parts up to 4096; down, up, residual and gate 16-byte
  * aligned; the rest as above.  workspace: 16-byte aligned, at least
- * tu_int8_gemm_adapters_workspace(m, rank) bytes (h).  cus: the device's
- * compute units.  Two launches.  No counterpart in the reference. */
+ * tu_int8_gemm_adapters_workspace(m, rank) bytes (h, and the rows' order).
+ * cus: the device's compute units.  Two launches, three where the rows are
+ * sorted by their adapter.  No counterpart in the reference. */
 int64_t tu_int8_gemm_adapters_workspace(int64_t m, int64_t rank);
 int32_t tu_int8_gemm_adapters(const int8_t *a, const int8_t *w, const float *a_scale, const float *w_scale,
                               const float *bias, const void *down_bf16, const void *up_bf16,

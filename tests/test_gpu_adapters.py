@@ -91,6 +91,21 @@ def test_many_rows(gpu_device, rank):
     _check(_inputs(gpu_device, 33001, 160, 64, rank, 5, 37, seed=rank))
 
 
+@pytest.mark.parametrize("m,count,rank,rows,k", [
+    (256, 8, 8, 1, 160), (255, 8, 8, 1, 160), (300, 5, 40, 1, 160), (257, 40, 16, 2, 160), (1000, 300, 24, 1, 160),
+    (1000, 1024, 8, 1, 160), (1000, 1025, 8, 1, 160), (5001, 33, 72, 1, 160), (9000, 4, 64, 1, 2560), (9000, 4, 64, 1, 160)])
+def test_many_rows_of_many_requests(gpu_device, m, count, rank, rows, k):
+    """Rows that are sorted by their adapter first, and sizes just past that."""
+    a = _inputs(gpu_device, m, k, 72, rank, count, rows, seed=m + count)
+    got = _check(a)
+    assert torch.equal(got, kernel.turing_int8_linear_adapters(**a))
+    # one adapter has nearly all rows, most have none
+    a["adapter_ids"][: 9 * a["adapter_ids"].numel() // 10] = count - 1
+    _check(a)
+    a["adapter_ids"].fill_(-1)
+    assert torch.equal(_check(a), _plain(a))
+
+
 @pytest.mark.parametrize("m,n,rank,parts", [
     (1, 32, 16, 2), (5, 144, 24, 3), (61, 240, 120, 3), (130, 96, 24, 3), (4096, 256, 64, 2), (512, 4800, 96, 3),
     (1024, 1584, 192, 3), (1024, 8976, 96, 3), (2050, 2064, 120, 3), (4100, 4800, 192, 3), (4100, 4800, 96, 3),
