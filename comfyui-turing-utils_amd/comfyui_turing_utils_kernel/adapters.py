@@ -72,6 +72,8 @@ def _linear_adapters(activation, weight, activation_scale, weight_scale, bias, d
     if gate is not None:
         gate = gate.to(torch.bfloat16).reshape(-1, n)
     down, up, residual, gate = (_aligned(t) for t in (down, up, residual, gate))
+    # (names of their own: a copy has to live until the launch)
+    scaling, adapter_ids = scaling.contiguous(), adapter_ids.contiguous()
     device = activation.device
     out = torch.empty((m, n), dtype=torch.bfloat16, device=device)
     if m == 0:
@@ -82,9 +84,8 @@ def _linear_adapters(activation, weight, activation_scale, weight_scale, bias, d
         workspace = torch.empty(nbytes, dtype=torch.uint8, device=device)
         _lib.call(
             "tu_int8_gemm_adapters", activation.data_ptr(), weight.data_ptr(), activation_scale.data_ptr(),
-            weight_scale.data_ptr(), _lib.ptr(bias), down.data_ptr(), up.data_ptr(), scaling.contiguous().data_ptr(),
-            adapter_ids.contiguous().data_ptr(), int(adapter_rows), rank, count, int(parts),
-            _lib.ptr(residual), _lib.ptr(gate),
+            weight_scale.data_ptr(), _lib.ptr(bias), down.data_ptr(), up.data_ptr(), scaling.data_ptr(),
+            adapter_ids.data_ptr(), int(adapter_rows), rank, count, int(parts), _lib.ptr(residual), _lib.ptr(gate),
             int(gate_rows) if gate is not None else 1, out.data_ptr(), m, n, k, cus, workspace.data_ptr(), nbytes,
             _lib.stream_of(device))
     return out
