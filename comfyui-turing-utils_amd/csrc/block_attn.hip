@@ -397,7 +397,8 @@ __global__ __launch_bounds__(kBlockThreads, kWgsPerCu<D>) void block_attn_kernel
     for (int qt = 0; qt < kQT; ++qt) {
         const int64_t qi = q0 + 16 * qt + lc;
         const float l = st.acc_l[qt][0];
-        const bool some = l > 0.0f && qi < q_end;
+        // (a sum of 0 is a row that saw no key; one that is NaN stays NaN)
+        const bool some = l != 0.0f && qi < q_end;
         const float inv = 1.0f / l;
 #pragma unroll
         for (int ds = 0; ds < Geo<D>::kDS; ds += 2) {
@@ -424,7 +425,9 @@ __global__ __launch_bounds__(kBlockThreads, kWgsPerCu<D>) void block_attn_kernel
 }
 
 // Merges the ranges of each row: M = max m_s, w_s = 2^(m_s - M),
-// out = sum w_s O_s / sum w_s l_s, zeros where no range saw a key.
+// out = sum w_s O_s / sum w_s l_s, zeros where no range saw a key.  A range saw
+// none where its l is 0 (its O may then be no number, and is left out); where
+// its l is NaN the row is.
 template <int D>
 __global__ __launch_bounds__(256) void block_merge_kernel(const float *__restrict__ part, BlockPlan plan, uint32_t hq,
                                                           int64_t lq, uint16_t *__restrict__ o, int64_t o_sb,
@@ -462,7 +465,7 @@ __global__ __launch_bounds__(256) void block_merge_kernel(const float *__restric
         for (int k = 0; k < 8; ++k) acc[k] *= old;
 #pragma unroll
         for (int u = 0; u < kAhead; ++u) {
-            if (p0 + u >= parts || !(x[u][1] > 0.0f)) continue;  // nothing seen in this range
+            if (p0 + u >= parts || x[u][1] == 0.0f) continue;  // nothing seen in this range
             const float w = __builtin_amdgcn_exp2f(x[u][0] - m);
             l = __builtin_fmaf(w, x[u][1], l);
 #pragma unroll
@@ -472,7 +475,7 @@ __global__ __launch_bounds__(256) void block_merge_kernel(const float *__restric
             }
         }
     }
-    const float inv = l > 0.0f ? 1.0f / l : 0.0f;
+    const float inv = l == 0.0f ? 0.0f : 1.0f / l;
     uint16_t *dst = o + (bh / hq) * o_sb + (bh % hq) * o_sh + q * o_sl + d0;
     u32x2 lo, hi;
     lo.x = pack_bf16x2(acc[0] * inv, acc[1] * inv);

@@ -1,0 +1,78 @@
+"""GPU: ``key_block_attention`` where scales are no numbers, infinite, tiny or
+huge, against the 64-bit reference of tests/operator_reference.py: a row is
+NaN where the softmax of the scores it sees is, and nowhere else.  Grids whose
+lists are split into ranges and grids whose lists are not."""
+from __future__ import annotations
+
+import pytest
+import torch
+
+from comfyui_turing_utils_kernel import _lib, turing_sage
+from tests import operator_reference as ref
+from tests import test_gpu_block_attn as attn
+
+pytestmark = pytest.mark.gpu
+
+NAN, INF = float("nan"), float("inf")
+# query rows, keys, entries of a list: up to six entries are never split
+FORMS = {"whole": (300, 700, 5), "split": (150, 9000, 100)}
+
+
+def _parts(b, hq, lq, d, width):
+    return _lib.load().tu_sage_block_attn_workspace(b, hq, lq, d, width, 256) > 0
+
+
+def _compare(args, index, causal=False, blkq=16, blkk=64, ql=None, kl=None):
+    """The call against the reference, NaN for NaN; returns (output, rows that are NaN)."""
+    q8, qs, k8, ks, vt = args
+    print(f"[block attn] Q{tuple(q8.shape)} K{tuple(k8.shape)} list {index.size(-1)} causal {causal}", flush=True)
+    got = turing_sage.key_block_attention(*args, index, is_causal=causal, blkq=blkq, blkk=blkk, query_lengths=ql,
+                                          key_lengths=kl)
+    want, size = ref.attend(*args, index, "HND", causal, q8.size(-1) ** -0.5, blkq, blkk, ql, kl)
+    none = want.isnan()
+    assert torch.equal(got.isnan(), none), (int(got.isnan().sum()), int(none.sum()))
+    off, bound = (got.double() - want).abs(), ref.attend_bound(want, size)
+    assert bool((off <= bound)[~none].all()), float((off / bound)[~none].max())
+    return got, none.any(-1)
+
+
+@pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("form", FORMS)
+@pytest.mark.parametrize("causal", [False, True])
+@pytest.mark.parametrize("value", [INF])
+@pytest.mark.parametrize("side", ["query", "key"])
+def test_scales_that_are_no_numbers(gpu_device, d, form, causal, value, side):
+    """As the quantizer leaves them: codes of zero where a scale is infinite.
+    Every third block of keys, or every fourth group of 16 queries; rows that
+    see none of such keys, and no such row itself, keep their values."""
+    lq, lk, width = FORMS[form]
+    q8, qs, k8, ks, vt, g = attn._inputs(gpu_device, 2, 4, 2, lq, lk, d, blkq=16, blkk=64, seed=d + lq)
+    assert _parts(2, 4, lq, d, width) == (form == "split")
+    index = attn._random_lists(2, 4, lq, lk, width, g, gpu_device)
+    if side == "key":
+        # few enough that some rows see none
+        ks[0, :, 1::(3 if form == "whole" else 60)] = value
+        at = (~ks.isfinite()).repeat_interleave(64, 2)[:, :, :lk]
+        k8[at] = 0
+        index[0, 0] = torch.arange(width, device=gpu_device)  # and the blocks on the diagonal
+    else:
+        qs[:, 1, ::4] = value
+        at = (~qs.isfinite()).repeat_interleave(16, 2)[:, :, :lq]
+        q8[at] = 0
+    _, rows = _compare((q8, qs, k8, ks, vt), index, causal)
+    assert rows.any() and not rows.all()
+
+
+@pytest.mark.parametrize("where", ["q", "k"])
+@pytest.mark.parametrize("lq,lk", [(300, 300), (1, 9000)])
+def test_an_infinite_input_gives_what_the_dense_attention_gives(gpu_device, where, lq, lk):
+    """One infinite element of Q (its block of rows is NaN) or, with K's mean
+    taken off, of K (its head is): every block kept, the rows that are NaN are
+    those of the dense attention."""
+    g = torch.Generator().manual_seed(8)
+    q = torch.randn(1, 2, lq, 128, generator=g).to(torch.bfloat16).to(gpu_device)
+    k, v = (torch.randn(1, 2, lk, 128, generator=g).to(torch.bfloat16).to(gpu_device) for _ in range(2))
+    (q if where == "q" else k)[0, 1, min(lq, lk) - 1, 5] = INF
+    dense = turing_sage.sageattn(q, k, v)
+    got = turing_sage.sparse_sageattn(q, k, v, keep=(lk + 63) // 64)
+    assert dense[:, 1].isnan().any() and torch.equal(got.isnan(), dense.isnan())
