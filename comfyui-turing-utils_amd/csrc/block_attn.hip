@@ -224,7 +224,9 @@ __global__ __launch_bounds__(kBlockThreads, kWgsPerCu<D>) void block_attn_kernel
 #pragma unroll
             for (int ds = 0; ds < kSl; ++ds)
                 qf[qt][ds] = *reinterpret_cast<const i32x4 *>(qp + qi * q_sl + 64 * ds + 16 * g);
-            qsc[qt] = q_scale[static_cast<int64_t>(bh) * nbq + static_cast<uint32_t>(qi) / blkq];
+            // (a row behind the sample's end takes no part in what a wave's rows
+            // decide together: when O is rescaled, how p is formed)
+            qsc[qt] = qi < q_end ? q_scale[static_cast<int64_t>(bh) * nbq + static_cast<uint32_t>(qi) / blkq] : 0.0f;
         }
     }
     int before = -1;  // largest entry in front of the segment

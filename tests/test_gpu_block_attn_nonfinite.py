@@ -63,6 +63,23 @@ def test_scales_that_are_no_numbers(gpu_device, d, form, causal, value, side):
     assert rows.any() and not rows.all()
 
 
+@pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("causal", [False, True])
+@pytest.mark.parametrize("value", [NAN, INF, 30.0, 0.0])
+def test_queries_behind_the_end_leave_the_others_their_bits(gpu_device, d, causal, value):
+    """Rows behind the sample's end that share a wave with rows in front of it:
+    any scales, any codes."""
+    *args, g = attn._inputs(gpu_device, 1, 2, 2, 300, 300, d, blkq=16, blkk=64, seed=4)
+    index = attn._random_lists(1, 2, 300, 300, 5, g, gpu_device)
+    ql = torch.tensor([131], dtype=torch.int32, device=gpu_device)
+    kw = dict(is_causal=causal, blkq=16, blkk=64, query_lengths=ql)
+    clean = turing_sage.key_block_attention(*args, index, **kw)
+    args[1][:, :, 9:] = value  # from row 144 on
+    args[0][:, :, 131:] = 127
+    got = turing_sage.key_block_attention(*args, index, **kw)
+    assert torch.equal(got, clean) and torch.isfinite(got).all()
+
+
 @pytest.mark.parametrize("where", ["q", "k"])
 @pytest.mark.parametrize("lq,lk", [(300, 300), (1, 9000)])
 def test_an_infinite_input_gives_what_the_dense_attention_gives(gpu_device, where, lq, lk):
