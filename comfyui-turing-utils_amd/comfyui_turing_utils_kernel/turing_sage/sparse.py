@@ -262,6 +262,8 @@ def key_block_attention(
     nothing.  Keys at or past ``key_lengths[b]`` are not seen, whatever codes
     and values stand there; rows at or past ``query_lengths[b]``, and rows that
     see no key, are zeros.  Causal masks are aligned at the first row and key.
+    Scales are not negative (a quantizer's are not); one that is infinite or NaN
+    makes NaN of the rows that see its keys, or that have it, and of no others.
     Values of the listed blocks in front of the sample's end must be finite, as
     in the dense attention: 0 times infinity is a NaN in every row of the tile.
     Output: bf16 in the layout and shape of ``query_int8``."""

@@ -45,8 +45,9 @@ constexpr int kSegment = 256;  // list entries compacted at a time
 // exponent base of a row that has seen no key yet: finite, so that a tile
 // without a visible key gives 2^-inf = 0 and not a NaN
 constexpr float kNoBase = -1e30f;
-// a scale of zero would make a masked score 0 * -inf
-constexpr float kLeastScale = 1e-18f;
+// Least factor of a masked tile's scores: 0 would make a masked one 0 * -inf.
+// (2^(score * 1e-18) is 1 for every score.)
+constexpr float kLeastFactor = 1e-18f;
 
 struct BlockPlan {
     uint32_t nqb;    // query blocks of a head
@@ -238,7 +239,7 @@ __global__ __launch_bounds__(kBlockThreads, kWgsPerCu<D>) void block_attn_kernel
     SoftmaxState<D> st;
 #pragma unroll
     for (int qt = 0; qt < kQT; ++qt) {
-        qsc[qt] = fmaxf(qsc[qt], kLeastScale) * sm_log2;
+        qsc[qt] *= sm_log2;
         st.m_used[qt] = kNoBase;
         st.acc_l[qt] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
@@ -311,12 +312,15 @@ __global__ __launch_bounds__(kBlockThreads, kWgsPerCu<D>) void block_attn_kernel
                 const int key_lim = min(k_end - key0, kBKey);
                 const int q_rel = static_cast<int>(max(min(q0 - key0, static_cast<int64_t>(kBKey)), static_cast<int64_t>(-kBlockRows)));
                 mask_tile<kCausal>(s, key_lim, q_rel, g, lc);
+                // a factor that is no number stays one, but not for a row that
+                // sees nothing of the tile
+#pragma unroll
+                for (int qt = 0; qt < kQT; ++qt)
+                    f[qt] = f[qt] < kLeastFactor || (kCausal && q_rel + 16 * qt + lc < 0) ? kLeastFactor : f[qt];
             }
             softmax_tile(s, f, st, pb);
         };
-        auto uniform = [](float x) {
-            return fmaxf(__int_as_float(__builtin_amdgcn_readfirstlane(__float_as_int(x))), kLeastScale);
-        };
+        auto uniform = [](float x) { return __int_as_float(__builtin_amdgcn_readfirstlane(__float_as_int(x))); };
         // scale1 .. 3: scales of tiles t + 1 .. t + 3; block2, block3: blocks of
         // tiles t + 2 and t + 3
         const int block0 = block_at(0), block1 = block_at(1);

@@ -376,8 +376,9 @@ int32_t tu_sage_block_select(const int8_t *q8, const float *q_scale, int64_t blk
  * ceil(lq / 128), width] names for them.  An entry counts if it lies in
  * [0, ceil(lk / 64)) and is larger than every entry before it.  Keys at or
  * past k_lengths[b] are not seen (codes and values there may be anything);
- * rows at or past q_lengths[b], and rows that see no key, are zeros.  Causal:
- * top-left aligned.  Grids of few workgroups on a device of `cus` compute
+ * rows at or past q_lengths[b], and rows that see no key, are zeros.  Scales
+ * are not negative; one that is no number makes NaN of the rows that see its
+ * keys, or that have it, and of no others.  Causal: top-left aligned.  Grids of few workgroups on a device of `cus` compute
  * units split their lists into ranges that a second kernel merges, as many as
  * `workspace` (16-byte aligned, workspace_bytes long) holds;
  * tu_sage_block_attn_workspace gives the bytes for all of them (0: no split),

@@ -39,7 +39,7 @@ def _compare(args, index, causal=False, blkq=16, blkk=64, ql=None, kl=None):
 @pytest.mark.parametrize("d", [64, 128])
 @pytest.mark.parametrize("form", FORMS)
 @pytest.mark.parametrize("causal", [False, True])
-@pytest.mark.parametrize("value", [INF])
+@pytest.mark.parametrize("value", [NAN, INF])
 @pytest.mark.parametrize("side", ["query", "key"])
 def test_scales_that_are_no_numbers(gpu_device, d, form, causal, value, side):
     """As the quantizer leaves them: codes of zero where a scale is infinite.
@@ -63,6 +63,19 @@ def test_scales_that_are_no_numbers(gpu_device, d, form, causal, value, side):
     assert rows.any() and not rows.all()
 
 
+@pytest.mark.parametrize("form", FORMS)
+def test_a_range_that_is_nan_is_not_left_out(gpu_device, form):
+    """One NaN block anywhere in a list makes every row of it NaN, however the list is cut."""
+    lq, lk, width = FORMS[form]
+    *args, _ = attn._inputs(gpu_device, 1, 2, 2, lq, lk, 128, blkq=16, blkk=64, seed=3)
+    index = torch.arange(width, dtype=torch.int32, device=gpu_device).expand(1, 2, (lq + 127) // 128, width).contiguous()
+    for at in sorted({0, 1, width // 2, width - 1}):
+        scales = args[3].clone()
+        scales[:, 0, at] = NAN
+        got, rows = _compare((args[0], args[1], args[2], scales, args[4]), index)
+        assert rows[:, 0].all() and not rows[:, 1].any()
+
+
 @pytest.mark.parametrize("d", [64, 128])
 @pytest.mark.parametrize("causal", [False, True])
 @pytest.mark.parametrize("value", [NAN, INF, 30.0, 0.0])
@@ -78,6 +91,19 @@ def test_queries_behind_the_end_leave_the_others_their_bits(gpu_device, d, causa
     args[0][:, :, 131:] = 127
     got = turing_sage.key_block_attention(*args, index, **kw)
     assert torch.equal(got, clean) and torch.isfinite(got).all()
+
+
+@pytest.mark.parametrize("form", FORMS)
+@pytest.mark.parametrize("power", [-100, -70, 70, 100])
+def test_scales_far_apart_whose_product_is_ordinary(gpu_device, form, power):
+    """2^-n beside 2^n: every product is the same number, and so is the result."""
+    lq, lk, width = FORMS[form]
+    q8, qs, k8, ks, vt, g = attn._inputs(gpu_device, 1, 2, 1, lq, lk, 128, blkq=16, blkk=64, seed=5)
+    index = attn._random_lists(1, 2, lq, lk, width, g, gpu_device)
+    for causal in (False, True):
+        want, _ = _compare((q8, qs, k8, ks, vt), index, causal)
+        got, _ = _compare((q8, qs * 2.0 ** power, k8, ks * 2.0 ** -power, vt), index, causal)
+        assert torch.equal(got, want)
 
 
 @pytest.mark.parametrize("where", ["q", "k"])
