@@ -42,9 +42,6 @@ constexpr int kBlockThreads = 256;
 constexpr int kBlockRows = 128;
 constexpr int kRing = 3;
 constexpr int kSegment = 256;  // list entries compacted at a time
-// exponent base of a row that has seen no key yet: finite, so that a tile
-// without a visible key gives 2^-inf = 0 and not a NaN
-constexpr float kNoBase = -1e30f;
 // Least factor of a masked tile's scores: 0 would make a masked one 0 * -inf.
 // (2^(score * 1e-18) is 1 for every score.)
 constexpr float kLeastFactor = 1e-18f;
@@ -96,6 +93,15 @@ __device__ __forceinline__ float load_scale(__amdgpu_buffer_rsrc_t rs, int at) {
 #undef TU_ISSUE
 #undef TU_ISSUE_K_BODY
 #undef TU_ISSUE_V_BODY
+
+// The largest value of 16 lanes, to all of them.
+__device__ __forceinline__ float row_max16(float v) {
+    // row_ror 8, 4, 2, 1
+    v = fmaxf(v, __int_as_float(__builtin_amdgcn_mov_dpp(__float_as_int(v), 0x128, 0xf, 0xf, true)));
+    v = fmaxf(v, __int_as_float(__builtin_amdgcn_mov_dpp(__float_as_int(v), 0x124, 0xf, 0xf, true)));
+    v = fmaxf(v, __int_as_float(__builtin_amdgcn_mov_dpp(__float_as_int(v), 0x122, 0xf, 0xf, true)));
+    return fmaxf(v, __int_as_float(__builtin_amdgcn_mov_dpp(__float_as_int(v), 0x121, 0xf, 0xf, true)));
+}
 
 __device__ __forceinline__ int sample_end(const int32_t *lengths, uint32_t b, int64_t len) {
     return lengths ? min(max(lengths[b], 0), static_cast<int>(len)) : static_cast<int>(len);
@@ -245,6 +251,7 @@ __global__ __launch_bounds__(kBlockThreads, kWgsPerCu<D>) void block_attn_kernel
 #pragma unroll
         for (int ds = 0; ds < Geo<D>::kDS; ++ds) st.acc_o[ds][qt] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
     }
+    const float largest_q = row_max16(fmaxf(qsc[0], qsc[1]));
     bf16x8 ones;
 #pragma unroll
     for (int i = 0; i < 8; ++i) ones[i] = static_cast<__bf16>(1.0f);
@@ -281,12 +288,15 @@ __global__ __launch_bounds__(kBlockThreads, kWgsPerCu<D>) void block_attn_kernel
             }
         }
         int n = 0, whole = 0, top = before;
+        float listed[4] = {};  // scales of the lane's entries, used when the first tile is done
 #pragma unroll
         for (int c = 0; c < 4; ++c) {
             if (64 * c >= end - seg) break;
             const bool counts = e[c] > prev[c] && e[c] >= 0 && e[c] < blocks;
             const uint64_t mask = __ballot(counts);
             if (counts) list[n + __builtin_popcountll(mask & ((1ull << lane) - 1))] = e[c];
+            // (past the buffer's end: 0)
+            listed[c] = load_scale(srs, counts ? e[c] >> kscale_shift : 0x1fffffff);
             n += __builtin_popcountll(mask);
             // tiles with masked keys stand last, as the list ascends
             whole += __builtin_popcountll(__ballot(counts && e[c] < masked_from));
@@ -318,7 +328,7 @@ __global__ __launch_bounds__(kBlockThreads, kWgsPerCu<D>) void block_attn_kernel
                 for (int qt = 0; qt < kQT; ++qt)
                     f[qt] = f[qt] < kLeastFactor || (kCausal && q_rel + 16 * qt + lc < 0) ? kLeastFactor : f[qt];
             }
-            softmax_tile(s, f, st, pb);
+            softmax_tile<decltype(mask_tag)::value>(s, f, st, pb);
         };
         auto uniform = [](float x) { return __int_as_float(__builtin_amdgcn_readfirstlane(__float_as_int(x))); };
         // scale1 .. 3: scales of tiles t + 1 .. t + 3; block2, block3: blocks of
@@ -343,7 +353,11 @@ __global__ __launch_bounds__(kBlockThreads, kWgsPerCu<D>) void block_attn_kernel
         // Interval t: QK of tile t + 1 and PV of tile t, then the softmax of
         // tile t + 1.  At its end a wave waits for its loads of K(t + 2) and
         // V(t + 1), issued an interval ago.
-        const int main_steps = max(0, min(n, whole) - 1);
+        // A wave with a factor past kFarFactor leaves its tiles to the second
+        // loop, which has the same barriers and fills the same stages: a test in
+        // this loop costs 2 to 6 % at head_dim 64.
+        const float largest_k = fmaxf(fmaxf(listed[0], listed[1]), fmaxf(listed[2], listed[3]));
+        const int main_steps = __any(largest_q * largest_k > kFarFactor) ? 0 : max(0, min(n, whole) - 1);
         int s0 = 0, s1 = 1, s2 = 2;  // stages of tiles t, t + 1, t + 2
 #pragma clang loop unroll(disable)
         for (int t = 0; t < main_steps; ++t) {

@@ -15,6 +15,10 @@ constexpr int kQT = 2;                   // 16-row query fragments per wave
 constexpr int kWaveQ = 16 * kQT;         // query rows per wave
 constexpr int kBKey = 64;                // keys per tile
 constexpr float kRescaleSlack = 8.0f;        // log2 of the largest p allowed
+constexpr float kFarFactor = 128.0f;         // f from which scores (22 bits times f) may pass 2^28
+// Exponent base of a row that has seen no key yet, where a tile may have none
+// for it: finite, so that such a tile gives 2^-inf = 0 and not a NaN.
+constexpr float kNoBase = -1e30f;
 
 // Head-dim geometry (D = 64 or 128).  K tile: 64 keys x D bytes; V^T tile:
 // D channels x 64 keys of bf16 (128-byte rows); group 0's 4 waves each move
@@ -180,7 +184,11 @@ __device__ __forceinline__ void mask_tile(i32x4 (&s)[4][kQT], int key_lim, int q
 // x = dot f - m_used is formed as fma(biased, f, c) with
 // c = -(1.5 * 2^23 f + m_used) when |c| < 2^12, which keeps the rounding of c
 // below 2^-13 in the exponent; otherwise the bias is subtracted exactly first.
-template <int D>
+// kAnySize: where f is past kFarFactor the product is rounded before m_used, a
+// rounded product too, is subtracted.  The FMA's exact product differs from
+// m_used by up to half a step of it, and from scores of 2^31 on that leaves the
+// exponent's range (all p infinite, or all 0).
+template <bool kAnySize = false, int D>
 __device__ __forceinline__ void softmax_tile(const i32x4 (&s)[4][kQT], const float (&f)[kQT], SoftmaxState<D> &st,
                                              bf16x8 (&p)[2][kQT]) {
     float mlane[kQT];
@@ -217,7 +225,9 @@ __device__ __forceinline__ void softmax_tile(const i32x4 (&s)[4][kQT], const flo
         c[qt] = -__builtin_fmaf(kBiasF, f[qt], st.m_used[qt]);
         exact = exact || !(fabsf(c[qt]) < 4096.0f);
     }
-    auto make_p = [&](auto exact_tag) {
+    // 0: an FMA on the biased score, 1: bias subtracted first, 2: product rounded as well
+    auto make_p = [&](auto form_tag) {
+        constexpr int kForm = decltype(form_tag)::value;
 #pragma unroll
         for (int qt = 0; qt < kQT; ++qt) {
             const float nm = -st.m_used[qt];
@@ -231,8 +241,9 @@ __device__ __forceinline__ void softmax_tile(const i32x4 (&s)[4][kQT], const flo
                     for (int t = 0; t < 2; ++t) {
                         const int e = 2 * j + t;  // keys 32 h + 8 g + e
                         const float v = __int_as_float(s[2 * h + (e >> 2)][qt][e & 3]);
-                        const float x = decltype(exact_tag)::value ? __builtin_fmaf(v - kBiasF, f[qt], nm)
-                                                                   : __builtin_fmaf(v, f[qt], c[qt]);
+                        const float x = kForm == 0   ? __builtin_fmaf(v, f[qt], c[qt])
+                                        : kForm == 1 ? __builtin_fmaf(v - kBiasF, f[qt], nm)
+                                                     : (v - kBiasF) * f[qt] + nm;
                         p2[t] = __builtin_amdgcn_exp2f(x);
                     }
                     packed[j] =
@@ -248,7 +259,7 @@ __device__ __forceinline__ void softmax_tile(const i32x4 (&s)[4][kQT], const flo
         // 95 -> 85 us.  At head_dim 128, where the other group's MFMAs are
         // twice as many, the runs are the better form (13.2 ms, 13.7 apart).
         if constexpr (D == 64) {
-            constexpr int kFma = decltype(exact_tag)::value ? 2 : 1;
+            constexpr int kFma = kForm + 1;
             __builtin_amdgcn_sched_group_barrier(0x002, 2 * kFma, 0);
 #pragma unroll
             for (int i = 0; i < 16; ++i) {
@@ -259,8 +270,13 @@ __device__ __forceinline__ void softmax_tile(const i32x4 (&s)[4][kQT], const flo
             }
         }
     };
-    if (__any(exact)) make_p(std::true_type{});
-    else make_p(std::false_type{});
+    if (__any(exact)) {
+        const bool far = kAnySize && __any(fmaxf(f[0], f[1]) > kFarFactor);
+        if (__builtin_expect(far, 0)) make_p(std::integral_constant<int, 2>{});
+        else make_p(std::integral_constant<int, 1>{});
+    } else {
+        make_p(std::integral_constant<int, 0>{});
+    }
 }
 
 // O^T += V^T P and l += 1 P for one tile.

@@ -106,6 +106,21 @@ def test_scales_far_apart_whose_product_is_ordinary(gpu_device, form, power):
         assert torch.equal(got, want)
 
 
+@pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("form", FORMS)
+@pytest.mark.parametrize("power", [3, 7, 9, 11, 13, 15, 17, 21, 40, 90])
+def test_scores_of_any_size(gpu_device, d, form, power):
+    """One factor of 2^power / 8 or so times whole numbers, positive and
+    negative: past 2^11 or so the largest score takes the row, and scores that
+    are equal share it."""
+    lq, lk, width = FORMS[form]
+    q8, qs, k8, ks, vt, g = attn._inputs(gpu_device, 1, 2, 2, lq, lk, d, blkq=16, blkk=64, seed=7)
+    qs.fill_(1.37), ks.fill_(2.0 ** power)
+    index = attn._random_lists(1, 2, lq, lk, width, g, gpu_device)
+    _, rows = _compare((q8, qs, k8, ks, vt), index)
+    assert not rows.any()
+
+
 @pytest.mark.parametrize("where", ["q", "k"])
 @pytest.mark.parametrize("lq,lk", [(300, 300), (1, 9000)])
 def test_an_infinite_input_gives_what_the_dense_attention_gives(gpu_device, where, lq, lk):
