@@ -17,8 +17,9 @@ constexpr int kBKey = 64;                // keys per tile
 constexpr float kRescaleSlack = 8.0f;        // log2 of the largest p allowed
 constexpr float kFarFactor = 128.0f;         // f from which scores (22 bits times f) may pass 2^28
 // Exponent base of a row that has seen no key yet, where a tile may have none
-// for it: finite, so that such a tile gives 2^-inf = 0 and not a NaN.
-constexpr float kNoBase = -1e30f;
+// for it: finite, so that such a tile gives 2^-inf = 0 and not a NaN, and below
+// every finite score.
+constexpr float kNoBase = -3.402823466e38f;
 
 // Head-dim geometry (D = 64 or 128).  K tile: 64 keys x D bytes; V^T tile:
 // D channels x 64 keys of bf16 (128-byte rows); group 0's 4 waves each move

@@ -106,6 +106,20 @@ def test_scales_far_apart_whose_product_is_ordinary(gpu_device, form, power):
         assert torch.equal(got, want)
 
 
+@pytest.mark.parametrize("form", FORMS)
+@pytest.mark.parametrize("causal", [False, True])
+def test_scores_below_every_ordinary_number(gpu_device, form, causal):
+    """Finite scores of -1e32 to -1e36 alone: the largest takes the row."""
+    lq, lk, width = FORMS[form]
+    q8, qs, k8, ks, vt, g = attn._inputs(gpu_device, 1, 2, 2, lq, lk, 128, blkq=16, blkk=64, seed=6)
+    q8, k8 = q8.abs().clamp_min(1), -k8.abs().clamp_min(1)
+    # one scale: scores are one factor times whole numbers, equal or far apart
+    qs.fill_(2.0 ** 50), ks.fill_(2.0 ** 50)
+    index = attn._random_lists(1, 2, lq, lk, width, g, gpu_device)
+    _, rows = _compare((q8, qs, k8, ks, vt), index, causal)
+    assert not rows.any()
+
+
 @pytest.mark.parametrize("d", [64, 128])
 @pytest.mark.parametrize("form", FORMS)
 @pytest.mark.parametrize("power", [3, 7, 9, 11, 13, 15, 17, 21, 40, 90])
