@@ -274,8 +274,9 @@ class WanBlockW8A8:
         self.adapters = dict(adapters)
 
     def _adapted(self, name: str, adapter_ids: Optional[torch.Tensor], rows: int) -> dict:
-        """The adapter arguments of a linear whose samples have ``rows`` rows each."""
-        if adapter_ids is None or name not in self.adapters:
+        """The adapter arguments of a linear whose samples have ``rows`` rows each
+        (none where they have no rows)."""
+        if adapter_ids is None or name not in self.adapters or rows == 0:
             return {}
         return dict(adapters=self.adapters[name], adapter_ids=adapter_ids, adapter_rows=rows)
 
@@ -309,7 +310,7 @@ class WanBlockW8A8:
 
     def _project(self, name: str, x2d: torch.Tensor, b: int, residual, gate, adapter_ids,
                  gelu: bool = False) -> torch.Tensor:
-        lin, adapted = getattr(self, name), self._adapted(name, adapter_ids, x2d.shape[0] // b)
+        lin, adapted = getattr(self, name), self._adapted(name, adapter_ids, x2d.shape[0] // b if b else 0)
         if residual is None:
             return lin(x2d, gelu=gelu, **adapted)
         b, l, c = residual.shape

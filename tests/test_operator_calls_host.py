@@ -58,3 +58,37 @@ def test_strided_scaling_and_ids_live_until_the_launch(entry_point, strided):
     for _ in range(20):  # (whether freed memory is taken again at once is the allocator's choice)
         kernel.turing_int8_linear_adapters(**a)
         assert (entry_point["scaling"], entry_point["ids"]) == want
+
+
+def _block(adapted):
+    """A Wan block without data; with adapters of every linear."""
+    from comfyui_turing_utils_kernel.wan_block import W8A8Linear, WanBlockConfig, WanBlockW8A8
+
+    def lin(n, k):
+        return W8A8Linear(torch.zeros(n, k, dtype=torch.int8, device="meta"), torch.ones(n, device="meta"), None)
+
+    ones = torch.ones(256, device="meta")
+    block = WanBlockW8A8(WanBlockConfig(dim=256, heads=2, ffn_dim=512, text_dim=256),
+                         modulation=torch.zeros(1, 6, 256, device="meta"), self_qkv=lin(768, 256),
+                         self_o=lin(256, 256), self_norm_q=ones, self_norm_k=ones, norm3_weight=ones,
+                         norm3_bias=ones * 0, cross_q=lin(256, 256), cross_kv=lin(512, 256), cross_o=lin(256, 256),
+                         cross_norm_q=ones, cross_norm_k=ones, ffn_up=lin(512, 256), ffn_down=lin(256, 512))
+    block.set_adapters({name: kernel.LinearAdapters(
+        torch.zeros(2, 8, getattr(block, name).in_features, dtype=torch.bfloat16, device="meta"),
+        torch.zeros(2, getattr(block, name).out_features, 8, dtype=torch.bfloat16, device="meta"),
+        torch.ones(2, device="meta")) for name in (block.LINEARS if adapted else ())})
+    return block
+
+
+@pytest.mark.parametrize("b,l", [(0, 5), (2, 0), (0, 0), (2, 5)])
+@pytest.mark.parametrize("with_ids", [False, True])
+def test_sublayers_without_rows(b, l, with_ids):
+    """An empty batch, or samples without rows, with or without adapters."""
+    block = _block(with_ids)
+    h = torch.empty(b, l, 256, dtype=torch.bfloat16, device="meta")
+    ids = torch.zeros(b, dtype=torch.int32, device="meta") if with_ids else None
+    gate = torch.empty(b, 1, 256, dtype=torch.bfloat16, device="meta")
+    assert block.ffn(h, adapter_ids=ids).shape == (b, l, 256)
+    if l:  # (a gate has a row for each of the output's)
+        assert block.ffn(h, residual=h, gate=gate, adapter_ids=ids).shape == (b, l, 256)
+    assert block._project("self_o", h.reshape(b * l, 256), b, h, None, ids).shape == (b * l, 256)
