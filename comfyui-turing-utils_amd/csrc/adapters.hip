@@ -35,6 +35,7 @@ namespace {
 
 constexpr int kSortThreads = 1024;   // and the most adapters that are sorted
 constexpr int64_t kLeastSorted = 256;  // rows
+constexpr float kLargestBf16 = 0x1.fep127f;
 
 // Tiles that the rows of `count` adapters fill at most.
 int64_t sorted_tiles(int64_t m, int64_t count, int64_t rows) { return (m + rows - 1) / rows + std::min(count, m); }
@@ -189,9 +190,12 @@ __global__ __launch_bounds__(64 * kWaves) void adapter_down_kernel(const int8_t 
             if ((kSorted ? row >= 0 : (mine >> (16 * i + lc) & 1) != 0) && rank < ad.rank) {
                 v *= scaling[which] * as[row];
                 u32x2 hi, lo;
+                // hi stops at bf16's largest number: what is past it, an infinity
+                // too, is in lo (hi infinite would make lo infinity - infinity)
+                auto held = [](float x) { return __builtin_amdgcn_fmed3f(x, -kLargestBf16, kLargestBf16); };
 #pragma unroll
                 for (int e = 0; e < 2; ++e) {
-                    hi[e] = hw_bf16x2_bits(v[2 * e], v[2 * e + 1]);
+                    hi[e] = hw_bf16x2_bits(held(v[2 * e]), held(v[2 * e + 1]));
                     lo[e] = hw_bf16x2_bits(v[2 * e] - __uint_as_float(hi[e] << 16),
                                            v[2 * e + 1] - __uint_as_float(hi[e] & 0xffff0000u));
                 }
