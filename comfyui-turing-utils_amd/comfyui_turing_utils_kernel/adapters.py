@@ -152,7 +152,8 @@ def turing_int8_linear_adapters(
     columns and the ranks are so many equal parts (of a multiple of 16 columns
     and 8 ranks each), the columns of a part see its own ranks alone, and ``up``
     is [count, N, rank / parts]: the projections of a fused q / k / v have
-    adapters of their own.  The op is
+    adapters of their own.  Infinite or NaN weights make infinity or NaN of their
+    own adapter's rows alone.  The op is
     ``torch.ops.turing_utils.int8_linear_adapters``; it has no backward."""
     args = (activation, weight, activation_scale, weight_scale, bias, down, up, scaling, adapter_ids, adapter_rows,
             residual, gate, gate_rows, parts)

@@ -173,7 +173,8 @@ int32_t tu_int8_gemm_bf16_residual(const int8_t *a, const int8_t *w, const float
  * residual bf16_rn(fma(bf16_rn(y), gate, residual)) as
  * tu_int8_gemm_bf16_residual.  Codes are those of a rotated activation, so
  * down holds the adapter's rows rotated alike.  h is summed in fp32 and kept
- * as two bf16 terms (to 2^-16 of it).  down: bf16 [count, rank, k]; up: bf16
+ * as two bf16 terms (to 2^-16 of it), infinities and NaN among them; an
+ * infinite element of up, which both terms meet, gives infinity or NaN.  down: bf16 [count, rank, k]; up: bf16
  * [count, n, rank / parts]: the columns and the ranks are `parts` equal parts
  * each (a multiple of 16 columns where there are several), and the columns of
  * a part see that part's ranks, as projections side by side have adapters of
