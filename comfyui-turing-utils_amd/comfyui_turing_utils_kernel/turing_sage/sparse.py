@@ -142,11 +142,12 @@ def select_key_blocks(
     Query block i (rows 128 i ..) sees key block j (keys 64 j ..) if the block
     has rows below ``query_lengths[b]``, the key block starts below
     ``key_lengths[b]`` and, when causal, at or below the query block's last
-    row.  Of those it takes the first ``keep`` by: forced blocks (the first
-    ``sink_blocks``, and with ``local_blocks`` = w the two beside the diagonal
-    and w - 1 more on each side), then the larger product of the blocks' mean
-    rows (64-bit, over the rows in front of the sample's end), NaN last, then
-    the lower j."""
+    row.  Of those it takes the first ``keep``: the forced blocks (the first
+    ``sink_blocks``, and with ``local_blocks`` = w the two on the diagonal, 2 i
+    and 2 i + 1, and w - 1 more on each side) in the order of j, whatever their
+    products; then the others by the larger product of the blocks' mean rows
+    (64-bit, over the rows in front of the sample's end), NaN last, the lower j
+    first among equals."""
     args = (tensor_layout, int(keep), bool(is_causal), int(sink_blocks), int(local_blocks), int(blkq), int(blkk),
             query_lengths, key_lengths)
     if tensor_layout in ("HND", "NHD") and query_int8.is_cuda and not torch.compiler.is_compiling():
@@ -262,8 +263,9 @@ def key_block_attention(
     nothing.  Keys at or past ``key_lengths[b]`` are not seen, whatever codes
     and values stand there; rows at or past ``query_lengths[b]``, and rows that
     see no key, are zeros.  Causal masks are aligned at the first row and key.
-    Scales are not negative (a quantizer's are not); one that is infinite or NaN
-    makes NaN of the rows that see its keys, or that have it, and of no others.
+    Scales are not negative (a quantizer's are not); one that is NaN, or infinite
+    with codes of zero as a quantizer leaves them, makes NaN of the rows that see
+    its keys, or that have it, and of no others.
     Values of the listed blocks in front of the sample's end must be finite, as
     in the dense attention: 0 times infinity is a NaN in every row of the tile.
     Output: bf16 in the layout and shape of ``query_int8``."""

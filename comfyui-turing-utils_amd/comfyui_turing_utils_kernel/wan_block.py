@@ -207,8 +207,10 @@ class WanBlockConfig:
 @dataclass(frozen=True)
 class BlockSparsity:
     """Self-attention over ``keep`` key blocks of 64 for each query block of
-    128, the first ``sink_blocks`` and the ``local_blocks`` on either side of
-    the query block's own always among them (``turing_sage.select_key_blocks``)."""
+    128.  Among them, as far as ``keep`` goes, are always the first
+    ``sink_blocks`` and, with ``local_blocks`` = w, the two key blocks of the
+    query block's own 128 tokens and w - 1 more on each side (so 1 keeps no
+    neighbour); see ``turing_sage.select_key_blocks``."""
     keep: int
     sink_blocks: int = 0
     local_blocks: int = 0

@@ -227,12 +227,14 @@ int32_t launch_down(const int8_t *a, const float *a_scale, const uint16_t *down,
     if (tiles() < cus) rows = 16;
     else if (ranks <= 32 && tiles() >= 4 * cus) rows = 64;
 #define TU_DOWN(R, F, S) adapter_down_kernel<R, F, 8, S><<<grid, 512, 0, st>>>(a, a_scale, down, scaling, ad, slots, h, m, k, sort, sort + 4)
-    // Requests of less than a tile's rows: a tile walks every adapter among its
-    // rows, all of K each time.  Where that is eight or more, or much work again,
-    // the rows are sorted by their adapter first, by a launch of 5 to 11 us (with
+    // Requests of few rows: a tile walks every adapter among its rows, all of K
+    // each time.  Where 16 rows have eight or more, or four and much work again,
+    // the rows are sorted by their adapter first, by a launch of 5 to 11 us: with
     // it 1564 rows of 11760, 29 adapters of rank 40: 269 -> 27 us; 4000 of 5120,
     // 16 of rank 32: 148 -> 30; 300 of 2048, 32 of rank 64: 18.5 -> 10.7; 10027 of
-    // 1344, 4 of rank 8 would go from 14 to 19 and is not sorted).
+    // 1344, 4 of rank 8 would go from 14 to 19 and is not sorted.  (Requests of 6
+    // to 15 rows never are, though a tile of 64 rows may have 5 to 12 of them, nor
+    // are more than 1024 adapters.)
     const int64_t walked = std::min<int64_t>(ad.count, (16 + ad.id_rows - 1) / ad.id_rows);
     if (ad.count <= kSortThreads && m >= kLeastSorted && m <= 0x7fffffff && walked >= 4 &&
         (walked >= 8 || (walked - 1) * m * k >= int64_t{1} << 26)) {

@@ -354,9 +354,10 @@ int32_t tu_sage_attn_fwd_auto(const int8_t *q8, const float *q_scale, int64_t bl
  *   S_ij = mq_i . mk_j in fp64
  * Block j is visible to block i if i has rows below the sample's length,
  * 64 j < the sample's key length and, causal, 64 j <= i's last row.  Of the
- * visible ones the first `keep` are taken by: forced blocks (j < sink_blocks;
- * with local_blocks = w > 0, 2 i - (w - 1) <= j <= 2 i + w), then the larger
- * S, NaN last, then the lower j.  index: int32 [batch, hq, ceil(lq / 128),
+ * visible ones the first `keep` are taken: the forced blocks (j < sink_blocks;
+ * with local_blocks = w > 0, 2 i - (w - 1) <= j <= 2 i + w) in the order of j,
+ * then the others by the larger S, NaN last, the lower j first among equals.
+ * index: int32 [batch, hq, ceil(lq / 128),
  * min(keep, ceil(lk / 64))], ascending, -1 behind the last.  Codes, scales and
  * strides as tu_sage_attn_fwd's.  workspace: 16-byte aligned, at least
  * tu_sage_block_select_workspace(...) bytes.  No counterpart in the reference
@@ -378,8 +379,9 @@ int32_t tu_sage_block_select(const int8_t *q8, const float *q_scale, int64_t blk
  * [0, ceil(lk / 64)) and is larger than every entry before it.  Keys at or
  * past k_lengths[b] are not seen (codes and values there may be anything);
  * rows at or past q_lengths[b], and rows that see no key, are zeros.  Scales
- * are not negative; one that is no number makes NaN of the rows that see its
- * keys, or that have it, and of no others.  Causal: top-left aligned.  Grids of few workgroups on a device of `cus` compute
+ * are not negative; one that is NaN, or infinite with codes of zero as
+ * tu_sage_quant leaves them, makes NaN of the rows that see its keys, or that
+ * have it, and of no others.  Causal: top-left aligned.  Grids of few workgroups on a device of `cus` compute
  * units split their lists into ranges that a second kernel merges, as many as
  * `workspace` (16-byte aligned, workspace_bytes long) holds;
  * tu_sage_block_attn_workspace gives the bytes for all of them (0: no split),
