@@ -19,8 +19,8 @@
 // share a tile's adapters; many rows of many adapters are sorted by it first.
 //
 // What bounds it: the loads of codes and ranks, half of the loop's time each;
-// its waves wait for 50 to 77 % of their cycles.  32760 rows of 5120, rank 32:
-// 53 us, 173 MB past the L2 (33 us of copy); 2050 rows, rank 64: 22 us, 54 MB.
+// its waves wait for 43 to 79 % of their cycles.  32760 rows of 5120, rank 32:
+// 51 us, 173 MB past the L2 (35 us of copy); 2050 rows, rank 64: 21 us, 54 MB.
 // Whole 128-byte lines a load (lanes lc and lc + 8 exchanging halves) and the
 // ranks of a row tile on one die were slower (134.5 -> 135.5, 132 -> 134.7 us
 // with the GEMM at 2050 rows).

@@ -274,11 +274,12 @@ __device__ __forceinline__ uint32_t residual_pair(uint32_t y, uint32_t r, uint32
 // masked zeros would carry an infinite weight of one request's adapter into
 // another's).
 //
-// What it costs beside the GEMM without adapters: 15 of 118 us at 2050 x 5120 x
+// What it costs beside the GEMM without adapters: 18 of 116 us at 2050 x 5120 x
 // 10240, rank 64, where a workgroup has a CU to itself and its loads of h and up
-// (100 KB) stand between its last MFMA and its first store; nothing that can be
-// told from the noise of 785 us at 32760 x 5120 x 5120, rank 32; 5 of 17 us at
-// 61 rows that have 16 adapters.
+// (100 KB) stand between its last MFMA and its first store; 7 of 762 us, less
+// than launches differ by, at 32760 x 5120 x 5120, rank 32; 5 of 16.5 us at 61
+// rows that have 16 adapters; 82 of 1976 us at 32760 x 5120 x 15360 with three
+// parts of rank 32.
 template <int kFragsM>
 struct RowAdapters {
     int id[kFragsM];
