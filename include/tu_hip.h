@@ -174,9 +174,9 @@ int32_t tu_int8_gemm_bf16_residual(const int8_t *a, const int8_t *w, const float
  * tu_int8_gemm_bf16_residual.  Codes are those of a rotated activation, so
  * down holds the adapter's rows rotated alike.  h is summed in fp32 and kept
  * as two bf16 terms (to 2^-16 of it), infinities and NaN among them; an
- * infinite element of up, which both terms meet, gives infinity or NaN.  down: bf16 [count, rank, k]; up: bf16
- * [count, n, rank / parts]: the columns and the ranks are `parts` equal parts
- * each (a multiple of 16 columns where there are several), and the columns of
+ * infinite element of up, which both terms meet, gives infinity or NaN.
+ * down: bf16 [count, rank, k]; up: bf16 [count, n, rank / parts]: the columns
+ * and the ranks are `parts` equal parts each (a multiple of 16 columns where there are several), and the columns of
  * a part see that part's ranks, as projections side by side have adapters of
  * their own; scaling: fp32 [count]; ids: int32 [ceil(m / id_rows)];
  * rank a multiple of 8 * parts up to 4096; down, up, residual and gate 16-byte
@@ -357,8 +357,7 @@ int32_t tu_sage_attn_fwd_auto(const int8_t *q8, const float *q_scale, int64_t bl
  * visible ones the first `keep` are taken: the forced blocks (j < sink_blocks;
  * with local_blocks = w > 0, 2 i - (w - 1) <= j <= 2 i + w) in the order of j,
  * then the others by the larger S, NaN last, the lower j first among equals.
- * index: int32 [batch, hq, ceil(lq / 128),
- * min(keep, ceil(lk / 64))], ascending, -1 behind the last.  Codes, scales and
+ * index: int32 [batch, hq, ceil(lq / 128), min(keep, ceil(lk / 64))], ascending, -1 behind the last.  Codes, scales and
  * strides as tu_sage_attn_fwd's.  workspace: 16-byte aligned, at least
  * tu_sage_block_select_workspace(...) bytes.  No counterpart in the reference
  * (its Sol router, comfyui_turing_utils/attention/sparse.py, selects by
@@ -381,8 +380,8 @@ int32_t tu_sage_block_select(const int8_t *q8, const float *q_scale, int64_t blk
  * rows at or past q_lengths[b], and rows that see no key, are zeros.  Scales
  * are not negative; one that is NaN, or infinite with codes of zero as
  * tu_sage_quant leaves them, makes NaN of the rows that see its keys, or that
- * have it, and of no others.  Causal: top-left aligned.  Grids of few workgroups on a device of `cus` compute
- * units split their lists into ranges that a second kernel merges, as many as
+ * have it, and of no others.  Causal: top-left aligned.  Grids of few
+ * workgroups on a device of `cus` compute units split their lists into ranges that a second kernel merges, as many as
  * `workspace` (16-byte aligned, workspace_bytes long) holds;
  * tu_sage_block_attn_workspace gives the bytes for all of them (0: no split),
  * and without one (NULL, 0) nothing is split.  The rest as tu_sage_attn_fwd.

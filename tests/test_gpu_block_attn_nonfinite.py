@@ -148,3 +148,25 @@ def test_an_infinite_input_gives_what_the_dense_attention_gives(gpu_device, wher
     dense = turing_sage.sageattn(q, k, v)
     got = turing_sage.sparse_sageattn(q, k, v, keep=(lk + 63) // 64)
     assert dense[:, 1].isnan().any() and torch.equal(got.isnan(), dense.isnan())
+
+
+@pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("causal", [False, True])
+def test_waves_of_ordinary_and_of_far_scores_side_by_side(gpu_device, d, causal):
+    """Rows 32 .. 63 of every query block have scores of 2^30 and more, the
+    others ordinary ones; 800 query blocks, so that no list is split, with lists
+    of up to 280 entries, a segment and some."""
+    lq, lk, width = 128 * 40 - 3, 64 * 320, 280
+    q8, qs, k8, ks, vt, g = attn._inputs(gpu_device, 1, 20, 20, lq, lk, d, blkq=16, blkk=64, seed=9)
+    assert not _parts(1, 20, lq, d, width)
+    ks.fill_(2.0 ** -6)
+    qs.fill_(1.0)
+    group = torch.arange(qs.size(2), device=gpu_device) % 8
+    qs[:, :, (group == 2) | (group == 3)] = 2.0 ** 24
+    index = attn._random_lists(1, 20, lq, lk, width, g, gpu_device)
+    got = turing_sage.key_block_attention(q8, qs, k8, ks, vt, index, is_causal=causal, blkq=16, blkk=64)
+    assert torch.equal(got, turing_sage.key_block_attention(q8, qs, k8, ks, vt, index, is_causal=causal, blkq=16, blkk=64))
+    two = [t[:, 3:5] for t in (q8, qs, k8, ks, vt, index)]
+    want, size = ref.attend(*two, "HND", causal, d ** -0.5, 16, 64)
+    off, bound = (got[:, 3:5].double() - want).abs(), ref.attend_bound(want, size)
+    assert bool((off <= bound).all()), float((off / bound.clamp_min(1e-30)).max())
