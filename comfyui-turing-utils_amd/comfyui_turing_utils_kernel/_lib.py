@@ -184,9 +184,27 @@ SIGNATURES: dict[str, tuple[object, list[object]]] = {
          _i64, _i64, _i64, _i64, _i64, _i64, _i64, _i64, _i64,
          _c_void_p, _c_void_p, _f32, _i32, _i32, _c_void_p, _i64, _c_void_p],
     ),
+    "tu_kv_cache_append": (
+        _i32,
+        [_c_void_p, _c_void_p, _c_void_p, _i32, _i64, _i64, _i64, _i64, _i64, _i64, _i64, _i64, _i64, _i64,
+         _c_void_p, _c_void_p, _i64, _c_void_p, _c_void_p, _c_void_p, _c_void_p, _c_void_p, _c_void_p, _i64,
+         _c_void_p, _c_void_p],
+    ),
+    "tu_kv_cache_read": (
+        _i32,
+        [_c_void_p, _c_void_p, _c_void_p, _c_void_p, _i64, _c_void_p, _i64, _c_void_p, _c_void_p, _c_void_p,
+         _c_void_p, _c_void_p, _i32, _i64, _i64, _i64, _i64, _i64, _i64, _i64, _i64, _i64, _i64, _c_void_p],
+    ),
+    "tu_kv_cache_attn_workspace": (_i64, [_i64, _i64, _i64, _i64, _i64, _i64, _i32]),
+    "tu_kv_cache_attn": (
+        _i32,
+        [_c_void_p, _c_void_p, _i32, _i64, _c_void_p, _c_void_p, _c_void_p, _c_void_p, _i64, _c_void_p, _i64,
+         _c_void_p, _c_void_p, _c_void_p, _i64, _i64, _i64, _i64, _i64, _i64, _i64, _i64, _i64, _i64, _i64,
+         _f32, _i32, _i64, _i32, _c_void_p, _i64, _c_void_p],
+    ),
 }
 
-ABI_VERSION = 19
+ABI_VERSION = 20
 
 _lock = threading.Lock()
 _lib: ctypes.CDLL | None = None
@@ -225,6 +243,7 @@ class _GeneralRoute:
         return None
 
     sageattn = w8a8attn = select_key_blocks = key_block_attention = int8_linear_adapters = int8_linear
+    kv_cache_append = kv_cache_read = kv_cache_attention = int8_linear
 
 
 _host = None

@@ -11,7 +11,9 @@ dense W8A8 path: ``w8a8attn``, ``w8a8attn_compiled``, ``prequantize_sol_sageattn
 Beside them, without a counterpart in the reference's facade (and so not in
 ``__all__``, which is the reference's list): the block-sparse attention of
 ``sparse.py``, ``sparse_sageattn``, ``sparse_sageattn_from_prequantized``,
-``select_key_blocks`` and ``key_block_attention``.
+``select_key_blocks`` and ``key_block_attention``, and the key/value cache in 8
+bits of ``kv_cache.py``, ``QuantizedKVCache``, ``SequenceKVCache``,
+``kv_cache_append``, ``kv_cache_read`` and ``kv_cache_attention``.
 """
 from __future__ import annotations
 
@@ -204,6 +206,13 @@ def preflight_w8a8(device: torch.device) -> None:
 
 # Registers the torch.ops.turing_utils attention ops on import.
 from . import custom_ops  # noqa: E402,F401
+from .kv_cache import (  # noqa: E402,F401
+    QuantizedKVCache,
+    SequenceKVCache,
+    kv_cache_append,
+    kv_cache_attention,
+    kv_cache_read,
+)
 from .sparse import (  # noqa: E402,F401
     key_block_attention,
     select_key_blocks,

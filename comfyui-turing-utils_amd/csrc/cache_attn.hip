@@ -1,0 +1,963 @@
+// Attention over the paged key/value cache in 8 bits (kv_cache.hip's pages).
+// No counterpart in the reference's kernels.
+//
+//   out_r = sum_j p_rj v_j / sum_j p_rj over the keys j the row sees,
+//   p = 2^(s - m), s = (q . k8) * (sm_scale * log2 e) * k_scale
+// with q int8 codes and their scales, or 16-bit floats.  A float row is taken as
+// integers of 16 bits, x ~ a (256 h + l) with h, l int8 and a = max |x| / 32512:
+// two INT8 products in place of one in 16-bit floats, which would need every key
+// converted; the error, 2^-16 of the row's largest, is below a bf16's own.
+//
+// Values are int8 codes with one scale a page.  They enter PV as fp16, exactly,
+// and the page's scale enters the exponent: w = 2^(s + log2 v_scale - m') is at
+// most about 1 for the largest p * v_scale of the row, so fp16 (11 bits) holds
+// the weights that matter, whatever the pages' scales are.  The row sum
+// sum w / v_scale is kept apart, in fp32 from the unrounded w.
+//   m' is held as the pair (score, log2 scale): far scores would swallow the
+// scale in a sum.  A page's log2 scale is taken as at least that of the base
+// less 64: its values are then too small to matter (2^-57 of the largest term),
+// and w stays a normal number for the row sum.
+//
+// Two kernels: few rows a K/V head (single tokens) read every code once from HBM
+// into registers; many rows share K and V tiles in LDS.  Both split a sequence's
+// pages into ranges where the grid would leave the chip empty; a third merges.
+#include <algorithm>
+#include <type_traits>
+
+#include "attn_common.h"
+#include "attn_plan.h"
+
+namespace tu {
+namespace {
+
+typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
+
+constexpr int kPage = 64;
+constexpr int kThreads = 256;
+constexpr float kNoBase = -3.402823466e38f;  // score of a row's base before its first key
+constexpr float kSlack = 8.0f;               // log2 of the largest w allowed
+constexpr float kLeastScale = -64.0f;        // least log2 of a page's V scale, less the base's
+constexpr float kZeroValues = -100.0f;       // log2 V scale of a page whose values count as zeros
+constexpr int kQInt8 = 2;                    // query types: 0 bf16, 1 fp16
+
+struct CacheCall {
+    const void *q;
+    const float *q_scale;  // int8 queries: [batch][hq][nbq]
+    uint32_t q_type, blkq, nbq;
+    const int8_t *k_codes, *v_codes;
+    const float *k_scale, *v_scale;
+    const int32_t *table, *lengths, *q_lengths;
+    int32_t width, pages;
+    uint32_t batch, hkv, group;  // group: query heads of a K/V head
+    uint32_t lq, rows;           // rows = lq * group, of one K/V head
+    uint32_t row_blocks, parts;
+    bool causal, out_fp16;
+    float sm_log2;
+    uint16_t *o;
+    int64_t q_sb, q_sh, q_sl, o_sb, o_sh, o_sl;
+    float *part_o, *part_m;  // [parts][batch * hkv * rows][D] and [..][4]: base score, base scale, sum
+};
+
+// A unit of work: rows of one K/V head over a range of its sequence's pages.
+struct Unit {
+    uint32_t b, hk, block, z;
+    int n, length;   // query tokens and keys of the sequence
+    int seen;        // keys that some row of the block sees
+    int first, end;  // pages of the range
+    int used;        // ranges that the block's pages fill
+};
+
+__device__ __forceinline__ int clamp_length(const int32_t *lengths, uint32_t b, int most) {
+    return lengths ? min(max(lengths[b], 0), most) : most;
+}
+
+// Keys that query token `t` of n sees: all, or up to its own place, the n queries
+// being the sequence's last tokens.
+__device__ __forceinline__ int keys_of(const CacheCall &c, int t, int n, int length) {
+    return c.causal ? min(length, max(length - n + t + 1, 0)) : length;
+}
+
+// Rows are numbered by token, then by head of the group.
+template <int kRows>
+__device__ __forceinline__ Unit unit_of(const CacheCall &c, uint32_t b, uint32_t hk, uint32_t block, uint32_t z) {
+    Unit u;
+    u.b = b, u.hk = hk, u.block = block, u.z = z;
+    u.n = clamp_length(c.q_lengths, b, static_cast<int>(c.lq));
+    u.length = clamp_length(c.lengths, b, c.width * kPage);
+    const uint32_t last = min(c.rows, (block + 1) * kRows) - 1;
+    const int token = min(static_cast<int>(last / c.group), u.n - 1);
+    u.seen = block * kRows < static_cast<uint32_t>(u.n) * c.group ? keys_of(c, token, u.n, u.length) : 0;
+    const int pages = (u.seen + kPage - 1) / kPage, per = (pages + c.parts - 1) / c.parts;
+    u.first = min(pages, static_cast<int>(z) * per);
+    u.end = min(pages, u.first + per);
+    u.used = per ? (pages + per - 1) / per : 1;
+    return u;
+}
+
+template <int kRows>
+__device__ __forceinline__ Unit unit_at(const CacheCall &c, uint32_t id) {
+    const uint32_t z = id % c.parts, rest = id / c.parts, block = rest % c.row_blocks, bh = rest / c.row_blocks;
+    return unit_of<kRows>(c, bh / c.hkv, bh % c.hkv, block, z);
+}
+
+// A row of the call: query token and head.  Rows past the last are the last.
+struct Row {
+    int token;
+    uint32_t head;
+};
+__device__ __forceinline__ Row row_at(const CacheCall &c, uint32_t hk, uint32_t r) {
+    r = min(r, c.rows - 1);
+    return Row{static_cast<int>(r / c.group), hk * c.group + r % c.group};
+}
+
+// 16 channels of a query row from `c0` on as bytes h and l, for each of kSl
+// pieces (c0 + step * i), and the row's factor (scale * sm_scale * log2 e of one
+// unit of 256 h + l).  The row's lanes are the four groups of 16.
+template <int kSl, bool kTerms>
+__device__ __forceinline__ float load_row(const CacheCall &c, const Row &row, uint32_t b, bool in, int c0, int step,
+                                          i32x4 (&hi)[kSl], i32x4 (&lo)[kSl]) {
+#pragma unroll
+    for (int i = 0; i < kSl; ++i) hi[i] = lo[i] = i32x4{0, 0, 0, 0};
+    const int64_t off = b * c.q_sb + row.head * c.q_sh + row.token * c.q_sl + c0;
+    if (!kTerms || c.q_type == kQInt8) {
+        if (!in) return 0.0f;
+#pragma unroll
+        for (int i = 0; i < kSl; ++i)
+            hi[i] = *reinterpret_cast<const i32x4 *>(static_cast<const int8_t *>(c.q) + off + step * i);
+        const int64_t at = static_cast<int64_t>(b * c.hkv * c.group + row.head) * c.nbq + static_cast<uint32_t>(row.token) / c.blkq;
+        return c.q_scale[at] * c.sm_log2 * (kTerms ? 0.00390625f : 1.0f);
+    }
+    float x[kSl][16] = {};
+    if (in) {
+#pragma unroll
+        for (int i = 0; i < kSl; ++i) {
+            const auto *src = reinterpret_cast<const u32x4 *>(static_cast<const uint16_t *>(c.q) + off + step * i);
+            const u32x4 w[2] = {src[0], src[1]};
+#pragma unroll
+            for (int e = 0; e < 16; ++e) {
+                const uint32_t pair = w[e >> 3][(e >> 1) & 3], bits = e & 1 ? pair >> 16 : pair & 0xffffu;
+                x[i][e] = c.q_type == 0 ? bf16_bits_to_f32(bits)
+                                        : static_cast<float>(__builtin_bit_cast(_Float16, static_cast<uint16_t>(bits)));
+            }
+        }
+    }
+    // (bit patterns: a NaN is the largest)
+    int top = 0;
+#pragma unroll
+    for (int i = 0; i < kSl; ++i)
+#pragma unroll
+        for (int e = 0; e < 16; ++e) top = max(top, static_cast<int>(__float_as_uint(x[i][e]) & 0x7fffffffu));
+    top = xmax_i32(top);
+    const float amax = __int_as_float(top);
+    const float inverse = 32512.0f / fmaxf(amax, 1e-30f);
+#pragma unroll
+    for (int i = 0; i < kSl; ++i)
+#pragma unroll
+        for (int e = 0; e < 16; ++e) {
+            const int v = static_cast<int>(rintf(x[i][e] * inverse));
+            const int h = (v + 128) >> 8, l = v - (h << 8);
+            hi[i][e >> 2] |= (h & 0xff) << (8 * (e & 3));
+            lo[i][e >> 2] |= (l & 0xff) << (8 * (e & 3));
+        }
+    return amax / 32512.0f * c.sm_log2;
+}
+
+// Four int8 codes as two pairs of fp16: the bytes biased by 128 below the
+// exponent of 1024, less 1152.
+__device__ __forceinline__ u32x2 codes_to_f16(uint32_t w) {
+    const f16x2_t bias = {static_cast<_Float16>(1152.0f), static_cast<_Float16>(1152.0f)};
+    const uint32_t x = w ^ 0x80808080u;
+    const uint32_t a = __builtin_amdgcn_perm(0x64646464u, x, 0x07010700u);
+    const uint32_t b = __builtin_amdgcn_perm(0x64646464u, x, 0x07030702u);
+    return u32x2{__builtin_bit_cast(uint32_t, __builtin_bit_cast(f16x2_t, a) - bias),
+                 __builtin_bit_cast(uint32_t, __builtin_bit_cast(f16x2_t, b) - bias)};
+}
+
+__device__ __forceinline__ float lane_value(float v, int lane) {
+    return __int_as_float(__builtin_amdgcn_readlane(__float_as_int(v), lane));
+}
+
+// Pages of a range, 64 at a time: lane i holds the i-th one's place in the pool
+// (-1: none), K scale and log2 of the V scale.
+struct PageWindow {
+    int page;
+    float k_scale, v_log2;
+    __device__ __forceinline__ void fetch(const CacheCall &c, const Unit &u, int from, int step, int lane) {
+        const int at = from + step * lane;
+        int p = -1;
+        if (at < u.end) p = c.table[static_cast<int64_t>(u.b) * c.width + at];
+        page = p >= 0 && p < c.pages ? p : -1;
+        const int64_t s = static_cast<int64_t>(max(page, 0)) * c.hkv + u.hk;
+        k_scale = c.k_scale[s];
+        // (a NaN stays; below 2^-100, where a sum of weights over the scale might be
+        // no number, the values count as zeros of that scale)
+        const float v = c.v_scale[s];
+        v_log2 = v <= 7.888609052e-31f ? kZeroValues : __builtin_amdgcn_logf(v);
+    }
+};
+
+// The softmax state of a row: base (score, log2 of a V scale), and in the lane
+// its share of the sum of w / v_scale.
+struct RowState {
+    float m = kNoBase, v = 0.0f, l = 0.0f;
+    // the page's log2 V scale less the base's (a NaN stays)
+    __device__ __forceinline__ float shift(float v_log2) const {
+        const float d = v_log2 - v;
+        return d < kLeastScale ? kLeastScale : d;
+    }
+};
+
+// Results of a unit's rows: o[ds][r] = channel 16 ds + 4 g + r of the row of the
+// lane's column, l its whole sum.  Written out, or for the merge.
+template <int D>
+__device__ __forceinline__ void store_row(const CacheCall &c, const Unit &u, const f32x4 (&o)[D / 16], float m, float v, float l,
+                                          uint32_t r, int g) {
+    const Row row = row_at(c, u.hk, r);
+    if (u.used > 1) {
+        if (r >= c.rows) return;
+        const int64_t rows = static_cast<int64_t>(c.batch) * c.hkv * c.rows;
+        const int64_t at = u.z * rows + static_cast<int64_t>(u.b * c.hkv + u.hk) * c.rows + r;
+#pragma unroll
+        for (int ds = 0; ds < D / 16; ++ds) *reinterpret_cast<f32x4 *>(c.part_o + at * D + 16 * ds + 4 * g) = o[ds];
+        if (g == 0) *reinterpret_cast<f32x4 *>(c.part_m + at * 4) = f32x4{m, v, l, 0.0f};
+        return;
+    }
+    // (a sum of 0 is a row that saw no key; one that is NaN stays NaN)
+    const bool some = l != 0.0f && row.token < u.n;
+    const float inv = 1.0f / l;
+    uint16_t *op = c.o + u.b * c.o_sb + row.head * c.o_sh + row.token * c.o_sl;
+#pragma unroll
+    for (int ds = 0; ds < D / 16; ds += 2) {
+        uint32_t w[2][2];
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+            const f32x4 a = o[ds + i] * inv;
+            const uint32_t p0 = c.out_fp16 ? hw_f16x2_bits(a[0], a[1]) : hw_bf16x2_bits(a[0], a[1]);
+            const uint32_t p1 = c.out_fp16 ? hw_f16x2_bits(a[2], a[3]) : hw_bf16x2_bits(a[2], a[3]);
+            w[i][0] = some ? p0 : 0;
+            w[i][1] = some ? p1 : 0;
+        }
+        // each lane ends with 8 contiguous channels of one row
+        auto lo = __builtin_amdgcn_permlane16_swap(w[0][0], w[1][0], false, false);
+        auto hi = __builtin_amdgcn_permlane16_swap(w[0][1], w[1][1], false, false);
+        if (r >= c.rows) continue;
+        auto *dst = reinterpret_cast<u32x2 *>(op + 16 * (ds + (g & 1)) + 8 * (g >> 1));
+        dst[0] = u32x2{lo[0], hi[0]};
+        dst[1] = u32x2{lo[1], hi[1]};
+    }
+}
+
+// The other of two bases where it is higher: by score, and log2 of the V scale.
+__device__ __forceinline__ bool higher(float m, float v, float than_m, float than_v) {
+    return (m - than_m) + (v - than_v) > 0.0f;
+}
+
+// ---------------------------------------------------------------------------
+// Few rows
+// ---------------------------------------------------------------------------
+// A workgroup of four waves has 16 kRT rows of one K/V head; its waves take the
+// pages of the unit's range in turn, each for itself, and are merged at the end.
+// A wave reads a page's codes straight into the MFMA operands: keys 16 g + e of a
+// page belong to lane group g throughout, so that a lane's 16 bytes of a V^T row
+// are the keys whose weights it holds, and a key row's bytes go to the lanes in
+// runs of D / 4.  The next page's loads (16 KiB a wave at D = 128) are in flight
+// while one is computed: what a CU needs to keep HBM busy.
+template <int D>
+struct PageRegs {
+    i32x4 k[4][D / 64];
+    u32x4 v[D / 16];
+    __device__ __forceinline__ void load(const CacheCall &c, int64_t at, int g, int lc) {
+        const int8_t *k_page = c.k_codes + at * kPage * D, *v_page = c.v_codes + at * kPage * D;
+#pragma unroll
+        for (int t = 0; t < 4; ++t)
+#pragma unroll
+            for (int i = 0; i < D / 64; ++i)
+                k[t][i] = *reinterpret_cast<const i32x4 *>(k_page + (16 * (lc >> 2) + 4 * t + (lc & 3)) * D + D / 4 * g + 16 * i);
+#pragma unroll
+        for (int ds = 0; ds < D / 16; ++ds)
+            v[ds] = *reinterpret_cast<const u32x4 *>(v_page + (16 * ds + lc) * kPage + 16 * g);
+    }
+};
+
+template <int D, int kRT>
+__global__ __launch_bounds__(kThreads, 2) void cache_few_kernel(CacheCall c) {
+    constexpr int kSl = D / 64, kDS = D / 16, kRows = 16 * kRT;
+    __shared__ __align__(16) float merge_o[3][kRT][kDS][64][4];
+    __shared__ float merge_m[4][kRT][64][3];
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int g = lane >> 4, lc = lane & 15;
+    const Unit u = unit_at<kRows>(c, xcd_chunk(blockIdx.x, gridDim.x));
+    if (u.z > 0 && static_cast<int>(u.z) >= u.used) return;  // the whole workgroup: nothing is left for the range
+    PageWindow window;
+    int base = u.first + wave;  // page of the window's lane 0; the wave's pages are 4 apart
+    window.fetch(c, u, base, 4, lane);
+    auto place = [&](int p) {  // of page p of the sequence, one of the window's
+        return static_cast<int64_t>(max(__builtin_amdgcn_readlane(window.page, (p - base) >> 2), 0)) * c.hkv + u.hk;
+    };
+    i32x4 qh[kRT][kSl], ql[kRT][kSl];
+    float factor[kRT];
+    int limit[kRT];
+    RowState st[kRT];
+    f32x4 o[kRT][kDS];
+#pragma unroll
+    for (int rt = 0; rt < kRT; ++rt) {
+        const uint32_t r = u.block * kRows + 16 * rt + lc;
+        const Row row = row_at(c, u.hk, r);
+        const bool in = r < c.rows && row.token < u.n;
+        factor[rt] = load_row<kSl, true>(c, row, u.b, in, D / 4 * g, 16, qh[rt], ql[rt]);
+        limit[rt] = in ? keys_of(c, row.token, u.n, u.length) : 0;
+#pragma unroll
+        for (int ds = 0; ds < kDS; ++ds) o[rt][ds] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+    }
+
+    auto compute = [&](const PageRegs<D> &r, int p) {
+        const int at = (p - base) >> 2;
+        const bool there = __builtin_amdgcn_readlane(window.page, at) >= 0;
+        const float k_scale = lane_value(window.k_scale, at), v_log2 = lane_value(window.v_log2, at);
+        const int key0 = p * kPage + 16 * g;  // the lane's keys are key0 ..+15
+#pragma unroll
+        for (int rt = 0; rt < kRT; ++rt) {
+            i32x4 s[4];
+#pragma unroll
+            for (int t = 0; t < 4; ++t) {
+                i32x4 acc = {0, 0, 0, 0};
+#pragma unroll
+                for (int i = 0; i < kSl; ++i) acc = __builtin_amdgcn_mfma_i32_16x16x64_i8(r.k[t][i], qh[rt][i], acc, 0, 0, 0);
+                acc <<= 8;
+#pragma unroll
+                for (int i = 0; i < kSl; ++i) acc = __builtin_amdgcn_mfma_i32_16x16x64_i8(r.k[t][i], ql[rt][i], acc, 0, 0, 0);
+                s[t] = acc;
+            }
+            const float f = factor[rt] * k_scale;
+            const int seen = there ? limit[rt] - key0 : 0;  // the first so many of the lane's keys
+            float x[16], top = -INFINITY;
+#pragma unroll
+            for (int e = 0; e < 16; ++e) {
+                x[e] = static_cast<float>(s[e >> 2][e & 3]) * f;
+                if (e < seen) top = fmaxf(top, x[e]);
+            }
+            const bool need = (top - st[rt].m) + (v_log2 - st[rt].v) > kSlack;
+            if (__any(need)) {
+                // a row's base moves by its own scores alone
+                const float row_top = xmax_f32(top);
+                if ((row_top - st[rt].m) + (v_log2 - st[rt].v) > kSlack) {
+                    const float alpha = __builtin_amdgcn_exp2f((st[rt].m - row_top) + (st[rt].v - v_log2));
+                    st[rt].m = row_top, st[rt].v = v_log2;
+                    st[rt].l *= alpha;
+#pragma unroll
+                    for (int ds = 0; ds < kDS; ++ds) o[rt][ds] *= alpha;
+                }
+            }
+            const float d = st[rt].shift(v_log2);
+            float sum = 0.0f;
+            f16x8 w[2];
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+                u32x4 packed;
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    float y[2];
+#pragma unroll
+                    for (int i = 0; i < 2; ++i) {
+                        const int e = 8 * h + 2 * j + i;
+                        y[i] = e < seen ? __builtin_amdgcn_exp2f((x[e] - st[rt].m) + d) : 0.0f;
+                        sum += y[i];
+                    }
+                    packed[j] = hw_f16x2_bits(y[0], y[1]);
+                }
+                w[h] = __builtin_bit_cast(f16x8, packed);
+            }
+            // w / v_scale, the scale being 2^(base's + d) (a lane without keys has no part in a NaN)
+            if (seen > 0) st[rt].l = __builtin_fmaf(sum, __builtin_amdgcn_exp2f(-(st[rt].v + d)), st[rt].l);
+            if (v_log2 == kZeroValues) continue;
+#pragma unroll
+            for (int ds = 0; ds < kDS; ++ds) {
+#pragma unroll
+                for (int h = 0; h < 2; ++h) {
+                    const u32x2 a = codes_to_f16(r.v[ds][2 * h]), b = codes_to_f16(r.v[ds][2 * h + 1]);
+                    const f16x8 v = __builtin_bit_cast(f16x8, (u32x4{a[0], a[1], b[0], b[1]}));
+                    o[rt][ds] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v, w[h], o[rt][ds], 0, 0, 0);
+                }
+            }
+        }
+    };
+
+    PageRegs<D> even, odd;
+    int p = base;
+    if (p < u.end) even.load(c, place(p), g, lc);
+    // Two pages a step, so that the registers of one are filled while the other is computed.
+#pragma clang loop unroll(disable)
+    for (; p < u.end; p += 8) {
+        if (p + 4 < u.end) odd.load(c, place(p + 4), g, lc);
+        compute(even, p);
+        if (p + 4 >= u.end) break;
+        const bool refill = p + 8 - base >= 64 * 4;
+        if (!refill && p + 8 < u.end) even.load(c, place(p + 8), g, lc);
+        compute(odd, p + 4);
+        if (refill && p + 8 < u.end) {
+            base = p + 8;
+            window.fetch(c, u, base, 4, lane);
+            even.load(c, place(p + 8), g, lc);
+        }
+    }
+
+    // The waves' states, merged by the first.
+    const bool alone = u.end - u.first <= 1;
+#pragma unroll
+    for (int rt = 0; rt < kRT; ++rt) {
+        st[rt].l = xsum_f32(st[rt].l);
+        if (alone) continue;
+        merge_m[wave][rt][lane][0] = st[rt].m;
+        merge_m[wave][rt][lane][1] = st[rt].v;
+        merge_m[wave][rt][lane][2] = st[rt].l;
+        if (wave > 0) {
+#pragma unroll
+            for (int ds = 0; ds < kDS; ++ds) *reinterpret_cast<f32x4 *>(merge_o[wave - 1][rt][ds][lane]) = o[rt][ds];
+        }
+    }
+    if (!alone) __syncthreads();
+    if (wave > 0) return;
+#pragma unroll
+    for (int rt = 0; rt < kRT; ++rt) {
+        if (!alone) {
+            float m = st[rt].m, v = st[rt].v;
+#pragma unroll
+            for (int i = 1; i < 4; ++i) {
+                const float mi = merge_m[i][rt][lane][0], vi = merge_m[i][rt][lane][1];
+                if (merge_m[i][rt][lane][2] != 0.0f && higher(mi, vi, m, v)) m = mi, v = vi;
+            }
+            float l = 0.0f;
+            f32x4 sum[kDS] = {};
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const float li = merge_m[i][rt][lane][2];
+                if (li == 0.0f) continue;  // saw nothing
+                const float wi = __builtin_amdgcn_exp2f((merge_m[i][rt][lane][0] - m) + (merge_m[i][rt][lane][1] - v));
+                l = __builtin_fmaf(wi, li, l);
+#pragma unroll
+                for (int ds = 0; ds < kDS; ++ds) {
+                    const f32x4 x = i == 0 ? o[rt][ds] : *reinterpret_cast<const f32x4 *>(merge_o[i - (i > 0)][rt][ds][lane]);
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) sum[ds][e] = __builtin_fmaf(wi, x[e], sum[ds][e]);
+                }
+            }
+            st[rt].m = m, st[rt].v = v, st[rt].l = l;
+#pragma unroll
+            for (int ds = 0; ds < kDS; ++ds) o[rt][ds] = sum[ds];
+        }
+        store_row<D>(c, u, o[rt], st[rt].m, st[rt].v, st[rt].l, u.block * kRows + 16 * rt + lc, g);
+    }
+}
+
+// ---------------------------------------------------------------------------
+// Many rows
+// ---------------------------------------------------------------------------
+// A workgroup of four waves has 128 rows of one K/V head, 32 a wave; two share a
+// CU, so that one's MFMAs run beside the other's softmax.  Pages stream through
+// LDS: keys as codes by direct-to-LDS loads, a ring of three; values through
+// registers, converted to fp16 once for the four waves, a ring of two.
+constexpr int kQT = 2;           // 16-row fragments of a wave
+constexpr int kWaveRows = 16 * kQT;
+constexpr int kManyRows = 4 * kWaveRows;
+constexpr int kKRing = 3;
+
+template <int D>
+struct Tiles {
+    static constexpr int kK = kPage * D;      // bytes of a K stage
+    static constexpr int kV = kPage * D * 2;  // of a V stage
+    static constexpr int kV0 = kKRing * kK;
+    static constexpr int kBytes = kV0 + 2 * kV;
+    static constexpr int kKLoads = kK / 4096;  // 16-byte loads of a thread for a page's keys, and for its values
+};
+
+// LDS row of a K tile -> key: within each half of 32, row 16 t + i holds key
+// 8 (i >> 2) + 4 t + (i & 3), so that a lane group owns 8 contiguous keys of a
+// half, one 16-byte piece of a V^T row.
+__device__ __forceinline__ int key_of_row(int row) {
+    return (row & ~31) + 8 * ((row & 15) >> 2) + 4 * ((row >> 4) & 1) + (row & 3);
+}
+
+template <int D>
+struct ManyGeom {
+    uint32_t k_src[Tiles<D>::kKLoads];  // a lane's 16 bytes of a page's keys
+    uint32_t k_rd[D / 64];              // operand of QK^T
+    uint32_t v_rd[2];                   // operand of PV, half 0 / 1
+    uint32_t v_wr[Tiles<D>::kKLoads][2];
+};
+
+// 16-byte pieces of a row are XORed with row bits, so that 16 lanes that read
+// one column of 16 rows meet distinct banks.
+template <int D>
+__device__ __forceinline__ ManyGeom<D> many_geom(int wave, int lane) {
+    ManyGeom<D> gm;
+    const int g = lane >> 4, lc = lane & 15;
+#pragma unroll
+    for (int i = 0; i < Tiles<D>::kKLoads; ++i) {
+        const int piece = (Tiles<D>::kKLoads * wave + i) * 64 + lane;  // of 16 bytes in LDS
+        const int row = piece / (D / 16), at = piece % (D / 16);
+        const int swizzle = D == 128 ? (row >> 1) & 7 : (row >> 2) & 3;
+        gm.k_src[i] = static_cast<uint32_t>(key_of_row(row) * D + (at ^ swizzle) * 16);
+        const int code = i * kThreads + wave * 64 + lane;  // of 16 bytes in the page's values
+        const int ch = code / 4;
+#pragma unroll
+        for (int e = 0; e < 2; ++e) gm.v_wr[i][e] = static_cast<uint32_t>(ch * 128 + (((2 * (code % 4) + e) ^ ((ch >> 1) & 7)) << 4));
+    }
+#pragma unroll
+    for (int i = 0; i < D / 64; ++i)
+        gm.k_rd[i] = static_cast<uint32_t>(lc * D + (D == 128 ? ((4 * i + g) ^ ((lc >> 1) & 7)) : (g ^ ((lc >> 2) & 3))) * 16);
+#pragma unroll
+    for (int i = 0; i < 2; ++i) gm.v_rd[i] = static_cast<uint32_t>(lc * 128 + (((4 * i + g) ^ ((lc >> 1) & 7)) << 4));
+    return gm;
+}
+
+template <int D>
+struct ManyState {
+    RowState row[kQT];
+    f32x4 o[D / 16][kQT];
+};
+
+// S^T of a tile: s[t][qt][r] = key 32 (t >> 1) + 8 g + 4 (t & 1) + r, row 16 qt +
+// lc.  One term: biased (kBias); two: the integer 256 q_h . k + q_l . k.
+template <int D, bool kTerms>
+__device__ __forceinline__ void many_qk(const int8_t *stage, const ManyGeom<D> &gm, const i32x4 (&qh)[kQT][D / 64],
+                                        const i32x4 (&ql)[kQT][D / 64], i32x4 (&s)[4][kQT]) {
+    constexpr int kSl = D / 64;
+    i32x4 kf[4][kSl];
+#pragma unroll
+    for (int i = 0; i < kSl; ++i)
+#pragma unroll
+        for (int t = 0; t < 4; ++t) kf[t][i] = *reinterpret_cast<const i32x4 *>(stage + gm.k_rd[i] + t * 16 * D);
+    constexpr int kFrom = kTerms ? 0 : kBias;
+#pragma unroll
+    for (int t = 0; t < 4; ++t)
+#pragma unroll
+        for (int qt = 0; qt < kQT; ++qt) {
+            i32x4 acc = {kFrom, kFrom, kFrom, kFrom};
+#pragma unroll
+            for (int i = 0; i < kSl; ++i) acc = __builtin_amdgcn_mfma_i32_16x16x64_i8(kf[t][i], qh[qt][i], acc, 0, 0, 0);
+            s[t][qt] = acc;
+        }
+    if constexpr (kTerms) {
+#pragma unroll
+        for (int t = 0; t < 4; ++t)
+#pragma unroll
+            for (int qt = 0; qt < kQT; ++qt) {
+                i32x4 acc = s[t][qt] << 8;
+#pragma unroll
+                for (int i = 0; i < kSl; ++i) acc = __builtin_amdgcn_mfma_i32_16x16x64_i8(kf[t][i], ql[qt][i], acc, 0, 0, 0);
+                s[t][qt] = acc;
+            }
+    }
+}
+
+// Softmax of a tile into the PV operands w[h][qt] (keys 32 h + 8 g ..+7).  f:
+// factors of the rows' integer scores.  kMask: keys of the tile at or past
+// `seen[qt]` (relative to the tile, per row) take no part.
+template <int D, bool kTerms, bool kMask>
+__device__ __forceinline__ void many_softmax(i32x4 (&s)[4][kQT], const float (&f)[kQT], float v_log2, const int (&seen)[kQT],
+                                             int g, ManyState<D> &st, f16x8 (&w)[2][kQT]) {
+    constexpr float kFrom = kTerms ? 0.0f : kBiasF;
+    constexpr int kLeast = static_cast<int>(0x80000000u);
+    float top[kQT];
+    bool need = false;
+#pragma unroll
+    for (int qt = 0; qt < kQT; ++qt) {
+        const int t0 = seen[qt] - 1 - 8 * g;  // key 8 g + c is seen iff c <= t0
+        if constexpr (kMask) {
+#pragma unroll
+            for (int t = 0; t < 4; ++t)
+#pragma unroll
+                for (int r = 0; r < 4; ++r) {
+                    const int hidden = (t0 - (32 * (t >> 1) + 4 * (t & 1) + r)) >> 31;
+                    s[t][qt][r] = (s[t][qt][r] & ~hidden) | (kLeast & hidden);
+                }
+        }
+        int mi = imax3(s[0][qt][0], s[0][qt][1], s[0][qt][2]);
+        mi = imax3(mi, s[0][qt][3], s[1][qt][0]);
+        mi = imax3(mi, s[1][qt][1], s[1][qt][2]);
+        mi = imax3(mi, s[1][qt][3], s[2][qt][0]);
+        mi = imax3(mi, s[2][qt][1], s[2][qt][2]);
+        mi = imax3(mi, s[2][qt][3], s[3][qt][0]);
+        mi = imax3(mi, s[3][qt][1], s[3][qt][2]);
+        mi = max(mi, s[3][qt][3]);
+        top[qt] = (kTerms ? static_cast<float>(mi) : __int_as_float(mi) - kFrom) * f[qt];
+        if (kMask && mi == kLeast) top[qt] = -INFINITY;
+        need = need || (top[qt] - st.row[qt].m) + (v_log2 - st.row[qt].v) > kSlack;
+    }
+    if (__any(need)) {
+#pragma unroll
+        for (int qt = 0; qt < kQT; ++qt) {
+            // a row's base moves by its own scores alone
+            const float row_top = xmax_f32(top[qt]);
+            const bool move = (row_top - st.row[qt].m) + (v_log2 - st.row[qt].v) > kSlack;
+            const float alpha = move ? __builtin_amdgcn_exp2f((st.row[qt].m - row_top) + (st.row[qt].v - v_log2)) : 1.0f;
+            st.row[qt].m = move ? row_top : st.row[qt].m;
+            st.row[qt].v = move ? v_log2 : st.row[qt].v;
+            st.row[qt].l *= alpha;
+#pragma unroll
+            for (int ds = 0; ds < D / 16; ++ds) st.o[ds][qt] *= alpha;
+        }
+    }
+    float d[kQT], c[kQT];
+    bool far = false;
+#pragma unroll
+    for (int qt = 0; qt < kQT; ++qt) {
+        d[qt] = st.row[qt].shift(v_log2);
+        c[qt] = d[qt] - __builtin_fmaf(kFrom, f[qt], st.row[qt].m);
+        far = far || !(fabsf(c[qt]) < 4096.0f);
+    }
+    auto weights = [&](auto far_tag) {
+#pragma unroll
+        for (int qt = 0; qt < kQT; ++qt) {
+            const int t0 = seen[qt] - 1 - 8 * g;
+            float sum = 0.0f;
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+                u32x4 packed;
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    float y[2];
+#pragma unroll
+                    for (int i = 0; i < 2; ++i) {
+                        const int e = 2 * j + i;  // key 32 h + 8 g + e
+                        const int si = s[2 * h + (e >> 2)][qt][e & 3];
+                        const float v = kTerms ? static_cast<float>(si) : __int_as_float(si);
+                        // far from the base's range the product is rounded as the base was
+                        const float x = decltype(far_tag)::value ? ((v - kFrom) * f[qt] - st.row[qt].m) + d[qt]
+                                                                 : __builtin_fmaf(v, f[qt], c[qt]);
+                        y[i] = __builtin_amdgcn_exp2f(x);
+                        if constexpr (kMask) {
+                            const int hidden = (t0 - (32 * h + e)) >> 31;
+                            y[i] = __int_as_float(__float_as_int(y[i]) & ~hidden);
+                        }
+                        sum += y[i];
+                    }
+                    packed[j] = hw_f16x2_bits(y[0], y[1]);
+                }
+                w[h][qt] = __builtin_bit_cast(f16x8, packed);
+            }
+            const float l = __builtin_fmaf(sum, __builtin_amdgcn_exp2f(-(st.row[qt].v + d[qt])), st.row[qt].l);
+            if (!kMask || t0 >= 0) st.row[qt].l = l;  // (a row that sees nothing of the tile has no part in a NaN)
+        }
+    };
+    if (__any(far)) weights(std::true_type{});
+    else weights(std::false_type{});
+}
+
+template <int D>
+__device__ __forceinline__ void many_pv(const int8_t *stage, const ManyGeom<D> &gm, const f16x8 (&w)[2][kQT], ManyState<D> &st) {
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+        f16x8 vf[D / 16];
+#pragma unroll
+        for (int ds = 0; ds < D / 16; ++ds) vf[ds] = *reinterpret_cast<const f16x8 *>(stage + gm.v_rd[h] + ds * 16 * 128);
+#pragma unroll
+        for (int ds = 0; ds < D / 16; ++ds)
+#pragma unroll
+            for (int qt = 0; qt < kQT; ++qt)
+                st.o[ds][qt] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vf[ds], w[h][qt], st.o[ds][qt], 0, 0, 0);
+    }
+}
+
+// A page's keys into a ring stage; its values into registers, and from there into one.
+#define TU_MANY_LOAD_K(D)                                                                                              \
+    __device__ __forceinline__ void many_load_k(int8_t *stage, __amdgpu_buffer_rsrc_t rs, const ManyGeom<D> &gm, int wave) {     \
+        _Pragma("unroll") for (int i = 0; i < Tiles<D>::kKLoads; ++i)                                                  \
+            __builtin_amdgcn_raw_ptr_buffer_load_lds(rs, (lds_void *)(stage + (Tiles<D>::kKLoads * wave + i) * 1024), 16, \
+                                                     gm.k_src[i], 0, 0, 0);                                            \
+    }
+TU_MANY_LOAD_K(128)
+TU_MANY_LOAD_K(64)
+#undef TU_MANY_LOAD_K
+
+template <int D>
+__device__ __forceinline__ void many_store_v(int8_t *stage, const ManyGeom<D> &gm, const u32x4 (&v)[Tiles<D>::kKLoads]) {
+#pragma unroll
+    for (int i = 0; i < Tiles<D>::kKLoads; ++i)
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+            const u32x2 a = codes_to_f16(v[i][2 * e]), b = codes_to_f16(v[i][2 * e + 1]);
+            *reinterpret_cast<u32x4 *>(stage + gm.v_wr[i][e]) = u32x4{a[0], a[1], b[0], b[1]};
+        }
+}
+
+template <int D, bool kTerms>
+__global__ __launch_bounds__(kThreads, 2) void cache_many_kernel(CacheCall c) {
+    constexpr int kSl = D / 64, kDS = D / 16, kLoads = Tiles<D>::kKLoads;
+    __shared__ __align__(1024) int8_t lds[Tiles<D>::kBytes];
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int g = lane >> 4, lc = lane & 15;
+    const Unit u = unit_at<kManyRows>(c, xcd_chunk(blockIdx.x, gridDim.x));
+    if (u.z > 0 && static_cast<int>(u.z) >= u.used) return;  // the whole workgroup: nothing is left for the range
+    PageWindow window;
+    int base = u.first;
+    window.fetch(c, u, base, 1, lane);
+    const ManyGeom<D> gm = many_geom<D>(wave, lane);
+
+    i32x4 qh[kQT][kSl], ql[kQT][kSl];
+    float factor[kQT];
+    int limit[kQT];
+    ManyState<D> st;
+    const uint32_t row0 = u.block * kManyRows + wave * kWaveRows;
+#pragma unroll
+    for (int qt = 0; qt < kQT; ++qt) {
+        const uint32_t r = row0 + 16 * qt + lc;
+        const Row row = row_at(c, u.hk, r);
+        const bool in = r < c.rows && row.token < u.n;
+        factor[qt] = load_row<kSl, kTerms>(c, row, u.b, in, 16 * g, 64, qh[qt], ql[qt]);
+        limit[qt] = keys_of(c, min(row.token, max(u.n - 1, 0)), u.n, u.length);
+#pragma unroll
+        for (int ds = 0; ds < kDS; ++ds) st.o[ds][qt] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+    }
+    // keys that all rows of the wave see: those of its first row
+    const int whole = __builtin_amdgcn_readfirstlane(
+        keys_of(c, min(row_at(c, u.hk, row0).token, max(u.n - 1, 0)), u.n, u.length) / kPage);
+
+    i32x4 s[4][kQT];
+    f16x8 w[2][kQT];
+    u32x4 v[kLoads];
+    auto at_of = [&](int p) { return min(max(p, base), u.end - 1) - base; };
+    auto place = [&](int p) {
+        return static_cast<int64_t>(max(__builtin_amdgcn_readlane(window.page, at_of(p)), 0)) * c.hkv + u.hk;
+    };
+    auto load_k = [&](int p) {
+        many_load_k(lds + (p - u.first) % kKRing * Tiles<D>::kK, make_rsrc(c.k_codes + place(p) * kPage * D, kPage * D), gm, wave);
+    };
+    auto load_v = [&](int p) {
+        const int8_t *page = c.v_codes + place(p) * kPage * D;
+#pragma unroll
+        for (int i = 0; i < kLoads; ++i) v[i] = *reinterpret_cast<const u32x4 *>(page + (i * kThreads + threadIdx.x) * 16);
+    };
+    auto store_v = [&](int p) {
+        if (lane_value(window.v_log2, at_of(p)) == kZeroValues) {
+#pragma unroll
+            for (int i = 0; i < kLoads; ++i) v[i] = u32x4{0, 0, 0, 0};
+        }
+        many_store_v<D>(lds + Tiles<D>::kV0 + (p - u.first) % 2 * Tiles<D>::kV, gm, v);
+    };
+    auto v_stage = [&](int p) { return lds + Tiles<D>::kV0 + (p - u.first) % 2 * Tiles<D>::kV; };
+    auto qk = [&](int p) { many_qk<D, kTerms>(lds + (p - u.first) % kKRing * Tiles<D>::kK, gm, qh, ql, s); };
+    auto softmax = [&](int p) {
+        const int at = at_of(p);
+        const float k_scale = lane_value(window.k_scale, at), v_log2 = lane_value(window.v_log2, at);
+        const bool there = __builtin_amdgcn_readlane(window.page, at) >= 0;
+        float f[kQT];
+        int seen[kQT];
+#pragma unroll
+        for (int qt = 0; qt < kQT; ++qt) {
+            f[qt] = factor[qt] * k_scale;
+            seen[qt] = there ? limit[qt] - p * kPage : 0;
+        }
+        if (there && p < whole) many_softmax<D, kTerms, false>(s, f, v_log2, seen, g, st, w);
+        else many_softmax<D, kTerms, true>(s, f, v_log2, seen, g, st, w);
+    };
+
+    if (u.first < u.end) {
+        load_v(u.first);
+        load_k(u.first);
+        load_k(u.first + 1);
+        store_v(u.first);
+        load_v(u.first + 1);
+        __builtin_amdgcn_s_waitcnt(vmcnt_imm(0));
+        __syncthreads();
+        qk(u.first);
+        softmax(u.first);
+        // Step p: QK of page p + 1 and PV of page p, then the softmax of page p + 1.
+        // Keys of p + 2 go into the stage that step p - 1 read last, values of p + 1
+        // into the one whose page PV finished a step ago.
+#pragma clang loop unroll(disable)
+        for (int p = u.first; p < u.end; ++p) {
+            if (p + 3 - base >= 64 && base + 64 < u.end) {
+                base = p;
+                window.fetch(c, u, base, 1, lane);
+            }
+            const bool more = p + 1 < u.end;
+            if (p + 2 < u.end) load_k(p + 2);
+            if (more) {
+                store_v(p + 1);
+                qk(p + 1);
+            }
+            if (p + 2 < u.end) load_v(p + 2);
+            many_pv<D>(v_stage(p), gm, w, st);
+            if (more) softmax(p + 1);
+            __builtin_amdgcn_s_waitcnt(vmcnt_imm(0));
+            __syncthreads();
+        }
+    }
+#pragma unroll
+    for (int qt = 0; qt < kQT; ++qt) {
+        f32x4 o[kDS];
+#pragma unroll
+        for (int ds = 0; ds < kDS; ++ds) o[ds] = st.o[ds][qt];
+        store_row<D>(c, u, o, st.row[qt].m, st.row[qt].v, xsum_f32(st.row[qt].l), row0 + 16 * qt + lc, g);
+    }
+}
+
+// ---------------------------------------------------------------------------
+// The merge
+// ---------------------------------------------------------------------------
+// A row's ranges: D / 8 threads a row, 8 channels each.  A range that saw none of
+// the row's keys has a sum of 0 and is left out; a NaN stays.
+template <int D, int kRows>
+__global__ __launch_bounds__(kThreads) void cache_merge_kernel(CacheCall c) {
+    constexpr int kTpr = D / 8;
+    const int64_t rows = static_cast<int64_t>(c.batch) * c.hkv * c.rows;
+    const int64_t at = static_cast<int64_t>(blockIdx.x) * (kThreads / kTpr) + threadIdx.x / kTpr;
+    if (at >= rows) return;
+    const uint32_t bh = static_cast<uint32_t>(at / c.rows), r = static_cast<uint32_t>(at % c.rows);
+    const Unit u = unit_of<kRows>(c, bh / c.hkv, bh % c.hkv, r / kRows, 0);
+    if (u.used <= 1) return;
+    const Row row = row_at(c, u.hk, r);
+    const int d0 = (threadIdx.x % kTpr) * 8;
+    float m = kNoBase, v = 0.0f, l = 0.0f, acc[8] = {};
+    constexpr int kAhead = 4;  // ranges whose loads are in flight together
+    for (int z0 = 0; z0 < u.used; z0 += kAhead) {
+        f32x4 x[kAhead], a[kAhead], b[kAhead];
+#pragma unroll
+        for (int i = 0; i < kAhead; ++i) {
+            const int64_t from = min(z0 + i, u.used - 1) * rows + at;
+            x[i] = *reinterpret_cast<const f32x4 *>(c.part_m + from * 4);
+            a[i] = *reinterpret_cast<const f32x4 *>(c.part_o + from * D + d0);
+            b[i] = *reinterpret_cast<const f32x4 *>(c.part_o + from * D + d0 + 4);
+        }
+        float m_new = m, v_new = v;
+#pragma unroll
+        for (int i = 0; i < kAhead; ++i)
+            if (x[i][2] != 0.0f && higher(x[i][0], x[i][1], m_new, v_new)) m_new = x[i][0], v_new = x[i][1];
+        const float old = l == 0.0f ? 0.0f : __builtin_amdgcn_exp2f((m - m_new) + (v - v_new));
+        m = m_new, v = v_new;
+        l *= old;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) acc[e] = old == 0.0f ? 0.0f : acc[e] * old;
+#pragma unroll
+        for (int i = 0; i < kAhead; ++i) {
+            if (z0 + i >= u.used || x[i][2] == 0.0f) continue;
+            const float wi = __builtin_amdgcn_exp2f((x[i][0] - m) + (x[i][1] - v));
+            l = __builtin_fmaf(wi, x[i][2], l);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                acc[e] = __builtin_fmaf(wi, a[i][e], acc[e]);
+                acc[4 + e] = __builtin_fmaf(wi, b[i][e], acc[4 + e]);
+            }
+        }
+    }
+    const bool some = l != 0.0f && row.token < u.n;
+    const float inv = 1.0f / l;
+    u32x4 out;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+        const float p = acc[2 * e] * inv, q = acc[2 * e + 1] * inv;
+        out[e] = some ? (c.out_fp16 ? hw_f16x2_bits(p, q) : hw_bf16x2_bits(p, q)) : 0;
+    }
+    auto *dst = reinterpret_cast<u32x2 *>(c.o + u.b * c.o_sb + row.head * c.o_sh + row.token * c.o_sl + d0);
+    dst[0] = u32x2{out[0], out[1]};
+    dst[1] = u32x2{out[2], out[3]};
+}
+
+// ---------------------------------------------------------------------------
+// The plan
+// ---------------------------------------------------------------------------
+struct CachePlan {
+    int32_t rows;  // of a row block: 16, 32 or 128
+    uint32_t row_blocks, parts;
+};
+
+CachePlan cache_plan(int64_t batch, int64_t hkv, int64_t rows, int64_t dim, int64_t max_pages, int64_t cus, int64_t max_bytes) {
+    CachePlan p{};
+    p.rows = rows <= 16 ? 16 : rows <= 32 ? 32 : kManyRows;
+    p.row_blocks = static_cast<uint32_t>((rows + p.rows - 1) / p.rows);
+    p.parts = 1;
+    const int64_t units = batch * hkv * p.row_blocks, slots = 2 * cus;
+    const int64_t least = p.rows == kManyRows ? 8 : 4;  // pages of a range
+    int64_t parts = std::min<int64_t>((slots + units - 1) / units, (max_pages + least - 1) / least);
+    const int64_t row_bytes = batch * hkv * rows * (dim + 4) * static_cast<int64_t>(sizeof(float));
+    parts = std::min<int64_t>(parts, max_bytes / row_bytes);
+    if (parts > 1) p.parts = static_cast<uint32_t>(parts);
+    return p;
+}
+
+int64_t cache_workspace(const CachePlan &p, int64_t batch, int64_t hkv, int64_t rows, int64_t dim) {
+    return p.parts > 1 ? p.parts * batch * hkv * rows * (dim + 4) * static_cast<int64_t>(sizeof(float)) : 0;
+}
+
+}  // namespace
+}  // namespace tu
+
+extern "C" int64_t tu_kv_cache_attn_workspace(int64_t batch, int64_t hq, int64_t hkv, int64_t lq, int64_t dim, int64_t max_length,
+                                              int32_t cus) {
+    using namespace tu;
+    if (batch <= 0 || hkv <= 0 || hq < hkv || lq <= 0 || dim <= 0 || max_length <= 0 || cus <= 0) return 0;
+    const int64_t rows = lq * (hq / hkv), pages = (max_length + kPage - 1) / kPage;
+    return cache_workspace(cache_plan(batch, hkv, rows, dim, pages, cus, INT64_MAX), batch, hkv, rows, dim);
+}
+
+extern "C" int32_t tu_kv_cache_attn(const void *q, const float *q_scale, int32_t q_type, int64_t blkq, const int8_t *k_codes,
+                                    const int8_t *v_codes, const float *k_scale, const float *v_scale, int64_t pages,
+                                    const int32_t *block_table, int64_t width, const int32_t *lengths,
+                                    const int32_t *q_lengths, void *o, int64_t batch, int64_t hq, int64_t hkv, int64_t lq,
+                                    int64_t dim, int64_t q_sb, int64_t q_sh, int64_t q_sl, int64_t o_sb, int64_t o_sh,
+                                    int64_t o_sl, float sm_scale, int32_t causal, int64_t max_length, int32_t cus,
+                                    void *workspace, int64_t workspace_bytes, void *stream) {
+    using namespace tu;
+    TU_REQUIRE(dim == 64 || dim == 128, "cache attention requires head_dim 64 or 128, got %lld", static_cast<long long>(dim));
+    TU_REQUIRE(q_type >= 0 && q_type <= kQInt8, "cache attention query type must be 0 (bf16), 1 (fp16) or 2 (int8), got %d", q_type);
+    TU_REQUIRE(batch > 0 && hq > 0 && hkv > 0 && hq % hkv == 0, "cache attention: hq must be a positive multiple of hkv");
+    TU_REQUIRE(lq > 0 && batch <= 65535 && hq <= 65535 && lq * (hq / hkv) <= 0x7fffff00 && cus > 0 && max_length > 0,
+               "cache attention sizes out of range");
+    TU_REQUIRE(width > 0 && width <= 0x7fffffff / kPage - 1 && pages > 0 && pages <= 0x7fffffff,
+               "cache attention block table or page count out of range");
+    TU_REQUIRE(q && k_codes && v_codes && k_scale && v_scale && block_table && lengths && o && (q_scale || q_type != kQInt8),
+               "cache attention pointers must be non-null");
+    TU_REQUIRE(q_type != kQInt8 || (blkq > 0 && blkq <= 0x7fffffff), "cache attention needs blkq > 0");
+    TU_REQUIRE(sm_scale > 0.0f, "cache attention sm_scale must be positive");
+    const int64_t piece = q_type == kQInt8 ? 16 : 8;
+    TU_REQUIRE(q_sb % piece == 0 && q_sh % piece == 0 && q_sl % piece == 0 && (reinterpret_cast<uintptr_t>(q) & 15) == 0,
+               "cache attention query rows must be 16-byte aligned");
+    TU_REQUIRE((reinterpret_cast<uintptr_t>(k_codes) & 15) == 0 && (reinterpret_cast<uintptr_t>(v_codes) & 15) == 0 &&
+                   o_sb % 4 == 0 && o_sh % 4 == 0 && o_sl % 4 == 0 && (reinterpret_cast<uintptr_t>(o) & 7) == 0,
+               "cache attention codes and output must be aligned");
+    TU_REQUIRE((reinterpret_cast<uintptr_t>(workspace) & 15) == 0, "cache attention workspace must be 16-byte aligned");
+    const int64_t rows = lq * (hq / hkv);
+    const CachePlan plan = cache_plan(batch, hkv, rows, dim, std::min<int64_t>((max_length + kPage - 1) / kPage, width), cus,
+                                      workspace ? workspace_bytes : 0);
+    const int64_t units = batch * hkv * plan.row_blocks * plan.parts;
+    constexpr int64_t kMost = 0x7fffffff;
+    TU_REQUIRE(units <= kMost && batch * hkv * rows <= kMost * 16, "cache attention grid too large");
+    if (require_gfx950()) return -1;
+    CacheCall c{};
+    c.q = q, c.q_scale = q_scale, c.q_type = static_cast<uint32_t>(q_type);
+    c.blkq = q_type == kQInt8 ? static_cast<uint32_t>(blkq) : 1;
+    c.nbq = q_type == kQInt8 ? static_cast<uint32_t>((lq + blkq - 1) / blkq) : 0;
+    c.k_codes = k_codes, c.v_codes = v_codes, c.k_scale = k_scale, c.v_scale = v_scale;
+    c.table = block_table, c.lengths = lengths, c.q_lengths = q_lengths;
+    c.width = static_cast<int32_t>(width), c.pages = static_cast<int32_t>(pages);
+    c.batch = static_cast<uint32_t>(batch), c.hkv = static_cast<uint32_t>(hkv), c.group = static_cast<uint32_t>(hq / hkv);
+    c.lq = static_cast<uint32_t>(lq), c.rows = static_cast<uint32_t>(rows);
+    c.row_blocks = plan.row_blocks, c.parts = plan.parts;
+    c.causal = causal != 0, c.out_fp16 = q_type == 1;
+    c.sm_log2 = sm_scale * kLog2e;
+    c.o = static_cast<uint16_t *>(o);
+    c.q_sb = q_sb, c.q_sh = q_sh, c.q_sl = q_sl, c.o_sb = o_sb, c.o_sh = o_sh, c.o_sl = o_sl;
+    c.part_o = static_cast<float *>(workspace);
+    c.part_m = c.part_o + plan.parts * batch * hkv * rows * dim;
+    hipStream_t s = static_cast<hipStream_t>(stream);
+    const dim3 grid(static_cast<unsigned>(units));
+#define TU_CACHE_ATTN(D)                                                                                               \
+    do {                                                                                                               \
+        if (plan.rows == 16) cache_few_kernel<D, 1><<<grid, kThreads, 0, s>>>(c);                                      \
+        else if (plan.rows == 32) cache_few_kernel<D, 2><<<grid, kThreads, 0, s>>>(c);                                 \
+        else if (q_type == kQInt8) cache_many_kernel<D, false><<<grid, kThreads, 0, s>>>(c);                           \
+        else cache_many_kernel<D, true><<<grid, kThreads, 0, s>>>(c);                                                  \
+        if (plan.parts > 1) {                                                                                          \
+            constexpr int64_t kRowsPerWg = kThreads / (D / 8);                                                         \
+            const dim3 merge(static_cast<unsigned>((batch * hkv * rows + kRowsPerWg - 1) / kRowsPerWg));               \
+            if (plan.rows == 16) cache_merge_kernel<D, 16><<<merge, kThreads, 0, s>>>(c);                              \
+            else if (plan.rows == 32) cache_merge_kernel<D, 32><<<merge, kThreads, 0, s>>>(c);                         \
+            else cache_merge_kernel<D, kManyRows><<<merge, kThreads, 0, s>>>(c);                                       \
+        }                                                                                                              \
+    } while (0)
+    if (dim == 128) TU_CACHE_ATTN(128);
+    else TU_CACHE_ATTN(64);
+#undef TU_CACHE_ATTN
+    return check_launch("tu_kv_cache_attn");
+}

@@ -15,6 +15,7 @@
 // launches are those of the general route, so results have the same bits.
 #include <torch/csrc/Exceptions.h>
 #include <torch/csrc/autograd/python_variable.h>
+#include <torch/csrc/utils/object_ptr.h>
 
 #include <ATen/ATen.h>
 #include <ATen/PythonTorchFunctionTLS.h>
@@ -467,10 +468,182 @@ PyObject *int8_linear_adapters(PyObject *, PyObject *const *args, Py_ssize_t nar
     END_HANDLE_TH_ERRORS
 }
 
+// The pool, block table and lengths of a key/value cache call: args[0 .. 5].
+struct Cache {
+    const Tensor *kc, *vc, *ks, *vs, *table, *length;
+    int64_t pages, heads, width, batch, row;
+    c10::Device device = c10::kCPU;
+};
+
+bool unpack_cache(PyObject *const *args, Cache &a) {
+    if (!THPVariable_CheckTypeExact(Py_TYPE(args[0]))) return false;
+    a.device = THPVariable_Unpack(args[0]).device();
+    if (!a.device.is_cuda() || !plain_context(a.device.index()) || !plain(args[0], &a.kc, a.device) ||
+        !plain(args[1], &a.vc, a.device) || !plain(args[2], &a.ks, a.device) || !plain(args[3], &a.vs, a.device) ||
+        !plain(args[4], &a.table, a.device) || !plain(args[5], &a.length, a.device))
+        return false;
+    const Tensor &kc = *a.kc, &vc = *a.vc, &ks = *a.ks, &vs = *a.vs, &table = *a.table, &length = *a.length;
+    if (kc.scalar_type() != at::kChar || vc.scalar_type() != at::kChar || ks.scalar_type() != at::kFloat ||
+        vs.scalar_type() != at::kFloat || table.scalar_type() != at::kInt || length.scalar_type() != at::kInt ||
+        kc.dim() != 4 || vc.dim() != 4 || ks.dim() != 2 || table.dim() != 2 || length.dim() != 1)
+        return false;
+    a.pages = kc.size(0), a.heads = kc.size(1), a.width = kc.size(3);
+    a.batch = table.size(0), a.row = table.size(1);
+    for (const Tensor *t : {a.kc, a.vc, a.ks, a.vs, a.table, a.length})
+        if (!t->is_contiguous()) return false;
+    return a.pages > 0 && a.heads > 0 && kc.size(2) == 64 && (a.width == 64 || a.width == 128) &&
+           vc.sizes() == at::IntArrayRef({a.pages, a.heads, a.width, 64}) && ks.sizes() == at::IntArrayRef({a.pages, a.heads}) &&
+           vs.sizes() == ks.sizes() && a.batch > 0 && a.row > 0 && length.size(0) == a.batch && aligned(kc, 16) &&
+           aligned(vc, 16);
+}
+
+// Token rows [batch, heads, tokens, width] (or NHD) as the cache's kernels read them.
+struct Tokens {
+    const Tensor *t;
+    int64_t heads, count, sb, sh, sl;
+};
+
+bool unpack_tokens(PyObject *obj, const Cache &c, bool nhd, Tokens &a) {
+    if (!plain(obj, &a.t, c.device) || a.t->dim() != 4) return false;
+    const Tensor &t = *a.t;
+    const int64_t piece = 16 / static_cast<int64_t>(t.element_size());
+    const int head = nhd ? 2 : 1, seq = nhd ? 1 : 2;
+    a.heads = t.size(head), a.count = t.size(seq);
+    a.sb = t.stride(0), a.sh = t.stride(head), a.sl = t.stride(seq);
+    return t.size(0) == c.batch && t.size(3) == c.width && a.heads > 0 && a.count > 0 && t.stride(3) == 1 &&
+           a.sb % piece == 0 && a.sh % piece == 0 && a.sl % piece == 0 && aligned(t, 16);
+}
+
+bool key_mean(PyObject *obj, const Cache &c, const Tensor **out) {
+    return optional(obj, out, c.device, at::kBFloat16) &&
+           (!*out || (*out)->sizes() == at::IntArrayRef({c.batch, c.heads, c.width}));
+}
+
+bool is_float16(const Tensor &t) { return t.scalar_type() == at::kHalf; }
+bool is_float(const Tensor &t) { return t.scalar_type() == at::kBFloat16 || is_float16(t); }
+
+// kv_cache_append(key, value, key_codes, value_codes, key_scale, value_scale, block_table, lengths, nhd, new_lengths,
+//                 key_in_scale, key_mean, stream)
+PyObject *kv_cache_append(PyObject *, PyObject *const *args, Py_ssize_t nargs) {
+    HANDLE_TH_ERRORS
+    int64_t nhd, stream;
+    Cache c;
+    Tokens k, v;
+    const int32_t *fresh;
+    const Tensor *scale, *mean;
+    if (nargs != 13 || !integer(args[8], &nhd) || !integer(args[12], &stream) || !unpack_cache(args + 2, c) ||
+        !unpack_tokens(args[0], c, nhd != 0, k) || !unpack_tokens(args[1], c, nhd != 0, v) ||
+        !lengths(args[9], &fresh, c.device, c.batch) || !optional(args[10], &scale, c.device, at::kFloat) ||
+        !key_mean(args[11], c, &mean))
+        Py_RETURN_NONE;
+    if (k.t->sizes() != v.t->sizes() || k.heads != c.heads || !is_float(*v.t) ||
+        k.t->scalar_type() != (scale ? at::kChar : v.t->scalar_type()) ||
+        (scale && scale->sizes() != at::IntArrayRef({c.batch, c.heads, ceil_div(k.count, 64)})))
+        Py_RETURN_NONE;
+    Tensor after;
+    {
+        ReleaseGil nogil;
+        after = empty({c.batch}, at::kInt, c.device);
+        if (tu_kv_cache_append(k.t->data_ptr(), scale ? scale->data_ptr<float>() : nullptr, v.t->data_ptr(),
+                               is_float16(*v.t), c.batch, c.heads, k.count, c.width, k.sb, k.sh, k.sl, v.sb, v.sh, v.sl,
+                               mean ? mean->data_ptr() : nullptr, c.table->data_ptr<int32_t>(), c.row,
+                               c.length->data_ptr<int32_t>(), fresh, c.kc->data_ptr<int8_t>(), c.vc->data_ptr<int8_t>(),
+                               c.ks->data_ptr<float>(), c.vs->data_ptr<float>(), c.pages, after.data_ptr<int32_t>(),
+                               reinterpret_cast<void *>(stream)))
+            failed("tu_kv_cache_append");
+    }
+    for (const Tensor *t : {c.kc, c.vc, c.ks, c.vs})
+        if (!t->is_inference()) t->unsafeGetTensorImpl()->bump_version();  // written in place
+    return THPVariable_Wrap(std::move(after));
+    END_HANDLE_TH_ERRORS
+}
+
+// kv_cache_read(key_codes, value_codes, key_scale, value_scale, block_table, lengths, max_length, nhd, float16, starts,
+//               key_mean, stream)
+PyObject *kv_cache_read(PyObject *, PyObject *const *args, Py_ssize_t nargs) {
+    HANDLE_TH_ERRORS
+    int64_t length, nhd, half, stream;
+    Cache c;
+    const int32_t *starts;
+    const Tensor *mean;
+    if (nargs != 12 || !integer(args[6], &length) || !integer(args[7], &nhd) || !integer(args[8], &half) ||
+        !integer(args[11], &stream) || !unpack_cache(args, c) || length < 1 || length > 0x7fffff00 ||
+        !lengths(args[9], &starts, c.device, c.batch) || !key_mean(args[10], c, &mean))
+        Py_RETURN_NONE;
+    Tensor k, v;
+    {
+        ReleaseGil nogil;
+        const int head = nhd ? 2 : 1, seq = nhd ? 1 : 2;
+        for (Tensor *t : {&k, &v})
+            *t = nhd ? empty({c.batch, length, c.heads, c.width}, half ? at::kHalf : at::kBFloat16, c.device)
+                     : empty({c.batch, c.heads, length, c.width}, half ? at::kHalf : at::kBFloat16, c.device);
+        if (tu_kv_cache_read(c.kc->data_ptr<int8_t>(), c.vc->data_ptr<int8_t>(), c.ks->data_ptr<float>(),
+                             c.vs->data_ptr<float>(), c.pages, c.table->data_ptr<int32_t>(), c.row,
+                             c.length->data_ptr<int32_t>(), starts, mean ? mean->data_ptr() : nullptr, k.data_ptr(),
+                             v.data_ptr(), half != 0, c.batch, c.heads, length, c.width, k.stride(0), k.stride(head),
+                             k.stride(seq), v.stride(0), v.stride(head), v.stride(seq), reinterpret_cast<void *>(stream)))
+            failed("tu_kv_cache_read");
+    }
+    THPObjectPtr out(PyTuple_New(2));
+    if (!out) throw python_error();
+    PyTuple_SET_ITEM(out.get(), 0, THPVariable_Wrap(std::move(k)));
+    PyTuple_SET_ITEM(out.get(), 1, THPVariable_Wrap(std::move(v)));
+    return out.release();
+    END_HANDLE_TH_ERRORS
+}
+
+// kv_cache_attention(query, key_codes, value_codes, key_scale, value_scale, block_table, lengths, nhd, causal, scale,
+//                    max_length, query_scale, blkq, query_lengths, cus, stream)
+PyObject *kv_cache_attention(PyObject *, PyObject *const *args, Py_ssize_t nargs) {
+    HANDLE_TH_ERRORS
+    int64_t nhd, causal, most, blkq, cus, stream;
+    Cache c;
+    Tokens q;
+    const int32_t *q_lengths;
+    const Tensor *q_scale;
+    if (nargs != 16 || !integer(args[7], &nhd) || !integer(args[8], &causal) || !PyFloat_Check(args[9]) ||
+        !integer(args[10], &most) || !integer(args[12], &blkq) || !integer(args[14], &cus) || !integer(args[15], &stream) ||
+        !unpack_cache(args + 1, c) || !unpack_tokens(args[0], c, nhd != 0, q) ||
+        !optional(args[11], &q_scale, c.device, at::kFloat) || !lengths(args[13], &q_lengths, c.device, c.batch))
+        Py_RETURN_NONE;
+    const double given = PyFloat_AS_DOUBLE(args[9]);
+    const float scale = given > 0.0 ? static_cast<float>(given) : static_cast<float>(1.0 / std::sqrt(static_cast<double>(c.width)));
+    if (!(scale > 0.0f && std::isfinite(scale)) || most < 1 || q.heads % c.heads ||
+        (q_scale ? q.t->scalar_type() != at::kChar || blkq < 1 ||
+                       q_scale->sizes() != at::IntArrayRef({c.batch, q.heads, ceil_div(q.count, blkq)})
+                 : !is_float(*q.t)))
+        Py_RETURN_NONE;
+    Tensor out;
+    {
+        ReleaseGil nogil;
+        const at::ScalarType type = q_scale ? at::kBFloat16 : q.t->scalar_type();
+        out = nhd ? empty({c.batch, q.count, q.heads, c.width}, type, c.device)
+                  : empty({c.batch, q.heads, q.count, c.width}, type, c.device);
+        most = most < c.row * 64 ? most : c.row * 64;
+        const int64_t bytes = tu_kv_cache_attn_workspace(c.batch, q.heads, c.heads, q.count, c.width, most,
+                                                         static_cast<int32_t>(cus));
+        Tensor work;
+        if (bytes > 0) work = empty({bytes}, at::kByte, c.device);
+        const int head = nhd ? 2 : 1, seq = nhd ? 1 : 2;
+        if (tu_kv_cache_attn(q.t->data_ptr(), q_scale ? q_scale->data_ptr<float>() : nullptr,
+                             q_scale ? 2 : is_float16(*q.t), blkq, c.kc->data_ptr<int8_t>(), c.vc->data_ptr<int8_t>(),
+                             c.ks->data_ptr<float>(), c.vs->data_ptr<float>(), c.pages, c.table->data_ptr<int32_t>(),
+                             c.row, c.length->data_ptr<int32_t>(), q_lengths, out.data_ptr(), c.batch, q.heads, c.heads,
+                             q.count, c.width, q.sb, q.sh, q.sl, out.stride(0), out.stride(head), out.stride(seq), scale,
+                             causal != 0, most, static_cast<int32_t>(cus), ptr(work), bytes,
+                             reinterpret_cast<void *>(stream)))
+            failed("tu_kv_cache_attn");
+    }
+    return THPVariable_Wrap(std::move(out));
+    END_HANDLE_TH_ERRORS
+}
+
 #define TU_METHOD(NAME) \
     {#NAME, reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(NAME)), METH_FASTCALL, nullptr}
 PyMethodDef methods[] = {TU_METHOD(int8_linear), TU_METHOD(sageattn), TU_METHOD(w8a8attn), TU_METHOD(select_key_blocks),
-                         TU_METHOD(key_block_attention), TU_METHOD(int8_linear_adapters), {nullptr, nullptr, 0, nullptr}};
+                         TU_METHOD(key_block_attention), TU_METHOD(int8_linear_adapters),
+                         TU_METHOD(kv_cache_append), TU_METHOD(kv_cache_read), TU_METHOD(kv_cache_attention),
+                         {nullptr, nullptr, 0, nullptr}};
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "_host_calls", nullptr, -1, methods, nullptr, nullptr, nullptr, nullptr};
 
 }  // namespace

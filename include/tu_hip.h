@@ -561,6 +561,74 @@ int32_t tu_layer_norm_affine_convrot_quant_i8(const void *x, const void *weight,
                                               float *row_scale, int64_t rows, int64_t hidden, float eps,
                                               void *stream);
 
+/* Key/value cache in 8 bits ------------------------------------------------ */
+
+/* A pool of `pages` pages of 64 tokens.  k_codes: int8 [pages, hkv, 64, dim];
+ * v_codes: int8 [pages, hkv, dim, 64]; k_scale, v_scale: fp32 [pages, hkv], not
+ * negative; codes 16-byte aligned, dim 64 or 128.  block_table: int32 [batch,
+ * width], the pages of each sequence in order (token t lies in page t / 64);
+ * lengths: int32 [batch], the tokens of each, taken within [0, 64 width].  An
+ * entry outside [0, pages) names no page: tokens written there are dropped,
+ * those read are zeros, and attention does not see them.  No counterpart in the
+ * reference. */
+
+/* Quantizes tokens behind each sequence's end: new_lengths[b] (int32 [batch],
+ * NULL: len) tokens of k and v, as many as its pages have room for.  Per page and
+ * head, K and V apart, in fp32:
+ *   s    = max(s of the tokens in the page before, max |new x| / 127, 1e-7 / 127)
+ *   code = rint(x * (1 / s)), within +-127
+ * and where s grows, the page's earlier codes become rint((code * s_before) *
+ * (1 / s)).  Codes behind the new end keep their bytes.  A NaN or infinite x
+ * makes the scale of its page and head one, with codes 0.
+ * k, v: bf16 (dtype 0) or fp16 (1) by element strides, 16-byte aligned rows; or,
+ * with k_in_scale (fp32 [batch, hkv, ceil(len / 64)]), k is int8 codes whose
+ * token t is code * k_in_scale[t / 64].  k_mean_bf16 (bf16 [batch, hkv, dim], or
+ * NULL) is subtracted from k first, in fp32.  lengths_out: int32 [batch], the
+ * lengths afterwards, not `lengths` itself.  A page named twice among the pages
+ * that are written holds what one of the writers left of each byte. */
+int32_t tu_kv_cache_append(const void *k, const float *k_in_scale, const void *v, int32_t dtype, int64_t batch,
+                           int64_t hkv, int64_t len, int64_t dim, int64_t k_sb, int64_t k_sh, int64_t k_sl,
+                           int64_t v_sb, int64_t v_sh, int64_t v_sl, const void *k_mean_bf16,
+                           const int32_t *block_table, int64_t width, const int32_t *lengths,
+                           const int32_t *new_lengths, int8_t *k_codes, int8_t *v_codes, float *k_scale,
+                           float *v_scale, int64_t pages, int32_t *lengths_out, void *stream);
+
+/* Tokens starts[b] (int32 [batch], NULL: 0) .. + len - 1 of each sequence as
+ * bf16 (dtype 0) or fp16 (1): T(code * s), K plus k_mean_bf16 in fp32 before the
+ * one rounding; zeros at and past the sequence's end.  k, v: outputs by element
+ * strides, 16-byte aligned rows. */
+int32_t tu_kv_cache_read(const int8_t *k_codes, const int8_t *v_codes, const float *k_scale, const float *v_scale,
+                         int64_t pages, const int32_t *block_table, int64_t width, const int32_t *lengths,
+                         const int32_t *starts, const void *k_mean_bf16, void *k, void *v, int32_t dtype,
+                         int64_t batch, int64_t hkv, int64_t len, int64_t dim, int64_t k_sb, int64_t k_sh,
+                         int64_t k_sl, int64_t v_sb, int64_t v_sh, int64_t v_sl, void *stream);
+
+/* Attention of lq query tokens a sequence over its cached keys and values:
+ *   s = (q . k_code) * sm_scale * k_scale, p = softmax over the keys seen,
+ *   out = sum p * v_code * v_scale
+ * A query sees every key of its sequence, or, causal, those up to its own place:
+ * the n = q_lengths[b] (int32 [batch], NULL: lq) queries are the sequence's last
+ * tokens, and token i sees keys j <= lengths[b] - n + i.  Rows that see no key,
+ * and rows at or past q_lengths[b], are zeros.
+ * q: bf16 (q_type 0), fp16 (1) or int8 codes (2) with q_scale fp32 [batch, hq,
+ * ceil(lq / blkq)], by element strides, 16-byte aligned rows; bf16 and fp16 rows
+ * are taken as integers of 16 bits with a scale a row.  o: bf16, fp16 where q is,
+ * by strides.  A scale that is NaN or infinite makes NaN of the rows that see its
+ * page (or have it) and of no others.  max_length: a bound of the lengths that
+ * the split into ranges is made for; longer sequences are right as well.
+ * workspace: 16-byte aligned, tu_kv_cache_attn_workspace(...) bytes for every
+ * range on a device of `cus` compute units (0: no split); with less of it fewer
+ * ranges, with none (NULL, 0) one. */
+int64_t tu_kv_cache_attn_workspace(int64_t batch, int64_t hq, int64_t hkv, int64_t lq, int64_t dim,
+                                   int64_t max_length, int32_t cus);
+int32_t tu_kv_cache_attn(const void *q, const float *q_scale, int32_t q_type, int64_t blkq, const int8_t *k_codes,
+                         const int8_t *v_codes, const float *k_scale, const float *v_scale, int64_t pages,
+                         const int32_t *block_table, int64_t width, const int32_t *lengths,
+                         const int32_t *q_lengths, void *o, int64_t batch, int64_t hq, int64_t hkv, int64_t lq,
+                         int64_t dim, int64_t q_sb, int64_t q_sh, int64_t q_sl, int64_t o_sb, int64_t o_sh,
+                         int64_t o_sl, float sm_scale, int32_t causal, int64_t max_length, int32_t cus,
+                         void *workspace, int64_t workspace_bytes, void *stream);
+
 #ifdef __cplusplus
 }
 #endif
