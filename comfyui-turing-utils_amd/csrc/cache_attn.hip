@@ -35,9 +35,10 @@ typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
 constexpr int kPage = 64;
 constexpr int kThreads = 256;
 constexpr float kNoBase = -3.402823466e38f;  // score of a row's base before its first key
-constexpr float kSlack = 8.0f;               // log2 of the largest w allowed
+constexpr float kUp = 7.0f;                  // log2 of w at the base: fp16's room is used from 2^15 down to 2^-24
+constexpr float kSlack = 8.0f;               // log2 of w above the base that moves it
 constexpr float kLeastScale = -64.0f;        // least log2 of a page's V scale, less the base's
-constexpr float kZeroValues = -100.0f;       // log2 V scale of a page whose values count as zeros
+constexpr float kZeroValues = -90.0f;        // log2 V scale of a page whose values count as zeros
 constexpr int kQInt8 = 2;                    // query types: 0 bf16, 1 fp16
 
 struct CacheCall {
@@ -189,10 +190,10 @@ struct PageWindow {
         page = p >= 0 && p < c.pages ? p : -1;
         const int64_t s = static_cast<int64_t>(max(page, 0)) * c.hkv + u.hk;
         k_scale = c.k_scale[s];
-        // (a NaN stays; below 2^-100, where a sum of weights over the scale might be
+        // (a NaN stays; below 2^-90, where a sum of weights over the scale might be
         // no number, the values count as zeros of that scale)
         const float v = c.v_scale[s];
-        v_log2 = v <= 7.888609052e-31f ? kZeroValues : __builtin_amdgcn_logf(v);
+        v_log2 = v <= 8.077935669e-28f ? kZeroValues : __builtin_amdgcn_logf(v);
     }
 };
 
@@ -280,7 +281,7 @@ struct PageRegs {
 };
 
 template <int D, int kRT>
-__global__ __launch_bounds__(kThreads, 2) void cache_few_kernel(CacheCall c) {
+__global__ __launch_bounds__(kThreads, D == 128 && kRT == 2 ? 1 : 2) void cache_few_kernel(CacheCall c) {
     constexpr int kSl = D / 64, kDS = D / 16, kRows = 16 * kRT;
     __shared__ __align__(16) float merge_o[3][kRT][kDS][64][4];
     __shared__ float merge_m[4][kRT][64][3];
@@ -360,7 +361,7 @@ __global__ __launch_bounds__(kThreads, 2) void cache_few_kernel(CacheCall c) {
 #pragma unroll
                     for (int i = 0; i < 2; ++i) {
                         const int e = 8 * h + 2 * j + i;
-                        y[i] = e < seen ? __builtin_amdgcn_exp2f((x[e] - st[rt].m) + d) : 0.0f;
+                        y[i] = e < seen ? __builtin_amdgcn_exp2f((x[e] - st[rt].m) + (d + kUp)) : 0.0f;
                         sum += y[i];
                     }
                     packed[j] = hw_f16x2_bits(y[0], y[1]);
@@ -513,29 +514,30 @@ __device__ __forceinline__ ManyGeom<D> many_geom(int wave, int lane) {
 template <int D>
 struct ManyState {
     RowState row[kQT];
+    float inverse[kQT];  // 1 / V scale of the page whose weights w holds
     f32x4 o[D / 16][kQT];
 };
 
-// S^T of a tile: s[t][qt][r] = key 32 (t >> 1) + 8 g + 4 (t & 1) + r, row 16 qt +
-// lc.  One term: biased (kBias); two: the integer 256 q_h . k + q_l . k.
+// S^T of a tile from its K fragments: s[t][qt][r] = key 32 (t >> 1) + 8 g + 4 (t &
+// 1) + r, row 16 qt + lc.  One term: biased (kBias); two: the integer 256 q_h . k +
+// q_l . k.
 template <int D, bool kTerms>
-__device__ __forceinline__ void many_qk(const int8_t *stage, const ManyGeom<D> &gm, const i32x4 (&qh)[kQT][D / 64],
+__device__ __forceinline__ void many_qk(const i32x4 (&kf)[4][D / 64], const i32x4 (&qh)[kQT][D / 64],
                                         const i32x4 (&ql)[kQT][D / 64], i32x4 (&s)[4][kQT]) {
     constexpr int kSl = D / 64;
-    i32x4 kf[4][kSl];
-#pragma unroll
-    for (int i = 0; i < kSl; ++i)
-#pragma unroll
-        for (int t = 0; t < 4; ++t) kf[t][i] = *reinterpret_cast<const i32x4 *>(stage + gm.k_rd[i] + t * 16 * D);
     constexpr int kFrom = kTerms ? 0 : kBias;
+    i32x4 z[4][kQT];
+#pragma unroll
+    for (int t = 0; t < 4; ++t)
+#pragma unroll
+        for (int qt = 0; qt < kQT; ++qt)
+            z[t][qt] = __builtin_amdgcn_mfma_i32_16x16x64_i8(kf[t][0], qh[qt][0], i32x4{kFrom, kFrom, kFrom, kFrom}, 0, 0, 0);
 #pragma unroll
     for (int t = 0; t < 4; ++t)
 #pragma unroll
         for (int qt = 0; qt < kQT; ++qt) {
-            i32x4 acc = {kFrom, kFrom, kFrom, kFrom};
-#pragma unroll
-            for (int i = 0; i < kSl; ++i) acc = __builtin_amdgcn_mfma_i32_16x16x64_i8(kf[t][i], qh[qt][i], acc, 0, 0, 0);
-            s[t][qt] = acc;
+            if constexpr (D == 128) z[t][qt] = __builtin_amdgcn_mfma_i32_16x16x64_i8(kf[t][kSl - 1], qh[qt][kSl - 1], z[t][qt], 0, 0, 0);
+            s[t][qt] = z[t][qt];
         }
     if constexpr (kTerms) {
 #pragma unroll
@@ -553,6 +555,12 @@ __device__ __forceinline__ void many_qk(const int8_t *stage, const ManyGeom<D> &
 // Softmax of a tile into the PV operands w[h][qt] (keys 32 h + 8 g ..+7).  f:
 // factors of the rows' integer scores.  kMask: keys of the tile at or past
 // `seen[qt]` (relative to the tile, per row) take no part.
+//
+// Weights are formed as fma(score, f, c), c = -m' less than 2^12, and summed by an
+// MFMA of the fp16 weights beside PV's.  A wave with larger scores, or with a page
+// whose V scale is far below the base's (its weights may then be too small for
+// fp16, and still count in the sum), takes the careful form: the product rounded as
+// the base was, and a sum in fp32.
 template <int D, bool kTerms, bool kMask>
 __device__ __forceinline__ void many_softmax(i32x4 (&s)[4][kQT], const float (&f)[kQT], float v_log2, const int (&seen)[kQT],
                                              int g, ManyState<D> &st, f16x8 (&w)[2][kQT]) {
@@ -562,8 +570,8 @@ __device__ __forceinline__ void many_softmax(i32x4 (&s)[4][kQT], const float (&f
     bool need = false;
 #pragma unroll
     for (int qt = 0; qt < kQT; ++qt) {
-        const int t0 = seen[qt] - 1 - 8 * g;  // key 8 g + c is seen iff c <= t0
         if constexpr (kMask) {
+            const int t0 = seen[qt] - 1 - 8 * g;  // key 8 g + c is seen iff c <= t0
 #pragma unroll
             for (int t = 0; t < 4; ++t)
 #pragma unroll
@@ -598,15 +606,15 @@ __device__ __forceinline__ void many_softmax(i32x4 (&s)[4][kQT], const float (&f
             for (int ds = 0; ds < D / 16; ++ds) st.o[ds][qt] *= alpha;
         }
     }
-    float d[kQT], c[kQT];
-    bool far = false;
+    float d[kQT];
+    bool careful = false;
 #pragma unroll
     for (int qt = 0; qt < kQT; ++qt) {
         d[qt] = st.row[qt].shift(v_log2);
-        c[qt] = d[qt] - __builtin_fmaf(kFrom, f[qt], st.row[qt].m);
-        far = far || !(fabsf(c[qt]) < 4096.0f);
+        st.inverse[qt] = __builtin_amdgcn_exp2f(-(st.row[qt].v + d[qt]));
+        careful = careful || !(fabsf(st.row[qt].m) < 4000.0f && d[qt] >= -8.0f && d[qt] < 64.0f);
     }
-    auto weights = [&](auto far_tag) {
+    if (kMask || __builtin_expect(__any(careful), 0)) {
 #pragma unroll
         for (int qt = 0; qt < kQT; ++qt) {
             const int t0 = seen[qt] - 1 - 8 * g;
@@ -621,11 +629,8 @@ __device__ __forceinline__ void many_softmax(i32x4 (&s)[4][kQT], const float (&f
                     for (int i = 0; i < 2; ++i) {
                         const int e = 2 * j + i;  // key 32 h + 8 g + e
                         const int si = s[2 * h + (e >> 2)][qt][e & 3];
-                        const float v = kTerms ? static_cast<float>(si) : __int_as_float(si);
-                        // far from the base's range the product is rounded as the base was
-                        const float x = decltype(far_tag)::value ? ((v - kFrom) * f[qt] - st.row[qt].m) + d[qt]
-                                                                 : __builtin_fmaf(v, f[qt], c[qt]);
-                        y[i] = __builtin_amdgcn_exp2f(x);
+                        const float v = kTerms ? static_cast<float>(si) : __int_as_float(si) - kFrom;
+                        y[i] = __builtin_amdgcn_exp2f((v * f[qt] - st.row[qt].m) + (d[qt] + kUp));
                         if constexpr (kMask) {
                             const int hidden = (t0 - (32 * h + e)) >> 31;
                             y[i] = __int_as_float(__float_as_int(y[i]) & ~hidden);
@@ -636,16 +641,40 @@ __device__ __forceinline__ void many_softmax(i32x4 (&s)[4][kQT], const float (&f
                 }
                 w[h][qt] = __builtin_bit_cast(f16x8, packed);
             }
-            const float l = __builtin_fmaf(sum, __builtin_amdgcn_exp2f(-(st.row[qt].v + d[qt])), st.row[qt].l);
-            if (!kMask || t0 >= 0) st.row[qt].l = l;  // (a row that sees nothing of the tile has no part in a NaN)
+            // (a row that sees nothing of the tile has no part in a NaN)
+            if (!kMask || seen[qt] > 0) st.row[qt].l = __builtin_fmaf(xsum_f32(sum), st.inverse[qt], st.row[qt].l);
+            st.inverse[qt] = 0.0f;
         }
-    };
-    if (__any(far)) weights(std::true_type{});
-    else weights(std::false_type{});
+    } else {
+#pragma unroll
+        for (int qt = 0; qt < kQT; ++qt) {
+            const float c = (d[qt] + kUp) - st.row[qt].m;
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+                u32x4 packed;
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    float y[2];
+#pragma unroll
+                    for (int i = 0; i < 2; ++i) {
+                        const int e = 2 * j + i;
+                        const int si = s[2 * h + (e >> 2)][qt][e & 3];
+                        const float v = kTerms ? static_cast<float>(si) : __int_as_float(si) - kFrom;
+                        y[i] = __builtin_amdgcn_exp2f(__builtin_fmaf(v, f[qt], c));
+                    }
+                    packed[j] = hw_f16x2_bits(y[0], y[1]);
+                }
+                w[h][qt] = __builtin_bit_cast(f16x8, packed);
+            }
+        }
+    }
 }
 
+// O^T += V^T w and the sum of the tile's weights.
 template <int D>
-__device__ __forceinline__ void many_pv(const int8_t *stage, const ManyGeom<D> &gm, const f16x8 (&w)[2][kQT], ManyState<D> &st) {
+__device__ __forceinline__ void many_pv(const int8_t *stage, const ManyGeom<D> &gm, const f16x8 (&w)[2][kQT], const f16x8 &ones,
+                                        ManyState<D> &st) {
+    f32x4 sum[kQT];
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
         f16x8 vf[D / 16];
@@ -656,7 +685,39 @@ __device__ __forceinline__ void many_pv(const int8_t *stage, const ManyGeom<D> &
 #pragma unroll
             for (int qt = 0; qt < kQT; ++qt)
                 st.o[ds][qt] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vf[ds], w[h][qt], st.o[ds][qt], 0, 0, 0);
+#pragma unroll
+        for (int qt = 0; qt < kQT; ++qt)
+            sum[qt] = __builtin_amdgcn_mfma_f32_16x16x32_f16(ones, w[h][qt], h ? sum[qt] : f32x4{0.0f, 0.0f, 0.0f, 0.0f}, 0, 0, 0);
     }
+#pragma unroll
+    for (int qt = 0; qt < kQT; ++qt) st.row[qt].l = __builtin_fmaf(sum[qt][0], st.inverse[qt], st.row[qt].l);
+}
+
+// A steady step's MFMAs: QK^T of one page, PV of the page before it.
+template <int D, bool kTerms>
+__device__ __forceinline__ void many_cluster(const int8_t *k_stage, const int8_t *v_stage, const ManyGeom<D> &gm,
+                                             const i32x4 (&qh)[kQT][D / 64], const i32x4 (&ql)[kQT][D / 64],
+                                             i32x4 (&s)[4][kQT], const f16x8 (&w)[2][kQT], const f16x8 &ones, ManyState<D> &st) {
+    constexpr int kSl = D / 64;
+    // (over the other workgroup's softmax on the same SIMD)
+    __builtin_amdgcn_s_setprio(3);
+    i32x4 kf[4][kSl];
+#pragma unroll
+    for (int i = 0; i < kSl; ++i)
+#pragma unroll
+        for (int t = 0; t < 4; ++t) kf[t][i] = *reinterpret_cast<const i32x4 *>(k_stage + gm.k_rd[i] + t * 16 * D);
+    many_qk<D, kTerms>(kf, qh, ql, s);
+    many_pv<D>(v_stage, gm, w, ones, st);
+    // Issue order, with at most 16 LDS reads in flight: the K reads, the first
+    // products, half of the V^T reads, products, the other half, the rest.
+    constexpr int kK = 4 * kSl, kV = D / 16, kQk = kK * kQT * (kTerms ? 2 : 1), kPv = 2 * kQT * (kV + 1);
+    __builtin_amdgcn_sched_group_barrier(0x100, kK, 0);
+    __builtin_amdgcn_sched_group_barrier(0x008, kK, 0);
+    __builtin_amdgcn_sched_group_barrier(0x100, kV, 0);
+    __builtin_amdgcn_sched_group_barrier(0x008, kQk - kK + kPv / 9, 0);
+    __builtin_amdgcn_sched_group_barrier(0x100, kV, 0);
+    __builtin_amdgcn_sched_group_barrier(0x008, kPv - kPv / 9, 0);
+    __builtin_amdgcn_s_setprio(0);
 }
 
 // A page's keys into a ring stage; its values into registers, and from there into one.
@@ -682,16 +743,16 @@ __device__ __forceinline__ void many_store_v(int8_t *stage, const ManyGeom<D> &g
 }
 
 template <int D, bool kTerms>
-__global__ __launch_bounds__(kThreads, 2) void cache_many_kernel(CacheCall c) {
+__global__ __launch_bounds__(kThreads, 2) void cache_many_kernel(CacheCall call) {
     constexpr int kSl = D / 64, kDS = D / 16, kLoads = Tiles<D>::kKLoads;
     __shared__ __align__(1024) int8_t lds[Tiles<D>::kBytes];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int g = lane >> 4, lc = lane & 15;
-    const Unit u = unit_at<kManyRows>(c, xcd_chunk(blockIdx.x, gridDim.x));
+    const Unit u = unit_at<kManyRows>(call, xcd_chunk(blockIdx.x, gridDim.x));
     if (u.z > 0 && static_cast<int>(u.z) >= u.used) return;  // the whole workgroup: nothing is left for the range
     PageWindow window;
     int base = u.first;
-    window.fetch(c, u, base, 1, lane);
+    window.fetch(call, u, base, 1, lane);
     const ManyGeom<D> gm = many_geom<D>(wave, lane);
 
     i32x4 qh[kQT][kSl], ql[kQT][kSl];
@@ -702,94 +763,134 @@ __global__ __launch_bounds__(kThreads, 2) void cache_many_kernel(CacheCall c) {
 #pragma unroll
     for (int qt = 0; qt < kQT; ++qt) {
         const uint32_t r = row0 + 16 * qt + lc;
-        const Row row = row_at(c, u.hk, r);
-        const bool in = r < c.rows && row.token < u.n;
-        factor[qt] = load_row<kSl, kTerms>(c, row, u.b, in, 16 * g, 64, qh[qt], ql[qt]);
-        limit[qt] = keys_of(c, min(row.token, max(u.n - 1, 0)), u.n, u.length);
+        const Row row = row_at(call, u.hk, r);
+        const bool in = r < call.rows && row.token < u.n;
+        factor[qt] = load_row<kSl, kTerms>(call, row, u.b, in, 16 * g, 64, qh[qt], ql[qt]);
+        limit[qt] = keys_of(call, min(row.token, max(u.n - 1, 0)), u.n, u.length);
 #pragma unroll
         for (int ds = 0; ds < kDS; ++ds) st.o[ds][qt] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
     }
-    // keys that all rows of the wave see: those of its first row
+    // pages that all rows of the wave see whole: those of its first row
     const int whole = __builtin_amdgcn_readfirstlane(
-        keys_of(c, min(row_at(c, u.hk, row0).token, max(u.n - 1, 0)), u.n, u.length) / kPage);
+        keys_of(call, min(row_at(call, u.hk, row0).token, max(u.n - 1, 0)), u.n, u.length) / kPage);
+    f16x8 ones;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) ones[e] = static_cast<_Float16>(1.0f);
+    const int8_t *k_codes = call.k_codes, *v_codes = call.v_codes;
+    const uint32_t hkv = call.hkv;
 
     i32x4 s[4][kQT];
     f16x8 w[2][kQT];
     u32x4 v[kLoads];
-    auto at_of = [&](int p) { return min(max(p, base), u.end - 1) - base; };
-    auto place = [&](int p) {
-        return static_cast<int64_t>(max(__builtin_amdgcn_readlane(window.page, at_of(p)), 0)) * c.hkv + u.hk;
-    };
-    auto load_k = [&](int p) {
-        many_load_k(lds + (p - u.first) % kKRing * Tiles<D>::kK, make_rsrc(c.k_codes + place(p) * kPage * D, kPage * D), gm, wave);
+    auto at_of = [&](int p) { return min(p, u.end - 1) - base; };
+    auto place = [&](int p) { return static_cast<int64_t>(max(__builtin_amdgcn_readlane(window.page, at_of(p)), 0)) * hkv + u.hk; };
+    auto k_stage = [&](int p) { return lds + (p - u.first) % kKRing * Tiles<D>::kK; };
+    auto v_stage = [&](int p) { return lds + Tiles<D>::kV0 + (p - u.first) % 2 * Tiles<D>::kV; };
+    auto load_k = [&](int8_t *stage, int p) {
+        many_load_k(stage, make_rsrc(k_codes + place(p) * kPage * D, kPage * D), gm, wave);
     };
     auto load_v = [&](int p) {
-        const int8_t *page = c.v_codes + place(p) * kPage * D;
+        const int8_t *page = v_codes + place(p) * kPage * D;
 #pragma unroll
         for (int i = 0; i < kLoads; ++i) v[i] = *reinterpret_cast<const u32x4 *>(page + (i * kThreads + threadIdx.x) * 16);
     };
-    auto store_v = [&](int p) {
+    auto store_v = [&](int8_t *stage, int p) {
         if (lane_value(window.v_log2, at_of(p)) == kZeroValues) {
 #pragma unroll
             for (int i = 0; i < kLoads; ++i) v[i] = u32x4{0, 0, 0, 0};
         }
-        many_store_v<D>(lds + Tiles<D>::kV0 + (p - u.first) % 2 * Tiles<D>::kV, gm, v);
+        many_store_v<D>(stage, gm, v);
     };
-    auto v_stage = [&](int p) { return lds + Tiles<D>::kV0 + (p - u.first) % 2 * Tiles<D>::kV; };
-    auto qk = [&](int p) { many_qk<D, kTerms>(lds + (p - u.first) % kKRing * Tiles<D>::kK, gm, qh, ql, s); };
-    auto softmax = [&](int p) {
-        const int at = at_of(p);
+    auto softmax = [&](int p, auto mask_tag) {
+        const int at = p - base;
         const float k_scale = lane_value(window.k_scale, at), v_log2 = lane_value(window.v_log2, at);
-        const bool there = __builtin_amdgcn_readlane(window.page, at) >= 0;
         float f[kQT];
         int seen[kQT];
 #pragma unroll
-        for (int qt = 0; qt < kQT; ++qt) {
-            f[qt] = factor[qt] * k_scale;
-            seen[qt] = there ? limit[qt] - p * kPage : 0;
+        for (int qt = 0; qt < kQT; ++qt) f[qt] = factor[qt] * k_scale, seen[qt] = kPage;
+        if constexpr (decltype(mask_tag)::value) {
+            const bool there = __builtin_amdgcn_readlane(window.page, at) >= 0;
+#pragma unroll
+            for (int qt = 0; qt < kQT; ++qt) seen[qt] = there ? limit[qt] - p * kPage : 0;
         }
-        if (there && p < whole) many_softmax<D, kTerms, false>(s, f, v_log2, seen, g, st, w);
-        else many_softmax<D, kTerms, true>(s, f, v_log2, seen, g, st, w);
+        many_softmax<D, kTerms, decltype(mask_tag)::value>(s, f, v_log2, seen, g, st, w);
+    };
+    auto qk = [&](int p) {
+        i32x4 kf[4][kSl];
+#pragma unroll
+        for (int i = 0; i < kSl; ++i)
+#pragma unroll
+            for (int t = 0; t < 4; ++t) kf[t][i] = *reinterpret_cast<const i32x4 *>(k_stage(p) + gm.k_rd[i] + t * 16 * D);
+        many_qk<D, kTerms>(kf, qh, ql, s);
     };
 
+    // Step p: QK^T of page p + 1 and PV of page p, then the softmax of page p + 1.
+    // Of the rings, keys of p + 3 go into the stage that step p - 1 read last, values
+    // of p + 1 into the one whose page step p - 1 finished; values of p + 2 are loaded
+    // into the registers that those left.  Each load has a step to land.
     if (u.first < u.end) {
         load_v(u.first);
-        load_k(u.first);
-        load_k(u.first + 1);
-        store_v(u.first);
+        load_k(k_stage(u.first), u.first);
+        load_k(k_stage(u.first + 1), u.first + 1);
+        store_v(v_stage(u.first), u.first);
+        load_k(k_stage(u.first + 2), u.first + 2);
         load_v(u.first + 1);
         __builtin_amdgcn_s_waitcnt(vmcnt_imm(0));
         __syncthreads();
         qk(u.first);
-        softmax(u.first);
-        // Step p: QK of page p + 1 and PV of page p, then the softmax of page p + 1.
-        // Keys of p + 2 go into the stage that step p - 1 read last, values of p + 1
-        // into the one whose page PV finished a step ago.
-#pragma clang loop unroll(disable)
-        for (int p = u.first; p < u.end; ++p) {
+        softmax(u.first, std::true_type{});
+        __builtin_amdgcn_s_waitcnt(lgkmcnt_imm(0));
+        wg_barrier();  // the first stage of keys is free
+        for (int p = u.first; p < u.end;) {
             if (p + 3 - base >= 64 && base + 64 < u.end) {
                 base = p;
-                window.fetch(c, u, base, 1, lane);
+                window.fetch(call, u, base, 1, lane);
             }
-            const bool more = p + 1 < u.end;
-            if (p + 2 < u.end) load_k(p + 2);
-            if (more) {
-                store_v(p + 1);
+            // steps whose next page every row sees whole: up to the first that is none,
+            // and as far as the window reaches three pages on
+            const uint64_t none = __ballot(window.page < 0) & (p + 1 - base < 64 ? ~0ull << (p + 1 - base) : 0);
+            int to = min(min(u.end, whole) - 1, base + 64 < u.end ? base + 61 : u.end);
+            if (none) to = min(to, base + static_cast<int>(__builtin_ctzll(none)) - 1);
+            int k0 = (p - u.first) % kKRing, v0 = (p - u.first) % 2;
+#pragma clang loop unroll(disable)
+            for (; p < to; ++p) {
+                const int k1 = k0 == kKRing - 1 ? 0 : k0 + 1;
+                many_cluster<D, kTerms>(lds + k1 * Tiles<D>::kK, lds + Tiles<D>::kV0 + v0 * Tiles<D>::kV, gm, qh, ql, s, w, ones, st);
+                store_v(lds + Tiles<D>::kV0 + (v0 ^ 1) * Tiles<D>::kV, p + 1);
+                load_k(lds + k0 * Tiles<D>::kK, p + 3);
+                load_v(p + 2);
+                softmax(p + 1, std::false_type{});
+                k0 = k1, v0 ^= 1;
+                // the keys of page p + 2 have landed: all but this step's loads
+                __builtin_amdgcn_s_waitcnt(vmcnt_imm(2 * kLoads));
+                __builtin_amdgcn_s_waitcnt(lgkmcnt_imm(0));
+                wg_barrier();
+            }
+            if (p + 3 - base >= 64 && base + 64 < u.end) continue;  // the window's end
+            // One step of another kind: a page that some row sees in part, or the last.
+            if (p + 1 < u.end) {
                 qk(p + 1);
+                store_v(v_stage(p + 1), p + 1);
+                if (p + 3 < u.end) load_k(k_stage(p + 3), p + 3);
+                if (p + 2 < u.end) load_v(p + 2);
             }
-            if (p + 2 < u.end) load_v(p + 2);
-            many_pv<D>(v_stage(p), gm, w, st);
-            if (more) softmax(p + 1);
-            __builtin_amdgcn_s_waitcnt(vmcnt_imm(0));
-            __syncthreads();
+            many_pv<D>(v_stage(p), gm, w, ones, st);
+            if (p + 1 < u.end) softmax(p + 1, std::true_type{});
+            __builtin_amdgcn_s_waitcnt(0);
+            wg_barrier();
+            ++p;
         }
     }
+    // (the call's fields are read again, not kept through the loop)
+    auto *again = (const CacheCall *)__builtin_amdgcn_kernarg_segment_ptr();
+    asm volatile("" : "+s"(again));
+    const CacheCall c = *again;
 #pragma unroll
     for (int qt = 0; qt < kQT; ++qt) {
         f32x4 o[kDS];
 #pragma unroll
         for (int ds = 0; ds < kDS; ++ds) o[ds] = st.o[ds][qt];
-        store_row<D>(c, u, o, st.row[qt].m, st.row[qt].v, xsum_f32(st.row[qt].l), row0 + 16 * qt + lc, g);
+        store_row<D>(c, u, o, st.row[qt].m, st.row[qt].v, st.row[qt].l, row0 + 16 * qt + lc, g);
     }
 }
 
