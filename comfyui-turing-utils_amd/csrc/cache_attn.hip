@@ -164,12 +164,20 @@ __device__ __forceinline__ float load_row(const CacheCall &c, const Row &row, ui
 }
 
 // Four int8 codes as two pairs of fp16: the bytes biased by 128 below the
-// exponent of 1024, less 1152.
-__device__ __forceinline__ u32x2 codes_to_f16(uint32_t w) {
+// exponent of 1024, less 1152.  With the selectors of zeros, four zeros.
+struct Selectors {
+    uint32_t low = 0x07010700u, high = 0x07030702u;
+    __device__ __forceinline__ static Selectors of(bool zeros) {
+        Selectors s;
+        if (zeros) s.low = s.high = 0x07060706u;
+        return s;
+    }
+};
+__device__ __forceinline__ u32x2 codes_to_f16(uint32_t w, const Selectors &sel) {
     const f16x2_t bias = {static_cast<_Float16>(1152.0f), static_cast<_Float16>(1152.0f)};
     const uint32_t x = w ^ 0x80808080u;
-    const uint32_t a = __builtin_amdgcn_perm(0x64646464u, x, 0x07010700u);
-    const uint32_t b = __builtin_amdgcn_perm(0x64646464u, x, 0x07030702u);
+    const uint32_t a = __builtin_amdgcn_perm(0x64806480u, x, sel.low);
+    const uint32_t b = __builtin_amdgcn_perm(0x64806480u, x, sel.high);
     return u32x2{__builtin_bit_cast(uint32_t, __builtin_bit_cast(f16x2_t, a) - bias),
                  __builtin_bit_cast(uint32_t, __builtin_bit_cast(f16x2_t, b) - bias)};
 }
@@ -182,7 +190,7 @@ __device__ __forceinline__ float lane_value(float v, int lane) {
 // (-1: none), K scale and log2 of the V scale.
 struct PageWindow {
     int page;
-    float k_scale, v_log2;
+    float k_scale, v_log2, v_inverse;
     __device__ __forceinline__ void fetch(const CacheCall &c, const Unit &u, int from, int step, int lane) {
         const int at = from + step * lane;
         int p = -1;
@@ -194,6 +202,7 @@ struct PageWindow {
         // no number, the values count as zeros of that scale)
         const float v = c.v_scale[s];
         v_log2 = v <= 8.077935669e-28f ? kZeroValues : __builtin_amdgcn_logf(v);
+        v_inverse = v <= 8.077935669e-28f ? 1.2379400392853803e27f : __builtin_amdgcn_rcpf(v);
     }
 };
 
@@ -375,7 +384,7 @@ __global__ __launch_bounds__(kThreads, D == 128 && kRT == 2 ? 1 : 2) void cache_
             for (int ds = 0; ds < kDS; ++ds) {
 #pragma unroll
                 for (int h = 0; h < 2; ++h) {
-                    const u32x2 a = codes_to_f16(r.v[ds][2 * h]), b = codes_to_f16(r.v[ds][2 * h + 1]);
+                    const u32x2 a = codes_to_f16(r.v[ds][2 * h], Selectors{}), b = codes_to_f16(r.v[ds][2 * h + 1], Selectors{});
                     const f16x8 v = __builtin_bit_cast(f16x8, (u32x4{a[0], a[1], b[0], b[1]}));
                     o[rt][ds] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v, w[h], o[rt][ds], 0, 0, 0);
                 }
@@ -455,12 +464,13 @@ __global__ __launch_bounds__(kThreads, D == 128 && kRT == 2 ? 1 : 2) void cache_
 // ---------------------------------------------------------------------------
 // A workgroup of four waves has 128 rows of one K/V head, 32 a wave; two share a
 // CU, so that one's MFMAs run beside the other's softmax.  Pages stream through
-// LDS: keys as codes by direct-to-LDS loads, a ring of three; values through
+// LDS: keys as codes by direct-to-LDS loads, a ring of four; values through
 // registers, converted to fp16 once for the four waves, a ring of two.
 constexpr int kQT = 2;           // 16-row fragments of a wave
 constexpr int kWaveRows = 16 * kQT;
 constexpr int kManyRows = 4 * kWaveRows;
-constexpr int kKRing = 3;
+constexpr int kKRing = 4;
+constexpr float kSummed = -1.0f;
 
 template <int D>
 struct Tiles {
@@ -483,7 +493,7 @@ struct ManyGeom {
     uint32_t k_src[Tiles<D>::kKLoads];  // a lane's 16 bytes of a page's keys
     uint32_t k_rd[D / 64];              // operand of QK^T
     uint32_t v_rd[2];                   // operand of PV, half 0 / 1
-    uint32_t v_wr[Tiles<D>::kKLoads][2];
+    uint32_t v_wr[2];                   // where the two halves of a lane's 16 values go (64 channels on for its next 16)
 };
 
 // 16-byte pieces of a row are XORed with row bits, so that 16 lanes that read
@@ -498,11 +508,10 @@ __device__ __forceinline__ ManyGeom<D> many_geom(int wave, int lane) {
         const int row = piece / (D / 16), at = piece % (D / 16);
         const int swizzle = D == 128 ? (row >> 1) & 7 : (row >> 2) & 3;
         gm.k_src[i] = static_cast<uint32_t>(key_of_row(row) * D + (at ^ swizzle) * 16);
-        const int code = i * kThreads + wave * 64 + lane;  // of 16 bytes in the page's values
-        const int ch = code / 4;
-#pragma unroll
-        for (int e = 0; e < 2; ++e) gm.v_wr[i][e] = static_cast<uint32_t>(ch * 128 + (((2 * (code % 4) + e) ^ ((ch >> 1) & 7)) << 4));
     }
+    const int ch = wave * 16 + lane / 4;
+#pragma unroll
+    for (int e = 0; e < 2; ++e) gm.v_wr[e] = static_cast<uint32_t>(ch * 128 + (((2 * (lane % 4) + e) ^ ((ch >> 1) & 7)) << 4));
 #pragma unroll
     for (int i = 0; i < D / 64; ++i)
         gm.k_rd[i] = static_cast<uint32_t>(lc * D + (D == 128 ? ((4 * i + g) ^ ((lc >> 1) & 7)) : (g ^ ((lc >> 2) & 3))) * 16);
@@ -511,11 +520,51 @@ __device__ __forceinline__ ManyGeom<D> many_geom(int wave, int lane) {
     return gm;
 }
 
+// Bases of the wave's rows.  Where every base is small in size (`ready`), a base
+// is also held as one number, base = m + v - kUp.
 template <int D>
 struct ManyState {
     RowState row[kQT];
-    float inverse[kQT];  // 1 / V scale of the page whose weights w holds
+    float base[kQT];
     f32x4 o[D / 16][kQT];
+    // of the wave:
+    float m_most;  // largest |m|; infinite while a row has seen no key
+    float v_most;  // largest v
+    __device__ __forceinline__ void init() {
+#pragma unroll
+        for (int qt = 0; qt < kQT; ++qt) {
+            base[qt] = kNoBase;
+#pragma unroll
+            for (int ds = 0; ds < D / 16; ++ds) o[ds][qt] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+        }
+        m_most = INFINITY, v_most = 0.0f;
+    }
+    // Moves the bases of rows that a page's scores pass by more than kSlack; top:
+    // each lane's largest.  A row's base moves by its own scores alone.
+    __device__ __forceinline__ void move(const float (&top)[kQT], float v_log2) {
+        float size = 0.0f, v = kZeroValues;
+#pragma unroll
+        for (int qt = 0; qt < kQT; ++qt) {
+            const float row_top = xmax_f32(top[qt]);
+            const bool go = (row_top - row[qt].m) + (v_log2 - row[qt].v) > kSlack;
+            const float alpha = go ? __builtin_amdgcn_exp2f((row[qt].m - row_top) + (row[qt].v - v_log2)) : 1.0f;
+            row[qt].m = go ? row_top : row[qt].m;
+            row[qt].v = go ? v_log2 : row[qt].v;
+            row[qt].l *= alpha;
+#pragma unroll
+            for (int ds = 0; ds < D / 16; ++ds) o[ds][qt] *= alpha;
+            base[qt] = (row[qt].m + row[qt].v) - kUp;
+            size = fmaxf(size, fabsf(row[qt].m));
+            v = fmaxf(v, row[qt].v);
+        }
+#pragma unroll
+        for (int i = 1; i < 16; i <<= 1) {
+            size = fmaxf(size, __shfl_xor(size, i));
+            v = fmaxf(v, __shfl_xor(v, i));
+        }
+        m_most = __int_as_float(__builtin_amdgcn_readfirstlane(__float_as_int(size)));
+        v_most = __int_as_float(__builtin_amdgcn_readfirstlane(__float_as_int(v)));
+    }
 };
 
 // S^T of a tile from its K fragments: s[t][qt][r] = key 32 (t >> 1) + 8 g + 4 (t &
@@ -552,73 +601,104 @@ __device__ __forceinline__ void many_qk(const i32x4 (&kf)[4][D / 64], const i32x
     }
 }
 
-// Softmax of a tile into the PV operands w[h][qt] (keys 32 h + 8 g ..+7).  f:
-// factors of the rows' integer scores.  kMask: keys of the tile at or past
-// `seen[qt]` (relative to the tile, per row) take no part.
-//
-// Weights are formed as fma(score, f, c), c = -m' less than 2^12, and summed by an
-// MFMA of the fp16 weights beside PV's.  A wave with larger scores, or with a page
-// whose V scale is far below the base's (its weights may then be too small for
-// fp16, and still count in the sum), takes the careful form: the product rounded as
-// the base was, and a sum in fp32.
-template <int D, bool kTerms, bool kMask>
-__device__ __forceinline__ void many_softmax(i32x4 (&s)[4][kQT], const float (&f)[kQT], float v_log2, const int (&seen)[kQT],
-                                             int g, ManyState<D> &st, f16x8 (&w)[2][kQT]) {
-    constexpr float kFrom = kTerms ? 0.0f : kBiasF;
+// The lane's largest score of a tile, an integer as many_qk leaves it.
+__device__ __forceinline__ int tile_top(const i32x4 (&s)[4][kQT], int qt) {
+    int mi = imax3(s[0][qt][0], s[0][qt][1], s[0][qt][2]);
+    mi = imax3(mi, s[0][qt][3], s[1][qt][0]);
+    mi = imax3(mi, s[1][qt][1], s[1][qt][2]);
+    mi = imax3(mi, s[1][qt][3], s[2][qt][0]);
+    mi = imax3(mi, s[2][qt][1], s[2][qt][2]);
+    mi = imax3(mi, s[2][qt][3], s[3][qt][0]);
+    mi = imax3(mi, s[3][qt][1], s[3][qt][2]);
+    return max(mi, s[3][qt][3]);
+}
+
+template <bool kTerms>
+__device__ __forceinline__ float score(int s) {
+    return kTerms ? static_cast<float>(s) : __int_as_float(s) - kBiasF;
+}
+
+// Weights w[h][qt] of a tile (keys 32 h + 8 g ..+7) in the careful form: for rows
+// that see a part of it (keys from `seen[qt]` on take no part), for scores whose
+// size would swallow fractions in a sum, and for pages whose V scale is far below
+// the base's, where weights too small for fp16 still count in the sum.  The product
+// is rounded as the base was, and the sum of weights is one of 32 bits, here.
+template <int D, bool kTerms>
+__device__ __forceinline__ void careful_weights(i32x4 (&s)[4][kQT], const float (&f)[kQT], float v_log2, const int (&seen)[kQT],
+                                                int g, ManyState<D> &st, f16x8 (&w)[2][kQT]) {
     constexpr int kLeast = static_cast<int>(0x80000000u);
     float top[kQT];
     bool need = false;
 #pragma unroll
     for (int qt = 0; qt < kQT; ++qt) {
-        if constexpr (kMask) {
-            const int t0 = seen[qt] - 1 - 8 * g;  // key 8 g + c is seen iff c <= t0
+        const int t0 = seen[qt] - 1 - 8 * g;  // key 8 g + c is seen iff c <= t0
 #pragma unroll
-            for (int t = 0; t < 4; ++t)
+        for (int t = 0; t < 4; ++t)
 #pragma unroll
-                for (int r = 0; r < 4; ++r) {
-                    const int hidden = (t0 - (32 * (t >> 1) + 4 * (t & 1) + r)) >> 31;
-                    s[t][qt][r] = (s[t][qt][r] & ~hidden) | (kLeast & hidden);
-                }
-        }
-        int mi = imax3(s[0][qt][0], s[0][qt][1], s[0][qt][2]);
-        mi = imax3(mi, s[0][qt][3], s[1][qt][0]);
-        mi = imax3(mi, s[1][qt][1], s[1][qt][2]);
-        mi = imax3(mi, s[1][qt][3], s[2][qt][0]);
-        mi = imax3(mi, s[2][qt][1], s[2][qt][2]);
-        mi = imax3(mi, s[2][qt][3], s[3][qt][0]);
-        mi = imax3(mi, s[3][qt][1], s[3][qt][2]);
-        mi = max(mi, s[3][qt][3]);
-        top[qt] = (kTerms ? static_cast<float>(mi) : __int_as_float(mi) - kFrom) * f[qt];
-        if (kMask && mi == kLeast) top[qt] = -INFINITY;
+            for (int r = 0; r < 4; ++r) {
+                const int hidden = (t0 - (32 * (t >> 1) + 4 * (t & 1) + r)) >> 31;
+                s[t][qt][r] = (s[t][qt][r] & ~hidden) | (kLeast & hidden);
+            }
+        const int mi = tile_top(s, qt);
+        top[qt] = mi == kLeast ? -INFINITY : score<kTerms>(mi) * f[qt];
         need = need || (top[qt] - st.row[qt].m) + (v_log2 - st.row[qt].v) > kSlack;
     }
-    if (__any(need)) {
-#pragma unroll
-        for (int qt = 0; qt < kQT; ++qt) {
-            // a row's base moves by its own scores alone
-            const float row_top = xmax_f32(top[qt]);
-            const bool move = (row_top - st.row[qt].m) + (v_log2 - st.row[qt].v) > kSlack;
-            const float alpha = move ? __builtin_amdgcn_exp2f((st.row[qt].m - row_top) + (st.row[qt].v - v_log2)) : 1.0f;
-            st.row[qt].m = move ? row_top : st.row[qt].m;
-            st.row[qt].v = move ? v_log2 : st.row[qt].v;
-            st.row[qt].l *= alpha;
-#pragma unroll
-            for (int ds = 0; ds < D / 16; ++ds) st.o[ds][qt] *= alpha;
-        }
-    }
-    float d[kQT];
-    bool careful = false;
+    if (__any(need)) st.move(top, v_log2);
 #pragma unroll
     for (int qt = 0; qt < kQT; ++qt) {
-        d[qt] = st.row[qt].shift(v_log2);
-        st.inverse[qt] = __builtin_amdgcn_exp2f(-(st.row[qt].v + d[qt]));
-        careful = careful || !(fabsf(st.row[qt].m) < 4000.0f && d[qt] >= -8.0f && d[qt] < 64.0f);
+        const int t0 = seen[qt] - 1 - 8 * g;
+        const float d = st.row[qt].shift(v_log2);
+        float sum = 0.0f;
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+            u32x4 packed;
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                float y[2];
+#pragma unroll
+                for (int i = 0; i < 2; ++i) {
+                    const int e = 2 * j + i;  // key 32 h + 8 g + e
+                    const int hidden = (t0 - (32 * h + e)) >> 31;
+                    const float x = (score<kTerms>(s[2 * h + (e >> 2)][qt][e & 3]) * f[qt] - st.row[qt].m) + (d + kUp);
+                    y[i] = __int_as_float(__float_as_int(__builtin_amdgcn_exp2f(x)) & ~hidden);
+                    sum += y[i];
+                }
+                packed[j] = hw_f16x2_bits(y[0], y[1]);
+            }
+            w[h][qt] = __builtin_bit_cast(f16x8, packed);
+        }
+        // (a row that sees nothing of the tile has no part in a NaN)
+        if (seen[qt] > 0)
+            st.row[qt].l = __builtin_fmaf(xsum_f32(sum), __builtin_amdgcn_exp2f(-(st.row[qt].v + d)), st.row[qt].l);
     }
-    if (kMask || __builtin_expect(__any(careful), 0)) {
+}
+
+// Softmax of a tile that every row of the wave sees whole.  Weights are
+// fma(score, f, c) with c = log2 v_scale - base, less than 2^12 in size and so exact
+// to 2^-13 (with the bias of the integer scores in it where that keeps it there),
+// and are summed, as fp16, by an MFMA beside PV's.  Returns what that sum is to be
+// multiplied by: 1 / v_scale, or kSummed where the careful form has summed.
+template <int D, bool kTerms>
+__device__ __forceinline__ float whole_weights(i32x4 (&s)[4][kQT], const float (&f)[kQT], float f_most, float v_log2,
+                                               float v_inverse, int g, ManyState<D> &st, f16x8 (&w)[2][kQT]) {
+    float top[kQT];
+    bool need = false;
+#pragma unroll
+    for (int qt = 0; qt < kQT; ++qt) {
+        top[qt] = score<kTerms>(tile_top(s, qt)) * f[qt];
+        need = need || (top[qt] + v_log2) - st.base[qt] > kSlack + kUp;
+    }
+    if (__any(need)) st.move(top, v_log2);
+    if (__builtin_expect(!(st.m_most < 4000.0f && v_log2 >= st.v_most - 8.0f), 0)) {
+        const int seen[kQT] = {kPage, kPage};
+        careful_weights<D, kTerms>(s, f, v_log2, seen, g, st, w);
+        return kSummed;
+    }
+    auto weights = [&](auto folded_tag) __attribute__((always_inline)) {
+        constexpr bool kFolded = decltype(folded_tag)::value;
 #pragma unroll
         for (int qt = 0; qt < kQT; ++qt) {
-            const int t0 = seen[qt] - 1 - 8 * g;
-            float sum = 0.0f;
+            const float c = v_log2 - (kFolded ? __builtin_fmaf(kBiasF, f[qt], st.base[qt]) : st.base[qt]);
 #pragma unroll
             for (int h = 0; h < 2; ++h) {
                 u32x4 packed;
@@ -629,51 +709,28 @@ __device__ __forceinline__ void many_softmax(i32x4 (&s)[4][kQT], const float (&f
                     for (int i = 0; i < 2; ++i) {
                         const int e = 2 * j + i;  // key 32 h + 8 g + e
                         const int si = s[2 * h + (e >> 2)][qt][e & 3];
-                        const float v = kTerms ? static_cast<float>(si) : __int_as_float(si) - kFrom;
-                        y[i] = __builtin_amdgcn_exp2f((v * f[qt] - st.row[qt].m) + (d[qt] + kUp));
-                        if constexpr (kMask) {
-                            const int hidden = (t0 - (32 * h + e)) >> 31;
-                            y[i] = __int_as_float(__float_as_int(y[i]) & ~hidden);
-                        }
-                        sum += y[i];
+                        const float x = kFolded ? __int_as_float(si) : score<kTerms>(si);
+                        y[i] = __builtin_amdgcn_exp2f(__builtin_fmaf(x, f[qt], c));
                     }
                     packed[j] = hw_f16x2_bits(y[0], y[1]);
                 }
                 w[h][qt] = __builtin_bit_cast(f16x8, packed);
             }
-            // (a row that sees nothing of the tile has no part in a NaN)
-            if (!kMask || seen[qt] > 0) st.row[qt].l = __builtin_fmaf(xsum_f32(sum), st.inverse[qt], st.row[qt].l);
-            st.inverse[qt] = 0.0f;
         }
+    };
+    if constexpr (kTerms) {
+        weights(std::false_type{});
     } else {
-#pragma unroll
-        for (int qt = 0; qt < kQT; ++qt) {
-            const float c = (d[qt] + kUp) - st.row[qt].m;
-#pragma unroll
-            for (int h = 0; h < 2; ++h) {
-                u32x4 packed;
-#pragma unroll
-                for (int j = 0; j < 4; ++j) {
-                    float y[2];
-#pragma unroll
-                    for (int i = 0; i < 2; ++i) {
-                        const int e = 2 * j + i;
-                        const int si = s[2 * h + (e >> 2)][qt][e & 3];
-                        const float v = kTerms ? static_cast<float>(si) : __int_as_float(si) - kFrom;
-                        y[i] = __builtin_amdgcn_exp2f(__builtin_fmaf(v, f[qt], c));
-                    }
-                    packed[j] = hw_f16x2_bits(y[0], y[1]);
-                }
-                w[h][qt] = __builtin_bit_cast(f16x8, packed);
-            }
-        }
+        if (__builtin_fmaf(kBiasF, f_most, st.m_most) < 4000.0f) weights(std::true_type{});
+        else weights(std::false_type{});
     }
+    return v_inverse;
 }
 
-// O^T += V^T w and the sum of the tile's weights.
+// O^T += V^T w and the sum of the tile's weights, times `inverse` (see whole_weights).
 template <int D>
 __device__ __forceinline__ void many_pv(const int8_t *stage, const ManyGeom<D> &gm, const f16x8 (&w)[2][kQT], const f16x8 &ones,
-                                        ManyState<D> &st) {
+                                        float inverse, ManyState<D> &st) {
     f32x4 sum[kQT];
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
@@ -689,15 +746,18 @@ __device__ __forceinline__ void many_pv(const int8_t *stage, const ManyGeom<D> &
         for (int qt = 0; qt < kQT; ++qt)
             sum[qt] = __builtin_amdgcn_mfma_f32_16x16x32_f16(ones, w[h][qt], h ? sum[qt] : f32x4{0.0f, 0.0f, 0.0f, 0.0f}, 0, 0, 0);
     }
+    if (!(inverse < 0.0f)) {
 #pragma unroll
-    for (int qt = 0; qt < kQT; ++qt) st.row[qt].l = __builtin_fmaf(sum[qt][0], st.inverse[qt], st.row[qt].l);
+        for (int qt = 0; qt < kQT; ++qt) st.row[qt].l = __builtin_fmaf(sum[qt][0], inverse, st.row[qt].l);
+    }
 }
 
 // A steady step's MFMAs: QK^T of one page, PV of the page before it.
 template <int D, bool kTerms>
 __device__ __forceinline__ void many_cluster(const int8_t *k_stage, const int8_t *v_stage, const ManyGeom<D> &gm,
                                              const i32x4 (&qh)[kQT][D / 64], const i32x4 (&ql)[kQT][D / 64],
-                                             i32x4 (&s)[4][kQT], const f16x8 (&w)[2][kQT], const f16x8 &ones, ManyState<D> &st) {
+                                             i32x4 (&s)[4][kQT], const f16x8 (&w)[2][kQT], const f16x8 &ones,
+                                             float inverse, ManyState<D> &st) {
     constexpr int kSl = D / 64;
     // (over the other workgroup's softmax on the same SIMD)
     __builtin_amdgcn_s_setprio(3);
@@ -707,7 +767,7 @@ __device__ __forceinline__ void many_cluster(const int8_t *k_stage, const int8_t
 #pragma unroll
         for (int t = 0; t < 4; ++t) kf[t][i] = *reinterpret_cast<const i32x4 *>(k_stage + gm.k_rd[i] + t * 16 * D);
     many_qk<D, kTerms>(kf, qh, ql, s);
-    many_pv<D>(v_stage, gm, w, ones, st);
+    many_pv<D>(v_stage, gm, w, ones, inverse, st);
     // Issue order, with at most 16 LDS reads in flight: the K reads, the first
     // products, half of the V^T reads, products, the other half, the rest.
     constexpr int kK = 4 * kSl, kV = D / 16, kQk = kK * kQT * (kTerms ? 2 : 1), kPv = 2 * kQT * (kV + 1);
@@ -732,13 +792,14 @@ TU_MANY_LOAD_K(64)
 #undef TU_MANY_LOAD_K
 
 template <int D>
-__device__ __forceinline__ void many_store_v(int8_t *stage, const ManyGeom<D> &gm, const u32x4 (&v)[Tiles<D>::kKLoads]) {
+__device__ __forceinline__ void many_store_v(int8_t *stage, const ManyGeom<D> &gm, const u32x4 (&v)[Tiles<D>::kKLoads],
+                                             const Selectors &sel) {
 #pragma unroll
     for (int i = 0; i < Tiles<D>::kKLoads; ++i)
 #pragma unroll
         for (int e = 0; e < 2; ++e) {
-            const u32x2 a = codes_to_f16(v[i][2 * e]), b = codes_to_f16(v[i][2 * e + 1]);
-            *reinterpret_cast<u32x4 *>(stage + gm.v_wr[i][e]) = u32x4{a[0], a[1], b[0], b[1]};
+            const u32x2 a = codes_to_f16(v[i][2 * e], sel), b = codes_to_f16(v[i][2 * e + 1], sel);
+            *reinterpret_cast<u32x4 *>(stage + gm.v_wr[e] + i * (kThreads / 4 * 128)) = u32x4{a[0], a[1], b[0], b[1]};
         }
 }
 
@@ -760,6 +821,8 @@ __global__ __launch_bounds__(kThreads, 2) void cache_many_kernel(CacheCall call)
     int limit[kQT];
     ManyState<D> st;
     const uint32_t row0 = u.block * kManyRows + wave * kWaveRows;
+    st.init();
+    float most = 0.0f;
 #pragma unroll
     for (int qt = 0; qt < kQT; ++qt) {
         const uint32_t r = row0 + 16 * qt + lc;
@@ -767,9 +830,11 @@ __global__ __launch_bounds__(kThreads, 2) void cache_many_kernel(CacheCall call)
         const bool in = r < call.rows && row.token < u.n;
         factor[qt] = load_row<kSl, kTerms>(call, row, u.b, in, 16 * g, 64, qh[qt], ql[qt]);
         limit[qt] = keys_of(call, min(row.token, max(u.n - 1, 0)), u.n, u.length);
-#pragma unroll
-        for (int ds = 0; ds < kDS; ++ds) st.o[ds][qt] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+        most = fmaxf(most, factor[qt]);
     }
+#pragma unroll
+    for (int i = 1; i < 16; i <<= 1) most = fmaxf(most, __shfl_xor(most, i));
+    const float factor_most = __int_as_float(__builtin_amdgcn_readfirstlane(__float_as_int(most)));
     // pages that all rows of the wave see whole: those of its first row
     const int whole = __builtin_amdgcn_readfirstlane(
         keys_of(call, min(row_at(call, u.hk, row0).token, max(u.n - 1, 0)), u.n, u.length) / kPage);
@@ -781,41 +846,45 @@ __global__ __launch_bounds__(kThreads, 2) void cache_many_kernel(CacheCall call)
 
     i32x4 s[4][kQT];
     f16x8 w[2][kQT];
+    float inverse = kSummed;  // of the page whose weights w holds
     u32x4 v[kLoads];
     auto at_of = [&](int p) { return min(p, u.end - 1) - base; };
-    auto place = [&](int p) { return static_cast<int64_t>(max(__builtin_amdgcn_readlane(window.page, at_of(p)), 0)) * hkv + u.hk; };
+    auto place = [&](int p) {
+        return static_cast<int64_t>(max(__builtin_amdgcn_readlane(window.page, at_of(p)), 0)) * hkv + u.hk;
+    };
     auto k_stage = [&](int p) { return lds + (p - u.first) % kKRing * Tiles<D>::kK; };
     auto v_stage = [&](int p) { return lds + Tiles<D>::kV0 + (p - u.first) % 2 * Tiles<D>::kV; };
-    auto load_k = [&](int8_t *stage, int p) {
-        many_load_k(stage, make_rsrc(k_codes + place(p) * kPage * D, kPage * D), gm, wave);
+    auto load_k = [&](int8_t *stage, int64_t at) __attribute__((always_inline)) {
+        many_load_k(stage, make_rsrc(k_codes + at * kPage * D, kPage * D), gm, wave);
     };
-    auto load_v = [&](int p) {
-        const int8_t *page = v_codes + place(p) * kPage * D;
+    auto load_v = [&](int64_t at) __attribute__((always_inline)) {
+        const int8_t *page = v_codes + at * kPage * D;
 #pragma unroll
         for (int i = 0; i < kLoads; ++i) v[i] = *reinterpret_cast<const u32x4 *>(page + (i * kThreads + threadIdx.x) * 16);
     };
-    auto store_v = [&](int8_t *stage, int p) {
-        if (lane_value(window.v_log2, at_of(p)) == kZeroValues) {
-#pragma unroll
-            for (int i = 0; i < kLoads; ++i) v[i] = u32x4{0, 0, 0, 0};
-        }
-        many_store_v<D>(stage, gm, v);
+    auto store_v = [&](int8_t *stage, int p) __attribute__((always_inline)) {
+        many_store_v<D>(stage, gm, v, Selectors::of(lane_value(window.v_log2, p - base) == kZeroValues));
     };
-    auto softmax = [&](int p, auto mask_tag) {
+    auto softmax_part = [&](int p) __attribute__((always_inline)) {
         const int at = p - base;
         const float k_scale = lane_value(window.k_scale, at), v_log2 = lane_value(window.v_log2, at);
+        const bool there = __builtin_amdgcn_readlane(window.page, at) >= 0;
         float f[kQT];
         int seen[kQT];
 #pragma unroll
-        for (int qt = 0; qt < kQT; ++qt) f[qt] = factor[qt] * k_scale, seen[qt] = kPage;
-        if constexpr (decltype(mask_tag)::value) {
-            const bool there = __builtin_amdgcn_readlane(window.page, at) >= 0;
-#pragma unroll
-            for (int qt = 0; qt < kQT; ++qt) seen[qt] = there ? limit[qt] - p * kPage : 0;
-        }
-        many_softmax<D, kTerms, decltype(mask_tag)::value>(s, f, v_log2, seen, g, st, w);
+        for (int qt = 0; qt < kQT; ++qt) f[qt] = factor[qt] * k_scale, seen[qt] = there ? limit[qt] - p * kPage : 0;
+        careful_weights<D, kTerms>(s, f, v_log2, seen, g, st, w);
+        inverse = kSummed;
     };
-    auto qk = [&](int p) {
+    auto softmax_whole = [&](int p) __attribute__((always_inline)) {
+        const int at = p - base;
+        const float k_scale = lane_value(window.k_scale, at), v_log2 = lane_value(window.v_log2, at);
+        float f[kQT];
+#pragma unroll
+        for (int qt = 0; qt < kQT; ++qt) f[qt] = factor[qt] * k_scale;
+        inverse = whole_weights<D, kTerms>(s, f, factor_most * k_scale, v_log2, lane_value(window.v_inverse, at), g, st, w);
+    };
+    auto qk = [&](int p) __attribute__((always_inline)) {
         i32x4 kf[4][kSl];
 #pragma unroll
         for (int i = 0; i < kSl; ++i)
@@ -825,22 +894,20 @@ __global__ __launch_bounds__(kThreads, 2) void cache_many_kernel(CacheCall call)
     };
 
     // Step p: QK^T of page p + 1 and PV of page p, then the softmax of page p + 1.
-    // Of the rings, keys of p + 3 go into the stage that step p - 1 read last, values
-    // of p + 1 into the one whose page step p - 1 finished; values of p + 2 are loaded
+    // Of the rings, keys of p + 3 go into a stage that step p - 2 read last, values of
+    // p + 1 into the one whose page step p - 1 finished; values of p + 2 are loaded
     // into the registers that those left.  Each load has a step to land.
     if (u.first < u.end) {
-        load_v(u.first);
-        load_k(k_stage(u.first), u.first);
-        load_k(k_stage(u.first + 1), u.first + 1);
+        load_v(place(u.first));
+        load_k(k_stage(u.first), place(u.first));
+        load_k(k_stage(u.first + 1), place(u.first + 1));
         store_v(v_stage(u.first), u.first);
-        load_k(k_stage(u.first + 2), u.first + 2);
-        load_v(u.first + 1);
+        load_k(k_stage(u.first + 2), place(u.first + 2));
+        load_v(place(u.first + 1));
         __builtin_amdgcn_s_waitcnt(vmcnt_imm(0));
         __syncthreads();
         qk(u.first);
-        softmax(u.first, std::true_type{});
-        __builtin_amdgcn_s_waitcnt(lgkmcnt_imm(0));
-        wg_barrier();  // the first stage of keys is free
+        softmax_part(u.first);
         for (int p = u.first; p < u.end;) {
             if (p + 3 - base >= 64 && base + 64 < u.end) {
                 base = p;
@@ -851,31 +918,43 @@ __global__ __launch_bounds__(kThreads, 2) void cache_many_kernel(CacheCall call)
             const uint64_t none = __ballot(window.page < 0) & (p + 1 - base < 64 ? ~0ull << (p + 1 - base) : 0);
             int to = min(min(u.end, whole) - 1, base + 64 < u.end ? base + 61 : u.end);
             if (none) to = min(to, base + static_cast<int>(__builtin_ctzll(none)) - 1);
-            int k0 = (p - u.first) % kKRing, v0 = (p - u.first) % 2;
+            if (p < to) {
+                int k1 = (p + 1 - u.first) % kKRing * Tiles<D>::kK;
+                int64_t next = place(p + 2);
+                auto step = [&](auto odd_tag) __attribute__((always_inline)) {
+                    constexpr int kOdd = decltype(odd_tag)::value;
+                    many_cluster<D, kTerms>(lds + k1, lds + Tiles<D>::kV0 + kOdd * Tiles<D>::kV, gm, qh, ql, s, w, ones, inverse, st);
+                    store_v(lds + Tiles<D>::kV0 + (kOdd ^ 1) * Tiles<D>::kV, p + 1);
+                    const int64_t after = place(p + 3);
+                    load_k(lds + (k1 + 2 * Tiles<D>::kK) % (kKRing * Tiles<D>::kK), after);
+                    load_v(next);
+                    next = after;
+                    softmax_whole(p + 1);
+                    k1 = (k1 + Tiles<D>::kK) % (kKRing * Tiles<D>::kK);
+                    ++p;
+                    // the keys of the next step have landed: all but this step's loads
+                    __builtin_amdgcn_s_waitcnt(vmcnt_imm(2 * kLoads));
+                    __builtin_amdgcn_s_waitcnt(lgkmcnt_imm(0));
+                    wg_barrier();
+                };
+                if ((p - u.first) % 2) step(std::integral_constant<int, 1>{});
 #pragma clang loop unroll(disable)
-            for (; p < to; ++p) {
-                const int k1 = k0 == kKRing - 1 ? 0 : k0 + 1;
-                many_cluster<D, kTerms>(lds + k1 * Tiles<D>::kK, lds + Tiles<D>::kV0 + v0 * Tiles<D>::kV, gm, qh, ql, s, w, ones, st);
-                store_v(lds + Tiles<D>::kV0 + (v0 ^ 1) * Tiles<D>::kV, p + 1);
-                load_k(lds + k0 * Tiles<D>::kK, p + 3);
-                load_v(p + 2);
-                softmax(p + 1, std::false_type{});
-                k0 = k1, v0 ^= 1;
-                // the keys of page p + 2 have landed: all but this step's loads
-                __builtin_amdgcn_s_waitcnt(vmcnt_imm(2 * kLoads));
-                __builtin_amdgcn_s_waitcnt(lgkmcnt_imm(0));
-                wg_barrier();
+                while (p + 1 < to) {
+                    step(std::integral_constant<int, 0>{});
+                    step(std::integral_constant<int, 1>{});
+                }
+                if (p < to) step(std::integral_constant<int, 0>{});
             }
             if (p + 3 - base >= 64 && base + 64 < u.end) continue;  // the window's end
             // One step of another kind: a page that some row sees in part, or the last.
             if (p + 1 < u.end) {
                 qk(p + 1);
                 store_v(v_stage(p + 1), p + 1);
-                if (p + 3 < u.end) load_k(k_stage(p + 3), p + 3);
-                if (p + 2 < u.end) load_v(p + 2);
+                if (p + 3 < u.end) load_k(k_stage(p + 3), place(p + 3));
+                if (p + 2 < u.end) load_v(place(p + 2));
             }
-            many_pv<D>(v_stage(p), gm, w, ones, st);
-            if (p + 1 < u.end) softmax(p + 1, std::true_type{});
+            many_pv<D>(v_stage(p), gm, w, ones, inverse, st);
+            if (p + 1 < u.end) softmax_part(p + 1);
             __builtin_amdgcn_s_waitcnt(0);
             wg_barrier();
             ++p;
