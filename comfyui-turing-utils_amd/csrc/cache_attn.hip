@@ -497,7 +497,14 @@ struct ManyGeom {
 };
 
 // 16-byte pieces of a row are XORed with row bits, so that 16 lanes that read
-// one column of 16 rows meet distinct banks.
+// one column of 16 rows meet distinct banks, and so do lanes that write V^T.
+__device__ __forceinline__ int v_swizzle(int ch) {
+#ifdef OLDSW
+    return (ch >> 1) & 7;
+#else
+    return ((ch >> 1) & 7) ^ (ch & 1);
+#endif
+}
 template <int D>
 __device__ __forceinline__ ManyGeom<D> many_geom(int wave, int lane) {
     ManyGeom<D> gm;
@@ -511,12 +518,12 @@ __device__ __forceinline__ ManyGeom<D> many_geom(int wave, int lane) {
     }
     const int ch = wave * 16 + lane / 4;
 #pragma unroll
-    for (int e = 0; e < 2; ++e) gm.v_wr[e] = static_cast<uint32_t>(ch * 128 + (((2 * (lane % 4) + e) ^ ((ch >> 1) & 7)) << 4));
+    for (int e = 0; e < 2; ++e) gm.v_wr[e] = static_cast<uint32_t>(ch * 128 + (((2 * (lane % 4) + e) ^ v_swizzle(ch)) << 4));
 #pragma unroll
     for (int i = 0; i < D / 64; ++i)
         gm.k_rd[i] = static_cast<uint32_t>(lc * D + (D == 128 ? ((4 * i + g) ^ ((lc >> 1) & 7)) : (g ^ ((lc >> 2) & 3))) * 16);
 #pragma unroll
-    for (int i = 0; i < 2; ++i) gm.v_rd[i] = static_cast<uint32_t>(lc * 128 + (((4 * i + g) ^ ((lc >> 1) & 7)) << 4));
+    for (int i = 0; i < 2; ++i) gm.v_rd[i] = static_cast<uint32_t>(lc * 128 + (((4 * i + g) ^ v_swizzle(lc)) << 4));
     return gm;
 }
 
@@ -847,7 +854,7 @@ __global__ __launch_bounds__(kThreads, 2) void cache_many_kernel(CacheCall call)
     i32x4 s[4][kQT];
     f16x8 w[2][kQT];
     float inverse = kSummed;  // of the page whose weights w holds
-    u32x4 v[kLoads];
+    u32x4 v[2][kLoads];  // values of the next two pages, by parity
     auto at_of = [&](int p) { return min(p, u.end - 1) - base; };
     auto place = [&](int p) {
         return static_cast<int64_t>(max(__builtin_amdgcn_readlane(window.page, at_of(p)), 0)) * hkv + u.hk;
@@ -857,12 +864,12 @@ __global__ __launch_bounds__(kThreads, 2) void cache_many_kernel(CacheCall call)
     auto load_k = [&](int8_t *stage, int64_t at) __attribute__((always_inline)) {
         many_load_k(stage, make_rsrc(k_codes + at * kPage * D, kPage * D), gm, wave);
     };
-    auto load_v = [&](int64_t at) __attribute__((always_inline)) {
+    auto load_v = [&](u32x4 (&v)[kLoads], int64_t at) __attribute__((always_inline)) {
         const int8_t *page = v_codes + at * kPage * D;
 #pragma unroll
         for (int i = 0; i < kLoads; ++i) v[i] = *reinterpret_cast<const u32x4 *>(page + (i * kThreads + threadIdx.x) * 16);
     };
-    auto store_v = [&](int8_t *stage, int p) __attribute__((always_inline)) {
+    auto store_v = [&](int8_t *stage, const u32x4 (&v)[kLoads], int p) __attribute__((always_inline)) {
         many_store_v<D>(stage, gm, v, Selectors::of(lane_value(window.v_log2, p - base) == kZeroValues));
     };
     auto softmax_part = [&](int p) __attribute__((always_inline)) {
@@ -895,15 +902,18 @@ __global__ __launch_bounds__(kThreads, 2) void cache_many_kernel(CacheCall call)
 
     // Step p: QK^T of page p + 1 and PV of page p, then the softmax of page p + 1.
     // Of the rings, keys of p + 3 go into a stage that step p - 2 read last, values of
-    // p + 1 into the one whose page step p - 1 finished; values of p + 2 are loaded
-    // into the registers that those left.  Each load has a step to land.
+    // p + 1 into the one whose page step p - 1 finished; values of p + 3 are loaded
+    // into the registers that those left.  Each load has two steps to land.
+    constexpr std::integral_constant<int, 0> kEven;
+    constexpr std::integral_constant<int, 1> kOdd;
     if (u.first < u.end) {
-        load_v(place(u.first));
+        load_v(v[0], place(u.first));
         load_k(k_stage(u.first), place(u.first));
         load_k(k_stage(u.first + 1), place(u.first + 1));
-        store_v(v_stage(u.first), u.first);
+        store_v(v_stage(u.first), v[0], u.first);
         load_k(k_stage(u.first + 2), place(u.first + 2));
-        load_v(place(u.first + 1));
+        load_v(v[1], place(u.first + 1));
+        load_v(v[0], place(u.first + 2));
         __builtin_amdgcn_s_waitcnt(vmcnt_imm(0));
         __syncthreads();
         qk(u.first);
@@ -920,38 +930,42 @@ __global__ __launch_bounds__(kThreads, 2) void cache_many_kernel(CacheCall call)
             if (none) to = min(to, base + static_cast<int>(__builtin_ctzll(none)) - 1);
             if (p < to) {
                 int k1 = (p + 1 - u.first) % kKRing * Tiles<D>::kK;
-                int64_t next = place(p + 2);
-                auto step = [&](auto odd_tag) __attribute__((always_inline)) {
-                    constexpr int kOdd = decltype(odd_tag)::value;
-                    many_cluster<D, kTerms>(lds + k1, lds + Tiles<D>::kV0 + kOdd * Tiles<D>::kV, gm, qh, ql, s, w, ones, inverse, st);
-                    store_v(lds + Tiles<D>::kV0 + (kOdd ^ 1) * Tiles<D>::kV, p + 1);
-                    const int64_t after = place(p + 3);
-                    load_k(lds + (k1 + 2 * Tiles<D>::kK) % (kKRing * Tiles<D>::kK), after);
-                    load_v(next);
-                    next = after;
+                auto step = [&](auto parity_tag) __attribute__((always_inline)) {
+                    constexpr int kParity = decltype(parity_tag)::value;
+                    many_cluster<D, kTerms>(lds + k1, lds + Tiles<D>::kV0 + kParity * Tiles<D>::kV, gm, qh, ql, s, w, ones, inverse, st);
+                    store_v(lds + Tiles<D>::kV0 + (kParity ^ 1) * Tiles<D>::kV, v[kParity ^ 1], p + 1);
+                    const int64_t next = place(p + 3);
+                    load_k(lds + (k1 + 2 * Tiles<D>::kK) % (kKRing * Tiles<D>::kK), next);
+                    __builtin_amdgcn_sched_barrier(0);  // (the wait below counts on the order)
+                    load_v(v[kParity ^ 1], next);
                     softmax_whole(p + 1);
                     k1 = (k1 + Tiles<D>::kK) % (kKRing * Tiles<D>::kK);
                     ++p;
                     // the keys of the next step have landed: all but this step's loads
-                    __builtin_amdgcn_s_waitcnt(vmcnt_imm(2 * kLoads));
+                    // and the values loaded behind them
+                    __builtin_amdgcn_s_waitcnt(vmcnt_imm(3 * kLoads));
                     __builtin_amdgcn_s_waitcnt(lgkmcnt_imm(0));
                     wg_barrier();
                 };
-                if ((p - u.first) % 2) step(std::integral_constant<int, 1>{});
+                if ((p - u.first) % 2) step(kOdd);
 #pragma clang loop unroll(disable)
                 while (p + 1 < to) {
-                    step(std::integral_constant<int, 0>{});
-                    step(std::integral_constant<int, 1>{});
+                    step(kEven);
+                    step(kOdd);
                 }
-                if (p < to) step(std::integral_constant<int, 0>{});
+                if (p < to) step(kEven);
             }
             if (p + 3 - base >= 64 && base + 64 < u.end) continue;  // the window's end
             // One step of another kind: a page that some row sees in part, or the last.
             if (p + 1 < u.end) {
                 qk(p + 1);
-                store_v(v_stage(p + 1), p + 1);
                 if (p + 3 < u.end) load_k(k_stage(p + 3), place(p + 3));
-                if (p + 2 < u.end) load_v(place(p + 2));
+                auto values = [&](u32x4 (&v)[kLoads]) __attribute__((always_inline)) {
+                    store_v(v_stage(p + 1), v, p + 1);
+                    if (p + 3 < u.end) load_v(v, place(p + 3));
+                };
+                if ((p - u.first) % 2) values(v[0]);
+                else values(v[1]);
             }
             many_pv<D>(v_stage(p), gm, w, ones, inverse, st);
             if (p + 1 < u.end) softmax_part(p + 1);
