@@ -88,16 +88,28 @@ __device__ __forceinline__ Unit unit_of(const CacheCall &c, uint32_t b, uint32_t
     const uint32_t last = min(c.rows, (block + 1) * kRows) - 1;
     const int token = min(static_cast<int>(last / c.group), u.n - 1);
     u.seen = block * kRows < static_cast<uint32_t>(u.n) * c.group ? keys_of(c, token, u.n, u.length) : 0;
-    const int pages = (u.seen + kPage - 1) / kPage, per = (pages + c.parts - 1) / c.parts;
+    // (of the whole sequence: ranges of a causal call's blocks have one size)
+    const int pages = (u.seen + kPage - 1) / kPage, per = ((u.length + kPage - 1) / kPage + c.parts - 1) / c.parts;
     u.first = min(pages, static_cast<int>(z) * per);
     u.end = min(pages, u.first + per);
     u.used = per ? (pages + per - 1) / per : 1;
     return u;
 }
 
+// Units by K/V head, so that the blocks of a head run on one XCD and its L2 reads
+// the head's codes once.  Causal: blocks from the last, longest one on, heads
+// fastest, so that the short ones fill the end.
 template <int kRows>
-__device__ __forceinline__ Unit unit_at(const CacheCall &c, uint32_t id) {
-    const uint32_t z = id % c.parts, rest = id / c.parts, block = rest % c.row_blocks, bh = rest / c.row_blocks;
+__device__ __forceinline__ Unit unit_at(const CacheCall &c) {
+    const uint32_t id = c.causal ? blockIdx.x : xcd_chunk(blockIdx.x, gridDim.x);
+    uint32_t bh, block, z;
+    if (c.causal) {
+        const uint32_t heads = c.batch * c.hkv, rest = id / heads;
+        bh = id % heads, z = rest % c.parts, block = c.row_blocks - 1 - rest / c.parts;
+    } else {
+        const uint32_t rest = id / c.parts;
+        z = id % c.parts, block = rest % c.row_blocks, bh = rest / c.row_blocks;
+    }
     return unit_of<kRows>(c, bh / c.hkv, bh % c.hkv, block, z);
 }
 
@@ -186,24 +198,32 @@ __device__ __forceinline__ float lane_value(float v, int lane) {
     return __int_as_float(__builtin_amdgcn_readlane(__float_as_int(v), lane));
 }
 
-// Pages of a range, 64 at a time: lane i holds the i-th one's place in the pool
-// (-1: none), K scale and log2 of the V scale.
+// Pages of a range, 64 at a time: lane i holds the i-th one's K and V planes' place
+// in the pool, its K scale, log2 of the V scale and the V scale's inverse; a bit
+// each: pages that are none (their place is the first's), and values of zero.
 struct PageWindow {
-    int page;
+    int at;
     float k_scale, v_log2, v_inverse;
+    uint64_t none, zero;
     __device__ __forceinline__ void fetch(const CacheCall &c, const Unit &u, int from, int step, int lane) {
-        const int at = from + step * lane;
         int p = -1;
-        if (at < u.end) p = c.table[static_cast<int64_t>(u.b) * c.width + at];
-        page = p >= 0 && p < c.pages ? p : -1;
-        const int64_t s = static_cast<int64_t>(max(page, 0)) * c.hkv + u.hk;
-        k_scale = c.k_scale[s];
+        if (from + step * lane < u.end) p = c.table[static_cast<int64_t>(u.b) * c.width + from + step * lane];
+        const bool there = p >= 0 && p < c.pages;
+        at = (there ? p : 0) * static_cast<int>(c.hkv) + static_cast<int>(u.hk);
+        none = __ballot(!there);
+        k_scale = c.k_scale[at];
         // (a NaN stays; below 2^-90, where a sum of weights over the scale might be
         // no number, the values count as zeros of that scale)
-        const float v = c.v_scale[s];
+        const float v = c.v_scale[at];
+        zero = __ballot(v <= 8.077935669e-28f);
         v_log2 = v <= 8.077935669e-28f ? kZeroValues : __builtin_amdgcn_logf(v);
         v_inverse = v <= 8.077935669e-28f ? 1.2379400392853803e27f : __builtin_amdgcn_rcpf(v);
+        // (used here, so that the wait for it is here too and not in a loop that uses it)
+        asm volatile("" : "+v"(k_scale));
     }
+    __device__ __forceinline__ int64_t place(int i) const { return __builtin_amdgcn_readlane(at, i); }
+    __device__ __forceinline__ bool there(int i) const { return !(none >> i & 1); }
+    __device__ __forceinline__ bool zeros(int i) const { return zero >> i & 1; }
 };
 
 // The softmax state of a row: base (score, log2 of a V scale), and in the lane
@@ -296,13 +316,13 @@ __global__ __launch_bounds__(kThreads, D == 128 && kRT == 2 ? 1 : 2) void cache_
     __shared__ float merge_m[4][kRT][64][3];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int g = lane >> 4, lc = lane & 15;
-    const Unit u = unit_at<kRows>(c, xcd_chunk(blockIdx.x, gridDim.x));
+    const Unit u = unit_at<kRows>(c);
     if (u.z > 0 && static_cast<int>(u.z) >= u.used) return;  // the whole workgroup: nothing is left for the range
     PageWindow window;
     int base = u.first + wave;  // page of the window's lane 0; the wave's pages are 4 apart
     window.fetch(c, u, base, 4, lane);
     auto place = [&](int p) {  // of page p of the sequence, one of the window's
-        return static_cast<int64_t>(max(__builtin_amdgcn_readlane(window.page, (p - base) >> 2), 0)) * c.hkv + u.hk;
+        return window.place((p - base) >> 2);
     };
     i32x4 qh[kRT][kSl], ql[kRT][kSl];
     float factor[kRT];
@@ -322,7 +342,7 @@ __global__ __launch_bounds__(kThreads, D == 128 && kRT == 2 ? 1 : 2) void cache_
 
     auto compute = [&](const PageRegs<D> &r, int p) {
         const int at = (p - base) >> 2;
-        const bool there = __builtin_amdgcn_readlane(window.page, at) >= 0;
+        const bool there = window.there(at);
         const float k_scale = lane_value(window.k_scale, at), v_log2 = lane_value(window.v_log2, at);
         const int key0 = p * kPage + 16 * g;  // the lane's keys are key0 ..+15
 #pragma unroll
@@ -379,7 +399,7 @@ __global__ __launch_bounds__(kThreads, D == 128 && kRT == 2 ? 1 : 2) void cache_
             }
             // w / v_scale, the scale being 2^(base's + d) (a lane without keys has no part in a NaN)
             if (seen > 0) st[rt].l = __builtin_fmaf(sum, __builtin_amdgcn_exp2f(-(st[rt].v + d)), st[rt].l);
-            if (v_log2 == kZeroValues) continue;
+            if (window.zeros(at)) continue;
 #pragma unroll
             for (int ds = 0; ds < kDS; ++ds) {
 #pragma unroll
@@ -462,13 +482,18 @@ __global__ __launch_bounds__(kThreads, D == 128 && kRT == 2 ? 1 : 2) void cache_
 // ---------------------------------------------------------------------------
 // Many rows
 // ---------------------------------------------------------------------------
-// A workgroup of four waves has 128 rows of one K/V head, 32 a wave; two share a
-// CU, so that one's MFMAs run beside the other's softmax.  Pages stream through
-// LDS: keys as codes by direct-to-LDS loads, a ring of four; values through
-// registers, converted to fp16 once for the four waves, a ring of two.
+// A workgroup has 128 or 256 rows of one K/V head: one or two groups of four waves,
+// 32 rows a wave.  Two groups of 128 share a CU either way; within one workgroup they
+// share the tiles too (half the reads from L2 and conversions of V), and run opposite
+// each other: one's MFMAs beside the other's softmax.  Pages stream through LDS: keys
+// as codes by direct-to-LDS loads, a ring of four; values through registers, converted
+// to fp16 once, a ring of two.
+//   Bound by instruction issue: a wave's step at D = 128 is 832 cycles of MFMAs of the
+// 1300 or so that it takes, and the two waves of a SIMD issue into the rest.  4680 rows
+// x 32760 keys, 40 heads, int8 queries: 2.26 ms, 1390 TFLOP/s (one group: 2.45 ms).
 constexpr int kQT = 2;           // 16-row fragments of a wave
 constexpr int kWaveRows = 16 * kQT;
-constexpr int kManyRows = 4 * kWaveRows;
+constexpr int kGroupRows = 4 * kWaveRows;
 constexpr int kKRing = 4;
 constexpr float kSummed = -1.0f;
 
@@ -478,7 +503,6 @@ struct Tiles {
     static constexpr int kV = kPage * D * 2;  // of a V stage
     static constexpr int kV0 = kKRing * kK;
     static constexpr int kBytes = kV0 + 2 * kV;
-    static constexpr int kKLoads = kK / 4096;  // 16-byte loads of a thread for a page's keys, and for its values
 };
 
 // LDS row of a K tile -> key: within each half of 32, row 16 t + i holds key
@@ -488,30 +512,32 @@ __device__ __forceinline__ int key_of_row(int row) {
     return (row & ~31) + 8 * ((row & 15) >> 2) + 4 * ((row >> 4) & 1) + (row & 3);
 }
 
-template <int D>
+// Loads of 1 KiB that a wave of kWaves has of a page's keys, and of its values (the
+// first waves only, where there are more waves than loads).
+template <int D, int kWaves>
+constexpr int kPieces = Tiles<D>::kK / 1024 >= kWaves ? Tiles<D>::kK / 1024 / kWaves : 1;
+
+template <int D, int kWaves>
 struct ManyGeom {
-    uint32_t k_src[Tiles<D>::kKLoads];  // a lane's 16 bytes of a page's keys
-    uint32_t k_rd[D / 64];              // operand of QK^T
-    uint32_t v_rd[2];                   // operand of PV, half 0 / 1
-    uint32_t v_wr[2];                   // where the two halves of a lane's 16 values go (64 channels on for its next 16)
+    uint32_t k_src[kPieces<D, kWaves>];  // a lane's 16 bytes of a page's keys
+    uint32_t k_rd[D / 64];               // operand of QK^T
+    uint32_t v_rd[2];                    // operand of PV, half 0 / 1
+    uint32_t v_wr[2];                    // where the two halves of a lane's 16 values go
+    static constexpr bool kAll = Tiles<D>::kK / 1024 >= kWaves;
+    bool loads;                          // whether the wave loads (kAll: every one does)
 };
 
 // 16-byte pieces of a row are XORed with row bits, so that 16 lanes that read
 // one column of 16 rows meet distinct banks, and so do lanes that write V^T.
-__device__ __forceinline__ int v_swizzle(int ch) {
-#ifdef OLDSW
-    return (ch >> 1) & 7;
-#else
-    return ((ch >> 1) & 7) ^ (ch & 1);
-#endif
-}
-template <int D>
-__device__ __forceinline__ ManyGeom<D> many_geom(int wave, int lane) {
-    ManyGeom<D> gm;
+__device__ __forceinline__ int v_swizzle(int ch) { return ((ch >> 1) & 7) ^ (ch & 1); }
+template <int D, int kWaves>
+__device__ __forceinline__ ManyGeom<D, kWaves> many_geom(int wave, int lane) {
+    ManyGeom<D, kWaves> gm;
     const int g = lane >> 4, lc = lane & 15;
+    gm.loads = wave < Tiles<D>::kK / 1024;
 #pragma unroll
-    for (int i = 0; i < Tiles<D>::kKLoads; ++i) {
-        const int piece = (Tiles<D>::kKLoads * wave + i) * 64 + lane;  // of 16 bytes in LDS
+    for (int i = 0; i < kPieces<D, kWaves>; ++i) {
+        const int piece = (kPieces<D, kWaves> * wave + i) * 64 + lane;  // of 16 bytes in LDS
         const int row = piece / (D / 16), at = piece % (D / 16);
         const int swizzle = D == 128 ? (row >> 1) & 7 : (row >> 2) & 3;
         gm.k_src[i] = static_cast<uint32_t>(key_of_row(row) * D + (at ^ swizzle) * 16);
@@ -735,8 +761,8 @@ __device__ __forceinline__ float whole_weights(i32x4 (&s)[4][kQT], const float (
 }
 
 // O^T += V^T w and the sum of the tile's weights, times `inverse` (see whole_weights).
-template <int D>
-__device__ __forceinline__ void many_pv(const int8_t *stage, const ManyGeom<D> &gm, const f16x8 (&w)[2][kQT], const f16x8 &ones,
+template <int D, int kWaves>
+__device__ __forceinline__ void many_pv(const int8_t *stage, const ManyGeom<D, kWaves> &gm, const f16x8 (&w)[2][kQT], const f16x8 &ones,
                                         float inverse, ManyState<D> &st) {
     f32x4 sum[kQT];
 #pragma unroll
@@ -760,8 +786,8 @@ __device__ __forceinline__ void many_pv(const int8_t *stage, const ManyGeom<D> &
 }
 
 // A steady step's MFMAs: QK^T of one page, PV of the page before it.
-template <int D, bool kTerms>
-__device__ __forceinline__ void many_cluster(const int8_t *k_stage, const int8_t *v_stage, const ManyGeom<D> &gm,
+template <int D, bool kTerms, int kWaves>
+__device__ __forceinline__ void many_cluster(const int8_t *k_stage, const int8_t *v_stage, const ManyGeom<D, kWaves> &gm,
                                              const i32x4 (&qh)[kQT][D / 64], const i32x4 (&ql)[kQT][D / 64],
                                              i32x4 (&s)[4][kQT], const f16x8 (&w)[2][kQT], const f16x8 &ones,
                                              float inverse, ManyState<D> &st) {
@@ -788,46 +814,57 @@ __device__ __forceinline__ void many_cluster(const int8_t *k_stage, const int8_t
 }
 
 // A page's keys into a ring stage; its values into registers, and from there into one.
-#define TU_MANY_LOAD_K(D)                                                                                              \
-    __device__ __forceinline__ void many_load_k(int8_t *stage, __amdgpu_buffer_rsrc_t rs, const ManyGeom<D> &gm, int wave) {     \
-        _Pragma("unroll") for (int i = 0; i < Tiles<D>::kKLoads; ++i)                                                  \
-            __builtin_amdgcn_raw_ptr_buffer_load_lds(rs, (lds_void *)(stage + (Tiles<D>::kKLoads * wave + i) * 1024), 16, \
-                                                     gm.k_src[i], 0, 0, 0);                                            \
+// (One overload for each, as the host's pass takes no template of the load.)
+#define TU_MANY_LOAD_K(D, WAVES)                                                                                       \
+    __device__ __forceinline__ void many_load_k(int8_t *stage, __amdgpu_buffer_rsrc_t rs, const ManyGeom<D, WAVES> &gm,  \
+                                                int wave) {                                                            \
+        constexpr int kN = kPieces<D, WAVES>;                                                                          \
+        _Pragma("unroll") for (int i = 0; i < kN; ++i)                                                                 \
+            __builtin_amdgcn_raw_ptr_buffer_load_lds(rs, (lds_void *)(stage + (kN * wave + i) * 1024), 16, gm.k_src[i], 0, 0, 0); \
     }
-TU_MANY_LOAD_K(128)
-TU_MANY_LOAD_K(64)
+TU_MANY_LOAD_K(128, 4)
+TU_MANY_LOAD_K(64, 4)
+TU_MANY_LOAD_K(128, 8)
+TU_MANY_LOAD_K(64, 8)
 #undef TU_MANY_LOAD_K
 
-template <int D>
-__device__ __forceinline__ void many_store_v(int8_t *stage, const ManyGeom<D> &gm, const u32x4 (&v)[Tiles<D>::kKLoads],
+// The compiler would wait for every load in flight before a write to LDS, as loads of
+// keys write there too (never to these places); so the writes are spelled out, and
+// the wait for them stands before the barrier that hands them over.
+__device__ __forceinline__ void write_lds(uint32_t at, u32x4 x) {
+    asm volatile("ds_write_b128 %0, %1" ::"v"(at), "v"(x) : "memory");
+}
+template <int D, int kWaves>
+__device__ __forceinline__ void many_store_v(uint32_t stage, const ManyGeom<D, kWaves> &gm, const u32x4 (&v)[kPieces<D, kWaves>],
                                              const Selectors &sel) {
 #pragma unroll
-    for (int i = 0; i < Tiles<D>::kKLoads; ++i)
+    for (int i = 0; i < kPieces<D, kWaves>; ++i)
 #pragma unroll
         for (int e = 0; e < 2; ++e) {
             const u32x2 a = codes_to_f16(v[i][2 * e], sel), b = codes_to_f16(v[i][2 * e + 1], sel);
-            *reinterpret_cast<u32x4 *>(stage + gm.v_wr[e] + i * (kThreads / 4 * 128)) = u32x4{a[0], a[1], b[0], b[1]};
+            write_lds(stage + gm.v_wr[e] + i * (16 * kWaves * 128), u32x4{a[0], a[1], b[0], b[1]});
         }
 }
 
-template <int D, bool kTerms>
-__global__ __launch_bounds__(kThreads, 2) void cache_many_kernel(CacheCall call) {
-    constexpr int kSl = D / 64, kDS = D / 16, kLoads = Tiles<D>::kKLoads;
+template <int D, bool kTerms, int kGroups>
+__global__ __launch_bounds__(256 * kGroups, 2 / kGroups) void cache_many_kernel(CacheCall call) {
+    constexpr int kSl = D / 64, kDS = D / 16, kWaves = 4 * kGroups, kLoads = kPieces<D, kWaves>, kRows = kGroupRows * kGroups;
     __shared__ __align__(1024) int8_t lds[Tiles<D>::kBytes];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int g = lane >> 4, lc = lane & 15;
-    const Unit u = unit_at<kManyRows>(call, xcd_chunk(blockIdx.x, gridDim.x));
+    const int group = wave >> 2;
+    const Unit u = unit_at<kRows>(call);
     if (u.z > 0 && static_cast<int>(u.z) >= u.used) return;  // the whole workgroup: nothing is left for the range
     PageWindow window;
     int base = u.first;
     window.fetch(call, u, base, 1, lane);
-    const ManyGeom<D> gm = many_geom<D>(wave, lane);
+    const ManyGeom<D, kWaves> gm = many_geom<D, kWaves>(wave, lane);
 
     i32x4 qh[kQT][kSl], ql[kQT][kSl];
     float factor[kQT];
     int limit[kQT];
     ManyState<D> st;
-    const uint32_t row0 = u.block * kManyRows + wave * kWaveRows;
+    const uint32_t row0 = u.block * kRows + wave * kWaveRows;
     st.init();
     float most = 0.0f;
 #pragma unroll
@@ -849,33 +886,33 @@ __global__ __launch_bounds__(kThreads, 2) void cache_many_kernel(CacheCall call)
 #pragma unroll
     for (int e = 0; e < 8; ++e) ones[e] = static_cast<_Float16>(1.0f);
     const int8_t *k_codes = call.k_codes, *v_codes = call.v_codes;
-    const uint32_t hkv = call.hkv;
+    const uint32_t lds_at = static_cast<uint32_t>(reinterpret_cast<uintptr_t>((__attribute__((address_space(3))) int8_t *)lds));
 
     i32x4 s[4][kQT];
     f16x8 w[2][kQT];
     float inverse = kSummed;  // of the page whose weights w holds
     u32x4 v[2][kLoads];  // values of the next two pages, by parity
     auto at_of = [&](int p) { return min(p, u.end - 1) - base; };
-    auto place = [&](int p) {
-        return static_cast<int64_t>(max(__builtin_amdgcn_readlane(window.page, at_of(p)), 0)) * hkv + u.hk;
-    };
+    auto place = [&](int p) { return window.place(at_of(p)); };
     auto k_stage = [&](int p) { return lds + (p - u.first) % kKRing * Tiles<D>::kK; };
     auto v_stage = [&](int p) { return lds + Tiles<D>::kV0 + (p - u.first) % 2 * Tiles<D>::kV; };
     auto load_k = [&](int8_t *stage, int64_t at) __attribute__((always_inline)) {
-        many_load_k(stage, make_rsrc(k_codes + at * kPage * D, kPage * D), gm, wave);
+        if (gm.kAll || gm.loads) many_load_k(stage, make_rsrc(k_codes + at * kPage * D, kPage * D), gm, wave);
     };
     auto load_v = [&](u32x4 (&v)[kLoads], int64_t at) __attribute__((always_inline)) {
         const int8_t *page = v_codes + at * kPage * D;
+        if (!gm.kAll && !gm.loads) return;
 #pragma unroll
-        for (int i = 0; i < kLoads; ++i) v[i] = *reinterpret_cast<const u32x4 *>(page + (i * kThreads + threadIdx.x) * 16);
+        for (int i = 0; i < kLoads; ++i) v[i] = *reinterpret_cast<const u32x4 *>(page + (i * 64 * kWaves + threadIdx.x) * 16);
     };
-    auto store_v = [&](int8_t *stage, const u32x4 (&v)[kLoads], int p) __attribute__((always_inline)) {
-        many_store_v<D>(stage, gm, v, Selectors::of(lane_value(window.v_log2, p - base) == kZeroValues));
+    auto store_v = [&](int parity, const u32x4 (&v)[kLoads], int p) __attribute__((always_inline)) {
+        if (gm.kAll || gm.loads)
+            many_store_v<D>(lds_at + Tiles<D>::kV0 + parity * Tiles<D>::kV, gm, v, Selectors::of(window.zeros(p - base)));
     };
     auto softmax_part = [&](int p) __attribute__((always_inline)) {
         const int at = p - base;
         const float k_scale = lane_value(window.k_scale, at), v_log2 = lane_value(window.v_log2, at);
-        const bool there = __builtin_amdgcn_readlane(window.page, at) >= 0;
+        const bool there = window.there(at);
         float f[kQT];
         int seen[kQT];
 #pragma unroll
@@ -901,23 +938,35 @@ __global__ __launch_bounds__(kThreads, 2) void cache_many_kernel(CacheCall call)
     };
 
     // Step p: QK^T of page p + 1 and PV of page p, then the softmax of page p + 1.
-    // Of the rings, keys of p + 3 go into a stage that step p - 2 read last, values of
-    // p + 1 into the one whose page step p - 1 finished; values of p + 3 are loaded
-    // into the registers that those left.  Each load has two steps to land.
+    // Interval p, between two barriers, has for group 0 step p, and for group 1 the
+    // softmax of page p and the MFMAs of step p: the groups' MFMAs and softmaxes stand
+    // opposite each other on a SIMD.  In interval p keys of p + 1 and values of p are
+    // read from LDS, values of p + 1 converted into the stage that interval p - 1 read
+    // last, and keys of p + 3 and values of p + 3 (into the registers that those of p +
+    // 1 left) loaded: each load has two intervals to land.
     constexpr std::integral_constant<int, 0> kEven;
     constexpr std::integral_constant<int, 1> kOdd;
+    auto landed = [&] __attribute__((always_inline)) {
+        // the keys that the next interval reads: all but this one's loads and the
+        // values loaded behind them
+        __builtin_amdgcn_s_waitcnt(vmcnt_imm(3 * kLoads));
+        __builtin_amdgcn_s_waitcnt(lgkmcnt_imm(0));
+        wg_barrier();
+    };
     if (u.first < u.end) {
         load_v(v[0], place(u.first));
         load_k(k_stage(u.first), place(u.first));
         load_k(k_stage(u.first + 1), place(u.first + 1));
-        store_v(v_stage(u.first), v[0], u.first);
+        store_v(0, v[0], u.first);
         load_k(k_stage(u.first + 2), place(u.first + 2));
         load_v(v[1], place(u.first + 1));
         load_v(v[0], place(u.first + 2));
-        __builtin_amdgcn_s_waitcnt(vmcnt_imm(0));
+        __builtin_amdgcn_s_waitcnt(0);
         __syncthreads();
         qk(u.first);
-        softmax_part(u.first);
+        if (kGroups == 1 || group == 0) softmax_part(u.first);
+        if (kGroups == 2) wg_barrier();
+        if (kGroups == 2 && group == 1) softmax_part(u.first);
         for (int p = u.first; p < u.end;) {
             if (p + 3 - base >= 64 && base + 64 < u.end) {
                 base = p;
@@ -925,28 +974,32 @@ __global__ __launch_bounds__(kThreads, 2) void cache_many_kernel(CacheCall call)
             }
             // steps whose next page every row sees whole: up to the first that is none,
             // and as far as the window reaches three pages on
-            const uint64_t none = __ballot(window.page < 0) & (p + 1 - base < 64 ? ~0ull << (p + 1 - base) : 0);
+            const uint64_t none = window.none & (p + 1 - base < 64 ? ~0ull << (p + 1 - base) : 0);
             int to = min(min(u.end, whole) - 1, base + 64 < u.end ? base + 61 : u.end);
             if (none) to = min(to, base + static_cast<int>(__builtin_ctzll(none)) - 1);
+            // the loads of interval p, and the values it converts
+            auto feed = [&](auto parity_tag, int8_t *k_to) __attribute__((always_inline)) {
+                constexpr int kParity = decltype(parity_tag)::value;
+                store_v(kParity ^ 1, v[kParity ^ 1], min(p + 1, u.end - 1));
+                const int64_t next = place(p + 3);
+                load_k(k_to, next);
+                __builtin_amdgcn_sched_barrier(0);  // (the wait before the barrier counts on the order)
+                load_v(v[kParity ^ 1], next);
+            };
             if (p < to) {
                 int k1 = (p + 1 - u.first) % kKRing * Tiles<D>::kK;
                 auto step = [&](auto parity_tag) __attribute__((always_inline)) {
                     constexpr int kParity = decltype(parity_tag)::value;
                     many_cluster<D, kTerms>(lds + k1, lds + Tiles<D>::kV0 + kParity * Tiles<D>::kV, gm, qh, ql, s, w, ones, inverse, st);
-                    store_v(lds + Tiles<D>::kV0 + (kParity ^ 1) * Tiles<D>::kV, v[kParity ^ 1], p + 1);
-                    const int64_t next = place(p + 3);
-                    load_k(lds + (k1 + 2 * Tiles<D>::kK) % (kKRing * Tiles<D>::kK), next);
-                    __builtin_amdgcn_sched_barrier(0);  // (the wait below counts on the order)
-                    load_v(v[kParity ^ 1], next);
+                    feed(parity_tag, lds + (k1 + 2 * Tiles<D>::kK) % (kKRing * Tiles<D>::kK));
+                    if (kGroups == 2 && group == 1) landed();
                     softmax_whole(p + 1);
                     k1 = (k1 + Tiles<D>::kK) % (kKRing * Tiles<D>::kK);
                     ++p;
-                    // the keys of the next step have landed: all but this step's loads
-                    // and the values loaded behind them
-                    __builtin_amdgcn_s_waitcnt(vmcnt_imm(3 * kLoads));
-                    __builtin_amdgcn_s_waitcnt(lgkmcnt_imm(0));
-                    wg_barrier();
+                    if (kGroups == 1 || group == 0) landed();
                 };
+                // (without it the compiler's waits inside would be for other ways to here)
+                __builtin_amdgcn_s_waitcnt(vmcnt_imm(0));
                 if ((p - u.first) % 2) step(kOdd);
 #pragma clang loop unroll(disable)
                 while (p + 1 < to) {
@@ -957,22 +1010,16 @@ __global__ __launch_bounds__(kThreads, 2) void cache_many_kernel(CacheCall call)
             }
             if (p + 3 - base >= 64 && base + 64 < u.end) continue;  // the window's end
             // One step of another kind: a page that some row sees in part, or the last.
-            if (p + 1 < u.end) {
-                qk(p + 1);
-                if (p + 3 < u.end) load_k(k_stage(p + 3), place(p + 3));
-                auto values = [&](u32x4 (&v)[kLoads]) __attribute__((always_inline)) {
-                    store_v(v_stage(p + 1), v, p + 1);
-                    if (p + 3 < u.end) load_v(v, place(p + 3));
-                };
-                if ((p - u.first) % 2) values(v[0]);
-                else values(v[1]);
-            }
+            if (p + 1 < u.end) qk(p + 1);
+            if ((p - u.first) % 2) feed(kOdd, k_stage(p + 3));
+            else feed(kEven, k_stage(p + 3));
             many_pv<D>(v_stage(p), gm, w, ones, inverse, st);
+            if (kGroups == 2 && group == 1) landed();
             if (p + 1 < u.end) softmax_part(p + 1);
-            __builtin_amdgcn_s_waitcnt(0);
-            wg_barrier();
+            if (kGroups == 1 || group == 0) landed();
             ++p;
         }
+        __builtin_amdgcn_s_waitcnt(vmcnt_imm(0));  // (loads past the range's end into LDS)
     }
     // (the call's fields are read again, not kept through the loop)
     auto *again = (const CacheCall *)__builtin_amdgcn_kernarg_segment_ptr();
@@ -990,42 +1037,28 @@ __global__ __launch_bounds__(kThreads, 2) void cache_many_kernel(CacheCall call)
 // ---------------------------------------------------------------------------
 // The merge
 // ---------------------------------------------------------------------------
-// A row's ranges: D / 8 threads a row, 8 channels each.  A range that saw none of
-// the row's keys has a sum of 0 and is left out; a NaN stays.
-template <int D, int kRows>
-__global__ __launch_bounds__(kThreads) void cache_merge_kernel(CacheCall c) {
-    constexpr int kTpr = D / 8;
-    const int64_t rows = static_cast<int64_t>(c.batch) * c.hkv * c.rows;
-    const int64_t at = static_cast<int64_t>(blockIdx.x) * (kThreads / kTpr) + threadIdx.x / kTpr;
-    if (at >= rows) return;
-    const uint32_t bh = static_cast<uint32_t>(at / c.rows), r = static_cast<uint32_t>(at % c.rows);
-    const Unit u = unit_of<kRows>(c, bh / c.hkv, bh % c.hkv, r / kRows, 0);
-    if (u.used <= 1) return;
-    const Row row = row_at(c, u.hk, r);
-    const int d0 = (threadIdx.x % kTpr) * 8;
+// A row's ranges: D / 8 threads for each, 8 channels a thread.  A range that saw
+// none of the row's keys has a sum of 0 and is left out; a NaN stays.  With few rows
+// a call has too few threads for one to walk a row's ranges (32 of them took 9.2 us
+// at 64 rows, D = 128): a workgroup has one row then, and kTurns = kThreads / (D / 8)
+// ranges at a time.
+struct MergeState {
     float m = kNoBase, v = 0.0f, l = 0.0f, acc[8] = {};
-    constexpr int kAhead = 4;  // ranges whose loads are in flight together
-    for (int z0 = 0; z0 < u.used; z0 += kAhead) {
-        f32x4 x[kAhead], a[kAhead], b[kAhead];
-#pragma unroll
-        for (int i = 0; i < kAhead; ++i) {
-            const int64_t from = min(z0 + i, u.used - 1) * rows + at;
-            x[i] = *reinterpret_cast<const f32x4 *>(c.part_m + from * 4);
-            a[i] = *reinterpret_cast<const f32x4 *>(c.part_o + from * D + d0);
-            b[i] = *reinterpret_cast<const f32x4 *>(c.part_o + from * D + d0 + 4);
-        }
+    // kN ranges' states (m, v, l) and 8 channels of their sums
+    template <int kN>
+    __device__ __forceinline__ void add(const f32x4 (&x)[kN], const f32x4 (&a)[kN], const f32x4 (&b)[kN], int there) {
         float m_new = m, v_new = v;
 #pragma unroll
-        for (int i = 0; i < kAhead; ++i)
-            if (x[i][2] != 0.0f && higher(x[i][0], x[i][1], m_new, v_new)) m_new = x[i][0], v_new = x[i][1];
+        for (int i = 0; i < kN; ++i)
+            if (i < there && x[i][2] != 0.0f && higher(x[i][0], x[i][1], m_new, v_new)) m_new = x[i][0], v_new = x[i][1];
         const float old = l == 0.0f ? 0.0f : __builtin_amdgcn_exp2f((m - m_new) + (v - v_new));
         m = m_new, v = v_new;
         l *= old;
 #pragma unroll
         for (int e = 0; e < 8; ++e) acc[e] = old == 0.0f ? 0.0f : acc[e] * old;
 #pragma unroll
-        for (int i = 0; i < kAhead; ++i) {
-            if (z0 + i >= u.used || x[i][2] == 0.0f) continue;
+        for (int i = 0; i < kN; ++i) {
+            if (i >= there || x[i][2] == 0.0f) continue;
             const float wi = __builtin_amdgcn_exp2f((x[i][0] - m) + (x[i][1] - v));
             l = __builtin_fmaf(wi, x[i][2], l);
 #pragma unroll
@@ -1035,12 +1068,58 @@ __global__ __launch_bounds__(kThreads) void cache_merge_kernel(CacheCall c) {
             }
         }
     }
-    const bool some = l != 0.0f && row.token < u.n;
-    const float inv = 1.0f / l;
+};
+
+template <int D, int kRows, int kTurns>
+__global__ __launch_bounds__(kThreads) void cache_merge_kernel(CacheCall c) {
+    constexpr int kTpr = D / 8;
+    const int64_t rows = static_cast<int64_t>(c.batch) * c.hkv * c.rows;
+    const int turn = kTurns > 1 ? threadIdx.x / kTpr : 0;
+    const int64_t at = kTurns > 1 ? blockIdx.x : static_cast<int64_t>(blockIdx.x) * (kThreads / kTpr) + threadIdx.x / kTpr;
+    if (at >= rows) return;
+    const uint32_t bh = static_cast<uint32_t>(at / c.rows), r = static_cast<uint32_t>(at % c.rows);
+    const Unit u = unit_of<kRows>(c, bh / c.hkv, bh % c.hkv, r / kRows, 0);
+    if (u.used <= 1) return;
+    const Row row = row_at(c, u.hk, r);
+    const int d0 = (threadIdx.x % kTpr) * 8;
+    MergeState st;
+    constexpr int kAhead = kTurns > 1 ? 2 : 4;  // ranges whose loads are in flight together
+    for (int z0 = turn; z0 < u.used; z0 += kAhead * kTurns) {
+        f32x4 x[kAhead], a[kAhead], b[kAhead];
+#pragma unroll
+        for (int i = 0; i < kAhead; ++i) {
+            const int64_t from = min(z0 + i * kTurns, u.used - 1) * rows + at;
+            x[i] = *reinterpret_cast<const f32x4 *>(c.part_m + from * 4);
+            a[i] = *reinterpret_cast<const f32x4 *>(c.part_o + from * D + d0);
+            b[i] = *reinterpret_cast<const f32x4 *>(c.part_o + from * D + d0 + 4);
+        }
+        st.add(x, a, b, (u.used - z0 + kTurns - 1) / kTurns);
+    }
+    if constexpr (kTurns > 1) {
+        __shared__ __align__(16) f32x4 all[3][kTurns][kTpr];
+        all[0][turn][threadIdx.x % kTpr] = f32x4{st.m, st.v, st.l, 0.0f};
+        all[1][turn][threadIdx.x % kTpr] = f32x4{st.acc[0], st.acc[1], st.acc[2], st.acc[3]};
+        all[2][turn][threadIdx.x % kTpr] = f32x4{st.acc[4], st.acc[5], st.acc[6], st.acc[7]};
+        __syncthreads();
+        if (turn > 0) return;
+        constexpr int kStep = 4;
+#pragma unroll
+        for (int t = 1; t < kTurns; t += kStep) {
+            f32x4 x[kStep], a[kStep], b[kStep];
+#pragma unroll
+            for (int i = 0; i < kStep; ++i) {
+                const int from = min(t + i, kTurns - 1);
+                x[i] = all[0][from][threadIdx.x], a[i] = all[1][from][threadIdx.x], b[i] = all[2][from][threadIdx.x];
+            }
+            st.add(x, a, b, kTurns - t);
+        }
+    }
+    const bool some = st.l != 0.0f && row.token < u.n;
+    const float inv = 1.0f / st.l;
     u32x4 out;
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
-        const float p = acc[2 * e] * inv, q = acc[2 * e + 1] * inv;
+        const float p = st.acc[2 * e] * inv, q = st.acc[2 * e + 1] * inv;
         out[e] = some ? (c.out_fp16 ? hw_f16x2_bits(p, q) : hw_bf16x2_bits(p, q)) : 0;
     }
     auto *dst = reinterpret_cast<u32x2 *>(c.o + u.b * c.o_sb + row.head * c.o_sh + row.token * c.o_sl + d0);
@@ -1052,22 +1131,68 @@ __global__ __launch_bounds__(kThreads) void cache_merge_kernel(CacheCall c) {
 // The plan
 // ---------------------------------------------------------------------------
 struct CachePlan {
-    int32_t rows;  // of a row block: 16, 32 or 128
+    int32_t rows;  // of a row block: 16 or 32 (few rows), 128 or 256 (many)
     uint32_t row_blocks, parts;
 };
 
-CachePlan cache_plan(int64_t batch, int64_t hkv, int64_t rows, int64_t dim, int64_t max_pages, int64_t cus, int64_t max_bytes) {
-    CachePlan p{};
-    p.rows = rows <= 16 ? 16 : rows <= 32 ? 32 : kManyRows;
-    p.row_blocks = static_cast<uint32_t>((rows + p.rows - 1) / p.rows);
-    p.parts = 1;
-    const int64_t units = batch * hkv * p.row_blocks, slots = 2 * cus;
-    const int64_t least = p.rows == kManyRows ? 8 : 4;  // pages of a range
-    int64_t parts = std::min<int64_t>((slots + units - 1) / units, (max_pages + least - 1) / least);
+// Ranges of a launch of few rows: as many as its workgroups have places at once (two
+// a CU, or one for 32 rows at D = 128), each of at least one page for every wave.  One
+// more would begin a second round: 131040 keys, 40 heads: 12 ranges 235 us, 13 319.
+// One workgroup a CU reads as fast as two (32 x 8 heads: 1 range 82, 2 ranges 87),
+// and up to 12 pages a merge costs more than it saves (513 keys at D = 64: 7.5, 9.9).
+int64_t few_parts(int64_t units, int64_t pages, int64_t slots, int64_t cus) {
+    return units >= cus || pages <= 12 ? 1 : std::min(slots / units, (pages + 3) / 4);
+}
+
+// Time of a launch of many rows, in steps of a page at 256 rows (1.6 us at D = 128).
+// Blocks of 128 rows run two to a CU, a step 1.08 of that for both, or 0.78 where
+// a CU has one; blocks of 256 run one to a CU.  A unit costs 4 steps over its pages, a
+// merge 3 and its bytes, 7 MB a step (at 256 CUs).
+//   Measured, us, 128 / 256 rows a block: 4680 rows x 32760 keys, 40 heads, int8
+// queries 2450 / 2240; 33 rows x 4 heads a K/V head, 8192 keys, 16 ranges 30.5 /
+// 34.8; 1560 x 9360, 12 heads, by ranges: 1: 184 / 214, 2: 133 / 125, 3: 99 / 97,
+// 4: 120 / 133, 6: 111 / 111.
+//   Causal: empty ranges of early blocks end at once, and long blocks go first.
+// 4001 x 4001, 2 x 16 heads: 1 range 143, 2 ranges 224; 2050 x 6000 at D = 64, 18
+// heads, 128 rows a block: 123, 87.
+double many_cost(int64_t units, int64_t parts, int64_t pages, double share, bool causal, bool one_a_cu, double part_bytes,
+                 int64_t cus) {
+    const int64_t slots = one_a_cu ? cus : 2 * cus;
+    const double n = static_cast<double>(units * parts) * share, full = n / static_cast<double>(slots);
+    const double rounds = full <= 1.0 ? 1.0 : causal ? full + 0.5 : static_cast<double>((units * parts + slots - 1) / slots);
+    const double step = one_a_cu ? 1.0 : n <= static_cast<double>(cus) ? 0.78 : 1.08;
+    const double per = static_cast<double>((pages + parts - 1) / parts);
+    const double merge = parts > 1 ? 3.0 + static_cast<double>(parts) * part_bytes * 2.0 / (7e6 * static_cast<double>(cus) / 256.0) : 0.0;
+    return rounds * (per + 4.0) * step + merge;
+}
+
+CachePlan cache_plan(int64_t batch, int64_t hkv, int64_t lq, int64_t group, int64_t dim, int64_t pages, bool causal, int64_t cus,
+                     int64_t max_bytes) {
+    const int64_t rows = lq * group;
     const int64_t row_bytes = batch * hkv * rows * (dim + 4) * static_cast<int64_t>(sizeof(float));
-    parts = std::min<int64_t>(parts, max_bytes / row_bytes);
-    if (parts > 1) p.parts = static_cast<uint32_t>(parts);
-    return p;
+    const int64_t most = std::min<int64_t>(max_bytes / row_bytes, 256);
+    auto plan = [&](int32_t block, int64_t parts) {
+        return CachePlan{block, static_cast<uint32_t>((rows + block - 1) / block), static_cast<uint32_t>(std::max<int64_t>(parts, 1))};
+    };
+    if (rows <= 32) {
+        const int64_t slots = rows > 16 && dim == 128 ? cus : 2 * cus;
+        return plan(rows <= 16 ? 16 : 32, std::min(few_parts(batch * hkv, pages, slots, cus), most));
+    }
+    // of a causal call's keys, the part that its mean row sees
+    const double tokens = static_cast<double>(pages * kPage);
+    const double share = causal ? std::max(0.5, 1.0 - 0.5 * static_cast<double>(lq) / tokens) : 1.0;
+    CachePlan best{};
+    double best_cost = 0.0;
+    for (const int32_t block : {256, 128}) {
+        const CachePlan one = plan(block, 1);
+        const int64_t units = batch * hkv * one.row_blocks;
+        for (int64_t parts = 1; parts == 1 || (parts <= std::min<int64_t>(most, 64) && 2 * parts <= pages && units * (parts - 1) < 4 * cus);
+             ++parts) {
+            const double cost = many_cost(units, parts, pages, share, causal, block == 256, static_cast<double>(row_bytes), cus);
+            if (!best.rows || cost < best_cost) best = plan(block, parts), best_cost = cost;
+        }
+    }
+    return best;
 }
 
 int64_t cache_workspace(const CachePlan &p, int64_t batch, int64_t hkv, int64_t rows, int64_t dim) {
@@ -1078,11 +1203,11 @@ int64_t cache_workspace(const CachePlan &p, int64_t batch, int64_t hkv, int64_t 
 }  // namespace tu
 
 extern "C" int64_t tu_kv_cache_attn_workspace(int64_t batch, int64_t hq, int64_t hkv, int64_t lq, int64_t dim, int64_t max_length,
-                                              int32_t cus) {
+                                              int32_t causal, int32_t cus) {
     using namespace tu;
     if (batch <= 0 || hkv <= 0 || hq < hkv || lq <= 0 || dim <= 0 || max_length <= 0 || cus <= 0) return 0;
-    const int64_t rows = lq * (hq / hkv), pages = (max_length + kPage - 1) / kPage;
-    return cache_workspace(cache_plan(batch, hkv, rows, dim, pages, cus, INT64_MAX), batch, hkv, rows, dim);
+    const int64_t group = hq / hkv, pages = (max_length + kPage - 1) / kPage;
+    return cache_workspace(cache_plan(batch, hkv, lq, group, dim, pages, causal != 0, cus, INT64_MAX), batch, hkv, lq * group, dim);
 }
 
 extern "C" int32_t tu_kv_cache_attn(const void *q, const float *q_scale, int32_t q_type, int64_t blkq, const int8_t *k_codes,
@@ -1100,6 +1225,7 @@ extern "C" int32_t tu_kv_cache_attn(const void *q, const float *q_scale, int32_t
                "cache attention sizes out of range");
     TU_REQUIRE(width > 0 && width <= 0x7fffffff / kPage - 1 && pages > 0 && pages <= 0x7fffffff,
                "cache attention block table or page count out of range");
+    TU_REQUIRE(pages * hkv <= 0x7fffffff, "cache attention: pages of all heads out of range");
     TU_REQUIRE(q && k_codes && v_codes && k_scale && v_scale && block_table && lengths && o && (q_scale || q_type != kQInt8),
                "cache attention pointers must be non-null");
     TU_REQUIRE(q_type != kQInt8 || (blkq > 0 && blkq <= 0x7fffffff), "cache attention needs blkq > 0");
@@ -1112,8 +1238,8 @@ extern "C" int32_t tu_kv_cache_attn(const void *q, const float *q_scale, int32_t
                "cache attention codes and output must be aligned");
     TU_REQUIRE((reinterpret_cast<uintptr_t>(workspace) & 15) == 0, "cache attention workspace must be 16-byte aligned");
     const int64_t rows = lq * (hq / hkv);
-    const CachePlan plan = cache_plan(batch, hkv, rows, dim, std::min<int64_t>((max_length + kPage - 1) / kPage, width), cus,
-                                      workspace ? workspace_bytes : 0);
+    const CachePlan plan = cache_plan(batch, hkv, lq, hq / hkv, dim, std::min<int64_t>((max_length + kPage - 1) / kPage, width),
+                                      causal != 0, cus, workspace ? workspace_bytes : 0);
     const int64_t units = batch * hkv * plan.row_blocks * plan.parts;
     constexpr int64_t kMost = 0x7fffffff;
     TU_REQUIRE(units <= kMost && batch * hkv * rows <= kMost * 16, "cache attention grid too large");
@@ -1136,22 +1262,34 @@ extern "C" int32_t tu_kv_cache_attn(const void *q, const float *q_scale, int32_t
     c.part_m = c.part_o + plan.parts * batch * hkv * rows * dim;
     hipStream_t s = static_cast<hipStream_t>(stream);
     const dim3 grid(static_cast<unsigned>(units));
+    // (the merge of many rows: one thread walks a row's few ranges)
+#define TU_CACHE_MERGE(D, ROWS, TURNS)                                                                                 \
+    do {                                                                                                               \
+        constexpr int64_t kRowsPerWg = TURNS > 1 ? 1 : kThreads / (D / 8);                                             \
+        const dim3 merge(static_cast<unsigned>((batch * hkv * rows + kRowsPerWg - 1) / kRowsPerWg));                   \
+        if (plan.parts > 1) cache_merge_kernel<D, ROWS, TURNS><<<merge, kThreads, 0, s>>>(c);                          \
+    } while (0)
 #define TU_CACHE_ATTN(D)                                                                                               \
     do {                                                                                                               \
-        if (plan.rows == 16) cache_few_kernel<D, 1><<<grid, kThreads, 0, s>>>(c);                                      \
-        else if (plan.rows == 32) cache_few_kernel<D, 2><<<grid, kThreads, 0, s>>>(c);                                 \
-        else if (q_type == kQInt8) cache_many_kernel<D, false><<<grid, kThreads, 0, s>>>(c);                           \
-        else cache_many_kernel<D, true><<<grid, kThreads, 0, s>>>(c);                                                  \
-        if (plan.parts > 1) {                                                                                          \
-            constexpr int64_t kRowsPerWg = kThreads / (D / 8);                                                         \
-            const dim3 merge(static_cast<unsigned>((batch * hkv * rows + kRowsPerWg - 1) / kRowsPerWg));               \
-            if (plan.rows == 16) cache_merge_kernel<D, 16><<<merge, kThreads, 0, s>>>(c);                              \
-            else if (plan.rows == 32) cache_merge_kernel<D, 32><<<merge, kThreads, 0, s>>>(c);                         \
-            else cache_merge_kernel<D, kManyRows><<<merge, kThreads, 0, s>>>(c);                                       \
+        if (plan.rows == 16) {                                                                                         \
+            cache_few_kernel<D, 1><<<grid, kThreads, 0, s>>>(c);                                                       \
+            TU_CACHE_MERGE(D, 16, kThreads / (D / 8));                                                                 \
+        } else if (plan.rows == 32) {                                                                                  \
+            cache_few_kernel<D, 2><<<grid, kThreads, 0, s>>>(c);                                                       \
+            TU_CACHE_MERGE(D, 32, kThreads / (D / 8));                                                                 \
+        } else if (plan.rows == 128) {                                                                                 \
+            if (q_type == kQInt8) cache_many_kernel<D, false, 1><<<grid, 256, 0, s>>>(c);                              \
+            else cache_many_kernel<D, true, 1><<<grid, 256, 0, s>>>(c);                                                \
+            TU_CACHE_MERGE(D, 128, 1);                                                                                 \
+        } else {                                                                                                       \
+            if (q_type == kQInt8) cache_many_kernel<D, false, 2><<<grid, 512, 0, s>>>(c);                              \
+            else cache_many_kernel<D, true, 2><<<grid, 512, 0, s>>>(c);                                                \
+            TU_CACHE_MERGE(D, 256, 1);                                                                                 \
         }                                                                                                              \
     } while (0)
     if (dim == 128) TU_CACHE_ATTN(128);
     else TU_CACHE_ATTN(64);
 #undef TU_CACHE_ATTN
+#undef TU_CACHE_MERGE
     return check_launch("tu_kv_cache_attn");
 }
