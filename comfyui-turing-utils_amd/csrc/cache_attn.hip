@@ -489,7 +489,7 @@ __global__ __launch_bounds__(kThreads, D == 128 && kRT == 2 ? 1 : 2) void cache_
 // as codes by direct-to-LDS loads, a ring of four; values through registers, converted
 // to fp16 once, a ring of two.
 //   Bound by instruction issue: a wave's step at D = 128 is 832 cycles of MFMAs of the
-// 1300 or so that it takes, and the two waves of a SIMD issue into the rest.  4680 rows
+// 1700 that it takes, and the two waves of a SIMD issue into the rest.  4680 rows
 // x 32760 keys, 40 heads, int8 queries: 2.26 ms, 1390 TFLOP/s (one group: 2.45 ms).
 constexpr int kQT = 2;           // 16-row fragments of a wave
 constexpr int kWaveRows = 16 * kQT;

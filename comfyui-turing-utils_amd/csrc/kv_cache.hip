@@ -14,8 +14,14 @@
 // the last new token keep their bytes.  The maximum is one of bit patterns, so
 // that a NaN or infinite x makes the scale one, and the page's codes 0.
 //
-// Bound by HBM where much is written (2 bytes read and 1 written an element),
-// by a chain of four loads (length, page, row, scale) for single tokens.
+// Bound by HBM where much is written or read (2 bytes of a 16-bit type and 1 of codes
+// an element): 32760 tokens of 40 heads, D = 128, are written and read in about 200 us
+// each, 5 TB/s, the rate of a large copy.  By a chain of four loads (length, page, row,
+// scale) for single tokens: 32 tokens of 8 heads in 5 us.
+//   Heads come fastest in the grid, so that workgroups that run together read whole
+// rows of a tensor with tokens first (a token for 32 sequences and back: 14 -> 12 us;
+// tensors with heads first lose 2 percent).  Each load and store of a wave covers
+// whole lines, V^T by way of LDS (479 -> 401 us for 32760 tokens and back).
 #include <algorithm>
 
 #include "tu_common.h"
@@ -98,50 +104,48 @@ struct Quantizer {
 template <int D, int kType, bool kCodes>
 __device__ void write_keys(const void *x, int64_t row_stride, const float *in_scale, int first_token, const uint16_t *mean,
                            int8_t *codes, float *scale, int front, int lo, int hi, uint32_t *part) {
-    constexpr int kItems = kPage * D / 16 / kThreads;  // pieces of 16 channels of a row
-    float v[kItems][16];
+    constexpr int kItems = kPage * D / 8 / kThreads;  // pieces of 8 channels of a row
+    float v[kItems][8];
     uint32_t amax = 0;
 #pragma unroll
     for (int it = 0; it < kItems; ++it) {
-        const int row = (it * kThreads + threadIdx.x) / (D / 16), c = threadIdx.x % (D / 16);
+        const int row = (it * kThreads + threadIdx.x) / (D / 8), c = threadIdx.x % (D / 8);
         if (row < lo || row >= hi) continue;
         if constexpr (kCodes) {
-            const u32x4 w = *reinterpret_cast<const u32x4 *>(static_cast<const int8_t *>(x) + row * row_stride + 16 * c);
+            const u32x2 w = *reinterpret_cast<const u32x2 *>(static_cast<const int8_t *>(x) + row * row_stride + 8 * c);
             const float s = in_scale[(first_token + row) / kPage];
 #pragma unroll
-            for (int e = 0; e < 16; ++e) v[it][e] = byte_of(w[e >> 2], e & 3) * s;
+            for (int e = 0; e < 8; ++e) v[it][e] = byte_of(w[e >> 2], e & 3) * s;
         } else {
-            const auto *src = reinterpret_cast<const u32x4 *>(static_cast<const uint16_t *>(x) + row * row_stride + 16 * c);
-            const u32x4 w[2] = {src[0], src[1]};
+            const u32x4 w = *reinterpret_cast<const u32x4 *>(static_cast<const uint16_t *>(x) + row * row_stride + 8 * c);
 #pragma unroll
-            for (int e = 0; e < 16; ++e) v[it][e] = element<kType>(w[e >> 3][(e >> 1) & 3], e & 1);
+            for (int e = 0; e < 8; ++e) v[it][e] = element<kType>(w[e >> 1], e & 1);
         }
         if (mean) {
-            const auto *src = reinterpret_cast<const u32x4 *>(mean + 16 * c);
-            const u32x4 w[2] = {src[0], src[1]};
+            const u32x4 w = *reinterpret_cast<const u32x4 *>(mean + 8 * c);
 #pragma unroll
-            for (int e = 0; e < 16; ++e) v[it][e] -= element<0>(w[e >> 3][(e >> 1) & 3], e & 1);
+            for (int e = 0; e < 8; ++e) v[it][e] -= element<0>(w[e >> 1], e & 1);
         }
 #pragma unroll
-        for (int e = 0; e < 16; ++e) amax = max(amax, magnitude(v[it][e]));
+        for (int e = 0; e < 8; ++e) amax = max(amax, magnitude(v[it][e]));
     }
     const float scale_before = *scale;
     const Quantizer q(group_max(amax, part), scale_before, front > 0);
     if (threadIdx.x == 0) *scale = q.scale;
 #pragma unroll
     for (int it = 0; it < kItems; ++it) {
-        const int row = (it * kThreads + threadIdx.x) / (D / 16), c = threadIdx.x % (D / 16);
-        auto *dst = reinterpret_cast<u32x4 *>(codes + row * D + 16 * c);
-        u32x4 w;
+        const int row = (it * kThreads + threadIdx.x) / (D / 8), c = threadIdx.x % (D / 8);
+        auto *dst = reinterpret_cast<u32x2 *>(codes + row * D + 8 * c);
+        u32x2 w;
         if (row >= lo && row < hi) {
 #pragma unroll
-            for (int e = 0; e < 4; ++e)
+            for (int e = 0; e < 2; ++e)
                 w[e] = q.code(v[it][4 * e]) | q.code(v[it][4 * e + 1]) << 8 | q.code(v[it][4 * e + 2]) << 16 |
                        q.code(v[it][4 * e + 3]) << 24;
         } else if (q.grown && row < front) {
             w = *dst;
 #pragma unroll
-            for (int e = 0; e < 4; ++e) w[e] = q.again(w[e]);
+            for (int e = 0; e < 2; ++e) w[e] = q.again(w[e]);
         } else {
             continue;
         }
@@ -149,25 +153,50 @@ __device__ void write_keys(const void *x, int64_t row_stride, const float *in_sc
     }
 }
 
+// A page of V^T in LDS on its way between rows of tokens (a thread has 4 of them) and
+// rows of channels: 68 bytes a channel, which spreads a wave's dwords over the banks.
+constexpr int kTurn = kPage / 4 + 1;  // dwords of a channel
+template <int D>
+struct Turn {
+    uint32_t at[D * kTurn];
+    __device__ __forceinline__ uint32_t &dword(int channel, int quad) { return at[channel * kTurn + quad]; }
+    // The thread's pieces of 16 bytes of a page's codes, contiguous over the workgroup.
+    __device__ __forceinline__ void out(int8_t *codes) {
+#pragma unroll
+        for (int it = 0; it < kPage * D / 16 / kThreads; ++it) {
+            const int i = it * kThreads + threadIdx.x;
+            u32x4 w;
+#pragma unroll
+            for (int e = 0; e < 4; ++e) w[e] = dword(i / 4, 4 * (i % 4) + e);
+            reinterpret_cast<u32x4 *>(codes)[i] = w;
+        }
+    }
+    __device__ __forceinline__ void in(const int8_t *codes) {
+#pragma unroll
+        for (int it = 0; it < kPage * D / 16 / kThreads; ++it) {
+            const int i = it * kThreads + threadIdx.x;
+            const u32x4 w = reinterpret_cast<const u32x4 *>(codes)[i];
+#pragma unroll
+            for (int e = 0; e < 4; ++e) dword(i / 4, 4 * (i % 4) + e) = w[e];
+        }
+    }
+};
+
 template <int D, int kType>
 __device__ void write_values(const void *x, int64_t row_stride, int8_t *codes, float *scale, int front, int lo, int hi,
-                             uint32_t *part) {
+                             uint32_t *part, Turn<D> &turn) {
     constexpr int kCh = D / 16;  // channels of a thread, times 4 tokens
     const int c = threadIdx.x % 16, t0 = 4 * (threadIdx.x / 16);
+    typedef uint32_t Row __attribute__((ext_vector_type(kCh / 2)));
     float v[4][kCh];
     uint32_t amax = 0;
 #pragma unroll
     for (int t = 0; t < 4; ++t) {
         const int row = t0 + t;
         const bool fresh = row >= lo && row < hi;
-        uint32_t w[kCh / 2] = {};
+        Row w = {};
         if (fresh) {
-            const auto *src = reinterpret_cast<const u32x2 *>(static_cast<const uint16_t *>(x) + row * row_stride + kCh * c);
-#pragma unroll
-            for (int e = 0; e < kCh / 4; ++e) {
-                const u32x2 p = src[e];
-                w[2 * e] = p[0], w[2 * e + 1] = p[1];
-            }
+            w = *reinterpret_cast<const Row *>(static_cast<const uint16_t *>(x) + row * row_stride + kCh * c);
         }
 #pragma unroll
         for (int e = 0; e < kCh; ++e) {
@@ -178,6 +207,14 @@ __device__ void write_values(const void *x, int64_t row_stride, int8_t *codes, f
     const float scale_before = *scale;
     const Quantizer q(group_max(amax, part), scale_before, front > 0);
     if (threadIdx.x == 0) *scale = q.scale;
+    if (lo == 0 && hi == kPage) {  // a page of new tokens alone
+#pragma unroll
+        for (int e = 0; e < kCh; ++e)
+            turn.dword(kCh * c + e, t0 / 4) = q.code(v[0][e]) | q.code(v[1][e]) << 8 | q.code(v[2][e]) << 16 | q.code(v[3][e]) << 24;
+        __syncthreads();
+        turn.out(codes);
+        return;
+    }
     uint32_t fresh = 0, earlier = 0;  // bytes of the thread's four tokens
 #pragma unroll
     for (int t = 0; t < 4; ++t) {
@@ -198,7 +235,7 @@ __device__ void write_values(const void *x, int64_t row_stride, int8_t *codes, f
     }
 }
 
-// Workgroup (block of the sequence's new tokens, head, 2 * sequence + (0: keys, 1: values)).
+// Workgroup (block of the sequence's new tokens * heads + head, 2 * sequence + (0: keys, 1: values)).
 template <int D, int kType, bool kCodes>
 __global__ __launch_bounds__(kThreads) void cache_append_kernel(
     const void *__restrict__ k, const float *__restrict__ k_in_scale, const void *__restrict__ v, int32_t len, int64_t k_sb,
@@ -206,12 +243,13 @@ __global__ __launch_bounds__(kThreads) void cache_append_kernel(
     const int32_t *__restrict__ new_lengths, int8_t *__restrict__ k_codes, int8_t *__restrict__ v_codes,
     float *__restrict__ k_scale, float *__restrict__ v_scale, int32_t *__restrict__ lengths_out) {
     __shared__ uint32_t part[kThreads / 64];
-    const uint32_t h = blockIdx.y, b = blockIdx.z >> 1;
-    const bool keys = (blockIdx.z & 1) == 0;
+    __shared__ Turn<D> turn;
+    const uint32_t h = blockIdx.x % pages.hkv, b = blockIdx.y >> 1, nth = blockIdx.x / pages.hkv;
+    const bool keys = (blockIdx.y & 1) == 0;
     const int before = held(pages, b);
     const int fresh = min(new_lengths ? min(max(new_lengths[b], 0), len) : len, pages.width * kPage - before);
-    if (blockIdx.x == 0 && h == 0 && keys && threadIdx.x == 0) lengths_out[b] = before + fresh;
-    const int block = before / kPage + static_cast<int>(blockIdx.x), base = block * kPage;
+    if (blockIdx.x == 0 && keys && threadIdx.x == 0) lengths_out[b] = before + fresh;
+    const int block = before / kPage + static_cast<int>(nth), base = block * kPage;
     const int lo = max(before - base, 0), hi = min(before + fresh - base, kPage);
     if (lo >= hi) return;
     const int page = page_of(pages, b, block);
@@ -227,7 +265,7 @@ __global__ __launch_bounds__(kThreads) void cache_append_kernel(
                                      k_codes + at * kPage * D, k_scale + at, lo, lo, hi, part);
     } else {
         write_values<D, kType>(static_cast<const uint16_t *>(v) + b * v_sb + h * v_sh + first * v_sl, v_sl,
-                               v_codes + at * kPage * D, v_scale + at, lo, lo, hi, part);
+                               v_codes + at * kPage * D, v_scale + at, lo, lo, hi, part, turn);
     }
 }
 
@@ -237,8 +275,8 @@ __device__ __forceinline__ uint32_t pack2(float a, float b) {
     else return pack_f16x2(a, b);
 }
 
-// Workgroup (block that the tokens read lie in, head, 2 * sequence + (0: keys,
-// 1: values)): rows of the output whose tokens lie in the block; zeros at and
+// Workgroup (block that the tokens read lie in * heads + head, 2 * sequence + (0:
+// keys, 1: values)): rows of the output whose tokens lie in the block; zeros at and
 // past the sequence's end and where the table names no page.
 template <int D, int kType>
 __global__ __launch_bounds__(kThreads) void cache_read_kernel(
@@ -246,11 +284,12 @@ __global__ __launch_bounds__(kThreads) void cache_read_kernel(
     const float *__restrict__ v_scale, Pages pages, const int32_t *__restrict__ starts, int32_t len,
     const uint16_t *__restrict__ k_mean, uint16_t *__restrict__ k, int64_t k_sb, int64_t k_sh, int64_t k_sl,
     uint16_t *__restrict__ v, int64_t v_sb, int64_t v_sh, int64_t v_sl) {
-    const uint32_t h = blockIdx.y, b = blockIdx.z >> 1;
-    const bool keys = (blockIdx.z & 1) == 0;
+    __shared__ Turn<D> turn;
+    const uint32_t h = blockIdx.x % pages.hkv, b = blockIdx.y >> 1, nth = blockIdx.x / pages.hkv;
+    const bool keys = (blockIdx.y & 1) == 0;
     const int end = held(pages, b);
     const int start = starts ? min(max(starts[b], 0), pages.width * kPage) : 0;
-    const int block = start / kPage + static_cast<int>(blockIdx.x);
+    const int block = start / kPage + static_cast<int>(nth);
     const int64_t base = static_cast<int64_t>(block) * kPage;
     const int lo = static_cast<int>(max(start - base, static_cast<int64_t>(0)));
     const int hi = static_cast<int>(min(start + static_cast<int64_t>(len) - base, static_cast<int64_t>(kPage)));
@@ -265,53 +304,49 @@ __global__ __launch_bounds__(kThreads) void cache_read_kernel(
         const uint16_t *mean = k_mean ? k_mean + static_cast<int64_t>(b * pages.hkv + h) * D : nullptr;
         uint16_t *out = k + b * k_sb + h * k_sh + first * k_sl;
 #pragma unroll
-        for (int it = 0; it < kPage * D / 16 / kThreads; ++it) {
-            const int row = (it * kThreads + threadIdx.x) / (D / 16), c = threadIdx.x % (D / 16);
+        for (int it = 0; it < kPage * D / 8 / kThreads; ++it) {
+            const int row = (it * kThreads + threadIdx.x) / (D / 8), c = threadIdx.x % (D / 8);
             if (row < lo || row >= hi) continue;
-            u32x4 r[2] = {};
+            u32x4 r = {};
             if (row < seen) {
-                const u32x4 w = *reinterpret_cast<const u32x4 *>(codes + row * D + 16 * c);
-                float x[16];
+                const u32x2 w = *reinterpret_cast<const u32x2 *>(codes + row * D + 8 * c);
+                float x[8];
 #pragma unroll
-                for (int e = 0; e < 16; ++e) x[e] = byte_of(w[e >> 2], e & 3) * s;
+                for (int e = 0; e < 8; ++e) x[e] = byte_of(w[e >> 2], e & 3) * s;
                 if (mean) {
-                    const auto *src = reinterpret_cast<const u32x4 *>(mean + 16 * c);
-                    const u32x4 m[2] = {src[0], src[1]};
+                    const u32x4 m = *reinterpret_cast<const u32x4 *>(mean + 8 * c);
 #pragma unroll
-                    for (int e = 0; e < 16; ++e) x[e] += element<0>(m[e >> 3][(e >> 1) & 3], e & 1);
+                    for (int e = 0; e < 8; ++e) x[e] += element<0>(m[e >> 1], e & 1);
                 }
 #pragma unroll
-                for (int e = 0; e < 8; ++e) r[e >> 2][e & 3] = pack2<kType>(x[2 * e], x[2 * e + 1]);
+                for (int e = 0; e < 4; ++e) r[e] = pack2<kType>(x[2 * e], x[2 * e + 1]);
             }
-            auto *dst = reinterpret_cast<u32x4 *>(out + row * k_sl + 16 * c);
-            dst[0] = r[0], dst[1] = r[1];
+            *reinterpret_cast<u32x4 *>(out + row * k_sl + 8 * c) = r;
         }
     } else {
         constexpr int kCh = D / 16;  // channels of a thread, times 4 tokens
         const int c = threadIdx.x % 16, t0 = 4 * (threadIdx.x / 16);
-        if (t0 + 4 <= lo || t0 >= hi) return;
         const int8_t *codes = v_codes + at * kPage * D;
         const float s = seen > 0 ? v_scale[at] : 0.0f;
+        if (seen > 0) turn.in(codes);
+        __syncthreads();
         uint16_t *out = v + b * v_sb + h * v_sh + first * v_sl;
         uint32_t w[kCh] = {};
         if (t0 < seen) {
 #pragma unroll
-            for (int e = 0; e < kCh; ++e) w[e] = *reinterpret_cast<const uint32_t *>(codes + (kCh * c + e) * kPage + t0);
+            for (int e = 0; e < kCh; ++e) w[e] = turn.dword(kCh * c + e, t0 / 4);
         }
 #pragma unroll
         for (int t = 0; t < 4; ++t) {
             const int row = t0 + t;
             if (row < lo || row >= hi) continue;
-            auto *dst = reinterpret_cast<u32x2 *>(out + row * v_sl + kCh * c);
+            typedef uint32_t Row __attribute__((ext_vector_type(kCh / 2)));
+            Row r = {};
+            if (row < seen) {
 #pragma unroll
-            for (int e = 0; e < kCh; e += 4) {
-                u32x2 r = {};
-                if (row < seen) {
-                    r[0] = pack2<kType>(byte_of(w[e], t) * s, byte_of(w[e + 1], t) * s);
-                    r[1] = pack2<kType>(byte_of(w[e + 2], t) * s, byte_of(w[e + 3], t) * s);
-                }
-                dst[e / 4] = r;
+                for (int e = 0; e < kCh / 2; ++e) r[e] = pack2<kType>(byte_of(w[2 * e], t) * s, byte_of(w[2 * e + 1], t) * s);
             }
+            *reinterpret_cast<Row *>(out + row * v_sl + kCh * c) = r;
         }
     }
 }
@@ -352,7 +387,8 @@ extern "C" int32_t tu_kv_cache_append(const void *k, const float *k_in_scale, co
     const Pages p{block_table, lengths, static_cast<int32_t>(width), static_cast<int32_t>(pages), static_cast<uint32_t>(hkv)};
     // len tokens touch one page more where they do not start at a page's start
     const int64_t blocks = std::min<int64_t>((len + 2 * kPage - 2) / kPage, width);
-    const dim3 grid(static_cast<unsigned>(blocks), static_cast<unsigned>(hkv), static_cast<unsigned>(2 * batch));
+    TU_REQUIRE(blocks * hkv <= 0x7fffffff, "cache append grid too large");
+    const dim3 grid(static_cast<unsigned>(blocks * hkv), static_cast<unsigned>(2 * batch));
     hipStream_t s = static_cast<hipStream_t>(stream);
 #define TU_APPEND(D, TYPE, CODES)                                                                                      \
     cache_append_kernel<D, TYPE, CODES><<<grid, kThreads, 0, s>>>(                                                     \
@@ -390,7 +426,8 @@ extern "C" int32_t tu_kv_cache_read(const int8_t *k_codes, const int8_t *v_codes
     if (require_gfx950()) return -1;
     const Pages p{block_table, lengths, static_cast<int32_t>(width), static_cast<int32_t>(pages), static_cast<uint32_t>(hkv)};
     const int64_t blocks = starts ? (len + 2 * kPage - 2) / kPage : (len + kPage - 1) / kPage;
-    const dim3 grid(static_cast<unsigned>(blocks), static_cast<unsigned>(hkv), static_cast<unsigned>(2 * batch));
+    TU_REQUIRE(blocks * hkv <= 0x7fffffff, "cache read grid too large");
+    const dim3 grid(static_cast<unsigned>(blocks * hkv), static_cast<unsigned>(2 * batch));
     hipStream_t s = static_cast<hipStream_t>(stream);
 #define TU_READ(D, TYPE)                                                                                               \
     cache_read_kernel<D, TYPE><<<grid, kThreads, 0, s>>>(                                                              \
