@@ -507,6 +507,11 @@ class SequenceKVCache:
                    torch.arange(batch * row, dtype=torch.int32, device=device).view(batch, row),
                    torch.zeros(batch, dtype=torch.int32, device=device))
 
+    @property
+    def max_length(self) -> int:
+        """Tokens that a sequence has places for."""
+        return self.block_table.size(1) * PAGE_TOKENS
+
     def append(self, key: torch.Tensor, value: torch.Tensor, **kwargs) -> None:
         """``kv_cache_append`` behind the sequences' ends; ``lengths`` grow."""
         self.lengths.copy_(kv_cache_append(key, value, self.cache, self.block_table, self.lengths, **kwargs))

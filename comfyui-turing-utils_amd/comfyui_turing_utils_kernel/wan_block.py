@@ -41,11 +41,13 @@ residual stream x is bf16; each residual add, x + y * gate, runs in the
 epilogue of the projection that produces y (``turing_utils::int8_linear_residual``):
 bf16_rn(fma(y, gate, x)) with y the bf16 projection output.
 
-Two options of a forward, off by default: each sample of a batch with the
+Three options of a forward, off by default: each sample of a batch with the
 low-rank adapters of its own request on any of the linears (``set_adapters``,
-``adapter_ids``; ``turing_utils::int8_linear_adapters``), and self-attention
+``adapter_ids``; ``turing_utils::int8_linear_adapters``), self-attention
 over the key blocks chosen per query block (``BlockSparsity``;
-``turing_sage.sparse_sageattn_from_prequantized``).
+``turing_sage.sparse_sageattn_from_prequantized``), and a video made chunk by
+chunk: self-attention over the keys and values of the chunks before, kept in 8
+bits, and over the chunk's own (``cache``; ``turing_sage.SequenceKVCache``).
 """
 from __future__ import annotations
 
@@ -58,6 +60,7 @@ import torch
 from . import ops  # noqa: F401  (registers torch.ops.turing_utils.*)
 from .adapters import LinearAdapters, turing_int8_linear_adapters
 from .turing_sage import core as sage_core
+from .turing_sage.kv_cache import SequenceKVCache
 from .turing_sage.sparse import sparse_sageattn_from_prequantized
 
 GROUP = 128
@@ -290,9 +293,12 @@ class WanBlockW8A8:
 
     def self_attention(self, h, freqs: torch.Tensor, residual: Optional[torch.Tensor] = None,
                        gate: Optional[torch.Tensor] = None, adapter_ids: Optional[torch.Tensor] = None,
-                       sparsity: Optional[BlockSparsity] = None) -> torch.Tensor:
+                       sparsity: Optional[BlockSparsity] = None,
+                       cache: Optional[SequenceKVCache] = None) -> torch.Tensor:
         """The attention output projected by o; with ``residual`` [B, L, C],
-        residual + that * gate (gate [B, 1, C] or None) from one epilogue."""
+        residual + that * gate (gate [B, 1, C] or None) from one epilogue.  With
+        ``cache`` the tokens' keys and values are appended to it and every query
+        sees all that its sequence has there then."""
         cfg = self.cfg
         b, l, c = h.shape
         qkv = self.self_qkv(_token_rows(h), **self._adapted("self_qkv", adapter_ids, l))
@@ -301,6 +307,11 @@ class WanBlockW8A8:
         qk = sage_core.prequantize_rms_rope_qk(
             q, k, self.self_norm_q, self.self_norm_k, freqs, epsilon=cfg.eps, rot_dim=cfg.head_dim,
             tensor_layout="NHD", norm_scope="row")
+        if cache is not None:
+            cache.append(qk.key_int8, v, tensor_layout="NHD", key_scale=qk.key_scale)
+            scale = qk.query_scale[..., :(l + 15) // 16].contiguous()  # (its blocks of 16 tokens fill blocks of 64)
+            out = cache.attend(qk.query_int8, tensor_layout="NHD", query_scale=scale, blkq=16, sm_scale=cfg.head_dim ** -0.5)
+            return self._project("self_o", out.reshape(b * l, c), b, residual, gate, adapter_ids).view(b, l, c)
         state = sage_core.prequantize_sageattn_from_qk(qk, v, sm_scale=cfg.head_dim ** -0.5)
         del qkv, q, k, qk
         if sparsity is None:
@@ -309,6 +320,16 @@ class WanBlockW8A8:
             out = sparse_sageattn_from_prequantized(state, keep=sparsity.keep, sink_blocks=sparsity.sink_blocks,
                                                     local_blocks=sparsity.local_blocks)
         return self._project("self_o", out.reshape(b * l, c), b, residual, gate, adapter_ids).view(b, l, c)
+
+    def _check_cache(self, cache: SequenceKVCache, batch: int, tokens: int, sparsity: Optional[BlockSparsity]) -> None:
+        if sparsity is not None:
+            raise ValueError("a cache and sparsity exclude each other")
+        heads, width = cache.cache.key_codes.shape[1], cache.cache.key_codes.shape[3]
+        if (heads, width) != (self.cfg.heads, self.cfg.head_dim) or cache.block_table.shape[0] != batch:
+            raise ValueError(f"the cache has {cache.block_table.shape[0]} sequences, {heads} heads of {width} channels, the "
+                             f"call {batch}, {self.cfg.heads} of {self.cfg.head_dim}")
+        if tokens > cache.max_length:
+            raise ValueError(f"{tokens} tokens do not fit a cache of {cache.max_length}")
 
     def _project(self, name: str, x2d: torch.Tensor, b: int, residual, gate, adapter_ids,
                  gelu: bool = False) -> torch.Tensor:
@@ -348,11 +369,18 @@ class WanBlockW8A8:
         return [mod[:, i:i + 1] for i in range(6)]
 
     def forward(self, x: torch.Tensor, e: torch.Tensor, context: torch.Tensor, freqs: torch.Tensor,
-                adapter_ids: Optional[torch.Tensor] = None, sparsity: Optional[BlockSparsity] = None) -> torch.Tensor:
+                adapter_ids: Optional[torch.Tensor] = None, sparsity: Optional[BlockSparsity] = None,
+                cache: Optional[SequenceKVCache] = None) -> torch.Tensor:
         """x bf16 [B, L, C]; e [B, 6, C] time modulation; context bf16 [B, Lc, C]
         (after the text embedding); freqs [1|B, L, 1, D/2, 2, 2]; adapter_ids
         int32 [B], the adapter (``set_adapters``) of each sample, none outside
-        [0, count); sparsity: which keys self-attention keeps, all when None."""
+        [0, count); sparsity: which keys self-attention keeps, all when None.
+
+        cache: this block's own, of B sequences with room for what is appended
+        (tokens past its end are neither kept nor seen).  x are then the next
+        tokens of the sequences, freqs those of their places, and self-attention
+        sees the tokens before as well.  The forward moves ``cache.lengths`` on;
+        for the next denoising step of the same chunk set them back, in place."""
         cfg = self.cfg
         if x.dtype != torch.bfloat16 or x.dim() != 3 or x.shape[2] != cfg.dim:
             raise TypeError(f"Wan block input must be bf16 [B, L, {cfg.dim}]")
@@ -364,6 +392,8 @@ class WanBlockW8A8:
             if adapter_ids.dtype != torch.int32 or adapter_ids.shape != (x.shape[0],):
                 raise ValueError(f"adapter_ids must be int32 [{x.shape[0]}], one adapter per sample")
         e0, e1, e2, e3, e4, e5 = self.modulation_chunks(e)
+        if cache is not None:
+            self._check_cache(cache, x.shape[0], x.shape[1], sparsity)
         x = x.contiguous()
         b, l, _ = x.shape
 
@@ -374,7 +404,7 @@ class WanBlockW8A8:
         # each norm runs with the next projection's quantizer, each residual
         # add in the epilogue of the projection before it
         x = self.self_attention(adaln_codes(x, e1, e0, self.self_qkv.group), freqs, residual=x, gate=e2,
-                                adapter_ids=adapter_ids, sparsity=sparsity)
+                                adapter_ids=adapter_ids, sparsity=sparsity, cache=cache)
         codes, rs = torch.ops.turing_utils.layer_norm_affine_int8_convrot_quantize(
             x, self.norm3_weight, self.norm3_bias, cfg.eps, self.cross_q.group)
         x = self.cross_attention(QuantizedActivation(codes, rs, b, l, self.cross_q.group), context, residual=x,
