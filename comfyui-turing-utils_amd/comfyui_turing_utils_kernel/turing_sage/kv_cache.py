@@ -412,10 +412,10 @@ def _attend_op(
         _, _, *o_strides = _layout_dims(out, tensor_layout)
         cus = _compute_units(device)
         max_length = min(max_length, row * PAGE_TOKENS)
-        nbytes = int(_lib.load().tu_kv_cache_attn_workspace(batch, hq, heads, tokens, width, max_length,
+        kind = 2 if query_scale is not None else int(query.dtype == torch.float16)
+        nbytes = int(_lib.load().tu_kv_cache_attn_workspace(batch, hq, heads, tokens, width, max_length, kind,
                                                             int(bool(is_causal)), cus))
         workspace = torch.empty(nbytes, dtype=torch.uint8, device=device) if nbytes else None
-        kind = 2 if query_scale is not None else int(query.dtype == torch.float16)
         _lib.call("tu_kv_cache_attn", query.data_ptr(), _lib.ptr(query_scale), kind, int(blkq), key_codes.data_ptr(),
                   value_codes.data_ptr(), key_scale.data_ptr(), value_scale.data_ptr(), pages, block_table.data_ptr(),
                   row, lengths.data_ptr(), _lib.ptr(query_lengths), out.data_ptr(), batch, hq, heads, tokens, width,

@@ -846,8 +846,10 @@ __device__ __forceinline__ void many_store_v(uint32_t stage, const ManyGeom<D, k
         }
 }
 
+// Four waves at D = 64 with one term leave the registers for a third workgroup on a CU
+// (8192 x 4096, 12 heads: 134 -> 115 us; with two terms they spill, and it gains nothing).
 template <int D, bool kTerms, int kGroups>
-__global__ __launch_bounds__(256 * kGroups, 2 / kGroups) void cache_many_kernel(CacheCall call) {
+__global__ __launch_bounds__(256 * kGroups, kGroups == 2 ? 1 : D == 64 && !kTerms ? 3 : 2) void cache_many_kernel(CacheCall call) {
     constexpr int kSl = D / 64, kDS = D / 16, kWaves = 4 * kGroups, kLoads = kPieces<D, kWaves>, kRows = kGroupRows * kGroups;
     __shared__ __align__(1024) int8_t lds[Tiles<D>::kBytes];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -1145,29 +1147,34 @@ int64_t few_parts(int64_t units, int64_t pages, int64_t slots, int64_t cus) {
 }
 
 // Time of a launch of many rows, in steps of a page at 256 rows (1.6 us at D = 128).
-// Blocks of 128 rows run two to a CU, a step 1.08 of that for both, or 0.78 where
-// a CU has one; blocks of 256 run one to a CU.  A unit costs 4 steps over its pages, a
-// merge 3 and its bytes, 7 MB a step (at 256 CUs).
+// Blocks of 128 rows run up to `places` to a CU: a step takes 0.78 of that for one, 1.08
+// for two and 1.4 for three.  Blocks of 256 run one to a CU.  A unit costs 4 steps over
+// its pages, a merge 3 and its bytes, 7 MB a step (at 256 CUs).
 //   Measured, us, 128 / 256 rows a block: 4680 rows x 32760 keys, 40 heads, int8
 // queries 2450 / 2240; 33 rows x 4 heads a K/V head, 8192 keys, 16 ranges 30.5 /
 // 34.8; 1560 x 9360, 12 heads, by ranges: 1: 184 / 214, 2: 133 / 125, 3: 99 / 97,
-// 4: 120 / 133, 6: 111 / 111.
+// 4: 120 / 133, 6: 111 / 111; 8192 x 4096 at D = 64, 12 heads: 115 / 147.
 //   Causal: empty ranges of early blocks end at once, and long blocks go first.
 // 4001 x 4001, 2 x 16 heads: 1 range 143, 2 ranges 224; 2050 x 6000 at D = 64, 18
 // heads, 128 rows a block: 123, 87.
-double many_cost(int64_t units, int64_t parts, int64_t pages, double share, bool causal, bool one_a_cu, double part_bytes,
+double many_cost(int64_t units, int64_t parts, int64_t pages, double share, bool causal, int64_t places, double part_bytes,
                  int64_t cus) {
-    const int64_t slots = one_a_cu ? cus : 2 * cus;
+    const int64_t slots = (places ? places : 1) * cus;
+    auto step = [&](double n) { return !places || n <= 0.0 ? (n > 0.0) * 1.0 : n <= cus ? 0.78 : n <= 2 * cus ? 1.08 : 1.4; };
     const double n = static_cast<double>(units * parts) * share, full = n / static_cast<double>(slots);
-    const double rounds = full <= 1.0 ? 1.0 : causal ? full + 0.5 : static_cast<double>((units * parts + slots - 1) / slots);
-    const double step = one_a_cu ? 1.0 : n <= static_cast<double>(cus) ? 0.78 : 1.08;
+    double steps = step(n);
+    if (full > 1.0) {
+        const int64_t rounds = units * parts / slots;
+        steps = causal ? (full + 0.5) * step(slots)
+                       : static_cast<double>(rounds) * step(slots) + step(static_cast<double>(units * parts - rounds * slots));
+    }
     const double per = static_cast<double>((pages + parts - 1) / parts);
     const double merge = parts > 1 ? 3.0 + static_cast<double>(parts) * part_bytes * 2.0 / (7e6 * static_cast<double>(cus) / 256.0) : 0.0;
-    return rounds * (per + 4.0) * step + merge;
+    return steps * (per + 4.0) + merge;
 }
 
-CachePlan cache_plan(int64_t batch, int64_t hkv, int64_t lq, int64_t group, int64_t dim, int64_t pages, bool causal, int64_t cus,
-                     int64_t max_bytes) {
+CachePlan cache_plan(int64_t batch, int64_t hkv, int64_t lq, int64_t group, int64_t dim, int64_t pages, bool int8, bool causal,
+                     int64_t cus, int64_t max_bytes) {
     const int64_t rows = lq * group;
     const int64_t row_bytes = batch * hkv * rows * (dim + 4) * static_cast<int64_t>(sizeof(float));
     const int64_t most = std::min<int64_t>(max_bytes / row_bytes, 256);
@@ -1188,7 +1195,8 @@ CachePlan cache_plan(int64_t batch, int64_t hkv, int64_t lq, int64_t group, int6
         const int64_t units = batch * hkv * one.row_blocks;
         for (int64_t parts = 1; parts == 1 || (parts <= std::min<int64_t>(most, 64) && 2 * parts <= pages && units * (parts - 1) < 4 * cus);
              ++parts) {
-            const double cost = many_cost(units, parts, pages, share, causal, block == 256, static_cast<double>(row_bytes), cus);
+            const double cost = many_cost(units, parts, pages, share, causal, block == 256 ? 0 : dim == 64 && int8 ? 3 : 2,
+                                          static_cast<double>(row_bytes), cus);
             if (!best.rows || cost < best_cost) best = plan(block, parts), best_cost = cost;
         }
     }
@@ -1203,11 +1211,11 @@ int64_t cache_workspace(const CachePlan &p, int64_t batch, int64_t hkv, int64_t 
 }  // namespace tu
 
 extern "C" int64_t tu_kv_cache_attn_workspace(int64_t batch, int64_t hq, int64_t hkv, int64_t lq, int64_t dim, int64_t max_length,
-                                              int32_t causal, int32_t cus) {
+                                              int32_t q_type, int32_t causal, int32_t cus) {
     using namespace tu;
     if (batch <= 0 || hkv <= 0 || hq < hkv || lq <= 0 || dim <= 0 || max_length <= 0 || cus <= 0) return 0;
     const int64_t group = hq / hkv, pages = (max_length + kPage - 1) / kPage;
-    return cache_workspace(cache_plan(batch, hkv, lq, group, dim, pages, causal != 0, cus, INT64_MAX), batch, hkv, lq * group, dim);
+    return cache_workspace(cache_plan(batch, hkv, lq, group, dim, pages, q_type == kQInt8, causal != 0, cus, INT64_MAX), batch, hkv, lq * group, dim);
 }
 
 extern "C" int32_t tu_kv_cache_attn(const void *q, const float *q_scale, int32_t q_type, int64_t blkq, const int8_t *k_codes,
@@ -1239,7 +1247,7 @@ extern "C" int32_t tu_kv_cache_attn(const void *q, const float *q_scale, int32_t
     TU_REQUIRE((reinterpret_cast<uintptr_t>(workspace) & 15) == 0, "cache attention workspace must be 16-byte aligned");
     const int64_t rows = lq * (hq / hkv);
     const CachePlan plan = cache_plan(batch, hkv, lq, hq / hkv, dim, std::min<int64_t>((max_length + kPage - 1) / kPage, width),
-                                      causal != 0, cus, workspace ? workspace_bytes : 0);
+                                      q_type == kQInt8, causal != 0, cus, workspace ? workspace_bytes : 0);
     const int64_t units = batch * hkv * plan.row_blocks * plan.parts;
     constexpr int64_t kMost = 0x7fffffff;
     TU_REQUIRE(units <= kMost && batch * hkv * rows <= kMost * 16, "cache attention grid too large");

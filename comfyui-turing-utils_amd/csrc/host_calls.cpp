@@ -621,7 +621,7 @@ PyObject *kv_cache_attention(PyObject *, PyObject *const *args, Py_ssize_t nargs
                   : empty({c.batch, q.heads, q.count, c.width}, type, c.device);
         most = most < c.row * 64 ? most : c.row * 64;
         const int64_t bytes = tu_kv_cache_attn_workspace(c.batch, q.heads, c.heads, q.count, c.width, most,
-                                                         causal != 0, static_cast<int32_t>(cus));
+                                                         q_scale ? 2 : is_float16(*q.t), causal != 0, static_cast<int32_t>(cus));
         Tensor work;
         if (bytes > 0) work = empty({bytes}, at::kByte, c.device);
         const int head = nhd ? 2 : 1, seq = nhd ? 1 : 2;

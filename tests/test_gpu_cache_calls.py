@@ -238,7 +238,7 @@ def test_little_workspace(gpu_device, lq):
     lengths = _ints([5700], gpu_device)
     want, bound = ref.attend(q, pool, table, lengths, "HND", True)
     lib, stream = _lib.load(), torch.cuda.current_stream(gpu_device).cuda_stream
-    full = lib.tu_kv_cache_attn_workspace(1, 4, 2, lq, 128, 5700, 1, 256)
+    full = lib.tu_kv_cache_attn_workspace(1, 4, 2, lq, 128, 5700, 0, 1, 256)
     assert full > 0
     for nbytes in (full, full // 2 + 16, 4 * lq * 132 * 4 * 2, 4 * lq * 132 * 4 - 16, 0):
         work = torch.full((nbytes + 256,), 0xa5, dtype=torch.uint8, device=gpu_device)

@@ -291,16 +291,16 @@ def test_workspace():
     """Bytes for whole ranges of rows; none where a call has no ranges or no sizes."""
     size = _lib.load().tu_kv_cache_attn_workspace
     row = 132 * 4
-    assert size(4, 16, 4, 1, 128, 8190, 0, 256) % (64 * row) == 0 < size(4, 16, 4, 1, 128, 8190, 0, 256)
-    assert size(1, 8, 8, 1, 64, 64, 0, 256) == 0  # one page
-    for bad in (0, 1, 2, 3, 4, 5, 7):
-        args = [4, 16, 4, 1, 128, 8190, 0, 256]
+    assert size(4, 16, 4, 1, 128, 8190, 0, 0, 256) % (64 * row) == 0 < size(4, 16, 4, 1, 128, 8190, 0, 0, 256)
+    assert size(1, 8, 8, 1, 64, 64, 0, 0, 256) == 0  # one page
+    for bad in (0, 1, 2, 3, 4, 5, 8):
+        args = [4, 16, 4, 1, 128, 8190, 0, 0, 256]
         args[bad] = 0
         assert size(*args) == 0
     for causal in (0, 1):  # ranges stay in number, and so does the memory
         for lq in (1, 3, 9, 40, 300, 5000, 32760):
             for pages in (1, 5, 63, 512, 2048):
-                got = size(1, 40, 40, lq, 128, 64 * pages, causal, 256)
+                got = size(1, 40, 40, lq, 128, 64 * pages, 2 * causal, causal, 256)
                 assert got % (40 * lq * row) == 0 and got <= 256 * 40 * lq * row, (lq, pages)
 
 
