@@ -469,7 +469,7 @@ def kv_cache_attention(
     if sm_scale is not None and not 0.0 < float(sm_scale) < float("inf"):
         raise ValueError("sm_scale must be a positive finite number")
     if max_length is None:
-        max_length = block_table.size(-1) * PAGE_TOKENS or 1
+        max_length = max(1, block_table.size(-1) * PAGE_TOKENS) if block_table.dim() else 1
     args = (bool(is_causal), -1.0 if sm_scale is None else float(sm_scale), int(max_length), query_scale, int(blkq),
             query_lengths)
     if tensor_layout in ("HND", "NHD") and query.is_cuda and not torch.compiler.is_compiling():

@@ -1203,6 +1203,13 @@ CachePlan cache_plan(int64_t batch, int64_t hkv, int64_t lq, int64_t group, int6
     return best;
 }
 
+// Sizes that the plan's and the kernels' arithmetic holds.
+bool cache_sizes(int64_t batch, int64_t hq, int64_t hkv, int64_t lq, int64_t max_length, int64_t cus) {
+    return batch > 0 && batch <= 65535 && hkv > 0 && hq >= hkv && hq <= 65535 && lq > 0 && lq <= 0x7fffff00 &&
+           lq * (hq / hkv) <= 0x7fffff00 && batch * hkv * (lq * (hq / hkv)) <= int64_t{0x7fffffff} * 16 && max_length > 0 && cus > 0 &&
+           cus <= 65535;
+}
+
 int64_t cache_workspace(const CachePlan &p, int64_t batch, int64_t hkv, int64_t rows, int64_t dim) {
     return p.parts > 1 ? p.parts * batch * hkv * rows * (dim + 4) * static_cast<int64_t>(sizeof(float)) : 0;
 }
@@ -1213,8 +1220,8 @@ int64_t cache_workspace(const CachePlan &p, int64_t batch, int64_t hkv, int64_t 
 extern "C" int64_t tu_kv_cache_attn_workspace(int64_t batch, int64_t hq, int64_t hkv, int64_t lq, int64_t dim, int64_t max_length,
                                               int32_t q_type, int32_t causal, int32_t cus) {
     using namespace tu;
-    if (batch <= 0 || hkv <= 0 || hq < hkv || lq <= 0 || dim <= 0 || max_length <= 0 || cus <= 0) return 0;
-    const int64_t group = hq / hkv, pages = (max_length + kPage - 1) / kPage;
+    if (!cache_sizes(batch, hq, hkv, lq, max_length, cus) || (dim != 64 && dim != 128)) return 0;
+    const int64_t group = hq / hkv, pages = std::min<int64_t>((max_length - 1) / kPage + 1, 0x7fffffff / kPage - 1);
     return cache_workspace(cache_plan(batch, hkv, lq, group, dim, pages, q_type == kQInt8, causal != 0, cus, INT64_MAX), batch, hkv, lq * group, dim);
 }
 
@@ -1229,8 +1236,7 @@ extern "C" int32_t tu_kv_cache_attn(const void *q, const float *q_scale, int32_t
     TU_REQUIRE(dim == 64 || dim == 128, "cache attention requires head_dim 64 or 128, got %lld", static_cast<long long>(dim));
     TU_REQUIRE(q_type >= 0 && q_type <= kQInt8, "cache attention query type must be 0 (bf16), 1 (fp16) or 2 (int8), got %d", q_type);
     TU_REQUIRE(batch > 0 && hq > 0 && hkv > 0 && hq % hkv == 0, "cache attention: hq must be a positive multiple of hkv");
-    TU_REQUIRE(lq > 0 && batch <= 65535 && hq <= 65535 && lq * (hq / hkv) <= 0x7fffff00 && cus > 0 && max_length > 0,
-               "cache attention sizes out of range");
+    TU_REQUIRE(cache_sizes(batch, hq, hkv, lq, max_length, cus), "cache attention sizes out of range");
     TU_REQUIRE(width > 0 && width <= 0x7fffffff / kPage - 1 && pages > 0 && pages <= 0x7fffffff,
                "cache attention block table or page count out of range");
     TU_REQUIRE(pages * hkv <= 0x7fffffff, "cache attention: pages of all heads out of range");
@@ -1246,11 +1252,11 @@ extern "C" int32_t tu_kv_cache_attn(const void *q, const float *q_scale, int32_t
                "cache attention codes and output must be aligned");
     TU_REQUIRE((reinterpret_cast<uintptr_t>(workspace) & 15) == 0, "cache attention workspace must be 16-byte aligned");
     const int64_t rows = lq * (hq / hkv);
-    const CachePlan plan = cache_plan(batch, hkv, lq, hq / hkv, dim, std::min<int64_t>((max_length + kPage - 1) / kPage, width),
+    const CachePlan plan = cache_plan(batch, hkv, lq, hq / hkv, dim, std::min<int64_t>((max_length - 1) / kPage + 1, width),
                                       q_type == kQInt8, causal != 0, cus, workspace ? workspace_bytes : 0);
     const int64_t units = batch * hkv * plan.row_blocks * plan.parts;
     constexpr int64_t kMost = 0x7fffffff;
-    TU_REQUIRE(units <= kMost && batch * hkv * rows <= kMost * 16, "cache attention grid too large");
+    TU_REQUIRE(units <= kMost, "cache attention grid too large");
     if (require_gfx950()) return -1;
     CacheCall c{};
     c.q = q, c.q_scale = q_scale, c.q_type = static_cast<uint32_t>(q_type);

@@ -97,7 +97,7 @@ def test_bad_caches_tables_and_lengths(call):
         with pytest.raises(error):
             call(cache=cache)
     for error, kw in ((TypeError, dict(table=_i(3, 2).long())), (TypeError, dict(lengths=_i(3).long())),
-                      (ValueError, dict(table=_i(6))), (ValueError, dict(table=_i(3, 0))), (ValueError, dict(lengths=_i(2))),
+                      (ValueError, dict(table=_i(6))), (ValueError, dict(table=_i())), (ValueError, dict(table=_i(3, 0))), (ValueError, dict(lengths=_i(2))),
                       (ValueError, dict(lengths=_i(3, 1))), (ValueError, dict(table=_i(3, 2, device="cpu"))),
                       (ValueError, dict(tensor_layout="BLHD"))):
         with pytest.raises(error):
@@ -277,7 +277,7 @@ def test_read_entry_refuses(change):
 
 @pytest.mark.parametrize("change", [
     dict(dim=96), dict(q_type=3), dict(q_type=-1), dict(batch=0), dict(hq=0), dict(hkv=0), dict(hq=7), dict(lq=0),
-    dict(lq=2 ** 31), dict(batch=70000), dict(hq=70002), dict(cus=0), dict(max_length=0), dict(width=0), dict(width=2 ** 31),
+    dict(lq=2 ** 31), dict(batch=70000), dict(hq=70002), dict(batch=65535, hq=65535, hkv=65535, lq=2 ** 30), dict(lq=2 ** 62), dict(cus=0), dict(max_length=0), dict(width=0), dict(width=2 ** 31),
     dict(pages=0), dict(pages=2 ** 31), dict(pages=2 ** 30), dict(q=None), dict(kc=None), dict(vc=None), dict(ks=None),
     dict(vs=None), dict(table=None), dict(lengths=None), dict(o=None), dict(q_type=2), dict(q_type=2, q_scale=P, blkq=0),
     dict(sm_scale=0.0), dict(sm_scale=float("nan")), dict(q=P + 8), dict(q_sl=68), dict(q_type=2, q_scale=P, q_sl=72),
@@ -297,6 +297,11 @@ def test_workspace():
         args = [4, 16, 4, 1, 128, 8190, 0, 0, 256]
         args[bad] = 0
         assert size(*args) == 0
+    huge = 2 ** 31 - 1
+    for args in ((65535, 65535, 65535, huge // 2, 128, huge, 0, 0, 256), (65535, 65535, 1, 2 ** 40, 128, 64, 0, 0, 256),
+                 (2 ** 40, 16, 4, 1, 128, 64, 0, 0, 256), (4, 2 ** 40, 4, 1, 128, 64, 0, 0, 256), (4, 16, 4, 1, 96, 64, 0, 0, 256)):
+        assert size(*args) == 0
+    assert size(1, 1, 1, 1, 128, 2 ** 62, 0, 0, 256) > 0
     for causal in (0, 1):  # ranges stay in number, and so does the memory
         for lq in (1, 3, 9, 40, 300, 5000, 32760):
             for pages in (1, 5, 63, 512, 2048):
