@@ -100,10 +100,12 @@ struct Quantizer {
 };
 
 // New rows [lo, hi) of a page, `front` earlier ones in front of them; x points
-// at the row that becomes the page's row 0 (which may lie before the tensor).
+// at the row that becomes the page's row 0 (which may lie before the tensor).  The
+// page (times heads, plus head) is looked at behind the rows' loads, so that its own
+// load runs beside them; negative, there is none.
 template <int D, int kType, bool kCodes>
 __device__ void write_keys(const void *x, int64_t row_stride, const float *in_scale, int first_token, const uint16_t *mean,
-                           int8_t *codes, float *scale, int front, int lo, int hi, uint32_t *part) {
+                           int8_t *codes, float *scale, int64_t at, int front, int lo, int hi, uint32_t *part) {
     constexpr int kItems = kPage * D / 8 / kThreads;  // pieces of 8 channels of a row
     float v[kItems][8];
     uint32_t amax = 0;
@@ -129,6 +131,8 @@ __device__ void write_keys(const void *x, int64_t row_stride, const float *in_sc
 #pragma unroll
         for (int e = 0; e < 8; ++e) amax = max(amax, magnitude(v[it][e]));
     }
+    if (at < 0) return;
+    codes += at * kPage * D, scale += at;
     const float scale_before = *scale;
     const Quantizer q(group_max(amax, part), scale_before, front > 0);
     if (threadIdx.x == 0) *scale = q.scale;
@@ -183,8 +187,8 @@ struct Turn {
 };
 
 template <int D, int kType>
-__device__ void write_values(const void *x, int64_t row_stride, int8_t *codes, float *scale, int front, int lo, int hi,
-                             uint32_t *part, Turn<D> &turn) {
+__device__ void write_values(const void *x, int64_t row_stride, int8_t *codes, float *scale, int64_t at, int front, int lo,
+                             int hi, uint32_t *part, Turn<D> &turn) {
     constexpr int kCh = D / 16;  // channels of a thread, times 4 tokens
     const int c = threadIdx.x % 16, t0 = 4 * (threadIdx.x / 16);
     typedef uint32_t Row __attribute__((ext_vector_type(kCh / 2)));
@@ -204,6 +208,8 @@ __device__ void write_values(const void *x, int64_t row_stride, int8_t *codes, f
             amax = max(amax, magnitude(v[t][e]));
         }
     }
+    if (at < 0) return;
+    codes += at * kPage * D, scale += at;
     const float scale_before = *scale;
     const Quantizer q(group_max(amax, part), scale_before, front > 0);
     if (threadIdx.x == 0) *scale = q.scale;
@@ -253,8 +259,7 @@ __global__ __launch_bounds__(kThreads) void cache_append_kernel(
     const int lo = max(before - base, 0), hi = min(before + fresh - base, kPage);
     if (lo >= hi) return;
     const int page = page_of(pages, b, block);
-    if (page < 0) return;
-    const int64_t at = static_cast<int64_t>(page) * pages.hkv + h;
+    const int64_t at = page < 0 ? -1 : static_cast<int64_t>(page) * pages.hkv + h;
     const int first = base - before;  // token of the call that is the page's row 0 (negative: one held before)
     if (keys) {
         const int64_t off = b * k_sb + h * k_sh + first * k_sl;
@@ -262,10 +267,10 @@ __global__ __launch_bounds__(kThreads) void cache_append_kernel(
                                : static_cast<const void *>(static_cast<const uint16_t *>(k) + off);
         const float *in = kCodes ? k_in_scale + static_cast<int64_t>(b * pages.hkv + h) * ((len + kPage - 1) / kPage) : nullptr;
         write_keys<D, kType, kCodes>(x, k_sl, in, first, k_mean ? k_mean + static_cast<int64_t>(b * pages.hkv + h) * D : nullptr,
-                                     k_codes + at * kPage * D, k_scale + at, lo, lo, hi, part);
+                                     k_codes, k_scale, at, lo, lo, hi, part);
     } else {
         write_values<D, kType>(static_cast<const uint16_t *>(v) + b * v_sb + h * v_sh + first * v_sl, v_sl,
-                               v_codes + at * kPage * D, v_scale + at, lo, lo, hi, part, turn);
+                               v_codes, v_scale, at, lo, lo, hi, part, turn);
     }
 }
 
