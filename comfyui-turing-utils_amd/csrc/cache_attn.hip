@@ -18,9 +18,9 @@
 // less 64: its values are then too small to matter (2^-57 of the largest term),
 // and w stays a normal number for the row sum.
 //
-// Two kernels: few rows a K/V head (single tokens) read every code once from HBM
-// into registers; many rows share K and V tiles in LDS.  Both split a sequence's
-// pages into ranges where the grid would leave the chip empty; a third merges.
+// Two kernels: blocks of 16 rows (single tokens) read codes straight into registers;
+// blocks of 128 or 256 share K and V tiles in LDS.  Both split a sequence's pages into
+// ranges where the grid would leave the chip empty; a third merges.
 #include <algorithm>
 #include <type_traits>
 
@@ -301,13 +301,15 @@ __device__ __forceinline__ bool higher(float m, float v, float than_m, float tha
 // ---------------------------------------------------------------------------
 // Few rows
 // ---------------------------------------------------------------------------
-// A workgroup of four waves has 16 kRT rows of one K/V head; its waves take the
+// A workgroup of four waves has 16 rows of one K/V head (more rows: more workgroups,
+// whose codes come from L2 but for the first); its waves take the
 // pages of the unit's range in turn, each for itself, and are merged at the end.
 // A wave reads a page's codes straight into the MFMA operands: keys 16 g + e of a
 // page belong to lane group g throughout, so that a lane's 16 bytes of a V^T row
 // are the keys whose weights it holds, and a key row's bytes go to the lanes in
 // runs of D / 4.  The next page's loads (16 KiB a wave at D = 128) are in flight
 // while one is computed: what a CU needs to keep HBM busy.
+constexpr int kFewRows = 16;
 template <int D>
 struct PageRegs {
     i32x4 k[4][D / 64];
@@ -325,24 +327,21 @@ struct PageRegs {
     }
 };
 
-template <int D, int kRT>
-__global__ __launch_bounds__(kThreads, D == 128 && kRT == 2 ? 1 : 2) void cache_few_kernel(CacheCall c) {
-    constexpr int kSl = D / 64, kDS = D / 16, kRows = 16 * kRT;
-    __shared__ __align__(16) float merge_o[3][kRT][kDS][64][4];
-    __shared__ float merge_m[4][kRT][64][3];
+template <int D>
+__global__ __launch_bounds__(kThreads, 2) void cache_few_kernel(CacheCall c) {
+    constexpr int kSl = D / 64, kDS = D / 16;
+    __shared__ __align__(16) float merge_o[3][kDS][64][4];
+    __shared__ float merge_m[4][64][3];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int g = lane >> 4, lc = lane & 15;
-    const Unit u = unit_at<kRows>(c);
+    const Unit u = unit_at<kFewRows>(c);
     if (u.z > 0 && static_cast<int>(u.z) >= u.used) return;  // the whole workgroup: nothing is left for the range
     // The loads of a start, in an order that leaves three in a row (length; rows and
     // table; codes and scales): one token of 32 heads over 4000, 12.3 -> 11.4 us.
-    RowBits<kSl> bits[kRT];
-#pragma unroll
-    for (int rt = 0; rt < kRT; ++rt) {
-        const uint32_t r = u.block * kRows + 16 * rt + lc;
-        const Row row = row_at(c, u.hk, r);
-        bits[rt] = fetch_row<kSl, true>(c, row, u.b, r < c.rows && row.token < u.n, D / 4 * g, 16);
-    }
+    const uint32_t r = u.block * kFewRows + lc;
+    const Row row = row_at(c, u.hk, r);
+    const bool in = r < c.rows && row.token < u.n;
+    const RowBits<kSl> bits = fetch_row<kSl, true>(c, row, u.b, in, D / 4 * g, 16);
     PageWindow window;
     int base = u.first + wave;  // page of the window's lane 0; the wave's pages are 4 apart
     window.fetch(c, u, base, 4, lane);
@@ -352,90 +351,79 @@ __global__ __launch_bounds__(kThreads, D == 128 && kRT == 2 ? 1 : 2) void cache_
     PageRegs<D> even, odd;
     int p = base;
     if (p < u.end) even.load(c, place(p), g, lc);
-    i32x4 qh[kRT][kSl], ql[kRT][kSl];
-    float factor[kRT];
-    int limit[kRT];
-    RowState st[kRT];
-    f32x4 o[kRT][kDS];
+    i32x4 qh[kSl], ql[kSl];
+    const float factor = row_codes<kSl, true>(c, bits, qh, ql);
+    const int limit = in ? keys_of(c, row.token, u.n, u.length) : 0;
+    RowState st;
+    f32x4 o[kDS];
 #pragma unroll
-    for (int rt = 0; rt < kRT; ++rt) {
-        const uint32_t r = u.block * kRows + 16 * rt + lc;
-        const Row row = row_at(c, u.hk, r);
-        const bool in = r < c.rows && row.token < u.n;
-        factor[rt] = row_codes<kSl, true>(c, bits[rt], qh[rt], ql[rt]);
-        limit[rt] = in ? keys_of(c, row.token, u.n, u.length) : 0;
-#pragma unroll
-        for (int ds = 0; ds < kDS; ++ds) o[rt][ds] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
-    }
+    for (int ds = 0; ds < kDS; ++ds) o[ds] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
 
     auto compute = [&](const PageRegs<D> &r, int p) {
         const int at = (p - base) >> 2;
         const bool there = window.there(at);
         const float k_scale = lane_value(window.k_scale, at), v_log2 = lane_value(window.v_log2, at);
         const int key0 = p * kPage + 16 * g;  // the lane's keys are key0 ..+15
+        i32x4 s[4];
 #pragma unroll
-        for (int rt = 0; rt < kRT; ++rt) {
-            i32x4 s[4];
+        for (int t = 0; t < 4; ++t) {
+            i32x4 acc = {0, 0, 0, 0};
 #pragma unroll
-            for (int t = 0; t < 4; ++t) {
-                i32x4 acc = {0, 0, 0, 0};
+            for (int i = 0; i < kSl; ++i) acc = __builtin_amdgcn_mfma_i32_16x16x64_i8(r.k[t][i], qh[i], acc, 0, 0, 0);
+            acc <<= 8;
 #pragma unroll
-                for (int i = 0; i < kSl; ++i) acc = __builtin_amdgcn_mfma_i32_16x16x64_i8(r.k[t][i], qh[rt][i], acc, 0, 0, 0);
-                acc <<= 8;
+            for (int i = 0; i < kSl; ++i) acc = __builtin_amdgcn_mfma_i32_16x16x64_i8(r.k[t][i], ql[i], acc, 0, 0, 0);
+            s[t] = acc;
+        }
+        const float f = factor * k_scale;
+        const int seen = there ? limit - key0 : 0;  // the first so many of the lane's keys
+        float x[16], top = -INFINITY;
 #pragma unroll
-                for (int i = 0; i < kSl; ++i) acc = __builtin_amdgcn_mfma_i32_16x16x64_i8(r.k[t][i], ql[rt][i], acc, 0, 0, 0);
-                s[t] = acc;
+        for (int e = 0; e < 16; ++e) {
+            x[e] = static_cast<float>(s[e >> 2][e & 3]) * f;
+            if (e < seen) top = fmaxf(top, x[e]);
+        }
+        const bool need = (top - st.m) + (v_log2 - st.v) > kSlack;
+        if (__any(need)) {
+            // a row's base moves by its own scores alone
+            const float row_top = xmax_f32(top);
+            if ((row_top - st.m) + (v_log2 - st.v) > kSlack) {
+                const float alpha = __builtin_amdgcn_exp2f((st.m - row_top) + (st.v - v_log2));
+                st.m = row_top, st.v = v_log2;
+                st.l *= alpha;
+#pragma unroll
+                for (int ds = 0; ds < kDS; ++ds) o[ds] *= alpha;
             }
-            const float f = factor[rt] * k_scale;
-            const int seen = there ? limit[rt] - key0 : 0;  // the first so many of the lane's keys
-            float x[16], top = -INFINITY;
+        }
+        const float d = st.shift(v_log2);
+        float sum = 0.0f;
+        f16x8 w[2];
 #pragma unroll
-            for (int e = 0; e < 16; ++e) {
-                x[e] = static_cast<float>(s[e >> 2][e & 3]) * f;
-                if (e < seen) top = fmaxf(top, x[e]);
-            }
-            const bool need = (top - st[rt].m) + (v_log2 - st[rt].v) > kSlack;
-            if (__any(need)) {
-                // a row's base moves by its own scores alone
-                const float row_top = xmax_f32(top);
-                if ((row_top - st[rt].m) + (v_log2 - st[rt].v) > kSlack) {
-                    const float alpha = __builtin_amdgcn_exp2f((st[rt].m - row_top) + (st[rt].v - v_log2));
-                    st[rt].m = row_top, st[rt].v = v_log2;
-                    st[rt].l *= alpha;
+        for (int h = 0; h < 2; ++h) {
+            u32x4 packed;
 #pragma unroll
-                    for (int ds = 0; ds < kDS; ++ds) o[rt][ds] *= alpha;
+            for (int j = 0; j < 4; ++j) {
+                float y[2];
+#pragma unroll
+                for (int i = 0; i < 2; ++i) {
+                    const int e = 8 * h + 2 * j + i;
+                    y[i] = e < seen ? __builtin_amdgcn_exp2f((x[e] - st.m) + (d + kUp)) : 0.0f;
+                    sum += y[i];
                 }
+                packed[j] = hw_f16x2_bits(y[0], y[1]);
             }
-            const float d = st[rt].shift(v_log2);
-            float sum = 0.0f;
-            f16x8 w[2];
+            w[h] = __builtin_bit_cast(f16x8, packed);
+        }
+        // w / v_scale, the scale being 2^(base's + d) (a lane without keys has no part in a NaN)
+        if (seen > 0) st.l = __builtin_fmaf(sum, __builtin_amdgcn_exp2f(-(st.v + d)), st.l);
+        if (window.zeros(at)) return;
+#pragma unroll
+        for (int ds = 0; ds < kDS; ++ds) {
 #pragma unroll
             for (int h = 0; h < 2; ++h) {
-                u32x4 packed;
-#pragma unroll
-                for (int j = 0; j < 4; ++j) {
-                    float y[2];
-#pragma unroll
-                    for (int i = 0; i < 2; ++i) {
-                        const int e = 8 * h + 2 * j + i;
-                        y[i] = e < seen ? __builtin_amdgcn_exp2f((x[e] - st[rt].m) + (d + kUp)) : 0.0f;
-                        sum += y[i];
-                    }
-                    packed[j] = hw_f16x2_bits(y[0], y[1]);
-                }
-                w[h] = __builtin_bit_cast(f16x8, packed);
-            }
-            // w / v_scale, the scale being 2^(base's + d) (a lane without keys has no part in a NaN)
-            if (seen > 0) st[rt].l = __builtin_fmaf(sum, __builtin_amdgcn_exp2f(-(st[rt].v + d)), st[rt].l);
-            if (window.zeros(at)) continue;
-#pragma unroll
-            for (int ds = 0; ds < kDS; ++ds) {
-#pragma unroll
-                for (int h = 0; h < 2; ++h) {
-                    const u32x2 a = codes_to_f16(r.v[ds][2 * h], Selectors{}), b = codes_to_f16(r.v[ds][2 * h + 1], Selectors{});
-                    const f16x8 v = __builtin_bit_cast(f16x8, (u32x4{a[0], a[1], b[0], b[1]}));
-                    o[rt][ds] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v, w[h], o[rt][ds], 0, 0, 0);
-                }
+                const u32x2 a = codes_to_f16(r.v[ds][2 * h], Selectors{}), b = codes_to_f16(r.v[ds][2 * h + 1], Selectors{});
+                const f16x8 v = __builtin_bit_cast(f16x8, (u32x4{a[0], a[1], b[0], b[1]}));
+                o[ds] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v, w[h], o[ds], 0, 0, 0);
             }
         }
     };
@@ -457,51 +445,45 @@ __global__ __launch_bounds__(kThreads, D == 128 && kRT == 2 ? 1 : 2) void cache_
     }
 
     // The waves' states, merged by the first.
-    const bool alone = u.end - u.first <= 1;
-#pragma unroll
-    for (int rt = 0; rt < kRT; ++rt) {
-        st[rt].l = xsum_f32(st[rt].l);
-        if (alone) continue;
-        merge_m[wave][rt][lane][0] = st[rt].m;
-        merge_m[wave][rt][lane][1] = st[rt].v;
-        merge_m[wave][rt][lane][2] = st[rt].l;
+    st.l = xsum_f32(st.l);
+    if (u.end - u.first > 1) {
+        merge_m[wave][lane][0] = st.m;
+        merge_m[wave][lane][1] = st.v;
+        merge_m[wave][lane][2] = st.l;
         if (wave > 0) {
 #pragma unroll
-            for (int ds = 0; ds < kDS; ++ds) *reinterpret_cast<f32x4 *>(merge_o[wave - 1][rt][ds][lane]) = o[rt][ds];
+            for (int ds = 0; ds < kDS; ++ds) *reinterpret_cast<f32x4 *>(merge_o[wave - 1][ds][lane]) = o[ds];
         }
+        __syncthreads();
     }
-    if (!alone) __syncthreads();
     if (wave > 0) return;
+    if (u.end - u.first > 1) {
+        float m = st.m, v = st.v;
 #pragma unroll
-    for (int rt = 0; rt < kRT; ++rt) {
-        if (!alone) {
-            float m = st[rt].m, v = st[rt].v;
-#pragma unroll
-            for (int i = 1; i < 4; ++i) {
-                const float mi = merge_m[i][rt][lane][0], vi = merge_m[i][rt][lane][1];
-                if (merge_m[i][rt][lane][2] != 0.0f && higher(mi, vi, m, v)) m = mi, v = vi;
-            }
-            float l = 0.0f;
-            f32x4 sum[kDS] = {};
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                const float li = merge_m[i][rt][lane][2];
-                if (li == 0.0f) continue;  // saw nothing
-                const float wi = __builtin_amdgcn_exp2f((merge_m[i][rt][lane][0] - m) + (merge_m[i][rt][lane][1] - v));
-                l = __builtin_fmaf(wi, li, l);
-#pragma unroll
-                for (int ds = 0; ds < kDS; ++ds) {
-                    const f32x4 x = i == 0 ? o[rt][ds] : *reinterpret_cast<const f32x4 *>(merge_o[i - (i > 0)][rt][ds][lane]);
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) sum[ds][e] = __builtin_fmaf(wi, x[e], sum[ds][e]);
-                }
-            }
-            st[rt].m = m, st[rt].v = v, st[rt].l = l;
-#pragma unroll
-            for (int ds = 0; ds < kDS; ++ds) o[rt][ds] = sum[ds];
+        for (int i = 1; i < 4; ++i) {
+            const float mi = merge_m[i][lane][0], vi = merge_m[i][lane][1];
+            if (merge_m[i][lane][2] != 0.0f && higher(mi, vi, m, v)) m = mi, v = vi;
         }
-        store_row<D>(c, u, o[rt], st[rt].m, st[rt].v, st[rt].l, u.block * kRows + 16 * rt + lc, g);
+        float l = 0.0f;
+        f32x4 sum[kDS] = {};
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const float li = merge_m[i][lane][2];
+            if (li == 0.0f) continue;  // saw nothing
+            const float wi = __builtin_amdgcn_exp2f((merge_m[i][lane][0] - m) + (merge_m[i][lane][1] - v));
+            l = __builtin_fmaf(wi, li, l);
+#pragma unroll
+            for (int ds = 0; ds < kDS; ++ds) {
+                const f32x4 x = i == 0 ? o[ds] : *reinterpret_cast<const f32x4 *>(merge_o[i - (i > 0)][ds][lane]);
+#pragma unroll
+                for (int e = 0; e < 4; ++e) sum[ds][e] = __builtin_fmaf(wi, x[e], sum[ds][e]);
+            }
+        }
+        st.m = m, st.v = v, st.l = l;
+#pragma unroll
+        for (int ds = 0; ds < kDS; ++ds) o[ds] = sum[ds];
     }
+    store_row<D>(c, u, o, st.m, st.v, st.l, r, g);
 }
 
 // ---------------------------------------------------------------------------
@@ -513,9 +495,10 @@ __global__ __launch_bounds__(kThreads, D == 128 && kRT == 2 ? 1 : 2) void cache_
 // each other: one's MFMAs beside the other's softmax.  Pages stream through LDS: keys
 // as codes by direct-to-LDS loads, a ring of four; values through registers, converted
 // to fp16 once, a ring of two.
-//   Bound by instruction issue: a wave's step at D = 128 is 832 cycles of MFMAs of the
-// 1700 that it takes, and the two waves of a SIMD issue into the rest.  4680 rows
-// x 32760 keys, 40 heads, int8 queries: 2.26 ms, 1390 TFLOP/s (one group: 2.45 ms).
+//   Bound by issue, near the power limit: a step of 256 rows takes 1.42 us at D = 128;
+// its MFMAs, LDS reads and softmax alone, in the same phases on random operands, 1.22,
+// at 1.9 GHz.  4680 rows x 32760 keys, 40 heads, int8 queries: 2.2 ms, 1400 TFLOP/s
+// (one group: 2.45 ms).
 constexpr int kQT = 2;           // 16-row fragments of a wave
 constexpr int kWaveRows = 16 * kQT;
 constexpr int kGroupRows = 4 * kWaveRows;
@@ -1160,34 +1143,39 @@ __global__ __launch_bounds__(kThreads) void cache_merge_kernel(CacheCall c) {
 // The plan
 // ---------------------------------------------------------------------------
 struct CachePlan {
-    int32_t rows;  // of a row block: 16 or 32 (few rows), 128 or 256 (many)
+    int32_t rows;  // of a row block: kFewRows, or 128 or 256 (many)
     uint32_t row_blocks, parts;
 };
 
-// Ranges of a launch of few rows: as many as its workgroups have places at once (two
-// a CU, or one for 32 rows at D = 128), each of at least one page for every wave.  One
-// more would begin a second round: 131040 keys, 40 heads: 12 ranges 235 us, 13 319.
-// One workgroup a CU reads as fast as two (32 x 8 heads: 1 range 82, 2 ranges 87),
-// and up to 12 pages a merge costs more than it saves (513 keys at D = 64: 7.5, 9.9).
-int64_t few_parts(int64_t units, int64_t pages, int64_t slots, int64_t cus) {
-    return units >= cus || pages <= 12 ? 1 : std::min(slots / units, (pages + 3) / 4);
-}
+// What a block of rows costs, in steps of a page at 256 rows (1.6 us at D = 128): a step
+// on a CU that has one, two or three of its workgroups (as many as `places`), and the
+// pages that a start and an end take as long as.
+struct BlockCost {
+    int32_t rows;
+    int64_t places;
+    double step[3], start;
+};
+constexpr BlockCost kFewCost = {kFewRows, 2, {0.28, 0.575, 0.0}, 7.0};
+constexpr BlockCost kManyCost = {kGroupRows, 2, {0.78, 1.08, 1.4}, 4.0};
+constexpr BlockCost kTwoGroupsCost = {2 * kGroupRows, 1, {1.0, 0.0, 0.0}, 4.0};
 
-// Time of a launch of many rows, in steps of a page at 256 rows (1.6 us at D = 128).
-// Blocks of 128 rows run up to `places` to a CU: a step takes 0.78 of that for one, 1.08
-// for two and 1.4 for three.  Blocks of 256 run one to a CU.  A unit costs 4 steps over
-// its pages, a merge 3 and its bytes, 7 MB a step (at 256 CUs).
-//   Measured, us, 128 / 256 rows a block: 4680 rows x 32760 keys, 40 heads, int8
-// queries 2450 / 2240; 33 rows x 4 heads a K/V head, 8192 keys, 16 ranges 30.5 /
-// 34.8; 1560 x 9360, 12 heads, by ranges: 1: 184 / 214, 2: 133 / 125, 3: 99 / 97,
-// 4: 120 / 133, 6: 111 / 111; 8192 x 4096 at D = 64, 12 heads: 115 / 147.
+// Time of a launch: its rounds of the places there are, and a merge: 3 steps and its
+// bytes, 7 MB a step (at 256 CUs).
+//   Measured, us, blocks of 16 / 128 rows, each at its best number of ranges: 64 rows of
+// 8 K/V heads x 8192 keys 18 / 27, 256 rows 37 / 34, 64 rows of 40 heads x 2048 19 / 24,
+// 64 of 128 heads 34 / 36, 77 of 12 heads x 513 at D = 64 7.2 / 13.  One round more is
+// dear: one row of 40 heads x 131040, 12 ranges 235, 13 319; and one workgroup a CU reads
+// as fast as two (one row of 256 heads x 8190: 1 range 82, 2 ranges 87).
+//   128 / 256 rows: 4680 rows x 32760 keys, 40 heads, int8 queries 2450 / 2240; 1560 x
+// 9360, 12 heads, by ranges: 1: 184 / 214, 2: 133 / 125, 3: 99 / 97, 4: 120 / 133, 6:
+// 111 / 111; 8192 x 4096 at D = 64, 12 heads: 115 / 147.
 //   Causal: empty ranges of early blocks end at once, and long blocks go first.
 // 4001 x 4001, 2 x 16 heads: 1 range 143, 2 ranges 224; 2050 x 6000 at D = 64, 18
 // heads, 128 rows a block: 123, 87.
-double many_cost(int64_t units, int64_t parts, int64_t pages, double share, bool causal, int64_t places, double part_bytes,
-                 int64_t cus) {
-    const int64_t slots = (places ? places : 1) * cus;
-    auto step = [&](double n) { return !places || n <= 0.0 ? (n > 0.0) * 1.0 : n <= cus ? 0.78 : n <= 2 * cus ? 1.08 : 1.4; };
+double launch_cost(const BlockCost &b, int64_t units, int64_t parts, int64_t per, double share, bool causal, double part_bytes,
+                   int64_t cus) {
+    const int64_t slots = b.places * cus;
+    auto step = [&](double n) { return n <= 0.0 ? 0.0 : n <= cus ? b.step[0] : n <= 2 * cus ? b.step[1] : b.step[2]; };
     const double n = static_cast<double>(units * parts) * share, full = n / static_cast<double>(slots);
     double steps = step(n);
     if (full > 1.0) {
@@ -1195,37 +1183,42 @@ double many_cost(int64_t units, int64_t parts, int64_t pages, double share, bool
         steps = causal ? (full + 0.5) * step(slots)
                        : static_cast<double>(rounds) * step(slots) + step(static_cast<double>(units * parts - rounds * slots));
     }
-    const double per = static_cast<double>((pages + parts - 1) / parts);
     const double merge = parts > 1 ? 3.0 + static_cast<double>(parts) * part_bytes * 2.0 / (7e6 * static_cast<double>(cus) / 256.0) : 0.0;
-    return steps * (per + 4.0) + merge;
+    return steps * (static_cast<double>(per) + b.start) + merge;
 }
 
 CachePlan cache_plan(int64_t batch, int64_t hkv, int64_t lq, int64_t group, int64_t dim, int64_t pages, bool int8, bool causal,
                      int64_t cus, int64_t max_bytes) {
     const int64_t rows = lq * group;
     const int64_t row_bytes = batch * hkv * rows * (dim + 4) * static_cast<int64_t>(sizeof(float));
-    const int64_t most = std::min<int64_t>(max_bytes / row_bytes, 256);
-    auto plan = [&](int32_t block, int64_t parts) {
-        return CachePlan{block, static_cast<uint32_t>((rows + block - 1) / block), static_cast<uint32_t>(std::max<int64_t>(parts, 1))};
-    };
-    if (rows <= 32) {
-        const int64_t slots = rows > 16 && dim == 128 ? cus : 2 * cus;
-        return plan(rows <= 16 ? 16 : 32, std::min(few_parts(batch * hkv, pages, slots, cus), most));
-    }
     // of a causal call's keys, the part that its mean row sees
     const double tokens = static_cast<double>(pages * kPage);
     const double share = causal ? std::max(0.5, 1.0 - 0.5 * static_cast<double>(lq) / tokens) : 1.0;
     CachePlan best{};
     double best_cost = 0.0;
-    for (const int32_t block : {256, 128}) {
-        const CachePlan one = plan(block, 1);
-        const int64_t units = batch * hkv * one.row_blocks;
-        for (int64_t parts = 1; parts == 1 || (parts <= std::min<int64_t>(most, 64) && 2 * parts <= pages && units * (parts - 1) < 4 * cus);
-             ++parts) {
-            const double cost = many_cost(units, parts, pages, share, causal, block == 256 ? 0 : dim == 64 && int8 ? 3 : 2,
-                                          static_cast<double>(row_bytes), cus);
-            if (!best.rows || cost < best_cost) best = plan(block, parts), best_cost = cost;
+    auto consider = [&](const BlockCost &b) {
+        const int64_t blocks = (rows + b.rows - 1) / b.rows, units = batch * hkv * blocks;
+        // (a page for each wave of few rows, two pages of many)
+        const int64_t most = std::min<int64_t>(max_bytes / row_bytes, b.rows == kFewRows ? std::min<int64_t>((pages + 3) / 4, 256)
+                                                                                         : std::min<int64_t>(pages / 2, 64));
+        for (int64_t parts = 1;;) {
+            const int64_t per = (pages + parts - 1) / parts;
+            const double cost = launch_cost(b, units, parts, per, share, causal, static_cast<double>(row_bytes), cus);
+            if (!best.rows || cost < best_cost) {
+                best = CachePlan{b.rows, static_cast<uint32_t>(blocks), static_cast<uint32_t>(parts)};
+                best_cost = cost;
+            }
+            if (per == 1 || units * parts > 3 * b.places * cus) break;
+            parts = (pages + per - 2) / (per - 1);  // the next number of ranges that are shorter
+            if (parts > most) break;
         }
+    };
+    consider(kFewCost);
+    if (rows > kFewRows) {
+        BlockCost many = kManyCost;
+        if (dim == 64 && int8) many.places = 3;
+        consider(many);
+        consider(kTwoGroupsCost);
     }
     return best;
 }
@@ -1312,12 +1305,9 @@ extern "C" int32_t tu_kv_cache_attn(const void *q, const float *q_scale, int32_t
     } while (0)
 #define TU_CACHE_ATTN(D)                                                                                               \
     do {                                                                                                               \
-        if (plan.rows == 16) {                                                                                         \
-            cache_few_kernel<D, 1><<<grid, kThreads, 0, s>>>(c);                                                       \
-            TU_CACHE_MERGE(D, 16, kThreads / (D / 8));                                                                 \
-        } else if (plan.rows == 32) {                                                                                  \
-            cache_few_kernel<D, 2><<<grid, kThreads, 0, s>>>(c);                                                       \
-            TU_CACHE_MERGE(D, 32, kThreads / (D / 8));                                                                 \
+        if (plan.rows == kFewRows) {                                                                                   \
+            cache_few_kernel<D><<<grid, kThreads, 0, s>>>(c);                                                          \
+            TU_CACHE_MERGE(D, kFewRows, kThreads / (D / 8));                                                           \
         } else if (plan.rows == 128) {                                                                                 \
             if (q_type == kQInt8) cache_many_kernel<D, false, 1><<<grid, 256, 0, s>>>(c);                              \
             else cache_many_kernel<D, true, 1><<<grid, 256, 0, s>>>(c);                                                \

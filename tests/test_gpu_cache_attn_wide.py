@@ -1,6 +1,6 @@
-"""GPU: attention over the key/value cache in 8 bits at calls that fill the chip: more
-blocks of 128 rows than compute units, which the launch takes as blocks of 256, with
-and without a split of the keys.  The same properties and bounds as at small calls."""
+"""GPU: attention over the key/value cache in 8 bits at calls of so many rows that the
+launch takes them in blocks of 128, or, with more of those than compute units, of 256,
+with and without a split of the keys.  The same properties and bounds as at small calls."""
 from __future__ import annotations
 
 import pytest
@@ -12,17 +12,23 @@ from tests.test_gpu_cache_attn import _check, _ints, _pool, _query
 
 pytestmark = pytest.mark.gpu
 
-HEADS = 66  # times two sequences, two blocks of 128 rows each: 264 blocks
+
+
+@pytest.fixture(params=[33, 66])
+def heads(request):
+    """K/V heads of two sequences: of two blocks of 128 rows each 132 blocks, taken as they are, or 264, taken as 132 of
+    256."""
+    return request.param
 
 
 @pytest.mark.parametrize("d", [64, 128])
 @pytest.mark.parametrize("kind", ["bf16", "f16", "int8"])
 @pytest.mark.parametrize("causal", [False, True])
 @pytest.mark.parametrize("lq,lengths,counts", [(256, [256, 130], None), (131, [131, 576], [131, 7]), (250, [2, 500], [2, 250])])
-def test_chunks(gpu_device, d, kind, causal, lq, lengths, counts):
-    pool, table, g = _pool(gpu_device, 2, HEADS, d, 9, d + lq)
+def test_chunks(gpu_device, heads, d, kind, causal, lq, lengths, counts):
+    pool, table, g = _pool(gpu_device, 2, heads, d, 9, d + lq)
     layout = "NHD" if lq % 2 else "HND"
-    q, kw = _query(gpu_device, 2, HEADS, lq, d, kind, layout, g)
+    q, kw = _query(gpu_device, 2, heads, lq, d, kind, layout, g)
     got = _check(q, pool, table, _ints(lengths, gpu_device), layout, causal, query_lengths=_ints(counts, gpu_device), **kw)
     again = turing_sage.kv_cache_attention(q, turing_sage.QuantizedKVCache(*pool), table, _ints(lengths, gpu_device),
                                            tensor_layout=layout, is_causal=causal, query_lengths=_ints(counts, gpu_device), **kw)
@@ -30,26 +36,26 @@ def test_chunks(gpu_device, d, kind, causal, lq, lengths, counts):
 
 
 @pytest.mark.parametrize("kind", ["bf16", "int8"])
-def test_shared_heads(gpu_device, kind):
-    pool, table, g = _pool(gpu_device, 2, HEADS, 64, 4, 3)
-    q, kw = _query(gpu_device, 2, 3 * HEADS, 70, 64, kind, "NHD", g)
+def test_shared_heads(gpu_device, heads, kind):
+    pool, table, g = _pool(gpu_device, 2, heads, 64, 4, 3)
+    q, kw = _query(gpu_device, 2, 3 * heads, 70, 64, kind, "NHD", g)
     _check(q, pool, table, _ints([200, 70], gpu_device), "NHD", True, **kw)
 
 
-def test_pages_that_are_none(gpu_device):
-    pool, table, g = _pool(gpu_device, 2, HEADS, 64, 9, 7)
+def test_pages_that_are_none(gpu_device, heads):
+    pool, table, g = _pool(gpu_device, 2, heads, 64, 9, 7)
     table[0, 2], table[0, 3], table[0, 8], table[1, 0] = -1, 10 ** 6, -5, -(10 ** 9)
-    q, kw = _query(gpu_device, 2, HEADS, 200, 64, "int8", "HND", g)
+    q, kw = _query(gpu_device, 2, heads, 200, 64, "int8", "HND", g)
     for causal in (False, True):
         _check(q, pool, table, _ints([570, 300], gpu_device), causal=causal, **kw)
 
 
 @pytest.mark.parametrize("which,value", [(2, float("nan")), (3, float("inf")), (3, float("nan"))])
-def test_scales_that_are_no_numbers(gpu_device, which, value):
+def test_scales_that_are_no_numbers(gpu_device, heads, which, value):
     """NaN in the rows that see the page, nothing elsewhere."""
-    pool, table, g = _pool(gpu_device, 2, HEADS, 64, 6, 9)
+    pool, table, g = _pool(gpu_device, 2, heads, 64, 6, 9)
     lengths = _ints([380, 384], gpu_device)
-    q, _ = _query(gpu_device, 2, HEADS, 200, 64, "bf16", "HND", g)
+    q, _ = _query(gpu_device, 2, heads, 200, 64, "bf16", "HND", g)
     want = _check(q, pool, table, lengths, causal=True)
     pool[which][int(table[0, 4]), 5] = value  # keys 256 .. 319: of rows 76 on
     got = turing_sage.kv_cache_attention(q, turing_sage.QuantizedKVCache(*pool), table, lengths, is_causal=True)
@@ -60,19 +66,19 @@ def test_scales_that_are_no_numbers(gpu_device, which, value):
 
 
 @pytest.mark.parametrize("ratio", [1e-9, 1e-25, 0.0])
-def test_pages_of_unlike_value_scales(gpu_device, ratio):
-    pool, table, g = _pool(gpu_device, 2, HEADS, 64, 6, 9)
+def test_pages_of_unlike_value_scales(gpu_device, heads, ratio):
+    pool, table, g = _pool(gpu_device, 2, heads, 64, 6, 9)
     scales = pool[3].clone()
     scales[table[0, ::2].long()] *= ratio
     scales[table[1, 1:3].long()] *= ratio
-    q, _ = _query(gpu_device, 2, HEADS, 140, 64, "bf16", "HND", g)
+    q, _ = _query(gpu_device, 2, heads, 140, 64, "bf16", "HND", g)
     _check(q, [*pool[:3], scales], table, _ints([384, 250], gpu_device))
 
 
 @pytest.mark.parametrize("size", [1e-6, 50.0, 1e4, 1e30])
-def test_scores_of_any_size(gpu_device, size):
-    pool, table, g = _pool(gpu_device, 2, HEADS, 64, 4, 11)
-    q, kw = _query(gpu_device, 2, HEADS, 140, 64, "int8", "HND", g)
+def test_scores_of_any_size(gpu_device, heads, size):
+    pool, table, g = _pool(gpu_device, 2, heads, 64, 4, 11)
+    q, kw = _query(gpu_device, 2, heads, 140, 64, "int8", "HND", g)
     kw["query_scale"] = kw["query_scale"] * size
     lengths = _ints([200, 256], gpu_device)
     if size < 1e30:
@@ -86,7 +92,7 @@ def test_scores_of_any_size(gpu_device, size):
     clear = 0
     for b, length in enumerate((200, 256)):
         k, v, ks, vs, _ = ref.sequence(pool, table, length, b)
-        for h in range(HEADS):
+        for h in range(heads):
             x = q[b, h].double() * kw["query_scale"][b, h].double().repeat_interleave(16)[:140, None]
             s = (x @ k[h].t()) * 0.125 * ks[h]
             s.masked_fill_(torch.arange(length, device=s.device) > length - 140 + torch.arange(140, device=s.device)[:, None], -torch.inf)
@@ -97,7 +103,7 @@ def test_scores_of_any_size(gpu_device, size):
             assert bool((off <= (2.0 ** -8 + 2.0 ** -20) * want.abs())[wins].all()), (b, h)
             assert bool((got[b, h].abs() <= (v[h] * vs[h][:, None]).abs().amax(0) * (1 + 2.0 ** -8 + 2.0 ** -9)).all()), (b, h)
             clear += int(wins.sum())
-    assert clear > 0.99 * 2 * HEADS * 140
+    assert clear > 0.99 * 2 * heads * 140
 
 
 @pytest.mark.parametrize("causal", [False, True])
@@ -113,10 +119,11 @@ def test_a_split_of_many_rows(gpu_device, causal, d, heads):
         _check(q, pool, table, _ints([length], gpu_device), "NHD", causal, **kw)
 
 
-def test_windows_of_pages(gpu_device):
-    """One range of more pages than a wave knows at once, at 256 rows a block."""
-    pool, table, g = _pool(gpu_device, 1, 130, 64, 150, 6)
-    q, kw = _query(gpu_device, 1, 130, 260, 64, "int8", "HND", g)
+@pytest.mark.parametrize("count", [60, 120])
+def test_windows_of_pages(gpu_device, count):
+    """One range of more pages than a wave knows at once, at 128 and at 256 rows a block."""
+    pool, table, g = _pool(gpu_device, 1, count, 64, 150, 6)
+    q, kw = _query(gpu_device, 1, count, 260, 64, "int8", "HND", g)
     table[0, 70] = -1
     for causal in (False, True):
         _check(q, pool, table, _ints([9570], gpu_device), causal=causal, **kw)
