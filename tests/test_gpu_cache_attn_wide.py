@@ -107,15 +107,17 @@ def test_scores_of_any_size(gpu_device, heads, size):
 
 
 @pytest.mark.parametrize("causal", [False, True])
-@pytest.mark.parametrize("d,heads", [(64, 18), (128, 12)])
-def test_a_split_of_many_rows(gpu_device, causal, d, heads):
-    """Long keys and too few blocks of rows for the chip (of 128 rows at d = 64, of 256 at d = 128): ranges of keys,
-    past the pages that a wave knows at once."""
+@pytest.mark.parametrize("d,heads,lq,kind", [(64, 18, 1020, "int8"), (64, 12, 1020, "bf16"), (128, 12, 1020, "int8"),
+                                             (128, 8, 120, "f16")])
+def test_a_split_of_many_rows(gpu_device, causal, d, heads, lq, kind):
+    """Long keys and too few blocks of rows for the chip (of 128 rows in the first and last case, of 256 in the others):
+    ranges of keys, past the pages that a wave knows at once."""
     pool, table, g = _pool(gpu_device, 1, heads, d, 400, 5)
-    q, kw = _query(gpu_device, 1, heads, 1020, d, "int8", "NHD", g)
+    q, kw = _query(gpu_device, 1, heads, lq, d, kind, "NHD", g)
     most, cus = 25600, torch.cuda.get_device_properties(gpu_device).multi_processor_count
-    assert _lib.load().tu_kv_cache_attn_workspace(1, heads, heads, 1020, d, most, 2, int(causal), cus) > 0
-    for length in (25555, 9000, 1020):
+    code = dict(bf16=0, f16=1, int8=2)[kind]
+    assert _lib.load().tu_kv_cache_attn_workspace(1, heads, heads, lq, d, most, code, int(causal), cus) > 0
+    for length in (25555, 9000, lq):
         _check(q, pool, table, _ints([length], gpu_device), "NHD", causal, **kw)
 
 
