@@ -228,15 +228,18 @@ struct PageWindow {
         at = (there ? p : 0) * static_cast<int>(c.hkv) + static_cast<int>(u.hk);
         none = __ballot(!there);
         k_scale = c.k_scale[at];
-        // (a NaN stays; below 2^-90, where a sum of weights over the scale might be
-        // no number, the values count as zeros of that scale)
-        const float v = c.v_scale[at];
+        v_log2 = c.v_scale[at];
+    }
+    // What follows from the scales, which have landed then (here, and not in a loop that
+    // uses them).  A NaN stays; below 2^-90, where a sum of weights over the scale might
+    // be no number, the values count as zeros of that scale.
+    __device__ __forceinline__ void landed() {
+        const float v = v_log2;
         zero = __ballot(v <= 8.077935669e-28f);
         v_log2 = v <= 8.077935669e-28f ? kZeroValues : __builtin_amdgcn_logf(v);
         v_inverse = v <= 8.077935669e-28f ? 1.2379400392853803e27f : __builtin_amdgcn_rcpf(v);
+        asm volatile("" : "+v"(k_scale));
     }
-    // (used here, so that the wait for it is here too and not in a loop that uses it)
-    __device__ __forceinline__ void landed() { asm volatile("" : "+v"(k_scale)); }
     __device__ __forceinline__ int64_t place(int i) const { return __builtin_amdgcn_readlane(at, i); }
     __device__ __forceinline__ bool there(int i) const { return !(none >> i & 1); }
     __device__ __forceinline__ bool zeros(int i) const { return zero >> i & 1; }
@@ -353,6 +356,7 @@ __global__ __launch_bounds__(kThreads, 2) void cache_few_kernel(CacheCall c) {
     if (p < u.end) even.load(c, place(p), g, lc);
     i32x4 qh[kSl], ql[kSl];
     const float factor = row_codes<kSl, true>(c, bits, qh, ql);
+    window.landed();
     const int limit = in ? keys_of(c, row.token, u.n, u.length) : 0;
     RowState st;
     f32x4 o[kDS];
@@ -440,6 +444,7 @@ __global__ __launch_bounds__(kThreads, 2) void cache_few_kernel(CacheCall c) {
         if (refill && p + 8 < u.end) {
             base = p + 8;
             window.fetch(c, u, base, 4, lane);
+            window.landed();
             even.load(c, place(p + 8), g, lc);
         }
     }
@@ -865,34 +870,21 @@ __global__ __launch_bounds__(256 * kGroups, kGroups == 2 ? 1 : D == 64 && !kTerm
     const int group = wave >> 2;
     const Unit u = unit_at<kRows>(call);
     if (u.z > 0 && static_cast<int>(u.z) >= u.used) return;  // the whole workgroup: nothing is left for the range
+    const uint32_t row0 = u.block * kRows + wave * kWaveRows;
+    auto row_of = [&](int qt) { return row_at(call, u.hk, row0 + 16 * qt + lc); };
+    // (as few rows' start: three loads in a row; the first pages' are on their way while
+    // the rows are taken apart)
+    RowBits<kSl> bits[kQT];
+#pragma unroll
+    for (int qt = 0; qt < kQT; ++qt) {
+        const Row row = row_of(qt);
+        bits[qt] = fetch_row<kSl, kTerms>(call, row, u.b, row0 + 16 * qt + lc < call.rows && row.token < u.n, 16 * g, 64);
+    }
     PageWindow window;
     int base = u.first;
     window.fetch(call, u, base, 1, lane);
-    window.landed();
     const ManyGeom<D, kWaves> gm = many_geom<D, kWaves>(wave, lane);
 
-    i32x4 qh[kQT][kSl], ql[kQT][kSl];
-    float factor[kQT];
-    int limit[kQT];
-    ManyState<D> st;
-    const uint32_t row0 = u.block * kRows + wave * kWaveRows;
-    st.init();
-    float most = 0.0f;
-#pragma unroll
-    for (int qt = 0; qt < kQT; ++qt) {
-        const uint32_t r = row0 + 16 * qt + lc;
-        const Row row = row_at(call, u.hk, r);
-        const bool in = r < call.rows && row.token < u.n;
-        factor[qt] = row_codes<kSl, kTerms>(call, fetch_row<kSl, kTerms>(call, row, u.b, in, 16 * g, 64), qh[qt], ql[qt]);
-        limit[qt] = keys_of(call, min(row.token, max(u.n - 1, 0)), u.n, u.length);
-        most = fmaxf(most, factor[qt]);
-    }
-#pragma unroll
-    for (int i = 1; i < 16; i <<= 1) most = fmaxf(most, __shfl_xor(most, i));
-    const float factor_most = __int_as_float(__builtin_amdgcn_readfirstlane(__float_as_int(most)));
-    // pages that all rows of the wave see whole: those of its first row
-    const int whole = __builtin_amdgcn_readfirstlane(
-        keys_of(call, min(row_at(call, u.hk, row0).token, max(u.n - 1, 0)), u.n, u.length) / kPage);
     f16x8 ones;
 #pragma unroll
     for (int e = 0; e < 8; ++e) ones[e] = static_cast<_Float16>(1.0f);
@@ -916,6 +908,33 @@ __global__ __launch_bounds__(256 * kGroups, kGroups == 2 ? 1 : D == 64 && !kTerm
 #pragma unroll
         for (int i = 0; i < kLoads; ++i) v[i] = *reinterpret_cast<const u32x4 *>(page + (i * 64 * kWaves + threadIdx.x) * 16);
     };
+    if (u.first < u.end) {
+        load_v(v[0], place(u.first));
+        load_k(k_stage(u.first), place(u.first));
+        load_k(k_stage(u.first + 1), place(u.first + 1));
+        load_v(v[1], place(u.first + 1));
+    }
+
+    i32x4 qh[kQT][kSl], ql[kQT][kSl];
+    float factor[kQT];
+    int limit[kQT];
+    ManyState<D> st;
+    st.init();
+    float most = 0.0f;
+#pragma unroll
+    for (int qt = 0; qt < kQT; ++qt) {
+        factor[qt] = row_codes<kSl, kTerms>(call, bits[qt], qh[qt], ql[qt]);
+        limit[qt] = keys_of(call, min(row_of(qt).token, max(u.n - 1, 0)), u.n, u.length);
+        most = fmaxf(most, factor[qt]);
+    }
+#pragma unroll
+    for (int i = 1; i < 16; i <<= 1) most = fmaxf(most, __shfl_xor(most, i));
+    const float factor_most = __int_as_float(__builtin_amdgcn_readfirstlane(__float_as_int(most)));
+    // pages that all rows of the wave see whole: those of its first row
+    const int whole = __builtin_amdgcn_readfirstlane(
+        keys_of(call, min(row_at(call, u.hk, row0).token, max(u.n - 1, 0)), u.n, u.length) / kPage);
+    window.landed();
+
     auto store_v = [&](int parity, const u32x4 (&v)[kLoads], int p) __attribute__((always_inline)) {
         if (gm.kAll || gm.loads)
             many_store_v<D>(lds_at + Tiles<D>::kV0 + parity * Tiles<D>::kV, gm, v, Selectors::of(window.zeros(p - base)));
@@ -965,12 +984,8 @@ __global__ __launch_bounds__(256 * kGroups, kGroups == 2 ? 1 : D == 64 && !kTerm
         wg_barrier();
     };
     if (u.first < u.end) {
-        load_v(v[0], place(u.first));
-        load_k(k_stage(u.first), place(u.first));
-        load_k(k_stage(u.first + 1), place(u.first + 1));
         store_v(0, v[0], u.first);
         load_k(k_stage(u.first + 2), place(u.first + 2));
-        load_v(v[1], place(u.first + 1));
         load_v(v[0], place(u.first + 2));
         __builtin_amdgcn_s_waitcnt(0);
         __syncthreads();
