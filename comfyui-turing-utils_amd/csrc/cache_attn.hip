@@ -9,10 +9,11 @@
 // converted; the error, 2^-16 of the row's largest, is below a bf16's own.
 //
 // Values are int8 codes with one scale a page.  They enter PV as fp16, exactly,
-// and the page's scale enters the exponent: w = 2^(s + log2 v_scale - m') is at
-// most about 1 for the largest p * v_scale of the row, so fp16 (11 bits) holds
+// and the page's scale enters the exponent: w = 2^(s + log2 v_scale - m') is about
+// 2^7 for the largest p * v_scale of the row, so fp16 (11 bits, from 2^-14 on) holds
 // the weights that matter, whatever the pages' scales are.  The row sum
-// sum w / v_scale is kept apart, in fp32 from the unrounded w.
+// sum w / v_scale is kept apart, in fp32: of the unrounded w, or, where an MFMA adds
+// up a tile's, of those that enter PV.
 //   m' is held as the pair (score, log2 scale): far scores would swallow the
 // scale in a sum.  A page's log2 scale is taken as at least that of the base
 // less 64: its values are then too small to matter (2^-57 of the largest term),
@@ -305,9 +306,8 @@ __device__ __forceinline__ bool higher(float m, float v, float than_m, float tha
 // Few rows
 // ---------------------------------------------------------------------------
 // A workgroup of four waves has 16 rows of one K/V head (more rows: more workgroups,
-// whose codes come from L2 but for the first); its waves take the
-// pages of the unit's range in turn, each for itself, and are merged at the end.
-// A wave reads a page's codes straight into the MFMA operands: keys 16 g + e of a
+// whose codes come from L2 but for the first); its waves take the pages of the unit's
+// range in turn, each for itself, and are merged at the end.  A wave reads a page's codes straight into the MFMA operands: keys 16 g + e of a
 // page belong to lane group g throughout, so that a lane's 16 bytes of a V^T row
 // are the keys whose weights it holds, and a key row's bytes go to the lanes in
 // runs of D / 4.  The next page's loads (16 KiB a wave at D = 128) are in flight
