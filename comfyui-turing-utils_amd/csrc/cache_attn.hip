@@ -307,11 +307,12 @@ __device__ __forceinline__ bool higher(float m, float v, float than_m, float tha
 // ---------------------------------------------------------------------------
 // A workgroup of four waves has 16 rows of one K/V head (more rows: more workgroups,
 // whose codes come from L2 but for the first); its waves take the pages of the unit's
-// range in turn, each for itself, and are merged at the end.  A wave reads a page's codes straight into the MFMA operands: keys 16 g + e of a
-// page belong to lane group g throughout, so that a lane's 16 bytes of a V^T row
-// are the keys whose weights it holds, and a key row's bytes go to the lanes in
-// runs of D / 4.  The next page's loads (16 KiB a wave at D = 128) are in flight
-// while one is computed: what a CU needs to keep HBM busy.
+// range in turn, each for itself, and are merged at the end.  A wave reads a page's
+// codes straight into the MFMA operands: keys 16 g + e of a page belong to lane group
+// g throughout, so that a lane's 16 bytes of a V^T row are the keys whose weights it
+// holds, and a key row's bytes go to the lanes in runs of D / 4.  The next page's
+// loads (16 KiB a wave at D = 128) are in flight while one is computed: what a CU
+// needs to keep HBM busy.
 constexpr int kFewRows = 16;
 template <int D>
 struct PageRegs {
@@ -1105,21 +1106,26 @@ __global__ __launch_bounds__(kThreads) void cache_merge_kernel(CacheCall c) {
     const int64_t at = kTurns > 1 ? blockIdx.x : static_cast<int64_t>(blockIdx.x) * (kThreads / kTpr) + threadIdx.x / kTpr;
     if (at >= rows) return;
     const uint32_t bh = static_cast<uint32_t>(at / c.rows), r = static_cast<uint32_t>(at % c.rows);
-    const Unit u = unit_of<kRows>(c, bh / c.hkv, bh % c.hkv, r / kRows, 0);
-    if (u.used <= 1) return;
-    const Row row = row_at(c, u.hk, r);
     const int d0 = (threadIdx.x % kTpr) * 8;
-    MergeState st;
     constexpr int kAhead = kTurns > 1 ? 2 : 4;  // ranges whose loads are in flight together
-    for (int z0 = turn; z0 < u.used; z0 += kAhead * kTurns) {
-        f32x4 x[kAhead], a[kAhead], b[kAhead];
+    f32x4 x[kAhead], a[kAhead], b[kAhead];
+    auto load = [&](int z0, int last) __attribute__((always_inline)) {
 #pragma unroll
         for (int i = 0; i < kAhead; ++i) {
-            const int64_t from = min(z0 + i * kTurns, u.used - 1) * rows + at;
+            const int64_t from = min(z0 + i * kTurns, last) * rows + at;
             x[i] = *reinterpret_cast<const f32x4 *>(c.part_m + from * 4);
             a[i] = *reinterpret_cast<const f32x4 *>(c.part_o + from * D + d0);
             b[i] = *reinterpret_cast<const f32x4 *>(c.part_o + from * D + d0 + 4);
         }
+    };
+    // (of few rows before the length is here, ranges that nothing fills among them)
+    if (kTurns > 1) load(turn, static_cast<int>(c.parts) - 1);
+    const Unit u = unit_of<kRows>(c, bh / c.hkv, bh % c.hkv, r / kRows, 0);
+    if (u.used <= 1) return;
+    const Row row = row_at(c, u.hk, r);
+    MergeState st;
+    for (int z0 = turn; z0 < u.used; z0 += kAhead * kTurns) {
+        if (kTurns == 1 || z0 > turn) load(z0, u.used - 1);
         st.add(x, a, b, (u.used - z0 + kTurns - 1) / kTurns);
     }
     if constexpr (kTurns > 1) {
@@ -1132,13 +1138,13 @@ __global__ __launch_bounds__(kThreads) void cache_merge_kernel(CacheCall c) {
         constexpr int kStep = 4;
 #pragma unroll
         for (int t = 1; t < kTurns; t += kStep) {
-            f32x4 x[kStep], a[kStep], b[kStep];
+            f32x4 xs[kStep], as[kStep], bs[kStep];
 #pragma unroll
             for (int i = 0; i < kStep; ++i) {
                 const int from = min(t + i, kTurns - 1);
-                x[i] = all[0][from][threadIdx.x], a[i] = all[1][from][threadIdx.x], b[i] = all[2][from][threadIdx.x];
+                xs[i] = all[0][from][threadIdx.x], as[i] = all[1][from][threadIdx.x], bs[i] = all[2][from][threadIdx.x];
             }
-            st.add(x, a, b, kTurns - t);
+            st.add(xs, as, bs, kTurns - t);
         }
     }
     const bool some = st.l != 0.0f && row.token < u.n;
