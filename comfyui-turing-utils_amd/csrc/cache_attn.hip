@@ -15,9 +15,10 @@
 // sum w / v_scale is kept apart, in fp32: of the unrounded w, or, where an MFMA adds
 // up a tile's, of those that enter PV.
 //   m' is held as the pair (score, log2 scale): far scores would swallow the
-// scale in a sum.  A page's log2 scale is taken as at least that of the base
-// less 64: its values are then too small to matter (2^-57 of the largest term),
-// and w stays a normal number for the row sum.
+// scale in a sum.  Of a page whose log2 scale is less than the base's by more than
+// 64, w may be no normal number where the page still matters in the row sum (its
+// scores may be far above the base's): its weights are summed apart, as
+// 2^(s - m' - log2 base scale).
 //
 // Two kernels: blocks of 16 rows (single tokens) read codes straight into registers;
 // blocks of 128 or 256 share K and V tiles in LDS.  Both split a sequence's pages into
@@ -38,7 +39,7 @@ constexpr int kThreads = 256;
 constexpr float kNoBase = -3.402823466e38f;  // score of a row's base before its first key
 constexpr float kUp = 7.0f;                  // log2 of w at the base: fp16's room is used from 2^15 down to 2^-24
 constexpr float kSlack = 8.0f;               // log2 of w above the base that moves it
-constexpr float kLeastScale = -64.0f;        // least log2 of a page's V scale, less the base's
+constexpr float kLeastScale = -64.0f;        // log2 of a page's V scale, less the base's, below which its sum is taken apart
 constexpr float kZeroValues = -90.0f;        // log2 V scale of a page whose values count as zeros
 constexpr int kQInt8 = 2;                    // query types: 0 bf16, 1 fp16
 
@@ -250,11 +251,9 @@ struct PageWindow {
 // its share of the sum of w / v_scale.
 struct RowState {
     float m = kNoBase, v = 0.0f, l = 0.0f;
-    // the page's log2 V scale less the base's (a NaN stays)
-    __device__ __forceinline__ float shift(float v_log2) const {
-        const float d = v_log2 - v;
-        return d < kLeastScale ? kLeastScale : d;
-    }
+    // Of a page far below the base's scale, w / v_scale of score x: at most 2^(kSlack + kUp
+    // - kZeroValues), as the base has not moved.
+    __device__ __forceinline__ float apart(float x) const { return __builtin_amdgcn_exp2f((x - m) + (kUp - v)); }
 };
 
 // Results of a unit's rows: o[ds][r] = channel 16 ds + 4 g + r of the row of the
@@ -400,7 +399,7 @@ __global__ __launch_bounds__(kThreads, 2) void cache_few_kernel(CacheCall c) {
                 for (int ds = 0; ds < kDS; ++ds) o[ds] *= alpha;
             }
         }
-        const float d = st.shift(v_log2);
+        const float d = v_log2 - st.v;
         float sum = 0.0f;
         f16x8 w[2];
 #pragma unroll
@@ -420,7 +419,14 @@ __global__ __launch_bounds__(kThreads, 2) void cache_few_kernel(CacheCall c) {
             w[h] = __builtin_bit_cast(f16x8, packed);
         }
         // w / v_scale, the scale being 2^(base's + d) (a lane without keys has no part in a NaN)
-        if (seen > 0) st.l = __builtin_fmaf(sum, __builtin_amdgcn_exp2f(-(st.v + d)), st.l);
+        float inverse = __builtin_amdgcn_exp2f(-(st.v + d));
+        if (__any(d < kLeastScale)) {
+            float apart = 0.0f;
+#pragma unroll
+            for (int e = 0; e < 16; ++e) apart += e < seen ? st.apart(x[e]) : 0.0f;
+            if (d < kLeastScale) sum = apart, inverse = 1.0f;
+        }
+        if (seen > 0) st.l = __builtin_fmaf(sum, inverse, st.l);
         if (window.zeros(at)) return;
 #pragma unroll
         for (int ds = 0; ds < kDS; ++ds) {
@@ -694,7 +700,7 @@ __device__ __forceinline__ void careful_weights(i32x4 (&s)[4][kQT], const float 
 #pragma unroll
     for (int qt = 0; qt < kQT; ++qt) {
         const int t0 = seen[qt] - 1 - 8 * g;
-        const float d = st.row[qt].shift(v_log2);
+        const float d = v_log2 - st.row[qt].v;
         float sum = 0.0f;
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
@@ -714,9 +720,20 @@ __device__ __forceinline__ void careful_weights(i32x4 (&s)[4][kQT], const float 
             }
             w[h][qt] = __builtin_bit_cast(f16x8, packed);
         }
+        float inverse = __builtin_amdgcn_exp2f(-(st.row[qt].v + d));
+        if (__any(d < kLeastScale)) {
+            float apart = 0.0f;
+#pragma unroll
+            for (int c = 0; c < 16; ++c) {  // key 32 (c >> 3) + 8 g + (c & 7)
+                const int hidden = (t0 - (32 * (c >> 3) + (c & 7))) >> 31;
+                const float x = score<kTerms>(s[c >> 2][qt][c & 3]) * f[qt];
+                apart += __int_as_float(__float_as_int(st.row[qt].apart(x)) & ~hidden);
+            }
+            if (d < kLeastScale) sum = apart, inverse = 1.0f;
+        }
         // (a row that sees nothing of the tile has no part in a NaN)
-        if (seen[qt] > 0)
-            st.row[qt].l = __builtin_fmaf(xsum_f32(sum), __builtin_amdgcn_exp2f(-(st.row[qt].v + d)), st.row[qt].l);
+        const float all = xsum_f32(sum);
+        if (seen[qt] > 0) st.row[qt].l = __builtin_fmaf(all, inverse, st.row[qt].l);
     }
 }
 
