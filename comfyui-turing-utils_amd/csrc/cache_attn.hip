@@ -40,6 +40,7 @@ constexpr float kNoBase = -3.402823466e38f;  // score of a row's base before its
 constexpr float kUp = 7.0f;                  // log2 of w at the base: fp16's room is used from 2^15 down to 2^-24
 constexpr float kSlack = 8.0f;               // log2 of w above the base that moves it
 constexpr float kLeastScale = -64.0f;        // log2 of a page's V scale, less the base's, below which its sum is taken apart
+constexpr float kFarMove = -100.0f;          // log2 of a factor that is taken in two steps
 constexpr float kZeroValues = -90.0f;        // log2 V scale of a page whose values count as zeros
 constexpr int kQInt8 = 2;                    // query types: 0 bf16, 1 fp16
 
@@ -296,6 +297,17 @@ __device__ __forceinline__ void store_row(const CacheCall &c, const Unit &u, con
     }
 }
 
+// to + l * 2^a, given 2^a.  A sum over V scales may lie as far above 1 as 2^a lies below
+// fp32's range (a base of scale 2^-30 left for one of 2^100): two steps then.
+__device__ __forceinline__ float moved(float l, float a, float power, float to = 0.0f) {
+    float sum = __builtin_fmaf(power, l, to);
+    if (__any(a < kFarMove)) {
+        const float half = __builtin_amdgcn_exp2f(0.5f * a);
+        if (a < kFarMove) sum = to + (l * half) * half;
+    }
+    return sum;
+}
+
 // The other of two bases where it is higher: by score, and log2 of the V scale.
 __device__ __forceinline__ bool higher(float m, float v, float than_m, float than_v) {
     return (m - than_m) + (v - than_v) > 0.0f;
@@ -392,9 +404,9 @@ __global__ __launch_bounds__(kThreads, 2) void cache_few_kernel(CacheCall c) {
             // a row's base moves by its own scores alone
             const float row_top = xmax_f32(top);
             if ((row_top - st.m) + (v_log2 - st.v) > kSlack) {
-                const float alpha = __builtin_amdgcn_exp2f((st.m - row_top) + (st.v - v_log2));
+                const float a = (st.m - row_top) + (st.v - v_log2), alpha = __builtin_amdgcn_exp2f(a);
                 st.m = row_top, st.v = v_log2;
-                st.l *= alpha;
+                st.l = moved(st.l, a, alpha);
 #pragma unroll
                 for (int ds = 0; ds < kDS; ++ds) o[ds] *= alpha;
             }
@@ -482,8 +494,8 @@ __global__ __launch_bounds__(kThreads, 2) void cache_few_kernel(CacheCall c) {
         for (int i = 0; i < 4; ++i) {
             const float li = merge_m[i][lane][2];
             if (li == 0.0f) continue;  // saw nothing
-            const float wi = __builtin_amdgcn_exp2f((merge_m[i][lane][0] - m) + (merge_m[i][lane][1] - v));
-            l = __builtin_fmaf(wi, li, l);
+            const float a = (merge_m[i][lane][0] - m) + (merge_m[i][lane][1] - v), wi = __builtin_amdgcn_exp2f(a);
+            l = moved(li, a, wi, l);
 #pragma unroll
             for (int ds = 0; ds < kDS; ++ds) {
                 const f32x4 x = i == 0 ? o[ds] : *reinterpret_cast<const f32x4 *>(merge_o[i - (i > 0)][ds][lane]);
@@ -600,10 +612,10 @@ struct ManyState {
         for (int qt = 0; qt < kQT; ++qt) {
             const float row_top = xmax_f32(top[qt]);
             const bool go = (row_top - row[qt].m) + (v_log2 - row[qt].v) > kSlack;
-            const float alpha = go ? __builtin_amdgcn_exp2f((row[qt].m - row_top) + (row[qt].v - v_log2)) : 1.0f;
+            const float a = go ? (row[qt].m - row_top) + (row[qt].v - v_log2) : 0.0f, alpha = __builtin_amdgcn_exp2f(a);
             row[qt].m = go ? row_top : row[qt].m;
             row[qt].v = go ? v_log2 : row[qt].v;
-            row[qt].l *= alpha;
+            row[qt].l = moved(row[qt].l, a, alpha);
 #pragma unroll
             for (int ds = 0; ds < D / 16; ++ds) o[ds][qt] *= alpha;
             base[qt] = (row[qt].m + row[qt].v) - kUp;
@@ -1096,21 +1108,32 @@ struct MergeState {
 #pragma unroll
         for (int i = 0; i < kN; ++i)
             if (i < there && x[i][2] != 0.0f && higher(x[i][0], x[i][1], m_new, v_new)) m_new = x[i][0], v_new = x[i][1];
-        const float old = l == 0.0f ? 0.0f : __builtin_amdgcn_exp2f((m - m_new) + (v - v_new));
+        const float l_old = l, a_old = l == 0.0f ? 0.0f : (m - m_new) + (v - v_new);
+        const float old = l == 0.0f ? 0.0f : __builtin_amdgcn_exp2f(a_old);
         m = m_new, v = v_new;
         l *= old;
 #pragma unroll
         for (int e = 0; e < 8; ++e) acc[e] = old == 0.0f ? 0.0f : acc[e] * old;
+        float least = a_old;
 #pragma unroll
         for (int i = 0; i < kN; ++i) {
             if (i >= there || x[i][2] == 0.0f) continue;
-            const float wi = __builtin_amdgcn_exp2f((x[i][0] - m) + (x[i][1] - v));
+            const float ai = (x[i][0] - m) + (x[i][1] - v), wi = __builtin_amdgcn_exp2f(ai);
+            least = fminf(least, ai);
             l = __builtin_fmaf(wi, x[i][2], l);
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
                 acc[e] = __builtin_fmaf(wi, a[i][e], acc[e]);
                 acc[4 + e] = __builtin_fmaf(wi, b[i][e], acc[4 + e]);
             }
+        }
+        if (!__any(least < kFarMove)) return;
+        l = moved(l_old, a_old, old);
+#pragma unroll
+        for (int i = 0; i < kN; ++i) {
+            if (i >= there || x[i][2] == 0.0f) continue;
+            const float ai = (x[i][0] - m) + (x[i][1] - v);
+            l = moved(x[i][2], ai, __builtin_amdgcn_exp2f(ai), l);
         }
     }
 };

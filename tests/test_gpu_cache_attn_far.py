@@ -50,3 +50,14 @@ def test_small_values_of_high_scores(gpu_device, lq, heads, kind, lead, ratio):
         for most in (None, 64):
             got = _check(q, pool, table, _ints([384, 290], gpu_device), max_length=most, **kw)
             assert torch.isfinite(got).all()
+
+
+@pytest.mark.parametrize("lq,heads", ROWS)
+@pytest.mark.parametrize("order", ["first", "later"])
+@pytest.mark.parametrize("lead", [0, 30, 100, 170])
+def test_scales_at_both_ends(gpu_device, lq, heads, order, lead):
+    """Values of 2^100 and pages of the least scale a cache writes (1e-7 / 127), 2^130 apart."""
+    q, pool, table, kw = _leads(gpu_device, lq, heads, "bf16", lead, 1.0, order)
+    pool[3].fill_(2.0 ** 100)
+    pool[3][table[:, 0 if order == "first" else 3].long()] = 1e-7 / 127
+    _check(q, pool, table, _ints([384, 250], gpu_device), **kw)
