@@ -40,6 +40,7 @@ constexpr float kNoBase = -3.402823466e38f;  // score of a row's base before its
 constexpr float kUp = 7.0f;                  // log2 of w at the base: fp16's room is used from 2^15 down to 2^-24
 constexpr float kSlack = 8.0f;               // log2 of w above the base that moves it
 constexpr float kLeastScale = -64.0f;        // log2 of a page's V scale, less the base's, below which its sum is taken apart
+constexpr float kLeastRow = 1e-33f;          // a float row's units are made for at least this
 constexpr float kFarMove = -100.0f;          // log2 of a factor that is taken in two steps
 constexpr float kZeroValues = -90.0f;        // log2 V scale of a page whose values count as zeros
 constexpr int kQInt8 = 2;                    // query types: 0 bf16, 1 fp16
@@ -178,8 +179,9 @@ __device__ __forceinline__ float row_codes(const CacheCall &c, const RowBits<kSl
 #pragma unroll
         for (int e = 0; e < 16; ++e) top = max(top, static_cast<int>(__float_as_uint(x[i][e]) & 0x7fffffffu));
     top = xmax_i32(top);
-    const float amax = __int_as_float(top);
-    const float inverse = 32512.0f / fmaxf(amax, 1e-30f);
+    // (a NaN stays; of smaller rows the inverse would be infinite)
+    const float amax = __int_as_float(max(top, __float_as_int(kLeastRow)));
+    const float inverse = 32512.0f / amax;
 #pragma unroll
     for (int i = 0; i < kSl; ++i) {
         hi[i] = lo[i] = i32x4{0, 0, 0, 0};
