@@ -109,8 +109,8 @@ def _rows(x: torch.Tensor, width: int) -> torch.Tensor:
         x = torch.nn.functional.pad(x, (0, width - x.size(-1)))
     piece = 16 // x.element_size()
     if x.stride(-1) != 1 or x.data_ptr() % 16 or any(s % piece for s in x.stride()[:-1]):
-        x = x.contiguous()
-        x = x.clone() if x.data_ptr() % 16 else x
+        # (contiguous() and clone() would keep any stride of an axis of one)
+        x = torch.empty(x.shape, dtype=x.dtype, device=x.device).copy_(x)
     return x
 
 

@@ -207,6 +207,26 @@ def test_strided_arguments_reach_the_entry_points_whole(entry_point):
     assert attend[14:19] == (3, 2, 2, 9, 64) and attend[27] == 128
 
 
+@pytest.mark.parametrize("layout", ["HND", "NHD"])
+def test_odd_strides_of_axes_of_one(entry_point, layout):
+    """One sequence, head and token of rows of 67 channels: torch calls it contiguous, with strides of no 16 bytes."""
+    cache = _cache(heads=1, device="cpu")
+    table, lengths = _i(1, 2, device="cpu"), _i(1, device="cpu")
+    x = torch.randn(1, 9, 2, 67).to(torch.bfloat16)[:, :1, :1, :64]
+    assert x.is_contiguous() and 67 in x.stride()
+    codes, scale = torch.zeros(1, 9, 2, 67, dtype=torch.int8)[:, :1, :1, :64], torch.ones(1, 1, 1)
+    mean = torch.randn(1, 3, 67).to(torch.bfloat16)[:, :1, :64]
+    kw = dict(tensor_layout=layout)
+    turing_sage.kv_cache_append(x, x, cache, table, lengths, key_mean=mean, **kw)
+    turing_sage.kv_cache_append(codes, x, cache, table, lengths, key_scale=scale, **kw)
+    turing_sage.kv_cache_attention(x, cache, table, lengths, **kw)
+    turing_sage.kv_cache_attention(codes, cache, table, lengths, query_scale=scale, **kw)
+    (_, bf16), (_, int8), (_, q), (_, q8) = entry_point
+    assert bf16[8:14] == int8[8:14] == (64, 64, 64) * 2
+    assert q[19:22] == q8[19:22] == (64, 64, 64)
+    assert all(args[i] % 16 == 0 for args, i in ((bf16, 0), (bf16, 2), (int8, 0), (int8, 2), (q, 0), (q8, 0)))
+
+
 def test_no_tokens(entry_point):
     cache, table = _cache(device="cpu"), _i(2, 2, device="cpu")
     lengths = torch.tensor([-3, 1000], dtype=torch.int32)
