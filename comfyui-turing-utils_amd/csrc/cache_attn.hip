@@ -1338,8 +1338,11 @@ extern "C" int32_t tu_kv_cache_attn(const void *q, const float *q_scale, int32_t
     const CachePlan plan = cache_plan(batch, hkv, lq, hq / hkv, dim, std::min<int64_t>((max_length - 1) / kPage + 1, width),
                                       q_type == kQInt8, causal != 0, cus, workspace ? workspace_bytes : 0);
     const int64_t units = batch * hkv * plan.row_blocks * plan.parts;
-    constexpr int64_t kMost = 0x7fffffff;
-    TU_REQUIRE(units <= kMost, "cache attention grid too large");
+    // a launch's threads are counted in 32 bits (a merge has no more workgroups than a row each)
+    constexpr int64_t kMost = 0xffffffff;
+    TU_REQUIRE(units <= kMost / (plan.rows == 2 * kGroupRows ? 512 : 256) &&
+                   (plan.parts == 1 || batch * hkv * rows <= kMost / kThreads),
+               "cache attention grid too large");
     if (require_gfx950()) return -1;
     CacheCall c{};
     c.q = q, c.q_scale = q_scale, c.q_type = static_cast<uint32_t>(q_type);

@@ -31,6 +31,7 @@ namespace {
 
 constexpr int kPage = 64;
 constexpr int kThreads = 256;
+constexpr int64_t kMostWgs = 0xffffffff / kThreads;  // a launch's threads are counted in 32 bits
 
 // Where a call's tokens lie in the pages.
 struct Pages {
@@ -388,11 +389,11 @@ extern "C" int32_t tu_kv_cache_append(const void *k, const float *k_in_scale, co
     TU_REQUIRE(dtype == 0 || dtype == 1, "cache append dtype must be 0 (bf16) or 1 (fp16), got %d", dtype);
     TU_REQUIRE((reinterpret_cast<uintptr_t>(k_mean_bf16) & 15) == 0, "cache append K mean must be 16-byte aligned");
     TU_REQUIRE(lengths_out != lengths, "cache append: the new lengths need memory of their own");
-    if (require_gfx950()) return -1;
-    const Pages p{block_table, lengths, static_cast<int32_t>(width), static_cast<int32_t>(pages), static_cast<uint32_t>(hkv)};
     // len tokens touch one page more where they do not start at a page's start
     const int64_t blocks = std::min<int64_t>((len + 2 * kPage - 2) / kPage, width);
-    TU_REQUIRE(blocks * hkv <= 0x7fffffff, "cache append grid too large");
+    TU_REQUIRE(blocks * hkv <= kMostWgs, "cache append grid too large");
+    if (require_gfx950()) return -1;
+    const Pages p{block_table, lengths, static_cast<int32_t>(width), static_cast<int32_t>(pages), static_cast<uint32_t>(hkv)};
     const dim3 grid(static_cast<unsigned>(blocks * hkv), static_cast<unsigned>(2 * batch));
     hipStream_t s = static_cast<hipStream_t>(stream);
 #define TU_APPEND(D, TYPE, CODES)                                                                                      \
@@ -428,10 +429,10 @@ extern "C" int32_t tu_kv_cache_read(const int8_t *k_codes, const int8_t *v_codes
     if (check_cache("cache read", batch, hkv, len, dim, width, pages, pointers, 8, strides, 8)) return -1;
     TU_REQUIRE(dtype == 0 || dtype == 1, "cache read dtype must be 0 (bf16) or 1 (fp16), got %d", dtype);
     TU_REQUIRE((reinterpret_cast<uintptr_t>(k_mean_bf16) & 15) == 0, "cache read K mean must be 16-byte aligned");
+    const int64_t blocks = starts ? (len + 2 * kPage - 2) / kPage : (len + kPage - 1) / kPage;
+    TU_REQUIRE(blocks * hkv <= kMostWgs, "cache read grid too large");
     if (require_gfx950()) return -1;
     const Pages p{block_table, lengths, static_cast<int32_t>(width), static_cast<int32_t>(pages), static_cast<uint32_t>(hkv)};
-    const int64_t blocks = starts ? (len + 2 * kPage - 2) / kPage : (len + kPage - 1) / kPage;
-    TU_REQUIRE(blocks * hkv <= 0x7fffffff, "cache read grid too large");
     const dim3 grid(static_cast<unsigned>(blocks * hkv), static_cast<unsigned>(2 * batch));
     hipStream_t s = static_cast<hipStream_t>(stream);
 #define TU_READ(D, TYPE)                                                                                               \

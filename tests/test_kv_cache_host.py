@@ -307,6 +307,17 @@ def test_attention_entry_refuses(change):
     assert status == -1 and "cache attention" in message
 
 
+@pytest.mark.parametrize("name,kw", [
+    ("tu_kv_cache_append", dict(hkv=65535, len=64 * 257, width=1000)),
+    ("tu_kv_cache_read", dict(hkv=65535, len=64 * 257, width=1000)),
+    ("tu_kv_cache_attn", dict(batch=65535, hq=257, hkv=257, lq=1, max_length=64)),
+    ("tu_kv_cache_attn", dict(batch=1, hq=65535, hkv=65535, lq=128 * 257, max_length=64))])
+def test_more_workgroups_than_a_launch_has(name, kw):
+    """More than 2^32 threads, in workgroups of 256."""
+    status, message = _entry(name, **kw)
+    assert status == -1 and "grid too large" in message
+
+
 def test_workspace():
     """Bytes for whole ranges of rows; none where a call has no ranges or no sizes."""
     size = _lib.load().tu_kv_cache_attn_workspace
