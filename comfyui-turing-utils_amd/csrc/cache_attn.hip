@@ -24,6 +24,7 @@
 // blocks of 128 or 256 share K and V tiles in LDS.  Both split a sequence's pages into
 // ranges where the grid would leave the chip empty; a third merges.
 #include <algorithm>
+#include <cmath>
 #include <type_traits>
 
 #include "attn_common.h"
@@ -1326,7 +1327,7 @@ extern "C" int32_t tu_kv_cache_attn(const void *q, const float *q_scale, int32_t
     TU_REQUIRE(q && k_codes && v_codes && k_scale && v_scale && block_table && lengths && o && (q_scale || q_type != kQInt8),
                "cache attention pointers must be non-null");
     TU_REQUIRE(q_type != kQInt8 || (blkq > 0 && blkq <= 0x7fffffff), "cache attention needs blkq > 0");
-    TU_REQUIRE(sm_scale > 0.0f, "cache attention sm_scale must be positive");
+    TU_REQUIRE(sm_scale > 0.0f && std::isfinite(sm_scale * kLog2e), "cache attention sm_scale must be positive and finite");
     const int64_t piece = q_type == kQInt8 ? 16 : 8;
     TU_REQUIRE(q_sb % piece == 0 && q_sh % piece == 0 && q_sl % piece == 0 && (reinterpret_cast<uintptr_t>(q) & 15) == 0,
                "cache attention query rows must be 16-byte aligned");

@@ -307,6 +307,13 @@ def test_attention_entry_refuses(change):
     assert status == -1 and "cache attention" in message
 
 
+@pytest.mark.parametrize("scale", [1e39, float("inf"), 3e38])
+def test_scales_past_32_bits_are_refused(scale):
+    """In 32 bits, log2 e of it included, an infinite scale would make a NaN of every row."""
+    status, message = _entry("tu_kv_cache_attn", sm_scale=scale)
+    assert status == -1 and "positive and finite" in message
+
+
 @pytest.mark.parametrize("name,kw", [
     ("tu_kv_cache_append", dict(hkv=65535, len=64 * 257, width=1000)),
     ("tu_kv_cache_read", dict(hkv=65535, len=64 * 257, width=1000)),
