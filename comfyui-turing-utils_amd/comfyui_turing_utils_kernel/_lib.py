@@ -196,6 +196,7 @@ SIGNATURES: dict[str, tuple[object, list[object]]] = {
          _c_void_p, _c_void_p, _i32, _i64, _i64, _i64, _i64, _i64, _i64, _i64, _i64, _i64, _i64, _c_void_p],
     ),
     "tu_kv_cache_attn_workspace": (_i64, [_i64, _i64, _i64, _i64, _i64, _i64, _i32, _i32, _i32]),
+    "tu_kv_cache_attn_plan": (_i32, [_i64, _i64, _i64, _i64, _i64, _i64, _i32, _i32, _i32]),
     "tu_kv_cache_attn": (
         _i32,
         [_c_void_p, _c_void_p, _i32, _i64, _c_void_p, _c_void_p, _c_void_p, _c_void_p, _i64, _c_void_p, _i64,
@@ -204,7 +205,7 @@ SIGNATURES: dict[str, tuple[object, list[object]]] = {
     ),
 }
 
-ABI_VERSION = 21
+ABI_VERSION = 22
 
 _lock = threading.Lock()
 _lib: ctypes.CDLL | None = None

@@ -1298,15 +1298,27 @@ int64_t cache_workspace(const CachePlan &p, int64_t batch, int64_t hkv, int64_t 
     return p.parts > 1 ? p.parts * batch * hkv * rows * (dim + 4) * static_cast<int64_t>(sizeof(float)) : 0;
 }
 
+// The plan of a call with all the workspace it wants; no rows for bad sizes.
+CachePlan whole_plan(int64_t batch, int64_t hq, int64_t hkv, int64_t lq, int64_t dim, int64_t max_length, int32_t q_type,
+                     int32_t causal, int32_t cus) {
+    if (!cache_sizes(batch, hq, hkv, lq, max_length, cus) || (dim != 64 && dim != 128)) return CachePlan{};
+    const int64_t pages = std::min<int64_t>((max_length - 1) / kPage + 1, 0x7fffffff / kPage - 1);
+    return cache_plan(batch, hkv, lq, hq / hkv, dim, pages, q_type == kQInt8, causal != 0, cus, INT64_MAX);
+}
+
 }  // namespace
 }  // namespace tu
 
 extern "C" int64_t tu_kv_cache_attn_workspace(int64_t batch, int64_t hq, int64_t hkv, int64_t lq, int64_t dim, int64_t max_length,
                                               int32_t q_type, int32_t causal, int32_t cus) {
-    using namespace tu;
-    if (!cache_sizes(batch, hq, hkv, lq, max_length, cus) || (dim != 64 && dim != 128)) return 0;
-    const int64_t group = hq / hkv, pages = std::min<int64_t>((max_length - 1) / kPage + 1, 0x7fffffff / kPage - 1);
-    return cache_workspace(cache_plan(batch, hkv, lq, group, dim, pages, q_type == kQInt8, causal != 0, cus, INT64_MAX), batch, hkv, lq * group, dim);
+    const tu::CachePlan plan = tu::whole_plan(batch, hq, hkv, lq, dim, max_length, q_type, causal, cus);
+    return plan.rows ? tu::cache_workspace(plan, batch, hkv, lq * (hq / hkv), dim) : 0;
+}
+
+extern "C" int32_t tu_kv_cache_attn_plan(int64_t batch, int64_t hq, int64_t hkv, int64_t lq, int64_t dim, int64_t max_length,
+                                         int32_t q_type, int32_t causal, int32_t cus) {
+    const tu::CachePlan plan = tu::whole_plan(batch, hq, hkv, lq, dim, max_length, q_type, causal, cus);
+    return plan.rows << 16 | static_cast<int32_t>(plan.parts);
 }
 
 extern "C" int32_t tu_kv_cache_attn(const void *q, const float *q_scale, int32_t q_type, int64_t blkq, const int8_t *k_codes,

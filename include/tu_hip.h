@@ -621,6 +621,10 @@ int32_t tu_kv_cache_read(const int8_t *k_codes, const int8_t *v_codes, const flo
  * ranges, with none (NULL, 0) one. */
 int64_t tu_kv_cache_attn_workspace(int64_t batch, int64_t hq, int64_t hkv, int64_t lq, int64_t dim,
                                    int64_t max_length, int32_t q_type, int32_t causal, int32_t cus);
+/* The form of a call with that workspace: rows of a workgroup (16, 128 or 256) << 16
+ * | ranges of a sequence's keys; 0 for bad arguments (host only, no HIP call). */
+int32_t tu_kv_cache_attn_plan(int64_t batch, int64_t hq, int64_t hkv, int64_t lq, int64_t dim, int64_t max_length,
+                              int32_t q_type, int32_t causal, int32_t cus);
 int32_t tu_kv_cache_attn(const void *q, const float *q_scale, int32_t q_type, int64_t blkq, const int8_t *k_codes,
                          const int8_t *v_codes, const float *k_scale, const float *v_scale, int64_t pages,
                          const int32_t *block_table, int64_t width, const int32_t *lengths,
