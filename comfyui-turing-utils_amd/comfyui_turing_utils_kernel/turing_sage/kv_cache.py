@@ -456,11 +456,14 @@ def kv_cache_attention(
     tokens, those up to their own: query i the keys j <= lengths[b] - n + i.  Rows
     that see no key, and rows at or past n, are zeros.
 
-    ``query`` is bf16 or fp16, taken as integers of 16 bits with a scale a row (an
-    error under half a step of bf16), or int8 codes with ``query_scale`` fp32 [B,
-    Hq, ceil(Lq / blkq)], the framework's own form, which needs half of the
-    products with the keys.  The result has the query's type and shape, bf16 for
-    codes.  ``sm_scale`` is head_dim^-0.5 unless given.
+    ``query`` is bf16 or fp16, or int8 codes with ``query_scale`` fp32 [B, Hq,
+    ceil(Lq / blkq)], the framework's own form, which needs half of the products
+    with the keys.  A float row is taken as integers of 16 bits with one scale: each
+    element is off by at most max |row| / 65024 (of a row below 1e-33, 1e-33 /
+    65024).  Elements below 1/128 of the row's largest lose bits of a bf16, those
+    below 1/16 of an fp16.  The result has the query's type and shape, bf16 for
+    codes.  ``sm_scale`` is head_dim^-0.5 unless given.  Scores are held in 32 bits:
+    a row with one that is infinite there is NaN.
 
     ``max_length``: a bound of the lengths, where it is known to be less than the
     64 n of the block table; the split of long sequences over the GPU is made for

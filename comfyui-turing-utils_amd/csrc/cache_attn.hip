@@ -6,7 +6,9 @@
 // with q int8 codes and their scales, or 16-bit floats.  A float row is taken as
 // integers of 16 bits, x ~ a (256 h + l) with h, l int8 and a = max |x| / 32512:
 // two INT8 products in place of one in 16-bit floats, which would need every key
-// converted; the error, 2^-16 of the row's largest, is below a bf16's own.
+// converted.  An element is off by max |x| / 65024 at most, half a unit, whatever its
+// own size: less than its own rounding where it is above 1/128 (bf16) or 1/16 (fp16)
+// of the row's largest, more where it is below.
 //
 // Values are int8 codes with one scale a page.  They enter PV as fp16, exactly,
 // and the page's scale enters the exponent: w = 2^(s + log2 v_scale - m') is about

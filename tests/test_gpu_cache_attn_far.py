@@ -8,12 +8,18 @@ import math
 import pytest
 import torch
 
+from comfyui_turing_utils_kernel import _lib
 from tests.test_gpu_cache_attn import _check, _ints, _pool, _query
 
-pytestmark = pytest.mark.gpu
+# (query tokens, K/V heads of the two sequences): rows a workgroup
+ROWS = {(1, 1): 16, (20, 1): 16, (140, 1): 16, (140, 33): 128, (256, 66): 256}
 
-# (query tokens, K/V heads of the two sequences): few rows, and so many that they are taken in blocks of 128 and of 256
-ROWS = [(1, 1), (20, 1), (140, 1), (140, 33), (256, 66)]
+
+def test_the_sizes_take_the_forms():
+    for (lq, heads), rows in ROWS.items():
+        for kind in (0, 2):
+            for most in (64, 384):
+                assert _lib.load().tu_kv_cache_attn_plan(2, heads, heads, lq, 64, most, kind, 0, 256) == rows << 16 | 1
 
 
 def _leads(device, lq, heads, kind, lead, ratio, order, row=6, page=3):
@@ -38,6 +44,7 @@ def _leads(device, lq, heads, kind, lead, ratio, order, row=6, page=3):
     return q, pool, table, kw
 
 
+@pytest.mark.gpu
 @pytest.mark.parametrize("lq,heads", ROWS)
 @pytest.mark.parametrize("kind", ["bf16", "int8"])
 @pytest.mark.parametrize("lead", [60, 68, 75, 85])
@@ -52,6 +59,7 @@ def test_small_values_of_high_scores(gpu_device, lq, heads, kind, lead, ratio):
             assert torch.isfinite(got).all()
 
 
+@pytest.mark.gpu
 @pytest.mark.parametrize("lq,heads", ROWS)
 @pytest.mark.parametrize("order", ["first", "later"])
 @pytest.mark.parametrize("lead", [0, 30, 100, 170])

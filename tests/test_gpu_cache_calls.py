@@ -326,3 +326,21 @@ def test_two_pools_at_once(gpu_device):
     torch.cuda.synchronize(gpu_device)
     for i in range(2):
         assert all(torch.equal(x, want[i]) for x in got[i])
+
+
+def test_a_backward_pass_is_refused(gpu_device, routes):
+    """Of a leaf the result is one that autograd knows, and its backward pass an error, on whichever route; the values
+    are those of a call without gradients."""
+    pool, table, g = _pool(gpu_device, 1, 2, 64, 3, 9)
+    cache, lengths = QuantizedKVCache(*pool), _ints([100], gpu_device)
+    q = _query(gpu_device, 1, 2, 3, 64, "bf16", "HND", g)[0].requires_grad_()
+    native, general, served = routes(lambda: turing_sage.kv_cache_attention(q, cache, table, lengths))
+    assert served == [False]
+    for out in (native, general):
+        assert out.requires_grad
+        with pytest.raises(RuntimeError, match="backward"):
+            out.float().sum().backward()
+    assert q.grad is None
+    with torch.no_grad():
+        again = turing_sage.kv_cache_attention(q, cache, table, lengths)
+    assert not again.requires_grad and torch.equal(again, native.detach())
