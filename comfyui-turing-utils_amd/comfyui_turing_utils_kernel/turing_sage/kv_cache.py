@@ -462,8 +462,8 @@ def kv_cache_attention(
     element is off by at most max |row| / 65024 (of a row below 1e-33, 1e-33 /
     65024).  Elements below 1/128 of the row's largest lose bits of a bf16, those
     below 1/16 of an fp16.  The result has the query's type and shape, bf16 for
-    codes.  ``sm_scale`` is head_dim^-0.5 unless given.  Scores are held in 32 bits:
-    a row with one that is infinite there is NaN.
+    codes.  ``sm_scale`` is head_dim^-0.5 unless given.  Scores are held in 32 bits: a
+    row whose largest is infinite there is NaN.
 
     ``max_length``: a bound of the lengths, where it is known to be less than the
     64 n of the block table; the split of long sequences over the GPU is made for

@@ -157,6 +157,9 @@ __device__ __forceinline__ RowBits<kSl> fetch_row(const CacheCall &c, const Row 
     return r;
 }
 
+// An infinite scale as NaN: a score of minus infinity would leave a row without its key.
+__device__ __forceinline__ float finite_or_nan(float scale) { return scale + (scale - scale); }
+
 // The row as bytes h and l, and its factor (scale * sm_scale * log2 e of one unit of
 // 256 h + l).  The row's lanes are the four groups of 16.
 template <int kSl, bool kTerms>
@@ -164,7 +167,7 @@ __device__ __forceinline__ float row_codes(const CacheCall &c, const RowBits<kSl
     if (!kTerms || c.q_type == kQInt8) {
 #pragma unroll
         for (int i = 0; i < kSl; ++i) hi[i] = __builtin_bit_cast(i32x4, bits.w[i][0]), lo[i] = i32x4{0, 0, 0, 0};
-        return bits.scale * c.sm_log2 * (kTerms ? 0.00390625f : 1.0f);
+        return finite_or_nan(bits.scale) * c.sm_log2 * (kTerms ? 0.00390625f : 1.0f);
     }
     float x[kSl][16];
 #pragma unroll
@@ -196,7 +199,7 @@ __device__ __forceinline__ float row_codes(const CacheCall &c, const RowBits<kSl
             lo[i][e >> 2] |= (l & 0xff) << (8 * (e & 3));
         }
     }
-    return amax / 32512.0f * c.sm_log2;
+    return finite_or_nan(amax) / 32512.0f * c.sm_log2;
 }
 
 // Four int8 codes as two pairs of fp16: the bytes biased by 128 below the
@@ -246,6 +249,7 @@ struct PageWindow {
         zero = __ballot(v <= 8.077935669e-28f);
         v_log2 = v <= 8.077935669e-28f ? kZeroValues : __builtin_amdgcn_logf(v);
         v_inverse = v <= 8.077935669e-28f ? 1.2379400392853803e27f : __builtin_amdgcn_rcpf(v);
+        k_scale = finite_or_nan(k_scale);
         asm volatile("" : "+v"(k_scale));
     }
     __device__ __forceinline__ int64_t place(int i) const { return __builtin_amdgcn_readlane(at, i); }

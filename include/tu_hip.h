@@ -614,9 +614,10 @@ int32_t tu_kv_cache_read(const int8_t *k_codes, const int8_t *v_codes, const flo
  * ceil(lq / blkq)], by element strides, 16-byte aligned rows; bf16 and fp16 rows
  * are taken as integers of 16 bits with a scale a row, each element off by at most
  * max(|row|, 1e-33) / 65024.  sm_scale: positive, sm_scale * log2 e finite in fp32.
- * o: bf16, fp16 where q is, by strides.  A scale that is NaN or infinite makes NaN of the rows that see its
- * page (or have it) and of no others.  max_length: a bound of the lengths that
- * the split into ranges is made for; longer sequences are right as well.
+ * o: bf16, fp16 where q is, by strides.  A scale that is NaN or infinite makes NaN
+ * of the rows that see its page (or have it) and of no others.  max_length: a
+ * bound of the lengths that the split into ranges is made for; longer sequences
+ * are right as well.
  * workspace: 16-byte aligned, tu_kv_cache_attn_workspace(...) bytes for every
  * range on a device of `cus` compute units (0: no split); with less of it fewer
  * ranges, with none (NULL, 0) one. */

@@ -135,6 +135,25 @@ def test_scales_that_are_no_numbers(gpu_device, form, which, value):
 
 @gpu
 @each_form
+@pytest.mark.parametrize("sign", [1, -1])
+def test_infinite_scales_of_codes_that_are_not_zero(gpu_device, form, sign):
+    """Of keys and of queries: NaN wherever they are seen, scores of minus infinity among them."""
+    call = _Call(gpu_device, form, 64, "int8", seed=9)
+    call.q.fill_(1)
+    call.pool[0].abs_().clamp_(min=1).mul_(sign)
+    want = call(False)
+    first = int(call.table[0, 3])
+    call.pool[2][first, 1] = float("inf")
+    call.kw["query_scale"][1, 0, 1] = float("inf")
+    got = call(False)
+    group = call.q.size(1) // call.heads
+    bad = torch.zeros(got.shape, dtype=torch.bool, device=gpu_device)
+    bad[0, group:2 * group] = bad[1, 0, 16:32] = True
+    assert got[bad].isnan().all() and torch.isfinite(want).all() and torch.isfinite(got[~bad]).all()
+
+
+@gpu
+@each_form
 def test_queries_that_are_no_numbers(gpu_device, form):
     """NaN of those rows, and no other's."""
     call = _Call(gpu_device, form, 64, seed=5)
