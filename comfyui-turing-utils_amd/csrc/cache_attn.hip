@@ -528,10 +528,12 @@ __global__ __launch_bounds__(kThreads, 2) void cache_few_kernel(CacheCall c) {
 // each other: one's MFMAs beside the other's softmax.  Pages stream through LDS: keys
 // as codes by direct-to-LDS loads, a ring of four; values through registers, converted
 // to fp16 once, a ring of two.
-//   Bound by issue, near the power limit: a step of 256 rows takes 1.42 us at D = 128;
-// its MFMAs, LDS reads and softmax alone, in the same phases on random operands, 1.22,
-// at 1.9 GHz.  4680 rows x 32760 keys, 40 heads, int8 queries: 2.2 ms, 1400 TFLOP/s
-// (one group: 2.45 ms).
+//   Bound by issue: a step of 256 rows takes 3300 cycles at D = 128 (1.4 us at 2.36
+// GHz), 48 of its 52 MFMAs a wave with their LDS reads and the softmax alone, in the
+// same phases, 2310 of them, on one box.  The other 30 % are loads, conversions of V and
+// waits; without them the card lowers its clock (random operands: 2.0 GHz, 1.17 us a
+// step).  4680 rows x 32760 keys, 40 heads, int8 queries: 2.15-2.26 ms, box to box,
+// 1390-1460 TFLOP/s (one group: 2.45 ms).
 constexpr int kQT = 2;           // 16-row fragments of a wave
 constexpr int kWaveRows = 16 * kQT;
 constexpr int kGroupRows = 4 * kWaveRows;
@@ -1217,9 +1219,10 @@ struct CachePlan {
     uint32_t row_blocks, parts;
 };
 
-// What a block of rows costs, in steps of a page at 256 rows (1.6 us at D = 128): a step
+// What a block of rows costs, in steps of a page at 256 rows (1.4 us at D = 128): a step
 // on a CU that has one, two or three of its workgroups (as many as `places`), and the
-// pages that a start and an end take as long as.
+// pages that a start and an end take as long as.  Fitted at D = 128; D = 64 takes the
+// same ratios.
 struct BlockCost {
     int32_t rows;
     int64_t places;

@@ -17,11 +17,11 @@
 // Bound by HBM where much is written or read (2 bytes of a 16-bit type and 1 of codes
 // an element): 32760 tokens of 40 heads, D = 128, are written and read in about 200 us
 // each, 5 TB/s, the rate of a large copy.  By a chain of four loads (length, page, row,
-// scale) for single tokens: 32 tokens of 8 heads in 5 us.
+// scale) for single tokens: 32 tokens of 8 heads in 5.8 us.
 //   Heads come fastest in the grid, so that workgroups that run together read whole
 // rows of a tensor with tokens first (a token for 32 sequences and back: 14 -> 12 us;
 // tensors with heads first lose 2 percent).  Each load and store of a wave covers
-// whole lines, V^T by way of LDS (479 -> 401 us for 32760 tokens and back).
+// whole lines, V^T by way of LDS (487 -> 401 us for 32760 tokens and back).
 #include <algorithm>
 
 #include "tu_common.h"
